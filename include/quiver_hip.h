@@ -33,6 +33,9 @@ extern "C" {
 #define QV_UINT8 0
 #define QV_FLOAT 1
 #define QV_INT8 2
+/* ... and of the scoring calls below only (no reference counterpart). */
+#define QV_BFLOAT16 3
+#define QV_FLOAT16 4
 
 /* Early-exit policies: quiver::EarlyExitPolicy (src/quiver/io_control.cuh:41-46)
  * as exposed by the CLI (bin/quiver_search.cu:48-54). */
@@ -457,6 +460,81 @@ int qv_index_copy_out(const qv_index* index, uint8_t* pages, uint8_t* codes, flo
 int qv_ground_truth(const void* d_base, int32_t data_type, int64_t n, int32_t dim,
                     const float* d_queries, int64_t nq, int32_t k, int32_t* d_ids,
                     float* d_dists, int device);
+
+/* ---- Dense scores and the distribution over them (no reference counterpart) --
+ * Scoring a whole catalogue (or a linear layer) by inner products in 8 bits, and
+ * what a model's answer or its training loss takes from scores: log
+ * probabilities of given columns, the entropy, the best alternatives, and the
+ * gradient.  All pointers are device pointers of `device`; matrices are
+ * row-major with a row stride in elements (at least the row's length) and need
+ * only their element's own alignment.  Unlike the rest of this library these
+ * calls do not wait: they enqueue on `stream` (a hipStream_t; NULL is the
+ * default stream), allocate nothing, keep nothing and can be captured into a
+ * HIP graph.  Every sum has a fixed order: equal calls give equal bits.  A call
+ * that returns an error has enqueued nothing. */
+
+/* Rows to 8 bits with a scale each: a = max_j |x_ij|, scales[i] = a / 127 and
+ * codes[i][j] = x_ij * (127 / a) rounded to the nearest whole number (halves to
+ * even), all in fp32.  A row whose a is below 2^-119 counts as zeros (scale 0);
+ * one that holds an infinity or a NaN gets the scale NaN and zero codes.  type:
+ * QV_FLOAT, QV_BFLOAT16 or QV_FLOAT16. */
+int qv_quantize_rows(const void* d_x, int32_t type, int64_t n, int64_t dim, int64_t x_stride,
+                     int8_t* d_codes, int64_t code_stride, float* d_scales, int device, void* stream);
+
+/* out[i][j] = (float(sum_k a[i][k] b[j][k]) * a_scales[i]) * b_scales[j] +
+ * bias[j] for i < m, j < n: the sum exact in 32-bit integers, the rest in fp32,
+ * rounded once to out_type (QV_FLOAT, QV_BFLOAT16 or QV_FLOAT16).  d_bias may be
+ * NULL; a bias of -inf takes a column out of a softmax.  k in [0,
+ * QV_PRODUCT_MAX_K], the largest whose sums cannot overflow (with k = 0 they
+ * are 0). */
+#define QV_PRODUCT_MAX_K 131071
+int qv_int8_product(const int8_t* d_a, int64_t a_stride, const float* d_a_scales, int64_t m,
+                    const int8_t* d_b, int64_t b_stride, const float* d_b_scales, const float* d_bias,
+                    int64_t n, int64_t k, void* d_out, int32_t out_type, int64_t out_stride,
+                    int device, void* stream);
+
+/* The softmax distribution of each row of logits at a temperature, z = x /
+ * temperature, in fp32: with M = max z and S = sum exp(z - M),
+ *   target[i][t] = z[targets[i][t]] - M - ln S   (0 where targets[i][t] < 0, an
+ *                  absent one; NaN where it is past the row's end)
+ *   entropy[i]   = -sum p ln p
+ *   top_ids[i], top[i]: the topk columns with the largest logits, in descending
+ *                  order, the lower column first among equal ones, and their
+ *                  log probabilities; -1 and -inf past the columns above -inf
+ *   stats[i]     = (max x, ln S), for the gradient; ln sum exp z is
+ *                  lse[i] = max x / temperature + ln S
+ * A column at -inf has probability 0.  A row with no column above -inf (or with
+ * no column): log probabilities and lse -inf, entropy 0.  A row that holds +inf
+ * or NaN has no distribution: NaN, ids -1.  type as qv_quantize_rows; cols <
+ * 2^31; targets_per_row in [0, QV_LOG_PROBS_MAX_TARGETS]; topk in [0,
+ * QV_LOG_PROBS_MAX_TOPK]; d_targets / d_target may be NULL with targets_per_row
+ * 0, d_top_ids / d_top with topk 0; d_entropy and d_lse may be NULL.
+ * d_workspace: qv_log_probs_workspace bytes (0: none; negative: a QV_* error),
+ * 16-byte aligned, free again once the call's work on the stream is done. */
+#define QV_LOG_PROBS_MAX_TOPK 64
+#define QV_LOG_PROBS_MAX_TARGETS 64
+int64_t qv_log_probs_workspace(int64_t rows, int64_t cols, int32_t topk);
+int qv_log_probs(const void* d_logits, int32_t type, int64_t rows, int64_t cols, int64_t stride,
+                 float temperature, const int32_t* d_targets, int32_t targets_per_row, int32_t topk,
+                 float* d_target, float* d_entropy, float* d_lse, float* d_stats,
+                 int32_t* d_top_ids, float* d_top, void* d_workspace, int64_t workspace_bytes,
+                 int device, void* stream);
+
+/* The gradient of sum_t g_target target + g_entropy entropy + g_lse lse + sum_j
+ * g_top top with respect to the logits, from the same logits, targets and
+ * temperature, and the stats, entropy and top_ids that qv_log_probs gave:
+ *   dz_j = -p_j G - g_entropy p_j (ln p_j + entropy) + [j = targets_t] g_target_t
+ *          + [j = top_ids_k] g_top_k,   G = sum g_target + sum g_top - g_lse
+ * with absent targets and alternatives (ids < 0) left out, and dx = dz /
+ * temperature rounded once to the logits' type.  Any of the four gradients may
+ * be NULL (none).  A row with nothing above -inf has the gradient 0, one without
+ * a distribution NaN.  d_grad may be the logits themselves. */
+int qv_log_probs_grad(const void* d_logits, int32_t type, int64_t rows, int64_t cols, int64_t stride,
+                      float temperature, const float* d_stats, const float* d_entropy,
+                      const int32_t* d_targets, int32_t targets_per_row, const int32_t* d_top_ids,
+                      int32_t topk, const float* d_g_target, const float* d_g_entropy,
+                      const float* d_g_lse, const float* d_g_top, void* d_grad, int64_t grad_stride,
+                      int device, void* stream);
 
 /* ---- Synthetic data: the seeded Gaussian mixture of the benchmark configs ----
  * Host generator (CPU) and device generator (HIP) produce identical values for

@@ -26,6 +26,11 @@ QV_EINDEX = -7
 QV_UINT8 = 0
 QV_FLOAT = 1
 QV_INT8 = 2
+QV_BFLOAT16 = 3
+QV_FLOAT16 = 4
+QV_PRODUCT_MAX_K = 131071
+QV_LOG_PROBS_MAX_TOPK = 64
+QV_LOG_PROBS_MAX_TARGETS = 64
 QV_EXIT_NONE = 0
 QV_EXIT_GPRUNING = 2
 QV_ADMIT_STREAMING = 0
@@ -193,6 +198,13 @@ SIGNATURES = {
     "qv_index_save": (_I32, [_P, C.c_char_p]),
     "qv_index_copy_out": (_I32, [_P, _P, _P, _P, _P, _P]),
     "qv_ground_truth": (_I32, [_P, _I32, _I64, _I32, _P, _I64, _I32, _P, _P, C.c_int]),
+    "qv_quantize_rows": (_I32, [_P, _I32, _I64, _I64, _I64, _P, _I64, _P, C.c_int, _P]),
+    "qv_int8_product": (_I32, [_P, _I64, _P, _I64, _P, _I64, _P, _P, _I64, _I64, _P, _I32, _I64, C.c_int, _P]),
+    "qv_log_probs_workspace": (_I64, [_I64, _I64, _I32]),
+    "qv_log_probs": (_I32, [_P, _I32, _I64, _I64, _I64, C.c_float, _P, _I32, _I32, _P, _P, _P, _P, _P, _P, _P, _I64,
+                            C.c_int, _P]),
+    "qv_log_probs_grad": (_I32, [_P, _I32, _I64, _I64, _I64, C.c_float, _P, _P, _P, _I32, _P, _I32, _P, _P, _P, _P,
+                                 _P, _I64, C.c_int, _P]),
     "qv_find_index_files": (_I32, [C.c_char_p, C.c_char_p, C.c_char_p, _I32]),
     "qv_read_layout": (_I32, [C.c_char_p, C.c_char_p, C.POINTER(IndexInfo)]),
     "qv_read_index_pages": (_I32, [C.c_char_p, _I64, _P]),
