@@ -1,5 +1,13 @@
 // qv_log_probs.hip -- log probabilities of given columns, entropy and best
 // alternatives of each row of logits, and their gradient.
+//
+// Everything is computed in base 2 relative to a running largest value m: with c =
+// log2(e) / T, s = sum 2^y and w = sum y 2^y over y = x c - m c, a row's ln S is
+// log2(s) ln 2 and its entropy ln 2 (log2(s) - w / s), which no cancellation
+// touches (w <= 0, s >= 1).  One pass over the row: a lane keeps its own m, s and w
+// and moves them to a new m only when a batch of its values holds a larger one.
+// The reference subtracted is fl(m c), not m c, so that y is one fused
+// multiply-add; the difference (fma(-m, c, fl(m c)), exact) enters once at the end.
 #include <algorithm>
 
 #include "qv_dense.hpp"
@@ -12,154 +20,612 @@ using namespace qv::dense;
 namespace {
 
 constexpr float kInf = __builtin_inff();
+constexpr float kLog2e = 1.44269504088896340736f, kLn2 = 0.69314718055994530942f;
+constexpr float kBig = 1e38f;    // |m c| from here on: differences are taken before they are multiplied
+constexpr float kNone = -200.f;  // 2^-200 is 0 in fp32: stands for -inf where it would be multiplied by 0
+
+// ---- values ------------------------------------------------------------------
+
+typedef uint32_t raw4 __attribute__((ext_vector_type(4)));
+typedef raw4 raw4_any __attribute__((aligned(2), may_alias));  // rows need only their elements' alignment
+
+template <class T>
+constexpr int kVec = 16 / (int)sizeof(T);
+
+template <class T>
+__device__ __forceinline__ raw4 load_raw(const T* p) {
+  return *reinterpret_cast<const raw4_any*>(p);
+}
+
+template <class T>
+__device__ __forceinline__ void unpack(raw4 r, float* v) {
+#pragma unroll
+  for (int i = 0; i < 4; i++) {
+    if constexpr (sizeof(T) == 4) {
+      v[i] = __uint_as_float(r[i]);
+    } else if constexpr (std::is_same<T, bf16>::value) {
+      v[2 * i] = __uint_as_float(r[i] << 16);
+      v[2 * i + 1] = __uint_as_float(r[i] & 0xffff0000u);
+    } else {
+      typedef f16 h2 __attribute__((ext_vector_type(2)));
+      const h2 h = __builtin_bit_cast(h2, (uint32_t)r[i]);
+      v[2 * i] = (float)h[0];
+      v[2 * i + 1] = (float)h[1];
+    }
+  }
+}
+
+// The vector at p of which `valid` elements are in the row, -inf past them.
+template <class T>
+__device__ __forceinline__ void load_tail(const T* p, int64_t valid, float* v) {
+  if (valid >= kVec<T>) {
+    unpack<T>(load_raw(p), v);
+  } else {
+#pragma unroll
+    for (int i = 0; i < kVec<T>; i++) v[i] = i < valid ? (float)p[i] : -kInf;
+  }
+}
+
+template <class T>
+__device__ __forceinline__ void store_vec(T* p, const float* v) {
+  raw4 r;
+#pragma unroll
+  for (int i = 0; i < 4; i++) {
+    if constexpr (sizeof(T) == 4) {
+      r[i] = __float_as_uint(v[i]);
+    } else {
+      typedef T t2 __attribute__((ext_vector_type(2)));
+      t2 h;
+      h[0] = (T)v[2 * i];
+      h[1] = (T)v[2 * i + 1];
+      r[i] = __builtin_bit_cast(uint32_t, h);
+    }
+  }
+  *reinterpret_cast<raw4_any*>(p) = r;
+}
+
+// Maxima without the compiler's quieting of each operand (a NaN among the values
+// shows in s).
+__device__ __forceinline__ float max2(float a, float b) {
+  float r;
+  asm("v_max_f32 %0, %1, %2" : "=v"(r) : "v"(a), "v"(b));
+  return r;
+}
+__device__ __forceinline__ float max3(float a, float b, float c) {
+  float r;
+  asm("v_max3_f32 %0, %1, %2, %3" : "=v"(r) : "v"(a), "v"(b), "v"(c));
+  return r;
+}
+
+// ---- keys of the alternatives --------------------------------------------------
 
 // Orders as the values do, larger first by larger key, equal values (the two
 // zeros among them) the lower column first; never 0 for a value above -inf.
-__device__ __forceinline__ uint64_t rank_key(float x, uint32_t column) {
+__device__ __forceinline__ uint32_t rank_of(float x) {
   const uint32_t b = __float_as_uint(x + 0.f);
-  const uint32_t order = b & 0x80000000u ? ~b : b | 0x80000000u;
-  return ((uint64_t)order << 32) | (uint32_t)~column;
+  return b & 0x80000000u ? ~b : b | 0x80000000u;
+}
+__device__ __forceinline__ float value_of(uint32_t rank) {
+  return __uint_as_float(rank & 0x80000000u ? rank ^ 0x80000000u : ~rank);
+}
+__device__ __forceinline__ uint64_t rank_key(float x, uint32_t column) {
+  return ((uint64_t)rank_of(x) << 32) | (uint32_t)~column;
 }
 
-template <class F>
-__device__ float block_fold(float v, float* tmp, F f) {
-  __syncthreads();
-  tmp[threadIdx.x] = v;
-  __syncthreads();
-  for (int s = 128; s; s >>= 1) {
-    if ((int)threadIdx.x < s) tmp[threadIdx.x] = f(tmp[threadIdx.x], tmp[threadIdx.x + s]);
-    __syncthreads();
+// The 64 largest of two lists of 64, both and the result in descending order.
+__device__ __forceinline__ uint64_t merge_desc(uint64_t a, uint64_t b) {
+  const int lane = opaque_lane();
+  const int from = (63 - lane) << 2;
+  const uint64_t r = ((uint64_t)(uint32_t)__builtin_amdgcn_ds_bpermute(from, (int)(uint32_t)(b >> 32)) << 32) |
+                     (uint32_t)__builtin_amdgcn_ds_bpermute(from, (int)(uint32_t)b);
+  uint64_t key = umax64(a, r);
+  key = cx_stage<32>(key, lane, false);
+  key = cx_stage<16>(key, lane, false);
+  key = cx_stage<8>(key, lane, false);
+  key = cx_stage<4>(key, lane, false);
+  key = cx_stage<2>(key, lane, false);
+  key = cx_stage<1>(key, lane, false);
+  return key;
+}
+
+// A wave's best keys: entry i of the list in lane i.  Candidates wait in LDS, 64 of
+// them are sorted and merged at once: a tenth of what placing them one by one
+// costs.
+constexpr int kPool = 128;
+
+struct Best {
+  uint64_t list = 0;
+  uint64_t* pool;  // [kPool], this wave's
+  int count = 0;
+  int k;
+
+  __device__ Best(uint64_t* pool_, int k_) : pool(pool_), k(k_) {}
+
+  __device__ __forceinline__ void merge(uint64_t key) { list = merge_desc(list, wave_sort_desc(key)); }
+
+  __device__ __forceinline__ void offer(bool take, uint64_t key) {
+    const uint64_t mask = __ballot(take);
+    if (mask == 0) return;
+    if (take) pool[count + __builtin_amdgcn_mbcnt_hi((uint32_t)(mask >> 32), __builtin_amdgcn_mbcnt_lo((uint32_t)mask, 0))] = key;
+    count += __popcll(mask);
+    if (count >= kWave) {
+      __builtin_amdgcn_fence(__ATOMIC_ACQ_REL, "wavefront");
+      count -= kWave;
+      merge(pool[count + lane_id()]);
+      __builtin_amdgcn_fence(__ATOMIC_ACQ_REL, "wavefront");
+    }
   }
-  return tmp[0];
+  __device__ __forceinline__ void finish() {
+    if (count == 0) return;
+    __builtin_amdgcn_fence(__ATOMIC_ACQ_REL, "wavefront");
+    merge(lane_id() < count ? pool[lane_id()] : 0);
+    count = 0;
+  }
+  // The k-th key so far (0 while there are fewer).
+  __device__ __forceinline__ uint64_t last() const { return read_lane_u64(list, k - 1); }
+};
+
+// ---- sums ----------------------------------------------------------------------
+
+__device__ __forceinline__ float scaled(float m, float c) { return m == -kInf ? 0.f : m * c; }
+__device__ __forceinline__ bool is_big(float mc) { return !(fabsf(mc) < kBig); }
+
+// log2 of what sums relative to m are multiplied by when the reference becomes
+// to >= m: their two rounded references' difference, or, where those overflow, the
+// difference's product (then 0 or far below every value that counts).
+__device__ __forceinline__ float shift_of(float m, float to, float c) {
+  const float a = scaled(m, c), b = scaled(to, c);
+  const float d = is_big(a) || is_big(b) ? (m == to ? 0.f : (m - to) * c) : a - b;
+  return m == -kInf ? kNone : max2(d, kNone);
 }
 
-// One workgroup per row; the row is read once for its largest value, once for the
-// sums, and once for each alternative.
+struct Sums {
+  float m = -kInf, s = 0.f, w = 0.f;
+
+  __device__ __forceinline__ void move(float to, float c) {
+    const float d = shift_of(m, to, c), f = __builtin_amdgcn_exp2f(d);
+    w = f * __fmaf_rn(d, s, w);
+    s = f * s;
+    m = to;
+  }
+  __device__ __forceinline__ void add(Sums o, float c) {
+    const float to = max2(m, o.m);
+    move(to, c);
+    o.move(to, c);
+    s = s + o.s;
+    w = w + o.w;
+  }
+  __device__ __forceinline__ float4 packed() const { return make_float4(m, s, w, 0.f); }
+  static __device__ __forceinline__ Sums of(float4 p) {
+    Sums o;
+    o.m = p.x;
+    o.s = p.y;
+    o.w = p.z;
+    return o;
+  }
+  // Over the wave, in a fixed order, the same in every lane.
+  __device__ __forceinline__ void fold(float c) {
+    float to = m;
+#pragma unroll
+    for (int x = 1; x < kWave; x *= 2) to = max2(to, __shfl_xor(to, x));
+    move(to, c);
+#pragma unroll
+    for (int x = 1; x < kWave; x *= 2) {
+      s = s + __shfl_xor(s, x);
+      w = w + __shfl_xor(w, x);
+    }
+  }
+};
+
+// One wave's pass over columns [from, to) of a row, every `step` batches of N U-vector loads.
+template <class T, int U, bool TOP>
+struct Pass {
+  static constexpr int N = U * kVec<T>;
+  static constexpr int kBatch = kWave * N;  // columns of a batch: vector u of lane l at (64 u + l) kVec
+  Sums sum;
+  float c, mc = 0.f;
+  bool big = false;
+  float least = -__FLT_MAX__;  // values below it are not among the k largest
+  Best best;
+
+  __device__ Pass(float c_, uint64_t* pool, int k) : c(c_), best(pool, k) {}
+
+  __device__ __forceinline__ void values(const float (&v)[N], int column, bool first) {
+    float top = v[0];
+#pragma unroll
+    for (int i = 1; i + 1 < N; i += 2) top = max3(top, v[i], v[i + 1]);
+    if constexpr (N % 2 == 0) top = max2(top, v[N - 1]);
+    if (__any(top > sum.m)) {
+      sum.move(max2(sum.m, top), c);
+      mc = scaled(sum.m, c);
+      big = __any(is_big(mc));
+    }
+    float s = 0.f, w = 0.f;
+    if (!big) {
+#pragma unroll
+      for (int i = 0; i < N; i++) {
+        const float y = __fmaf_rn(v[i], c, -mc), e = __builtin_amdgcn_exp2f(y);
+        s = s + e;
+        w = __fmaf_rn(e, max2(y, kNone), w);
+      }
+    } else {
+      const bool far = is_big(mc);
+#pragma unroll
+      for (int i = 0; i < N; i++) {
+        const float y = far ? (v[i] - sum.m) * c : __fmaf_rn(v[i], c, -mc), e = __builtin_amdgcn_exp2f(y);
+        s = s + e;
+        w = __fmaf_rn(e, max2(y, kNone), w);
+      }
+    }
+    sum.s = sum.s + s;
+    sum.w = sum.w + w;
+    if constexpr (TOP) {
+      if (first) {
+        // the k-th of the lanes' largest: k values are at least that large
+        const uint64_t order = wave_sort_desc(rank_key(top, (uint32_t)lane_id()));
+        least = max2(least, value_of((uint32_t)(read_lane_u64(order, best.k - 1) >> 32)));
+      }
+      if (__any(top >= least)) {
+#pragma unroll
+        for (int i = 0; i < N; i++) {
+          const int at = column + (i / kVec<T>)*kWave * kVec<T> + i % kVec<T>;
+          best.offer(v[i] >= least, rank_key(v[i], (uint32_t)at));
+        }
+        raise(best.last());
+      }
+    }
+  }
+  __device__ __forceinline__ void raise(uint64_t key) {
+    if (key) least = max2(least, value_of((uint32_t)(key >> 32)));
+  }
+
+  // Batches [b, end) in steps; shared: the block's largest k-th value so far (ranks), or null.
+  __device__ void run(const T* __restrict__ x, int64_t from, int64_t to, int b, int step, uint32_t* shared) {
+    const int lane = lane_id();
+    bool first = true;
+    for (int64_t at = from + (int64_t)b * kBatch; at < to; at += (int64_t)step * kBatch) {
+      float v[N];
+      const int64_t mine = at + lane * kVec<T>;
+      if (at + kBatch <= to) {
+        raw4 r[U];
+#pragma unroll
+        for (int u = 0; u < U; u++) r[u] = load_raw(x + mine + u * kWave * kVec<T>);
+#pragma unroll
+        for (int u = 0; u < U; u++) unpack<T>(r[u], v + u * kVec<T>);
+      } else {
+#pragma unroll
+        for (int u = 0; u < U; u++)
+          load_tail(x + mine + u * kWave * kVec<T>, to - mine - u * kWave * kVec<T>, v + u * kVec<T>);
+      }
+      if (TOP && shared) least = max2(least, value_of(max(rank_of(least), *(volatile uint32_t*)shared)));
+      values(v, (int)mine, first);
+      if (TOP && shared && lane == 0) atomicMax(shared, rank_of(least));
+      first = false;
+    }
+    if constexpr (TOP) best.finish();
+    sum.fold(c);
+  }
+};
+
+struct Out {
+  const int32_t* targets;
+  int per_row, topk;
+  float *target, *entropy, *lse, *stats;
+  int32_t* top_ids;
+  float* top;
+};
+
+// A row's results from its sums (in every lane) and its list, by one wave.
 template <class T>
-__global__ __launch_bounds__(256) void log_probs_kernel(const T* __restrict__ logits, int64_t rows, int cols,
-                                                        int64_t stride, float inv_t, const int32_t* __restrict__ targets,
-                                                        int per_row, int topk, float* __restrict__ target,
-                                                        float* __restrict__ entropy, float* __restrict__ lse,
-                                                        float* __restrict__ stats, int32_t* __restrict__ top_ids,
-                                                        float* __restrict__ top) {
-  __shared__ float tmp[256];
-  __shared__ uint64_t keys[256];
-  const int64_t row = blockIdx.x;
-  const T* x = logits + row * stride;
-  const int tid = threadIdx.x;
-  float m = -kInf, odd = 0.f;
-  for (int64_t j = tid; j < cols; j += 256) {
-    const float v = (float)x[j];
-    if (!(v < kInf)) odd = 1.f;
-    m = fmaxf(m, v);
-  }
-  m = block_fold(m, tmp, [](float a, float b) { return fmaxf(a, b); });
-  odd = block_fold(odd, tmp, [](float a, float b) { return fmaxf(a, b); });
-  const float ref = m == -kInf ? 0.f : m;
-  float s = 0.f, w = 0.f;
-  for (int64_t j = tid; j < cols; j += 256) {
-    const float y = fmaxf(((float)x[j] - ref) * inv_t, -200.f);
-    const float e = expf(y);
-    s += e;
-    w += e * y;
-  }
-  s = block_fold(s, tmp, [](float a, float b) { return a + b; });
-  w = block_fold(w, tmp, [](float a, float b) { return a + b; });
-  const bool empty = m == -kInf && odd == 0.f;
+__device__ __forceinline__ void finish_row(const T* __restrict__ x, int64_t row, int cols, const Sums& sum,
+                                           uint64_t list, float c, float inv_t, const Out& o) {
+  const int lane = lane_id();
+  const bool odd = sum.s != sum.s, empty = sum.s == 0.f;
   const float nan = __builtin_nanf("");
-  const float ln_s = odd != 0.f ? nan : empty ? -kInf : logf(s);
-  if (odd != 0.f) m = nan;
-  auto lp = [&](float v) { return odd != 0.f ? nan : v == -kInf ? -kInf : (v - ref) * inv_t - ln_s; };
-  if (tid == 0) {
-    if (entropy) entropy[row] = odd != 0.f ? nan : empty ? 0.f : ln_s - w / s;
-    if (lse) lse[row] = empty ? -kInf : m * inv_t + ln_s;
-    stats[2 * row] = m;
-    stats[2 * row + 1] = ln_s;
+  const float mc = scaled(sum.m, c);
+  // log2 of the sum relative to m c itself
+  const float log2_s = log2f(sum.s) + (is_big(mc) ? 0.f : __fmaf_rn(-sum.m, c, mc));
+  const float ln_s = odd ? nan : empty ? -kInf : log2_s * kLn2;
+  auto lp = [&](float v) { return odd ? nan : v == -kInf ? -kInf : __fmaf_rn(v - sum.m, inv_t, -ln_s); };
+  if (lane == 0) {
+    if (o.entropy) o.entropy[row] = odd ? nan : empty ? 0.f : (log2f(sum.s) - sum.w / sum.s) * kLn2;
+    if (o.lse) o.lse[row] = odd ? nan : empty ? -kInf : __fmaf_rn(sum.m, inv_t, ln_s);
+    o.stats[2 * row] = odd ? nan : sum.m;
+    o.stats[2 * row + 1] = ln_s;
   }
-  for (int t = tid; t < per_row; t += 256) {
-    const int32_t j = targets[row * per_row + t];
-    target[row * per_row + t] = j < 0 ? 0.f : j >= cols ? nan : lp((float)x[j]);
+  if (lane < o.per_row) {
+    const int32_t j = o.targets[row * o.per_row + lane];
+    o.target[row * o.per_row + lane] = j < 0 ? 0.f : j >= cols ? nan : lp((float)x[j]);
   }
-  uint64_t last = ~0ull;
-  for (int k = 0; k < topk; k++) {
-    uint64_t best = 0;
-    for (int64_t j = tid; j < cols; j += 256) {
-      const float v = (float)x[j];
-      const uint64_t key = rank_key(v, (uint32_t)j);
-      if (v > -kInf && key < last && key > best) best = key;
-    }
-    __syncthreads();
-    keys[tid] = best;
-    __syncthreads();
-    for (int q = 128; q; q >>= 1) {
-      if (tid < q) keys[tid] = umax64(keys[tid], keys[tid + q]);
-      __syncthreads();
-    }
-    last = keys[0];
-    if (tid == 0) {
-      const bool none = last == 0 || odd != 0.f;
-      top_ids[row * topk + k] = none ? -1 : (int32_t)~(uint32_t)last;
-      top[row * topk + k] = odd != 0.f ? nan : none ? -kInf : lp((float)x[~(uint32_t)last]);
-    }
+  if (lane < o.topk) {
+    const bool none = odd || list == 0;
+    o.top_ids[row * o.topk + lane] = none ? -1 : (int32_t)~(uint32_t)list;
+    o.top[row * o.topk + lane] = odd ? nan : none ? -kInf : lp(value_of((uint32_t)(list >> 32)));
   }
 }
 
-// One workgroup per row: every column by the formula's first two terms, then the
-// columns that targets or alternatives name.
-template <class T>
-__global__ __launch_bounds__(256) void log_probs_grad_kernel(
-    const T* logits, int64_t rows, int cols, int64_t stride, float inv_t, const float* __restrict__ stats,
-    const float* __restrict__ entropy, const int32_t* __restrict__ targets, int per_row,
-    const int32_t* __restrict__ top_ids, int topk, const float* __restrict__ g_target,
-    const float* __restrict__ g_entropy, const float* __restrict__ g_lse, const float* __restrict__ g_top, T* grad,
-    int64_t grad_stride) {
+// One wave per row: no barrier, no join.
+template <class T, int U, bool TOP>
+__global__ __launch_bounds__(256) void log_probs_wave_kernel(const T* __restrict__ logits, int64_t rows, int cols,
+                                                             int64_t stride, float c, float inv_t, Out o) {
+  __shared__ uint64_t pool[TOP ? 4 * kPool : 1];
+  const int wave = threadIdx.x / kWave;
+  const int64_t row = (int64_t)blockIdx.x * 4 + wave;
+  if (row >= rows) return;
+  const T* x = logits + row * stride;
+  Pass<T, U, TOP> pass(c, TOP ? pool + wave * kPool : pool, o.topk);
+  pass.run(x, 0, cols, 0, 1, nullptr);
+  finish_row(x, row, cols, pass.sum, pass.best.list, c, inv_t, o);
+}
+
+// One workgroup per chunk of a row.  With one chunk per row its results, else the
+// chunk's sums and keys, for join_kernel.
+template <class T, int U, bool TOP>
+__global__ __launch_bounds__(256) void log_probs_block_kernel(const T* __restrict__ logits, int cols, int64_t stride,
+                                                              float c, float inv_t, int64_t chunk, int splits, Out o,
+                                                              float4* __restrict__ part,
+                                                              uint64_t* __restrict__ part_keys) {
+  __shared__ uint64_t pool[TOP ? 4 * kPool : 1];
+  __shared__ float4 sums[4];
+  __shared__ uint32_t least;
+  const int tid = threadIdx.x, wave = tid / kWave, lane = lane_id();
+  const int64_t row = blockIdx.x / (unsigned)splits;
+  const int split = (int)(blockIdx.x - row * splits);
+  const T* x = logits + row * stride;
+  if constexpr (TOP) {
+    if (tid == 0) least = 0;
+    __syncthreads();
+  }
+  Pass<T, U, TOP> pass(c, TOP ? pool + wave * kPool : pool, o.topk);
+  const int64_t from = (int64_t)split * chunk;
+  pass.run(x, from, min((int64_t)cols, from + chunk), wave, 4, &least);
+  if (lane == 0) sums[wave] = pass.sum.packed();
+  if constexpr (TOP) pool[wave * kPool + lane] = pass.best.list;
+  __syncthreads();
+  if (wave) return;
+  Sums sum = Sums::of(sums[0]);
+#pragma unroll
+  for (int q = 1; q < 4; q++) sum.add(Sums::of(sums[q]), c);
+  uint64_t list = pass.best.list;
+  if constexpr (TOP) {
+#pragma unroll
+    for (int q = 1; q < 4; q++) list = merge_desc(list, pool[q * kPool + lane]);
+  }
+  if (splits == 1) {
+    finish_row(x, row, cols, sum, list, c, inv_t, o);
+  } else {
+    if (lane == 0) part[blockIdx.x] = sum.packed();
+    if (TOP && lane < o.topk) part_keys[(int64_t)blockIdx.x * o.topk + lane] = list;
+  }
+}
+
+// One workgroup per row joins its chunks.
+template <class T, bool TOP>
+__global__ __launch_bounds__(256) void join_kernel(const T* __restrict__ logits, int cols, int64_t stride, float c,
+                                                   float inv_t, int splits, Out o, const float4* __restrict__ part,
+                                                   const uint64_t* __restrict__ part_keys) {
+  __shared__ uint64_t pool[TOP ? 4 * kPool : 1];
+  __shared__ float4 sums[4];
+  const int tid = threadIdx.x, wave = tid / kWave, lane = lane_id();
   const int64_t row = blockIdx.x;
+  Sums sum;
+  for (int i = tid; i < splits; i += 256) {
+    sum.add(Sums::of(part[row * splits + i]), c);
+  }
+  sum.fold(c);
+  Best best(TOP ? pool + wave * kPool : pool, o.topk);
+  if constexpr (TOP) {
+    const uint64_t* keys = part_keys + row * splits * o.topk;
+    // the k-th of 64 chunks' largest keys: k keys are at least that large
+    const int head = wave * kWave + lane;
+    const uint64_t order = wave_sort_desc(head < splits ? keys[(int64_t)head * o.topk] : 0);
+    uint64_t least = read_lane_u64(order, o.topk - 1);
+    const int total = splits * o.topk;
+    for (int i = wave * kWave; i < total; i += 256) {
+      const uint64_t key = i + lane < total ? keys[i + lane] : 0;
+      best.offer(key && key >= least, key);
+      least = umax64(least, best.last());
+    }
+    best.finish();
+    pool[wave * kPool + lane] = best.list;
+  }
+  if (lane == 0) sums[wave] = sum.packed();
+  __syncthreads();
+  if (wave) return;
+  sum = Sums::of(sums[0]);
+#pragma unroll
+  for (int q = 1; q < 4; q++) sum.add(Sums::of(sums[q]), c);
+  uint64_t list = best.list;
+  if constexpr (TOP) {
+#pragma unroll
+    for (int q = 1; q < 4; q++) list = merge_desc(list, pool[q * kPool + lane]);
+  }
+  finish_row(logits + row * stride, row, cols, sum, list, c, inv_t, o);
+}
+
+// ---- gradient ------------------------------------------------------------------
+
+struct Weights {
+  const float *stats, *entropy;
+  const int32_t* targets;
+  int per_row;  // 0 without g_target
+  const int32_t* top_ids;
+  int topk;     // 0 without g_top
+  const float *g_target, *g_entropy, *g_lse, *g_top;
+};
+
+// One wave per chunk of a row: every column by the first two terms, p (a + b log2
+// p), then the columns that targets or alternatives name, whose weights add up in
+// their order.  The named columns' logits are read before any column is written
+// (the gradient may take the logits' place); a wave's stores to one address stay
+// in order.
+template <class T, int U>
+__global__ __launch_bounds__(256) void log_probs_grad_kernel(const T* logits, int64_t units, int cols, int64_t stride,
+                                                             float c, float inv_t, int chunk, int splits, Weights g,
+                                                             T* grad, int64_t grad_stride) {
+  constexpr int N = U * kVec<T>, kBatch = kWave * N;
+  const int64_t unit = (int64_t)blockIdx.x * 4 + threadIdx.x / kWave;
+  if (unit >= units) return;
+  const int lane = lane_id();
+  const int64_t row = unit / splits;
+  const int64_t from = (unit - row * splits) * chunk, to = min((int64_t)cols, from + chunk);
   const T* x = logits + row * stride;
   T* dx = grad + row * grad_stride;
-  const int tid = threadIdx.x;
-  const float m = stats[2 * row], ln_s = stats[2 * row + 1];
-  const float ge = g_entropy ? g_entropy[row] : 0.f, h = g_entropy ? entropy[row] : 0.f;
-  float g = g_lse ? -g_lse[row] : 0.f;
-  const int named = (g_target ? per_row : 0) + (g_top ? topk : 0);
-  auto name = [&](int i, float& w) {
-    const int t = g_target ? per_row : 0;
-    const int32_t j = i < t ? targets[row * per_row + i] : top_ids[row * topk + i - t];
-    w = i < t ? g_target[row * per_row + i] : g_top[row * topk + i - t];
-    return j;
-  };
-  for (int i = 0; i < named; i++) {
-    float w;
-    if (name(i, w) >= 0) g += w;
+  const float m = g.stats[2 * row], ln_s = g.stats[2 * row + 1], log2_s = ln_s * kLog2e;
+  const bool odd = m != m, empty = m == -kInf;
+
+  int32_t id[2] = {-1, -1};
+  float weight[2] = {0.f, 0.f}, total = 0.f;
+  const int named = g.per_row + g.topk;
+#pragma unroll
+  for (int h = 0; h < 2; h++) {
+    const int i = h * kWave + lane;
+    if (i >= named) continue;
+    const bool t = i < g.per_row;
+    const int64_t at = t ? row * g.per_row + i : row * g.topk + i - g.per_row;
+    id[h] = t ? g.targets[at] : g.top_ids[at];
+    weight[h] = t ? g.g_target[at] : g.g_top[at];
+    if (id[h] >= 0) total = total + weight[h];
   }
+  if (named) {
+#pragma unroll
+    for (int q = 1; q < kWave; q *= 2) total = total + __shfl_xor(total, q);
+  }
+  if (g.g_lse) total = total - g.g_lse[row];
+  const float ge = g.g_entropy ? g.g_entropy[row] : 0.f, h = g.g_entropy ? g.entropy[row] : 0.f;
+  const float nan = __builtin_nanf("");
+  const float a = odd ? nan : empty ? 0.f : -(total + ge * h) * inv_t;
+  const float b = empty ? 0.f : -(ge * kLn2) * inv_t;
   auto dense = [&](float v) {
-    if (m == -kInf || m != m) return m == -kInf ? 0.f : m;
-    const float lp = fmaxf((v - m) * inv_t - ln_s, -1000.f);
-    const float p = expf(lp);
-    return v == -kInf ? 0.f : -p * g - ge * (p * (lp + h));
+    const float y = max2(__fmaf_rn(v - m, c, -log2_s), kNone);
+    // the instruction gives 0 below 2^-126: probabilities down there are taken 2^64 larger
+    const bool low = y < -126.f;
+    const float p = __builtin_amdgcn_exp2f(low ? y + 64.f : y);
+    return p * (__fmaf_rn(b, y, a) * (low ? 0x1p-64f : 1.f));
   };
-  // a named column's value: its weights added in their order
-  auto value = [&](int i, float v) {
-    float w, sum = dense(v);
-    const int32_t j = name(i, w);
-    for (int q = 0; q < named; q++)
-      if (name(q, w) == j && m != -kInf) sum += w;
-    return sum * inv_t;
-  };
-  float w, patch = 0.f;
-  __shared__ float kept[256];
-  const bool shared_rows = named <= 256;
-  if (shared_rows && tid < named) {
-    const int32_t j = name(tid, w);
-    if (j >= 0 && j < cols) patch = (float)x[j];
+
+  float extra[2] = {0.f, 0.f}, kept[2] = {0.f, 0.f};
+  uint64_t here[2] = {0, 0};
+  if (named) {
+#pragma unroll
+    for (int q = 0; q < 2; q++) {
+      here[q] = __ballot(id[q] >= from && id[q] < to);
+      if (here[q] >> lane & 1) kept[q] = (float)x[id[q]];
+    }
+#pragma unroll
+    for (int q = 0; q < 2; q++) {
+      for (uint64_t left = here[q]; left; left &= left - 1) {
+        const int l = __ffsll((long long)left) - 1;
+        const int32_t j = read_lane_i32(id[q], l);
+        const float w = read_lane_f32(weight[q], l);
+        if (id[0] == j) extra[0] = extra[0] + w;
+        if (id[1] == j) extra[1] = extra[1] + w;
+      }
+    }
   }
-  kept[tid] = patch;
-  __syncthreads();
-  for (int64_t j = tid; j < cols; j += 256) dx[j] = (T)(dense((float)x[j]) * inv_t);
-  __syncthreads();
-  if (tid < named) {
-    const int32_t j = name(tid, w);
-    if (j >= 0 && j < cols) dx[j] = (T)value(tid, kept[tid]);
+  for (int64_t at = from; at < to; at += kBatch) {
+    const int64_t mine = at + lane * kVec<T>;
+    if (at + kBatch <= to) {
+      raw4 r[U];
+#pragma unroll
+      for (int u = 0; u < U; u++) r[u] = load_raw(x + mine + u * kWave * kVec<T>);
+#pragma unroll
+      for (int u = 0; u < U; u++) {
+        float v[kVec<T>];
+        unpack<T>(r[u], v);
+#pragma unroll
+        for (int i = 0; i < kVec<T>; i++) v[i] = dense(v[i]);
+        store_vec(dx + mine + u * kWave * kVec<T>, v);
+      }
+    } else {
+#pragma unroll
+      for (int u = 0; u < U; u++) {
+        const int64_t p = mine + u * kWave * kVec<T>, valid = to - p;
+        float v[kVec<T>];
+        load_tail(x + p, valid, v);
+#pragma unroll
+        for (int i = 0; i < kVec<T>; i++) v[i] = dense(v[i]);
+        if (valid >= kVec<T>) {
+          store_vec(dx + p, v);
+        } else {
+#pragma unroll
+          for (int i = 0; i < kVec<T>; i++)
+            if (i < valid) dx[p + i] = (T)v[i];
+        }
+      }
+    }
   }
+  if (here[0] | here[1]) {
+    __builtin_amdgcn_fence(__ATOMIC_ACQ_REL, "wavefront");
+#pragma unroll
+    for (int q = 0; q < 2; q++)
+      if (here[q] >> lane & 1)
+        dx[id[q]] = (T)(dense(kept[q]) + (empty ? 0.f : extra[q] * inv_t));
+  }
+}
+
+// ---- launches --------------------------------------------------------------------
+
+// How a call's rows are cut.
+struct Plan {
+  bool waves;     // one wave per row
+  int splits;     // chunks per row (workgroups)
+  int64_t chunk;  // columns
+};
+
+constexpr int64_t kStep = 4096;  // columns: one batch of each of a workgroup's four waves
+
+Plan plan_of(int64_t rows, int64_t cols) {
+  if (cols <= 1024 || (rows >= 4096 && cols <= 8192)) return {true, 1, cols};
+  const int64_t most = (cols + kStep - 1) / kStep;
+  const int64_t want = std::min<int64_t>(std::min<int64_t>(most, 1024), (2048 + rows - 1) / rows);
+  const int64_t steps = (most + want - 1) / want;
+  return {false, (int)((most + steps - 1) / steps), steps * kStep};
+}
+
+template <class T, bool TOP>
+void log_probs(const T* x, int64_t rows, int64_t cols, int64_t stride, float temperature, const Out& o, void* work,
+               hipStream_t st) {
+  const float c = (float)(1.44269504088896340736 / (double)temperature), inv_t = (float)(1.0 / (double)temperature);
+  const Plan p = plan_of(rows, cols);
+  if (p.waves) {
+    const dim3 grid((unsigned)((rows + 3) / 4));
+    if (cols <= kWave * kVec<T>)
+      hipLaunchKernelGGL((log_probs_wave_kernel<T, 1, TOP>), grid, dim3(256), 0, st, x, rows, (int)cols, stride, c,
+                         inv_t, o);
+    else
+      hipLaunchKernelGGL((log_probs_wave_kernel<T, 16 / kVec<T>, TOP>), grid, dim3(256), 0, st, x, rows, (int)cols, stride, c,
+                         inv_t, o);
+    HIP_OK(hipGetLastError());
+    return;
+  }
+  float4* part = static_cast<float4*>(work);
+  uint64_t* keys = reinterpret_cast<uint64_t*>(part + rows * p.splits);
+  hipLaunchKernelGGL((log_probs_block_kernel<T, 16 / kVec<T>, TOP>), dim3((unsigned)(rows * p.splits)), dim3(256), 0, st, x,
+                     (int)cols, stride, c, inv_t, p.chunk, p.splits, o, part, keys);
+  HIP_OK(hipGetLastError());
+  if (p.splits > 1) {
+    hipLaunchKernelGGL((join_kernel<T, TOP>), dim3((unsigned)rows), dim3(256), 0, st, x, (int)cols, stride, c, inv_t,
+                       p.splits, o, part, keys);
+    HIP_OK(hipGetLastError());
+  }
+}
+
+template <class T>
+void log_probs_grad(const T* x, int64_t rows, int64_t cols, int64_t stride, float temperature, const Weights& g,
+                    T* grad, int64_t grad_stride, hipStream_t st) {
+  constexpr int U = 16 / kVec<T>;
+  const float c = (float)(1.44269504088896340736 / (double)temperature), inv_t = (float)(1.0 / (double)temperature);
+  const int64_t chunk = 4 * kWave * U * kVec<T>;
+  const int64_t splits = (cols + chunk - 1) / chunk, units = rows * splits;
+  hipLaunchKernelGGL((log_probs_grad_kernel<T, U>), dim3((unsigned)((units + 3) / 4)), dim3(256), 0, st, x, units,
+                     (int)cols, stride, c, inv_t, (int)chunk, (int)splits, g, grad, grad_stride);
+  HIP_OK(hipGetLastError());
+}
+
+int64_t workspace_of(int64_t rows, int64_t cols, int32_t topk) {
+  const Plan p = plan_of(rows, cols);
+  return p.splits > 1 ? rows * p.splits * (int64_t)(sizeof(float4) + sizeof(uint64_t) * topk) : 0;
 }
 
 void check_rows(int32_t type, int64_t rows, int64_t cols, int64_t stride, const void* x, float temperature,
@@ -184,6 +650,8 @@ int64_t qv_log_probs_workspace(int64_t rows, int64_t cols, int32_t topk) {
   const int rc = qv::guard([&] {
     if (rows < 0 || cols < 0 || topk < 0) qv::fail(QV_EINVAL, "negative size");
     if (topk > QV_LOG_PROBS_MAX_TOPK) qv::fail(QV_EUNSUPPORTED, "topk above 64");
+    if (rows > INT32_MAX || cols > INT32_MAX) qv::fail(QV_EUNSUPPORTED, "more than 2^31 - 1 rows or columns");
+    if (rows) bytes = workspace_of(rows, cols, topk);
   });
   return rc == QV_OK ? bytes : rc;
 }
@@ -199,12 +667,18 @@ int qv_log_probs(const void* d_logits, int32_t type, int64_t rows, int64_t cols,
     check_vector("top_ids", d_top_ids, rows * topk);
     check_vector("top", d_top, rows * topk);
     if (rows == 0) return;
+    const int64_t need = workspace_of(rows, cols, topk);
+    if (need) {
+      if (workspace_bytes < need) qv::fail(QV_EINVAL, "workspace too small");
+      check_matrix("workspace", d_workspace, 1, need, need, 16);
+    }
     const OnDevice on(device);
+    const Out o{d_targets, targets_per_row, topk, d_target, d_entropy, d_lse, d_stats, d_top_ids, d_top};
     auto go = [&](auto* x) {
-      hipLaunchKernelGGL(log_probs_kernel, dim3((unsigned)rows), dim3(256), 0, static_cast<hipStream_t>(stream), x, rows,
-                         (int)cols, stride, 1.f / temperature, d_targets, targets_per_row, topk, d_target, d_entropy,
-                         d_lse, d_stats, d_top_ids, d_top);
-      HIP_OK(hipGetLastError());
+      using T = std::remove_const_t<std::remove_pointer_t<decltype(x)>>;
+      const hipStream_t st = static_cast<hipStream_t>(stream);
+      if (topk) log_probs<T, true>(x, rows, cols, stride, temperature, o, d_workspace, st);
+      else log_probs<T, false>(x, rows, cols, stride, temperature, o, d_workspace, st);
     };
     if (type == QV_FLOAT) go(static_cast<const float*>(d_logits));
     else if (type == QV_BFLOAT16) go(static_cast<const bf16*>(d_logits));
@@ -224,14 +698,13 @@ int qv_log_probs_grad(const void* d_logits, int32_t type, int64_t rows, int64_t 
     if (d_g_entropy) check_vector("entropy", d_entropy, rows);
     if (d_g_top) check_vector("top_ids", d_top_ids, rows * topk);
     if (rows == 0 || cols == 0) return;
+    const Weights g{d_stats, d_entropy, d_targets, d_g_target ? targets_per_row : 0, d_top_ids, d_g_top ? topk : 0,
+                    d_g_target, d_g_entropy, d_g_lse, d_g_top};
     const OnDevice on(device);
     auto go = [&](auto* x) {
       using T = std::remove_const_t<std::remove_pointer_t<decltype(x)>>;
-      hipLaunchKernelGGL(log_probs_grad_kernel, dim3((unsigned)rows), dim3(256), 0, static_cast<hipStream_t>(stream), x,
-                         rows, (int)cols, stride, 1.f / temperature, d_stats, d_entropy, d_targets, targets_per_row,
-                         d_top_ids, topk, d_g_target, d_g_entropy, d_g_lse, d_g_top, static_cast<T*>(d_grad),
-                         grad_stride);
-      HIP_OK(hipGetLastError());
+      log_probs_grad<T>(x, rows, cols, stride, temperature, g, static_cast<T*>(d_grad), grad_stride,
+                        static_cast<hipStream_t>(stream));
     };
     if (type == QV_FLOAT) go(static_cast<const float*>(d_logits));
     else if (type == QV_BFLOAT16) go(static_cast<const bf16*>(d_logits));

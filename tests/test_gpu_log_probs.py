@@ -351,6 +351,23 @@ def test_empty_sizes(scoring):
     assert scoring.log_probs_grad(x, r, targets, grad_target=torch.ones((3, 1), device="cuda")).shape == (3, 0)
 
 
+def test_long_matrix(scoring):
+    """Rows that begin past 2^31 elements."""
+    say("log probs, offsets past 32 bits")
+    n, v = 3, 1_500_000_000
+    x = torch.empty((n, v), dtype=torch.bfloat16, device="cuda")
+    x.fill_(-40.0)
+    x[2, v - 1], x[2, 7], x[1, 0] = 3.0, 2.0, 1.0
+    targets = torch.tensor([[5], [0], [v - 1]], dtype=torch.int32, device="cuda")
+    r = scoring.log_probs(x, targets, top_k=3)
+    assert r.top_ids.tolist() == [[0, 1, 2], [0, 1, 2], [v - 1, 7, 0]]
+    s = math.exp(-43) * (v - 2) + 1 + math.exp(-1)
+    assert abs(r.target[2, 0].item() + math.log(s)) < 1e-6
+    assert abs(r.logsumexp[0].item() - (math.log(v) - 40)) < 1e-4
+    grad = scoring.log_probs_grad(x, r, targets, grad_target=torch.ones((3, 1), device="cuda"), out=x)
+    assert abs(grad[2, v - 1].item() - (1 - 1 / s)) < 2e-3 and abs(grad[2, 7].item() + math.exp(-1) / s) < 2e-3
+
+
 def test_other_stream_reuse_and_repeat(scoring):
     """Results written again through out=, on a stream of their own, in a captured graph; equal calls, equal bits."""
     say("log probs, streams and graphs")
