@@ -43,33 +43,321 @@ __global__ __launch_bounds__(256) void quantize_kernel(const T* __restrict__ x, 
   if (lane == 0) scales[row] = odd ? __builtin_nanf("") : some ? top / 127.f : 0.f;
 }
 
-// A 16 x 16 tile of the output per workgroup, one thread per element, both
-// operands' rows staged 64 bytes at a time.
+// ---- product -------------------------------------------------------------------
+//
+// Sums of int8 products on the matrix cores (v_mfma_i32_32x32x32_i8, exact in
+// int32).  The rows of b are the instruction's rows and the rows of a its columns,
+// so a lane ends with four consecutive columns j of one output row i.
+//
+// k goes in stages of 128 bytes of each row, eight pieces of 16.  The last piece of
+// a row whose length is no multiple of 16 is its last 16 bytes; what it repeats is
+// zeroed in a, so every load is a whole one inside the row and b needs no mask.
+// Rows past the end repeat the last row; what they give is not stored.
+
+typedef int32_t i4 __attribute__((ext_vector_type(4)));
+typedef int32_t i16v __attribute__((ext_vector_type(16)));
+typedef float f4 __attribute__((ext_vector_type(4)));
+typedef i4 i4_any __attribute__((aligned(1), may_alias));
+typedef f4 f4_any __attribute__((aligned(4), may_alias));
+
+constexpr int kStage = 128;   // bytes of k per stage
+constexpr int64_t kFar = 1 << 23;  // row strides from here on: 256 rows' offsets pass 31 bits
+
 template <class O>
-__global__ __launch_bounds__(256) void product_kernel(const int8_t* __restrict__ a, int64_t a_stride,
-                                                      const float* __restrict__ a_scales, int64_t m,
-                                                      const int8_t* __restrict__ b, int64_t b_stride,
-                                                      const float* __restrict__ b_scales,
-                                                      const float* __restrict__ bias, int64_t n, int64_t k,
-                                                      O* __restrict__ out, int64_t out_stride, int64_t tiles_n) {
+struct Product {
+  const int8_t* a;
+  int64_t a_stride;
+  const float* a_scales;
+  int64_t m;
+  const int8_t* b;
+  int64_t b_stride;
+  const float* b_scales;
+  const float* bias;
+  int64_t n, k;
+  O* out;
+  int64_t out_stride;
+};
+
+// What a piece starting `over` bytes before its place repeats, zeroed.
+__device__ __forceinline__ i4 without_first(i4 v, int over) {
+#pragma unroll
+  for (int w = 0; w < 4; w++) {
+    const int cut = over - 4 * w;
+    v[w] = cut <= 0 ? v[w] : cut >= 4 ? 0 : (int32_t)((uint32_t)v[w] & (~0u << (8 * cut)));
+  }
+  return v;
+}
+
+__device__ __forceinline__ i16v mfma(i4 x, i4 y, i16v acc) {
+  return __builtin_amdgcn_mfma_i32_32x32x32_i8(x, y, acc, 0, 0, 0);
+}
+
+// Puts an instruction's result, 32 columns j from j0 of 32 rows i, into a wave's tile
+// [32][stride] in LDS.
+__device__ __forceinline__ void put_sums(int32_t* tile, int stride, int j0, const i16v& acc) {
+  const int lane = lane_id();
+#pragma unroll
+  for (int g = 0; g < 4; g++) {
+    i4 v;
+#pragma unroll
+    for (int e = 0; e < 4; e++) v[e] = acc[4 * g + e];
+    *reinterpret_cast<i4*>(tile + (lane % 32) * stride + j0 + 8 * g + 4 * (lane / 32)) = v;
+  }
+}
+
+// Scales and stores a wave's tile of 32 rows and J columns: 16 bytes of a row per lane.
+template <int J, class O>
+__device__ __forceinline__ void store_tile(const int32_t* tile, int stride, int64_t i0, int64_t j0,
+                                           const Product<O>& p) {
+  constexpr int V = 16 / (int)sizeof(O), L = J / V, R = kWave / L;  // columns per lane, lanes per row, rows at once
+  const int lane = lane_id(), jl = lane % L * V;
+  const int64_t j = j0 + jl;
+  if (j >= p.n) return;
+  const bool whole = j + V <= p.n;
+  float sb[V], add[V];
+#pragma unroll
+  for (int v = 0; v < V; v += 4) {
+    if (whole) {
+      const f4 s = *reinterpret_cast<const f4_any*>(p.b_scales + j + v);
+      const f4 t = p.bias ? (f4)*reinterpret_cast<const f4_any*>(p.bias + j + v) : f4{0.f, 0.f, 0.f, 0.f};
+#pragma unroll
+      for (int e = 0; e < 4; e++) sb[v + e] = s[e], add[v + e] = t[e];
+    } else {
+#pragma unroll
+      for (int e = 0; e < 4; e++) {
+        const int64_t q = min(j + v + e, p.n - 1);
+        sb[v + e] = p.b_scales[q];
+        add[v + e] = p.bias ? p.bias[q] : 0.f;
+      }
+    }
+  }
+#pragma unroll 4
+  for (int r = lane / L; r < 32; r += R) {
+    const int64_t i = i0 + r;
+    if (i >= p.m) break;
+    const float sa = p.a_scales[i];
+    union {
+      O o[V];
+      i4 raw;
+    } u;
+#pragma unroll
+    for (int v = 0; v < V; v += 4) {
+      const i4 sums = *reinterpret_cast<const i4*>(tile + r * stride + jl + v);
+#pragma unroll
+      for (int e = 0; e < 4; e++) {
+        const float x = ((float)sums[e] * sa) * sb[v + e];
+        u.o[v + e] = (O)(p.bias ? x + add[v + e] : x);
+      }
+    }
+    O* dst = p.out + i * p.out_stride + j;
+    if (whole) {
+      *reinterpret_cast<i4_any*>(dst) = u.raw;
+    } else {
+#pragma unroll
+      for (int v = 0; v < V; v++)
+        if (j + v < p.n) dst[v] = u.o[v];
+    }
+  }
+}
+
+// Workgroups go round the eight XCDs: each XCD gets a run of consecutive tiles.
+__device__ __forceinline__ int64_t tile_of_block(int64_t block, int64_t tiles) {
+  const int64_t xcd = block % 8, per = tiles / 8, more = tiles % 8;
+  return xcd * per + min(xcd, more) + block / 8;
+}
+
+// A tile of BM x BN outputs per workgroup, WM x WN waves of 32 TM x 32 TN each.  Both
+// operands' stages go through registers into LDS, the next one in flight while the
+// matrix cores work on this one; piece q of row r lies at q ^ (r mod 8), which keeps
+// both the writes and the reads free of bank conflicts.
+template <int BM, int BN, int WM, int WN, class O>
+__global__ __launch_bounds__(64 * WM * WN, 1) void product_tile_kernel(Product<O> p, int64_t tiles_m, int64_t tiles_n,
+                                                                       int64_t group) {
+  constexpr int T = 64 * WM * WN, TM = BM / WM / 32, TN = BN / WN / 32;
+  constexpr int LA = BM * 8 / T, LB = BN * 8 / T, kRows = T / 8;
+  constexpr int kBuffer = (BM + BN) * kStage;
+  extern __shared__ __align__(16) char lds[];
+  const int tid = threadIdx.x, wave = tid / kWave, lane = lane_id();
+  const int wm = wave / WN, wn = wave % WN;
+  // tiles in groups of `group` rows of tiles, down the rows first
+  const int64_t t = tile_of_block(blockIdx.x, tiles_m * tiles_n);
+  const int64_t g = t / (group * tiles_n), gm = min(group, tiles_m - g * group), in = t - g * group * tiles_n;
+  const int64_t i0 = (g * group + in % gm) * BM, j0 = in / gm * BN;
+
+  const int piece = tid % 8, r0 = tid / 8;
+  const int8_t *a = p.a + i0 * p.a_stride, *b = p.b + j0 * p.b_stride;
+  uint32_t at_a[LA], at_b[LB];
+#pragma unroll
+  for (int q = 0; q < LA; q++) at_a[q] = (uint32_t)(min((int64_t)(r0 + q * kRows), p.m - 1 - i0) * p.a_stride);
+#pragma unroll
+  for (int q = 0; q < LB; q++) at_b[q] = (uint32_t)(min((int64_t)(r0 + q * kRows), p.n - 1 - j0) * p.b_stride);
+  const int k = (int)p.k, stages = (k + kStage - 1) / kStage;
+  i4 ra[LA], rb[LB];
+  auto load = [&](int s) {
+    const int place = s * kStage + piece * 16, from = min(place, k - 16);
+#pragma unroll
+    for (int q = 0; q < LA; q++) ra[q] = *reinterpret_cast<const i4_any*>(a + (at_a[q] + (uint32_t)from));
+#pragma unroll
+    for (int q = 0; q < LB; q++) rb[q] = *reinterpret_cast<const i4_any*>(b + (at_b[q] + (uint32_t)from));
+  };
+  auto keep = [&](int s) {
+    char* to = lds + (s & 1) * kBuffer + r0 * kStage + (piece ^ (r0 & 7)) * 16;
+    if ((s + 1) * kStage > k) {
+      const int over = max(0, s * kStage + piece * 16 - (k - 16));
+#pragma unroll
+      for (int q = 0; q < LA; q++) ra[q] = without_first(ra[q], over);
+    }
+#pragma unroll
+    for (int q = 0; q < LA; q++) *reinterpret_cast<i4*>(to + q * kRows * kStage) = ra[q];
+#pragma unroll
+    for (int q = 0; q < LB; q++) *reinterpret_cast<i4*>(to + BM * kStage + q * kRows * kStage) = rb[q];
+  };
+  i16v acc[TM][TN];
+#pragma unroll
+  for (int x = 0; x < TM; x++)
+#pragma unroll
+    for (int y = 0; y < TN; y++) acc[x][y] = i16v{};
+  const int row = lane % 32, half = lane / 32;
+  auto step = [&](int s, int q) {  // 32 bytes of k
+    const char* from = lds + (s & 1) * kBuffer + ((2 * q + half) ^ (row & 7)) * 16 + row * kStage;
+    i4 fa[TM], fb[TN];
+#pragma unroll
+    for (int x = 0; x < TM; x++) fa[x] = *reinterpret_cast<const i4*>(from + (wm * TM + x) * 32 * kStage);
+#pragma unroll
+    for (int y = 0; y < TN; y++) fb[y] = *reinterpret_cast<const i4*>(from + BM * kStage + (wn * TN + y) * 32 * kStage);
+#pragma unroll
+    for (int x = 0; x < TM; x++)
+#pragma unroll
+      for (int y = 0; y < TN; y++) acc[x][y] = mfma(fb[y], fa[x], acc[x][y]);
+  };
+  load(0);
+  keep(0);
+  __syncthreads();
+  for (int s = 0; s + 1 < stages; s++) {
+    load(s + 1);
+#pragma unroll
+    for (int q = 0; q < 4; q++) step(s, q);
+    keep(s + 1);
+    __syncthreads();
+  }
+  const int last = stages - 1, steps = (k - last * kStage + 31) / 32;
+  if (steps == 4) {
+#pragma unroll
+    for (int q = 0; q < 4; q++) step(last, q);
+  } else {
+    for (int q = 0; q < steps; q++) step(last, q);
+  }
+  __syncthreads();
+  constexpr int J = 32 * TN, kTile = J + 4;
+  int32_t* tile = reinterpret_cast<int32_t*>(lds) + wave * 32 * kTile;
+#pragma unroll
+  for (int x = 0; x < TM; x++) {
+    if (x) __builtin_amdgcn_fence(__ATOMIC_ACQ_REL, "wavefront");
+#pragma unroll
+    for (int y = 0; y < TN; y++) put_sums(tile, kTile, 32 * y, acc[x][y]);
+    __builtin_amdgcn_fence(__ATOMIC_ACQ_REL, "wavefront");
+    store_tile<J>(tile, kTile, i0 + (wm * TM + x) * 32, j0 + wn * J, p);
+  }
+}
+
+// Up to 32 rows of a against strips of 32 rows of b, one strip per wave at a time (WK =
+// 1), or a strip's k cut over the WK waves of its workgroup.  A wave's stage of b goes
+// through registers into an LDS area of its own, so no barrier holds it; the next one
+// is in flight meanwhile.  a's operands come from the caches, once for all strips
+// while k is a single stage.
+template <int WK, class O>
+__global__ __launch_bounds__(256) void product_strip_kernel(Product<O> p, int64_t strips, int64_t step) {
+  constexpr int kTile = 32 + 4;
+  __shared__ __align__(16) char lds[4][32 * kTile * 4];  // a stage of b, then the strip's sums
+  const int wave = threadIdx.x / kWave, lane = lane_id();
+  const int row = lane % 32, half = lane / 32;
+  const int k = (int)p.k, stages = (k + kStage - 1) / kStage;
+  const int r0 = lane / 8, piece = lane % 8;
+  const int8_t* a_row = p.a + min((int64_t)row, p.m - 1) * p.a_stride;
+  char* area = lds[wave];
+  i4 fa[4], rb[4];
+  auto load_a = [&](int s) {
+#pragma unroll
+    for (int q = 0; q < 4; q++) {
+      const int place = s * kStage + (2 * q + half) * 16, from = min(place, k - 16);
+      fa[q] = without_first(*reinterpret_cast<const i4_any*>(a_row + from), place - from);
+    }
+  };
+  auto load_b = [&](int64_t strip, int s) {
+    const int from = min(s * kStage + piece * 16, k - 16);
+#pragma unroll
+    for (int q = 0; q < 4; q++) {
+      const int64_t r = min(strip * 32 + r0 + 8 * q, p.n - 1);
+      rb[q] = *reinterpret_cast<const i4_any*>(p.b + r * p.b_stride + from);
+    }
+  };
+  const int s0 = WK == 1 ? 0 : wave;
+  int64_t strip = WK == 1 ? (int64_t)blockIdx.x * 4 + wave : blockIdx.x;
+  if (WK == 1 && strip >= strips) return;
+  if (s0 < stages) load_b(strip, s0);
+  if (stages == 1 && s0 < stages) load_a(0);
+  for (; strip < strips; strip += step) {
+    i16v acc{};
+    for (int s = s0; s < stages; s += WK) {
+      if (stages > 1) load_a(s);
+#pragma unroll
+      for (int q = 0; q < 4; q++)
+        *reinterpret_cast<i4*>(area + (r0 + 8 * q) * kStage + (piece ^ ((r0 + 8 * q) & 7)) * 16) = rb[q];
+      __builtin_amdgcn_fence(__ATOMIC_ACQ_REL, "wavefront");
+      if (s + WK < stages) load_b(strip, s + WK);
+      else if (strip + step < strips) load_b(strip + step, s0);
+      const char* from = area + row * kStage;
+#pragma unroll
+      for (int q = 0; q < 4; q++)
+        acc = mfma(*reinterpret_cast<const i4*>(from + ((2 * q + half) ^ (row & 7)) * 16), fa[q], acc);
+      __builtin_amdgcn_fence(__ATOMIC_ACQ_REL, "wavefront");
+    }
+    int32_t* tile = reinterpret_cast<int32_t*>(area);
+    put_sums(tile, kTile, 0, acc);
+    __builtin_amdgcn_fence(__ATOMIC_ACQ_REL, "wavefront");
+    if constexpr (WK > 1) {
+      __syncthreads();
+      // each wave adds up and stores the rows of a quarter of the tile: the sums go to wave 0's tile
+      int32_t* sum = reinterpret_cast<int32_t*>(lds[0]);
+      for (int e = threadIdx.x; e < 32 * kTile; e += 256) {
+        int32_t v = sum[e];
+#pragma unroll
+        for (int w = 1; w < WK; w++) v += reinterpret_cast<const int32_t*>(lds[w])[e];
+        sum[e] = v;
+      }
+      __syncthreads();
+      if (wave == 0) store_tile<32>(sum, kTile, 0, strip * 32, p);
+      __syncthreads();
+    } else {
+      store_tile<32>(tile, kTile, 0, strip * 32, p);
+      __builtin_amdgcn_fence(__ATOMIC_ACQ_REL, "wavefront");
+    }
+  }
+}
+
+// Rows shorter than one piece (16 bytes), or further apart than 32-bit offsets reach:
+// a 16 x 16 tile of the output per workgroup, one thread per element, both operands'
+// rows staged 64 bytes at a time.
+template <class O>
+__global__ __launch_bounds__(256) void product_small_kernel(Product<O> p, int64_t tiles_n) {
   __shared__ int8_t sa[16][68], sb[16][68];
   const int tid = threadIdx.x, r = tid / 16, c = tid % 16;
   const int64_t i0 = (int64_t)blockIdx.x / tiles_n * 16, j0 = (int64_t)blockIdx.x % tiles_n * 16;
   int32_t acc = 0;
-  for (int64_t k0 = 0; k0 < k; k0 += 64) {
+  for (int64_t k0 = 0; k0 < p.k; k0 += 64) {
     for (int u = tid; u < 16 * 64; u += 256) {
       const int64_t row = u / 64, at = k0 + u % 64;
-      sa[row][u % 64] = i0 + row < m && at < k ? a[(i0 + row) * a_stride + at] : (int8_t)0;
-      sb[row][u % 64] = j0 + row < n && at < k ? b[(j0 + row) * b_stride + at] : (int8_t)0;
+      sa[row][u % 64] = i0 + row < p.m && at < p.k ? p.a[(i0 + row) * p.a_stride + at] : (int8_t)0;
+      sb[row][u % 64] = j0 + row < p.n && at < p.k ? p.b[(j0 + row) * p.b_stride + at] : (int8_t)0;
     }
     __syncthreads();
     for (int u = 0; u < 64; u++) acc += (int32_t)sa[r][u] * (int32_t)sb[c][u];
     __syncthreads();
   }
-  if (i0 + r < m && j0 + c < n) {
-    float v = ((float)acc * a_scales[i0 + r]) * b_scales[j0 + c];
-    if (bias) v = v + bias[j0 + c];
-    out[(i0 + r) * out_stride + j0 + c] = (O)v;
+  if (i0 + r < p.m && j0 + c < p.n) {
+    float v = ((float)acc * p.a_scales[i0 + r]) * p.b_scales[j0 + c];
+    if (p.bias) v = v + p.bias[j0 + c];
+    p.out[(i0 + r) * p.out_stride + j0 + c] = (O)v;
   }
 }
 
@@ -81,14 +369,40 @@ void quantize(const void* x, int64_t n, int64_t dim, int64_t stride, int8_t* cod
   HIP_OK(hipGetLastError());
 }
 
-template <class O>
-void product(const int8_t* a, int64_t a_stride, const float* a_scales, int64_t m, const int8_t* b, int64_t b_stride,
-             const float* b_scales, const float* bias, int64_t n, int64_t k, void* out, int64_t out_stride,
-             hipStream_t st) {
-  const int64_t tm = (m + 15) / 16, tn = (n + 15) / 16;
-  hipLaunchKernelGGL(product_kernel<O>, dim3((unsigned)(tm * tn)), dim3(256), 0, st, a, a_stride, a_scales, m, b,
-                     b_stride, b_scales, bias, n, k, static_cast<O*>(out), out_stride, tn);
+template <int BM, int BN, int WM, int WN, class O>
+void launch_tiles(const Product<O>& p, hipStream_t st) {
+  const int64_t tm = (p.m + BM - 1) / BM, tn = (p.n + BN - 1) / BN;
+  // down a group of tiles' rows first: as many as keep their rows of a within 2 MB of an XCD's L2, eight at least
+  const int64_t group = std::min(tm, std::max<int64_t>(8, (2 << 20) / (BM * p.k)));
+  const int buffers = p.k > kStage ? 2 : 1;
+  const int lds = std::max(buffers * (BM + BN) * kStage, WM * WN * 32 * (BN / WN + 4) * 4);
+  auto* kernel = product_tile_kernel<BM, BN, WM, WN, O>;
+  if (lds > 65536) HIP_OK(hipFuncSetAttribute(reinterpret_cast<const void*>(kernel), hipFuncAttributeMaxDynamicSharedMemorySize, lds));
+  hipLaunchKernelGGL(kernel, dim3((unsigned)(tm * tn)), dim3(64 * WM * WN), lds, st, p, tm, tn, group);
   HIP_OK(hipGetLastError());
+}
+
+template <class O>
+void product(const Product<O>& p, hipStream_t st) {
+  if (p.k < 16 || p.a_stride >= kFar || p.b_stride >= kFar) {
+    const int64_t tm = (p.m + 15) / 16, tn = (p.n + 15) / 16;
+    if (tm * tn > INT32_MAX) fail(QV_EUNSUPPORTED, "more tiles than one launch has");
+    hipLaunchKernelGGL(product_small_kernel<O>, dim3((unsigned)(tm * tn)), dim3(256), 0, st, p, tn);
+    HIP_OK(hipGetLastError());
+  } else if (p.m <= 32) {
+    const int64_t strips = (p.n + 31) / 32;
+    if (strips < 2048 && p.k > kStage) {
+      hipLaunchKernelGGL((product_strip_kernel<4, O>), dim3((unsigned)strips), dim3(256), 0, st, p, strips, strips);
+    } else {
+      const int64_t blocks = std::min<int64_t>((strips + 3) / 4, 256 * 6);
+      hipLaunchKernelGGL((product_strip_kernel<1, O>), dim3((unsigned)blocks), dim3(256), 0, st, p, strips, blocks * 4);
+    }
+    HIP_OK(hipGetLastError());
+  } else if (p.k >= 512 && ((p.m + 255) / 256) * ((p.n + 255) / 256) >= 200) {
+    launch_tiles<256, 256, 2, 2>(p, st);
+  } else {
+    launch_tiles<128, 128, 2, 2>(p, st);
+  }
 }
 
 }  // namespace
@@ -125,17 +439,17 @@ int qv_int8_product(const int8_t* d_a, int64_t a_stride, const float* d_a_scales
     check_vector("a_scales", d_a_scales, m);
     check_vector("b_scales", d_b_scales, n);
     if (d_bias) check_vector("bias", d_bias, n);
-    if (m > INT32_MAX || n > INT32_MAX || (m + 15) / 16 * ((n + 15) / 16) > INT32_MAX)
+    if (m > INT32_MAX || n > INT32_MAX || (m + 127) / 128 * ((n + 127) / 128) > INT32_MAX)
       qv::fail(QV_EUNSUPPORTED, "more tiles than one launch has");
     const OnDevice on(device);
     const hipStream_t st = static_cast<hipStream_t>(stream);
     auto go = [&](auto* o) {
-      product<std::remove_pointer_t<decltype(o)>>(d_a, a_stride, d_a_scales, m, d_b, b_stride, d_b_scales, d_bias, n, k,
-                                                  d_out, out_stride, st);
+      using O = std::remove_pointer_t<decltype(o)>;
+      product(Product<O>{d_a, a_stride, d_a_scales, m, d_b, b_stride, d_b_scales, d_bias, n, k, o, out_stride}, st);
     };
-    if (out_type == QV_FLOAT) go(static_cast<float*>(nullptr));
-    else if (out_type == QV_BFLOAT16) go(static_cast<bf16*>(nullptr));
-    else go(static_cast<f16*>(nullptr));
+    if (out_type == QV_FLOAT) go(static_cast<float*>(d_out));
+    else if (out_type == QV_BFLOAT16) go(static_cast<bf16*>(d_out));
+    else go(static_cast<f16*>(d_out));
   });
 }
 
