@@ -44,6 +44,10 @@ inline int value_size(int32_t type) {
   fail(QV_EINVAL, "type must be float, bfloat16 or float16");
 }
 
+// The wave's number in its workgroup, in a scalar register: what is derived from it
+// (row pointers, tile corners) is then scalar arithmetic.
+__device__ __forceinline__ int wave_id() { return __builtin_amdgcn_readfirstlane((int)(threadIdx.x / 64)); }
+
 // A matrix that the call reads or writes: there, aligned to its elements, rows that do not overlap.
 inline void check_matrix(const char* name, const void* p, int64_t rows, int64_t cols, int64_t stride, int size) {
   if (rows < 0 || cols < 0) fail(QV_EINVAL, std::string(name) + ": negative size");

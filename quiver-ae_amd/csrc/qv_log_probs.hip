@@ -349,7 +349,7 @@ template <class T, int U, bool TOP>
 __global__ __launch_bounds__(256) void log_probs_wave_kernel(const T* __restrict__ logits, int64_t rows, int cols,
                                                              int64_t stride, float c, float inv_t, Out o) {
   __shared__ uint64_t pool[TOP ? 4 * kPool : 1];
-  const int wave = threadIdx.x / kWave;
+  const int wave = wave_id();
   const int64_t row = (int64_t)blockIdx.x * 4 + wave;
   if (row >= rows) return;
   const T* x = logits + row * stride;
@@ -368,7 +368,7 @@ __global__ __launch_bounds__(256) void log_probs_block_kernel(const T* __restric
   __shared__ uint64_t pool[TOP ? 4 * kPool : 1];
   __shared__ float4 sums[4];
   __shared__ uint32_t least;
-  const int tid = threadIdx.x, wave = tid / kWave, lane = lane_id();
+  const int tid = threadIdx.x, wave = wave_id(), lane = lane_id();
   const int64_t row = blockIdx.x / (unsigned)splits;
   const int split = (int)(blockIdx.x - row * splits);
   const T* x = logits + row * stride;
@@ -406,7 +406,7 @@ __global__ __launch_bounds__(256) void join_kernel(const T* __restrict__ logits,
                                                    const uint64_t* __restrict__ part_keys) {
   __shared__ uint64_t pool[TOP ? 4 * kPool : 1];
   __shared__ float4 sums[4];
-  const int tid = threadIdx.x, wave = tid / kWave, lane = lane_id();
+  const int tid = threadIdx.x, wave = wave_id(), lane = lane_id();
   const int64_t row = blockIdx.x;
   Sums sum;
   for (int i = tid; i < splits; i += 256) {
@@ -464,7 +464,7 @@ __global__ __launch_bounds__(256) void log_probs_grad_kernel(const T* logits, in
                                                              float c, float inv_t, int chunk, int splits, Weights g,
                                                              T* grad, int64_t grad_stride) {
   constexpr int N = U * kVec<T>, kBatch = kWave * N;
-  const int64_t unit = (int64_t)blockIdx.x * 4 + threadIdx.x / kWave;
+  const int64_t unit = (int64_t)blockIdx.x * 4 + wave_id();
   if (unit >= units) return;
   const int lane = lane_id();
   const int64_t row = unit / splits;

@@ -61,7 +61,8 @@ typedef i4 i4_any __attribute__((aligned(1), may_alias));
 typedef f4 f4_any __attribute__((aligned(4), may_alias));
 
 constexpr int kStage = 128;   // bytes of k per stage
-constexpr int64_t kFar = 1 << 23;  // row strides from here on: 256 rows' offsets pass 31 bits
+constexpr int64_t kFar = 1 << 23;     // row strides from here on: 256 rows' offsets pass 31 bits
+constexpr int64_t kFarOut = 1 << 27;  // the same of the output, for 4 rows of floats
 
 template <class O>
 struct Product {
@@ -177,7 +178,7 @@ __global__ __launch_bounds__(64 * WM * WN, 1) void product_tile_kernel(Product<O
   constexpr int LA = BM * 8 / T, LB = BN * 8 / T, kRows = T / 8;
   constexpr int kBuffer = (BM + BN) * kStage;
   extern __shared__ __align__(16) char lds[];
-  const int tid = threadIdx.x, wave = tid / kWave, lane = lane_id();
+  const int tid = threadIdx.x, wave = wave_id(), lane = lane_id();
   const int wm = wave / WN, wn = wave % WN;
   // tiles in groups of `group` rows of tiles, down the rows first
   const int64_t t = tile_of_block(blockIdx.x, tiles_m * tiles_n);
@@ -260,6 +261,152 @@ __global__ __launch_bounds__(64 * WM * WN, 1) void product_tile_kernel(Product<O
   }
 }
 
+// Short rows, k <= 32 KS, whose product is mostly writing: 32 rows of a stay in a wave's
+// registers while its workgroup (128 rows) walks over tiles of 64 rows of b, through
+// LDS with the next two tiles on their way.
+//
+// Memory takes whole aligned lines of 128 bytes at 5.4 TB/s and rows cut elsewhere at
+// 3.3 to 3.8, and rows of an odd length begin anywhere.  So a wave keeps, per row, a
+// ring of two lines in LDS in which an element's place follows its address: a line is
+// written whole as soon as its last column is there, and only the first and the last
+// one of a walk are written in parts.
+template <int KS, class O>
+__global__ __launch_bounds__(256, KS == 4 ? 3 : 2) void product_panel_kernel(Product<O> p, int64_t panels, int64_t tiles_n,
+                                                               int64_t slices) {
+  constexpr int PC = 2 * KS, kRow = 32 * KS, L = 64 * PC / 256, kRows = 256 / PC;
+  constexpr int S = (int)sizeof(O), E = 128 / S, V = 16 / S;   // elements of a line, of 16 bytes
+  constexpr int kRing = 256, Y = E / 32;  // bytes of a row's ring; 32-column results to a line
+  __shared__ __align__(16) char lds[2][64 * kRow];
+  __shared__ __align__(16) char rings[4][32 * kRing];
+  __shared__ __align__(16) float sa[128];
+  const int tid = threadIdx.x, wave = wave_id(), lane = lane_id(), row = lane % 32, half = lane / 32;
+  const int64_t t = tile_of_block(blockIdx.x, panels * slices), slice = t / panels, i0 = (t - slice * panels) * 128;
+  const int64_t first = tiles_n * slice / slices, end = tiles_n * (slice + 1) / slices;
+  const int k = (int)p.k, piece = tid % PC, r0 = tid / PC, from = min(piece * 16, k - 16);
+  i4 rb[L];
+  auto load = [&](int64_t tile) {
+    const int8_t* b = p.b + tile * 64 * p.b_stride;
+#pragma unroll
+    for (int q = 0; q < L; q++) {
+      const int64_t r = min((int64_t)(r0 + q * kRows), p.n - 1 - tile * 64);
+      rb[q] = *reinterpret_cast<const i4_any*>(b + (uint32_t)(r * p.b_stride + from));
+    }
+  };
+  auto keep = [&](int buffer) {
+#pragma unroll
+    for (int q = 0; q < L; q++) {
+      const int r = r0 + q * kRows;
+      *reinterpret_cast<i4*>(lds[buffer] + r * kRow + (piece ^ (r & 7)) * 16) = rb[q];
+    }
+  };
+  load(first);
+  const int64_t it = i0 + wave * 32;  // the wave's rows
+  const int rows = (int)min(p.m - it, (int64_t)32);
+  i4 fa[KS];
+  {
+    const int8_t* a = p.a + min(it + row, p.m - 1) * p.a_stride;
+#pragma unroll
+    for (int q = 0; q < KS; q++) {
+      const int place = (2 * q + half) * 16, at = min(place, k - 16);
+      fa[q] = without_first(*reinterpret_cast<const i4_any*>(a + at), place - at);
+    }
+  }
+  if (tid < 128) sa[tid] = p.a_scales[min(i0 + tid, p.m - 1)];
+  // elements of its line before a row's first one
+  auto shift = [&](int r) { return (int)(reinterpret_cast<uintptr_t>(p.out + (it + r) * p.out_stride) % 128) / S; };
+  char* ring = rings[wave];
+  // where the columns of a line go in the ring, register 4 g + e of result y; those of the next line
+  // half a ring on
+  int place[Y][16];
+#pragma unroll
+  for (int g = 0; g < 4; g++)
+#pragma unroll
+    for (int e = 0; e < 4; e++)
+#pragma unroll
+      for (int y = 0; y < Y; y++) {
+        const int at = (int)(first & 1) * 64 + 32 * y + row + shift(8 * g + 4 * half + e);
+        place[y][4 * g + e] = 4 * half * kRing + (at * S & (kRing - 1));
+      }
+  // lines as they leave: 8 lanes a line, 8 rows at once
+  constexpr int G = 4;
+  const int c = lane % 8;
+  char* line_to[G];
+  int rel[G];
+#pragma unroll
+  for (int g = 0; g < G; g++) {
+    const int r = 8 * g + lane / 8, sh = shift(r);
+    rel[g] = c * V - sh;
+    line_to[g] = reinterpret_cast<char*>(p.out + (it + r) * p.out_stride + (first * 64 + rel[g]));
+  }
+  // line number `line` (the E elements from column line E - shift on) of every row, columns [lo, hi) of it
+  const int64_t lo = first * 64;
+  auto leave = [&](int64_t line, int64_t hi, int64_t step) {
+    const int least = (int)max(lo - line * E, (int64_t)-1024), most = (int)min(hi - line * E, (int64_t)1024);
+    const char* from = ring + (int)(line & 1) * 128 + c * 16;
+#pragma unroll
+    for (int g = 0; g < G; g++) {
+      const int r = 8 * g + lane / 8;
+      union {
+        i4 raw;
+        O o[V];
+      } u;
+      u.raw = *reinterpret_cast<const i4*>(from + r * kRing);
+      if (r < rows) {
+        if (rel[g] >= least && rel[g] + V <= most) {
+          *reinterpret_cast<i4*>(line_to[g]) = u.raw;
+        } else {
+#pragma unroll
+          for (int v = 0; v < V; v++)
+            if (rel[g] + v >= least && rel[g] + v < most) reinterpret_cast<O*>(line_to[g])[v] = u.o[v];
+        }
+      }
+      line_to[g] += step;
+    }
+  };
+  keep(0);
+  if (first + 1 < end) load(first + 1);
+  __syncthreads();
+  for (int64_t tile = first; tile < end; tile++) {
+    const char* b = lds[(tile - first) & 1] + row * kRow;
+    i16v acc[2] = {i16v{}, i16v{}};
+#pragma unroll
+    for (int q = 0; q < KS; q++)
+#pragma unroll
+      for (int y = 0; y < 2; y++)
+        acc[y] = mfma(fa[q], *reinterpret_cast<const i4*>(b + y * 32 * kRow + ((2 * q + half) ^ (row & 7)) * 16), acc[y]);
+    if (tile + 1 < end) keep((int)(tile + 1 - first) & 1);
+    if (tile + 2 < end) load(tile + 2);
+#pragma unroll
+    for (int l = 0; l < 2 / Y; l++) {
+      float sb[Y], add[Y];
+#pragma unroll
+      for (int y = 0; y < Y; y++) {
+        const int64_t j = min(tile * 64 + (l * Y + y) * 32 + row, p.n - 1);
+        sb[y] = p.b_scales[j];
+        add[y] = p.bias ? p.bias[j] : 0.f;
+      }
+#pragma unroll
+      for (int g = 0; g < 4; g++) {
+        const f4 s = *reinterpret_cast<const f4*>(sa + wave * 32 + 8 * g + 4 * half);
+#pragma unroll
+        for (int e = 0; e < 4; e++)
+#pragma unroll
+          for (int y = 0; y < Y; y++) {
+            float x = ((float)acc[l * Y + y][4 * g + e] * s[e]) * sb[y];
+            if (p.bias) x = x + add[y];
+            *reinterpret_cast<O*>(ring + place[y][4 * g + e] + (8 * g + e) * kRing) = (O)x;
+            place[y][4 * g + e] ^= 128;
+          }
+      }
+      __builtin_amdgcn_fence(__ATOMIC_ACQ_REL, "wavefront");
+      leave(tile * (2 / Y) + l, p.n, 128);
+      __builtin_amdgcn_fence(__ATOMIC_ACQ_REL, "wavefront");
+    }
+    __syncthreads();
+  }
+  leave(end * (2 / Y), min(end * 64, p.n), 0);
+}
+
 // Up to 32 rows of a against strips of 32 rows of b, one strip per wave at a time (WK =
 // 1), or a strip's k cut over the WK waves of its workgroup.  A wave's stage of b goes
 // through registers into an LDS area of its own, so no barrier holds it; the next one
@@ -269,7 +416,7 @@ template <int WK, class O>
 __global__ __launch_bounds__(256) void product_strip_kernel(Product<O> p, int64_t strips, int64_t step) {
   constexpr int kTile = 32 + 4;
   __shared__ __align__(16) char lds[4][32 * kTile * 4];  // a stage of b, then the strip's sums
-  const int wave = threadIdx.x / kWave, lane = lane_id();
+  const int wave = wave_id(), lane = lane_id();
   const int row = lane % 32, half = lane / 32;
   const int k = (int)p.k, stages = (k + kStage - 1) / kStage;
   const int r0 = lane / 8, piece = lane % 8;
@@ -382,9 +529,19 @@ void launch_tiles(const Product<O>& p, hipStream_t st) {
   HIP_OK(hipGetLastError());
 }
 
+template <int KS, class O>
+void launch_panels(const Product<O>& p, hipStream_t st) {
+  const int64_t panels = (p.m + 127) / 128, tiles_n = (p.n + 63) / 64;
+  // as many workgroups as run at once, each with a like share of b's tiles
+  const int64_t slices = std::min(tiles_n, std::max<int64_t>(1, 256 * (KS == 4 ? 3 : 2) / panels));
+  hipLaunchKernelGGL((product_panel_kernel<KS, O>), dim3((unsigned)(panels * slices)), dim3(256), 0, st, p, panels,
+                     tiles_n, slices);
+  HIP_OK(hipGetLastError());
+}
+
 template <class O>
 void product(const Product<O>& p, hipStream_t st) {
-  if (p.k < 16 || p.a_stride >= kFar || p.b_stride >= kFar) {
+  if (p.k < 16 || p.a_stride >= kFar || p.b_stride >= kFar || p.out_stride >= kFarOut) {
     const int64_t tm = (p.m + 15) / 16, tn = (p.n + 15) / 16;
     if (tm * tn > INT32_MAX) fail(QV_EUNSUPPORTED, "more tiles than one launch has");
     hipLaunchKernelGGL(product_small_kernel<O>, dim3((unsigned)(tm * tn)), dim3(256), 0, st, p, tn);
@@ -398,6 +555,10 @@ void product(const Product<O>& p, hipStream_t st) {
       hipLaunchKernelGGL((product_strip_kernel<1, O>), dim3((unsigned)blocks), dim3(256), 0, st, p, strips, blocks * 4);
     }
     HIP_OK(hipGetLastError());
+  } else if (p.k <= 128) {
+    launch_panels<4>(p, st);
+  } else if (p.k <= 256) {
+    launch_panels<8>(p, st);
   } else if (p.k >= 512 && ((p.m + 255) / 256) * ((p.n + 255) / 256) >= 200) {
     launch_tiles<256, 256, 2, 2>(p, st);
   } else {
