@@ -60,6 +60,7 @@ typedef float f4 __attribute__((ext_vector_type(4)));
 typedef i4 i4_any __attribute__((aligned(1), may_alias));
 typedef f4 f4_any __attribute__((aligned(4), may_alias));
 
+constexpr int kLoadsDone = 0x0f70;  // s_waitcnt vmcnt(0)
 constexpr int kStage = 128;   // bytes of k per stage
 constexpr int64_t kFar = 1 << 23;     // row strides from here on: 256 rows' offsets pass 31 bits
 constexpr int64_t kFarOut = 1 << 27;  // the same of the output, for 4 rows of floats
@@ -279,18 +280,21 @@ __global__ __launch_bounds__(256, KS == 4 ? 3 : 2) void product_panel_kernel(Pro
   __shared__ __align__(16) char lds[2][64 * kRow];
   __shared__ __align__(16) char rings[4][32 * kRing];
   __shared__ __align__(16) float sa[128];
+  __shared__ float sb[2][2][64];  // a tile's scales and biases
   const int tid = threadIdx.x, wave = wave_id(), lane = lane_id(), row = lane % 32, half = lane / 32;
   const int64_t t = tile_of_block(blockIdx.x, panels * slices), slice = t / panels, i0 = (t - slice * panels) * 128;
   const int64_t first = tiles_n * slice / slices, end = tiles_n * (slice + 1) / slices;
   const int k = (int)p.k, piece = tid % PC, r0 = tid / PC, from = min(piece * 16, k - 16);
   i4 rb[L];
+  float rs = 0.f;
+  const bool scales = tid < 128 && (tid < 64 || p.bias);
+  const float* scale_of = tid < 64 ? p.b_scales : p.bias;
   auto load = [&](int64_t tile) {
     const int8_t* b = p.b + tile * 64 * p.b_stride;
+    const int last = (int)min(p.n - 1 - tile * 64, (int64_t)63);
 #pragma unroll
-    for (int q = 0; q < L; q++) {
-      const int64_t r = min((int64_t)(r0 + q * kRows), p.n - 1 - tile * 64);
-      rb[q] = *reinterpret_cast<const i4_any*>(b + (uint32_t)(r * p.b_stride + from));
-    }
+    for (int q = 0; q < L; q++) rb[q] = *reinterpret_cast<const i4_any*>(b + (uint32_t)(min(r0 + q * kRows, last) * (int)p.b_stride + from));
+    if (scales) rs = scale_of[tile * 64 + min(tid % 64, last)];
   };
   auto keep = [&](int buffer) {
 #pragma unroll
@@ -298,6 +302,7 @@ __global__ __launch_bounds__(256, KS == 4 ? 3 : 2) void product_panel_kernel(Pro
       const int r = r0 + q * kRows;
       *reinterpret_cast<i4*>(lds[buffer] + r * kRow + (piece ^ (r & 7)) * 16) = rb[q];
     }
+    if (tid < 128) sb[buffer][tid / 64][tid % 64] = scales ? rs : -0.f;  // x + -0 is x
   };
   load(first);
   const int64_t it = i0 + wave * 32;  // the wave's rows
@@ -343,6 +348,14 @@ __global__ __launch_bounds__(256, KS == 4 ? 3 : 2) void product_panel_kernel(Pro
   auto leave = [&](int64_t line, int64_t hi, int64_t step) {
     const int least = (int)max(lo - line * E, (int64_t)-1024), most = (int)min(hi - line * E, (int64_t)1024);
     const char* from = ring + (int)(line & 1) * 128 + c * 16;
+    if (rows == 32 && least <= 1 - E && most >= E) {  // whole lines of all rows
+#pragma unroll
+      for (int g = 0; g < G; g++) {
+        *reinterpret_cast<i4*>(line_to[g]) = *reinterpret_cast<const i4*>(from + (8 * g + lane / 8) * kRing);
+        line_to[g] += step;
+      }
+      return;
+    }
 #pragma unroll
     for (int g = 0; g < G; g++) {
       const int r = 8 * g + lane / 8;
@@ -362,28 +375,37 @@ __global__ __launch_bounds__(256, KS == 4 ? 3 : 2) void product_panel_kernel(Pro
       }
       line_to[g] += step;
     }
+    // every store of this way is done: a later wait for loads then need not count them, and on the other way
+    // waits for the loads before its four stores only
+    __builtin_amdgcn_s_waitcnt(kLoadsDone);
   };
   keep(0);
   if (first + 1 < end) load(first + 1);
   __syncthreads();
+#pragma unroll
+  for (int q = 0; q < KS; q++) asm volatile("" : "+v"(fa[q]));  // these are there: the loop's waits count its own
+#pragma unroll
+  for (int q = 0; q < L; q++) asm volatile("" : "+v"(rb[q]));
+  asm volatile("" : "+v"(rs));
   for (int64_t tile = first; tile < end; tile++) {
-    const char* b = lds[(tile - first) & 1] + row * kRow;
+    const int buffer = (int)(tile - first) & 1;
+    const char* b = lds[buffer] + row * kRow;
     i16v acc[2] = {i16v{}, i16v{}};
 #pragma unroll
     for (int q = 0; q < KS; q++)
 #pragma unroll
       for (int y = 0; y < 2; y++)
         acc[y] = mfma(fa[q], *reinterpret_cast<const i4*>(b + y * 32 * kRow + ((2 * q + half) ^ (row & 7)) * 16), acc[y]);
-    if (tile + 1 < end) keep((int)(tile + 1 - first) & 1);
+    if (tile + 1 < end) keep(buffer ^ 1);
     if (tile + 2 < end) load(tile + 2);
 #pragma unroll
     for (int l = 0; l < 2 / Y; l++) {
-      float sb[Y], add[Y];
+      float scale[Y], add[Y];
 #pragma unroll
       for (int y = 0; y < Y; y++) {
-        const int64_t j = min(tile * 64 + (l * Y + y) * 32 + row, p.n - 1);
-        sb[y] = p.b_scales[j];
-        add[y] = p.bias ? p.bias[j] : 0.f;
+        const int j = (l * Y + y) * 32 + row;
+        scale[y] = sb[buffer][0][j];
+        add[y] = sb[buffer][1][j];
       }
 #pragma unroll
       for (int g = 0; g < 4; g++) {
@@ -392,8 +414,7 @@ __global__ __launch_bounds__(256, KS == 4 ? 3 : 2) void product_panel_kernel(Pro
         for (int e = 0; e < 4; e++)
 #pragma unroll
           for (int y = 0; y < Y; y++) {
-            float x = ((float)acc[l * Y + y][4 * g + e] * s[e]) * sb[y];
-            if (p.bias) x = x + add[y];
+            const float x = ((float)acc[l * Y + y][4 * g + e] * s[e]) * scale[y] + add[y];
             *reinterpret_cast<O*>(ring + place[y][4 * g + e] + (8 * g + e) * kRing) = (O)x;
             place[y][4 * g + e] ^= 128;
           }
