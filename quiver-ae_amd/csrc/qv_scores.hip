@@ -170,8 +170,8 @@ __device__ __forceinline__ int64_t tile_of_block(int64_t block, int64_t tiles) {
 
 // A tile of BM x BN outputs per workgroup, WM x WN waves of 32 TM x 32 TN each.  Both
 // operands' stages go through registers into LDS, the next one in flight while the
-// matrix cores work on this one; piece q of row r lies at q ^ (r mod 8), which keeps
-// both the writes and the reads free of bank conflicts.
+// matrix cores work on this one; piece q of row r lies at q ^ (r / 2 mod 8), so that the
+// 16 rows that are read at once (64 banks, 256 bytes) lie in 16 different places.
 template <int BM, int BN, int WM, int WN, class O>
 __global__ __launch_bounds__(64 * WM * WN, 1) void product_tile_kernel(Product<O> p, int64_t tiles_m, int64_t tiles_n,
                                                                        int64_t group) {
@@ -203,7 +203,7 @@ __global__ __launch_bounds__(64 * WM * WN, 1) void product_tile_kernel(Product<O
     for (int q = 0; q < LB; q++) rb[q] = *reinterpret_cast<const i4_any*>(b + (at_b[q] + (uint32_t)from));
   };
   auto keep = [&](int s) {
-    char* to = lds + (s & 1) * kBuffer + r0 * kStage + (piece ^ (r0 & 7)) * 16;
+    char* to = lds + (s & 1) * kBuffer + r0 * kStage + (piece ^ (r0 / 2 & 7)) * 16;
     if ((s + 1) * kStage > k) {
       const int over = max(0, s * kStage + piece * 16 - (k - 16));
 #pragma unroll
@@ -220,36 +220,138 @@ __global__ __launch_bounds__(64 * WM * WN, 1) void product_tile_kernel(Product<O
 #pragma unroll
     for (int y = 0; y < TN; y++) acc[x][y] = i16v{};
   const int row = lane % 32, half = lane / 32;
-  auto step = [&](int s, int q) {  // 32 bytes of k
-    const char* from = lds + (s & 1) * kBuffer + ((2 * q + half) ^ (row & 7)) * 16 + row * kStage;
-    i4 fa[TM], fb[TN];
+  i4 fa[2][TM], fb[2][TN];
+  auto read = [&](int s, int q) {  // a step's operands: 32 bytes of k
+    const char* from = lds + (s & 1) * kBuffer + ((2 * q + half) ^ (row / 2 & 7)) * 16 + row * kStage;
 #pragma unroll
-    for (int x = 0; x < TM; x++) fa[x] = *reinterpret_cast<const i4*>(from + (wm * TM + x) * 32 * kStage);
+    for (int x = 0; x < TM; x++) fa[q & 1][x] = *reinterpret_cast<const i4*>(from + (wm * TM + x) * 32 * kStage);
 #pragma unroll
-    for (int y = 0; y < TN; y++) fb[y] = *reinterpret_cast<const i4*>(from + BM * kStage + (wn * TN + y) * 32 * kStage);
-#pragma unroll
-    for (int x = 0; x < TM; x++)
-#pragma unroll
-      for (int y = 0; y < TN; y++) acc[x][y] = mfma(fb[y], fa[x], acc[x][y]);
+    for (int y = 0; y < TN; y++)
+      fb[q & 1][y] = *reinterpret_cast<const i4*>(from + BM * kStage + (wn * TN + y) * 32 * kStage);
   };
   load(0);
   keep(0);
   __syncthreads();
-  for (int s = 0; s + 1 < stages; s++) {
-    load(s + 1);
+  for (int s = 0; s < stages; s++) {
+    const bool more = s + 1 < stages;
+    if (more) load(s + 1);
+    read(s, 0);
 #pragma unroll
-    for (int q = 0; q < 4; q++) step(s, q);
-    keep(s + 1);
+    for (int q = 0; q < 4; q++) {
+      if (q < 3) read(s, q + 1);
+      if (q == 3 && more) keep(s + 1);
+      __builtin_amdgcn_sched_barrier(0);
+#pragma unroll
+      for (int x = 0; x < TM; x++)
+#pragma unroll
+        for (int y = 0; y < TN; y++) acc[x][y] = mfma(fb[q & 1][y], fa[q & 1][x], acc[x][y]);
+      __builtin_amdgcn_sched_barrier(0);
+    }
     __syncthreads();
   }
-  const int last = stages - 1, steps = (k - last * kStage + 31) / 32;
-  if (steps == 4) {
+  constexpr int J = 32 * TN, kTile = J + 4;
+  int32_t* tile = reinterpret_cast<int32_t*>(lds) + wave * 32 * kTile;
 #pragma unroll
-    for (int q = 0; q < 4; q++) step(last, q);
-  } else {
-    for (int q = 0; q < steps; q++) step(last, q);
+  for (int x = 0; x < TM; x++) {
+    if (x) __builtin_amdgcn_fence(__ATOMIC_ACQ_REL, "wavefront");
+#pragma unroll
+    for (int y = 0; y < TN; y++) put_sums(tile, kTile, 32 * y, acc[x][y]);
+    __builtin_amdgcn_fence(__ATOMIC_ACQ_REL, "wavefront");
+    store_tile<J>(tile, kTile, i0 + (wm * TM + x) * 32, j0 + wn * J, p);
   }
-  __syncthreads();
+}
+
+// The same tiles where the matrix cores are what bounds the product: stages of 64 bytes
+// of k go straight from memory to LDS (no registers, no LDS writes to issue), NB of
+// them at a time, so NB - 1 are on their way while one is used.  A stage is two steps
+// of 32 bytes; the second step's operands are read while the first one's products run,
+// and the next stage's first operands while the second one's do, so the one barrier
+// per stage, between the two, finds the operands of what follows it in registers.
+// Needs 16-byte aligned rows and k a multiple of 64.
+constexpr int kReadsDone = 0xc07f;  // s_waitcnt lgkmcnt(0)
+template <int N>
+constexpr int kWaitFor = (N & 15) | (N >> 4 << 14) | 0x0070;  // s_waitcnt vmcnt(N) lgkmcnt(0)
+
+template <int BM, int BN, int WM, int WN, int NB, class O>
+__global__ __launch_bounds__(64 * WM * WN, 1) void product_deep_kernel(Product<O> p, int64_t tiles_m, int64_t tiles_n,
+                                                                       int64_t group) {
+  constexpr int TM = BM / WM / 32, TN = BN / WN / 32, kRow = 64;
+  constexpr int I = (BM + BN) / 16 / (WM * WN);  // loads of 16 rows per wave and stage
+  constexpr int kBuffer = (BM + BN) * kRow;
+  extern __shared__ __align__(16) char lds[];
+  const int wave = wave_id(), lane = lane_id(), wm = wave / WN, wn = wave % WN;
+  const int64_t t = tile_of_block(blockIdx.x, tiles_m * tiles_n);
+  const int64_t g = t / (group * tiles_n), gm = min(group, tiles_m - g * group), in = t - g * group * tiles_n;
+  const int64_t i0 = (g * group + in % gm) * BM, j0 = in / gm * BN;
+  const int stages = (int)p.k / kRow;
+
+  // piece q of row r lies at q ^ (r / 4 mod 4): the lanes of a load write 1 KB in a row, so what they load is
+  // permuted instead
+  const int piece = (lane % 4) ^ (lane / 16);
+  const int8_t* src[I];
+#pragma unroll
+  for (int q = 0; q < I; q++) {
+    const int r = (wave * I + q) * 16 + lane / 4;
+    src[q] = (r < BM ? p.a + min(i0 + r, p.m - 1) * p.a_stride : p.b + min(j0 + r - BM, p.n - 1) * p.b_stride) + piece * 16;
+  }
+  // (stages past the last one repeat it: as many loads per turn as the waits count)
+  auto issue = [&](int s) {
+    char* to = lds + s % NB * kBuffer + wave * I * 1024;
+    const int from = min(s, stages - 1) * kRow;
+#pragma unroll
+    for (int q = 0; q < I; q++)
+      __builtin_amdgcn_global_load_lds((const __attribute__((address_space(1))) void*)(src[q] + from),
+                                       (__attribute__((address_space(3))) void*)(to + q * 1024), 16, 0, 0);
+  };
+  i16v acc[TM][TN];
+#pragma unroll
+  for (int x = 0; x < TM; x++)
+#pragma unroll
+    for (int y = 0; y < TN; y++) acc[x][y] = i16v{};
+  const int row = lane % 32, half = lane / 32;
+  i4 fa[2][TM], fb[2][TN];
+  auto read = [&](int s, int q) {
+    const char* from = lds + s % NB * kBuffer + ((2 * q + half) ^ (row / 4 % 4)) * 16 + row * kRow;
+#pragma unroll
+    for (int x = 0; x < TM; x++) fa[q][x] = *reinterpret_cast<const i4*>(from + (wm * TM + x) * 32 * kRow);
+#pragma unroll
+    for (int y = 0; y < TN; y++) fb[q][y] = *reinterpret_cast<const i4*>(from + (BM + (wn * TN + y) * 32) * kRow);
+  };
+  auto products = [&](int q) {
+#pragma unroll
+    for (int x = 0; x < TM; x++)
+#pragma unroll
+      for (int y = 0; y < TN; y++) acc[x][y] = mfma(fb[q][y], fa[q][x], acc[x][y]);
+  };
+  auto meet = [] {  // nothing of a stage moves over it
+    asm volatile("" ::: "memory");
+    __builtin_amdgcn_s_barrier();
+    asm volatile("" ::: "memory");
+    __builtin_amdgcn_sched_barrier(0);
+  };
+#pragma unroll
+  for (int s = 0; s < NB; s++) issue(s);
+  __builtin_amdgcn_s_waitcnt(kWaitFor<(NB - 1) * I>);
+  meet();
+  read(0, 0);
+  __builtin_amdgcn_s_waitcnt(kReadsDone);
+  for (int s = 0; s < stages; s++) {
+    read(s, 1);
+    __builtin_amdgcn_sched_barrier(0);  // the reads go first: the products below hide them
+    products(0);
+    __builtin_amdgcn_sched_barrier(0);
+    // stage s + 1 is there and every wave has read stage s
+    __builtin_amdgcn_s_waitcnt(kWaitFor<(NB - 2) * I>);
+    meet();
+    read(s + 1, 0);
+    __builtin_amdgcn_sched_barrier(0);
+    issue(s + NB);
+    products(1);
+    __builtin_amdgcn_s_waitcnt(kReadsDone);  // long since: said for the compiler, which else waits at the loop's top
+    __builtin_amdgcn_sched_barrier(0);
+  }
+  __builtin_amdgcn_s_waitcnt(kWaitFor<0>);
+  meet();
   constexpr int J = 32 * TN, kTile = J + 4;
   int32_t* tile = reinterpret_cast<int32_t*>(lds) + wave * 32 * kTile;
 #pragma unroll
@@ -285,6 +387,7 @@ __global__ __launch_bounds__(256, KS == 4 ? 3 : 2) void product_panel_kernel(Pro
   const int64_t t = tile_of_block(blockIdx.x, panels * slices), slice = t / panels, i0 = (t - slice * panels) * 128;
   const int64_t first = tiles_n * slice / slices, end = tiles_n * (slice + 1) / slices;
   const int k = (int)p.k, piece = tid % PC, r0 = tid / PC, from = min(piece * 16, k - 16);
+  auto swap = [](int r) { return KS == 4 ? r / 2 & 7 : r & 15; };  // as in the tiles, for rows of 128 or 256 bytes
   i4 rb[L];
   float rs = 0.f;
   const bool scales = tid < 128 && (tid < 64 || p.bias);
@@ -300,7 +403,7 @@ __global__ __launch_bounds__(256, KS == 4 ? 3 : 2) void product_panel_kernel(Pro
 #pragma unroll
     for (int q = 0; q < L; q++) {
       const int r = r0 + q * kRows;
-      *reinterpret_cast<i4*>(lds[buffer] + r * kRow + (piece ^ (r & 7)) * 16) = rb[q];
+      *reinterpret_cast<i4*>(lds[buffer] + r * kRow + (piece ^ swap(r)) * 16) = rb[q];
     }
     if (tid < 128) sb[buffer][tid / 64][tid % 64] = scales ? rs : -0.f;  // x + -0 is x
   };
@@ -395,7 +498,7 @@ __global__ __launch_bounds__(256, KS == 4 ? 3 : 2) void product_panel_kernel(Pro
     for (int q = 0; q < KS; q++)
 #pragma unroll
       for (int y = 0; y < 2; y++)
-        acc[y] = mfma(fa[q], *reinterpret_cast<const i4*>(b + y * 32 * kRow + ((2 * q + half) ^ (row & 7)) * 16), acc[y]);
+        acc[y] = mfma(fa[q], *reinterpret_cast<const i4*>(b + y * 32 * kRow + ((2 * q + half) ^ swap(row)) * 16), acc[y]);
     if (tile + 1 < end) keep(buffer ^ 1);
     if (tile + 2 < end) load(tile + 2);
 #pragma unroll
@@ -470,14 +573,14 @@ __global__ __launch_bounds__(256) void product_strip_kernel(Product<O> p, int64_
       if (stages > 1) load_a(s);
 #pragma unroll
       for (int q = 0; q < 4; q++)
-        *reinterpret_cast<i4*>(area + (r0 + 8 * q) * kStage + (piece ^ ((r0 + 8 * q) & 7)) * 16) = rb[q];
+        *reinterpret_cast<i4*>(area + (r0 + 8 * q) * kStage + (piece ^ ((r0 + 8 * q) / 2 & 7)) * 16) = rb[q];
       __builtin_amdgcn_fence(__ATOMIC_ACQ_REL, "wavefront");
       if (s + WK < stages) load_b(strip, s + WK);
       else if (strip + step < strips) load_b(strip + step, s0);
       const char* from = area + row * kStage;
 #pragma unroll
       for (int q = 0; q < 4; q++)
-        acc = mfma(*reinterpret_cast<const i4*>(from + ((2 * q + half) ^ (row & 7)) * 16), fa[q], acc);
+        acc = mfma(*reinterpret_cast<const i4*>(from + ((2 * q + half) ^ (row / 2 & 7)) * 16), fa[q], acc);
       __builtin_amdgcn_fence(__ATOMIC_ACQ_REL, "wavefront");
     }
     int32_t* tile = reinterpret_cast<int32_t*>(area);
@@ -550,6 +653,17 @@ void launch_tiles(const Product<O>& p, hipStream_t st) {
   HIP_OK(hipGetLastError());
 }
 
+template <int BM, int BN, int WM, int WN, int NB, class O>
+void launch_deep(const Product<O>& p, hipStream_t st) {
+  const int64_t tm = (p.m + BM - 1) / BM, tn = (p.n + BN - 1) / BN;
+  const int64_t group = std::min<int64_t>(tm, 8);
+  const int lds = std::max(NB * (BM + BN) * 64, WM * WN * 32 * (BN / WN + 4) * 4);
+  auto* kernel = product_deep_kernel<BM, BN, WM, WN, NB, O>;
+  if (lds > 65536) HIP_OK(hipFuncSetAttribute(reinterpret_cast<const void*>(kernel), hipFuncAttributeMaxDynamicSharedMemorySize, lds));
+  hipLaunchKernelGGL(kernel, dim3((unsigned)(tm * tn)), dim3(64 * WM * WN), lds, st, p, tm, tn, group);
+  HIP_OK(hipGetLastError());
+}
+
 template <int KS, class O>
 void launch_panels(const Product<O>& p, hipStream_t st) {
   const int64_t panels = (p.m + 127) / 128, tiles_n = (p.n + 63) / 64;
@@ -581,7 +695,9 @@ void product(const Product<O>& p, hipStream_t st) {
   } else if (p.k <= 256) {
     launch_panels<8>(p, st);
   } else if (p.k >= 512 && ((p.m + 255) / 256) * ((p.n + 255) / 256) >= 200) {
-    launch_tiles<256, 256, 2, 2>(p, st);
+    const bool aligned = (reinterpret_cast<uintptr_t>(p.a) | reinterpret_cast<uintptr_t>(p.b) | p.a_stride | p.b_stride) % 16 == 0 && p.k % 64 == 0;
+    if (aligned) launch_deep<256, 256, 2, 2, 4>(p, st);
+    else launch_tiles<256, 256, 2, 2>(p, st);
   } else {
     launch_tiles<128, 128, 2, 2>(p, st);
   }
