@@ -268,6 +268,19 @@ __global__ __launch_bounds__(64 * WM * WN, 1) void product_tile_kernel(Product<O
 // and the next stage's first operands while the second one's do, so the one barrier
 // per stage, between the two, finds the operands of what follows it in registers.
 // Needs 16-byte aligned rows and k a multiple of 64.
+// The schedule's next N x (P matrix instructions, one of the given kind): a matrix
+// instruction takes 32 cycles, in which a wave can issue a few others; in a run of
+// their own they would leave the matrix pipe idle.
+constexpr int kMfma = 0x008, kVmem = 0x010, kDsRead = 0x100;
+template <int N, int KIND, int P>
+__device__ __forceinline__ void between() {
+#pragma unroll
+  for (int i = 0; i < N; i++) {
+    __builtin_amdgcn_sched_group_barrier(kMfma, P, 0);
+    __builtin_amdgcn_sched_group_barrier(KIND, 1, 0);
+  }
+}
+
 constexpr int kReadsDone = 0xc07f;  // s_waitcnt lgkmcnt(0)
 template <int N>
 constexpr int kWaitFor = (N & 15) | (N >> 4 << 14) | 0x0070;  // s_waitcnt vmcnt(N) lgkmcnt(0)
@@ -295,11 +308,11 @@ __global__ __launch_bounds__(64 * WM * WN, 1) void product_deep_kernel(Product<O
     src[q] = (r < BM ? p.a + min(i0 + r, p.m - 1) * p.a_stride : p.b + min(j0 + r - BM, p.n - 1) * p.b_stride) + piece * 16;
   }
   // (stages past the last one repeat it: as many loads per turn as the waits count)
-  auto issue = [&](int s) {
+  auto issue = [&](int s, int part) {  // a half of a stage's loads
     char* to = lds + s % NB * kBuffer + wave * I * 1024;
     const int from = min(s, stages - 1) * kRow;
 #pragma unroll
-    for (int q = 0; q < I; q++)
+    for (int q = part * I / 2; q < (part + 1) * I / 2; q++)
       __builtin_amdgcn_global_load_lds((const __attribute__((address_space(1))) void*)(src[q] + from),
                                        (__attribute__((address_space(3))) void*)(to + q * 1024), 16, 0, 0);
   };
@@ -330,23 +343,29 @@ __global__ __launch_bounds__(64 * WM * WN, 1) void product_deep_kernel(Product<O
     __builtin_amdgcn_sched_barrier(0);
   };
 #pragma unroll
-  for (int s = 0; s < NB; s++) issue(s);
-  __builtin_amdgcn_s_waitcnt(kWaitFor<(NB - 1) * I>);
+  for (int s = 0; s < NB; s++) {
+    issue(s, 0);
+    if (s + 1 < NB) issue(s, 1);
+  }
+  __builtin_amdgcn_s_waitcnt(kWaitFor<(NB - 1) * I - I / 2>);
   meet();
   read(0, 0);
   __builtin_amdgcn_s_waitcnt(kReadsDone);
   for (int s = 0; s < stages; s++) {
     read(s, 1);
-    __builtin_amdgcn_sched_barrier(0);  // the reads go first: the products below hide them
+    issue(s + NB - 1, 1);
     products(0);
+    between<TM + TN, kDsRead, 1>();
+    between<I / 2, kVmem, 2>();
     __builtin_amdgcn_sched_barrier(0);
     // stage s + 1 is there and every wave has read stage s
     __builtin_amdgcn_s_waitcnt(kWaitFor<(NB - 2) * I>);
     meet();
     read(s + 1, 0);
-    __builtin_amdgcn_sched_barrier(0);
-    issue(s + NB);
+    issue(s + NB, 0);
     products(1);
+    between<TM + TN, kDsRead, 1>();
+    between<I / 2, kVmem, 2>();
     __builtin_amdgcn_s_waitcnt(kReadsDone);  // long since: said for the compiler, which else waits at the loop's top
     __builtin_amdgcn_sched_barrier(0);
   }
