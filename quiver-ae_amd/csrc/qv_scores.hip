@@ -290,6 +290,7 @@ __global__ __launch_bounds__(64 * WM * WN, 1) void product_deep_kernel(Product<O
                                                                        int64_t group) {
   constexpr int TM = BM / WM / 32, TN = BN / WN / 32, kRow = 64;
   constexpr int I = (BM + BN) / 16 / (WM * WN);  // loads of 16 rows per wave and stage
+  static_assert(I % 2 == 0, "issued in halves");
   constexpr int kBuffer = (BM + BN) * kRow;
   extern __shared__ __align__(16) char lds[];
   const int wave = wave_id(), lane = lane_id(), wm = wave / WN, wn = wave % WN;
@@ -713,12 +714,19 @@ void product(const Product<O>& p, hipStream_t st) {
     launch_panels<4>(p, st);
   } else if (p.k <= 256) {
     launch_panels<8>(p, st);
-  } else if (p.k >= 512 && ((p.m + 255) / 256) * ((p.n + 255) / 256) >= 200) {
-    const bool aligned = (reinterpret_cast<uintptr_t>(p.a) | reinterpret_cast<uintptr_t>(p.b) | p.a_stride | p.b_stride) % 16 == 0 && p.k % 64 == 0;
-    if (aligned) launch_deep<256, 256, 2, 2, 4>(p, st);
-    else launch_tiles<256, 256, 2, 2>(p, st);
   } else {
-    launch_tiles<128, 128, 2, 2>(p, st);
+    // By how many tiles there are for the 256 CUs.  Measured to bfloat16, us, with tiles of 256, 128 and 64 straight
+    // to LDS and of 128 through registers: 4,096^3: 73, 87, 136, 84; 2,048 x 4,096 x 4,096: 56, 48, 73, 46;
+    // 1,024: 53, 26, 42, 31; 512: 51, 22, 20, 29; 64: 45, 20, 13, 27; 4,096 x 4,096 x 1,024: 32, 32, 41, 31;
+    // 1,024 x 20,032 x 512: 42, 28, 32, 27.
+    auto tiles = [&](int64_t size) { return (p.m + size - 1) / size * ((p.n + size - 1) / size); };
+    const bool direct = (reinterpret_cast<uintptr_t>(p.a) | reinterpret_cast<uintptr_t>(p.b) | p.a_stride | p.b_stride) % 16 == 0 &&
+                        p.k % 64 == 0;
+    if (direct && p.k >= 2048 && tiles(256) >= 200) launch_deep<256, 256, 2, 2, 4>(p, st);
+    else if (direct && tiles(64) <= 512) launch_deep<64, 64, 2, 2, 4>(p, st);
+    else if (direct && tiles(128) <= 256) launch_deep<128, 128, 2, 2, 4>(p, st);
+    else if (tiles(64) <= 512) launch_tiles<64, 64, 2, 2>(p, st);
+    else launch_tiles<128, 128, 2, 2>(p, st);
   }
 }
 

@@ -147,7 +147,8 @@ def _check_product(out, a, sa, b, sb, bias, dtype):
     (1, 1, 1), (1, 1, 16), (1, 1000, 128), (2, 77, 5), (3, 129, 15), (16, 300, 96), (17, 31, 17), (31, 257, 100),
     (32, 512, 128), (33, 513, 129), (64, 64, 64), (65, 127, 200), (100, 1001, 33), (127, 255, 256), (128, 128, 1024),
     (129, 300, 31), (255, 257, 144), (256, 256, 384), (300, 200, 1000), (511, 513, 112), (1, 5000, 4096), (20, 700, 2049),
-    (600, 700, 769), (1030, 2100, 260)])
+    (600, 700, 769), (1030, 2100, 260), (33, 70, 320), (200, 900, 4096), (1000, 3000, 576), (130, 20000, 640),
+    (1500, 3300, 384), (1500, 3300, 1001), (100, 900, 4001), (4096, 3329, 2048)])
 def test_product(scoring, dtype, m, n, k):
     say("product", dtype, m, n, k)
     a, sa, b, sb, bias = _inputs(m, n, k, m * 31 + n * 7 + k)
