@@ -11,36 +11,162 @@ using namespace qv::dense;
 
 namespace {
 
-constexpr float kTiny = 0x1p-119f;  // below it 127 / a comes near the largest float: the row counts as zeros
+// ---- rows to 8 bits --------------------------------------------------------------
+//
+// A row is read once, by a group of G lanes that hold it in registers (E loads of 16
+// bytes each) between the search for its largest magnitude and the rounding; R rows
+// per group at once keep more loads in flight.  Bound by memory: one read, a quarter (half) of it
+// written.  Magnitudes are compared as whole numbers, whose order is theirs, with
+// infinities and NaN above all.
 
-__device__ __forceinline__ float wave_max(float v) {
-  for (int m = 32; m; m >>= 1) v = fmaxf(v, __shfl_xor(v, m));
+typedef uint32_t raw4 __attribute__((ext_vector_type(4)));
+typedef raw4 raw4_any __attribute__((aligned(2), may_alias));
+
+constexpr uint32_t kTinyBits = 0x04000000u;  // 2^-119: below it 127 / a comes near the largest float, the row counts as zeros
+constexpr uint32_t kInfBits = 0x7f800000u;
+
+template <class T>
+constexpr int kVec = 16 / (int)sizeof(T);
+
+template <class T>
+__device__ __forceinline__ void to_floats(raw4 r, float* v) {
+#pragma unroll
+  for (int i = 0; i < 4; i++) {
+    if constexpr (sizeof(T) == 4) {
+      v[i] = __uint_as_float(r[i]);
+    } else if constexpr (std::is_same<T, bf16>::value) {
+      v[2 * i] = __uint_as_float(r[i] << 16);
+      v[2 * i + 1] = __uint_as_float(r[i] & 0xffff0000u);
+    } else {
+      typedef f16 h2 __attribute__((ext_vector_type(2)));
+      const h2 h = __builtin_bit_cast(h2, (uint32_t)r[i]);
+      v[2 * i] = (float)h[0];
+      v[2 * i + 1] = (float)h[1];
+    }
+  }
+}
+
+// The vector at column j of a row of dim, zeros past it.
+template <class T>
+__device__ __forceinline__ void load_floats(const T* row, int64_t j, int64_t dim, float* v) {
+  if (j + kVec<T> <= dim) {
+    to_floats<T>(*reinterpret_cast<const raw4_any*>(row + j), v);
+  } else {
+#pragma unroll
+    for (int i = 0; i < kVec<T>; i++) v[i] = j + i < dim ? (float)row[j + i] : 0.f;
+  }
+}
+
+// Largest value over the group of G lanes (a power of two) that the lane is in.
+template <int G>
+__device__ __forceinline__ uint32_t group_max(uint32_t v) {
+  if constexpr (G >= 2) v = max(v, (uint32_t)__builtin_amdgcn_mov_dpp((int)v, 0xB1, 0xF, 0xF, true));
+  if constexpr (G >= 4) v = max(v, (uint32_t)__builtin_amdgcn_mov_dpp((int)v, 0x4E, 0xF, 0xF, true));
+  if constexpr (G >= 8) v = max(v, (uint32_t)__builtin_amdgcn_mov_dpp((int)v, 0x141, 0xF, 0xF, true));  // row_half_mirror
+  if constexpr (G >= 16) v = max(v, (uint32_t)__builtin_amdgcn_mov_dpp((int)v, 0x128, 0xF, 0xF, true));  // row_ror:8
+  if constexpr (G >= 32) {
+    const auto p = __builtin_amdgcn_permlane16_swap(v, v, false, false);
+    v = max(p[0], p[1]);
+  }
+  if constexpr (G >= 64) {
+    const auto p = __builtin_amdgcn_permlane32_swap(v, v, false, false);
+    v = max(p[0], p[1]);
+  }
   return v;
 }
 
-// One wave per row, the row read twice.
+struct RowScale {
+  float inv, scale;
+};
+__device__ __forceinline__ RowScale scale_of(uint32_t top) {
+  const float a = __uint_as_float(top);
+  if (top >= kInfBits) return {0.f, __builtin_nanf("")};
+  if (top < kTinyBits) return {0.f, 0.f};
+  return {127.f / a, a / 127.f};
+}
+
+// x (127 / a) to the nearest whole number, halves to even, in the low byte: adding 1.5 2^23
+// rounds to it (|x| 127 / a <= 127).  inv 0 gives 0 for every x, infinities and NaN too.
+__device__ __forceinline__ uint32_t code_of(float x, float inv) {
+  return inv != 0.f ? __float_as_uint(x * inv + 12582912.f) : 0u;
+}
+
 template <class T>
+__device__ __forceinline__ void store_codes(int8_t* row, int64_t j, int64_t dim, const float* v, float inv) {
+  uint32_t word[kVec<T> / 4];
+#pragma unroll
+  for (int w = 0; w < kVec<T> / 4; w++) {
+    uint32_t c[4];
+#pragma unroll
+    for (int i = 0; i < 4; i++) c[i] = code_of(v[4 * w + i], inv);
+    // bytes 0 of four words into one
+    const uint32_t lo = __builtin_amdgcn_perm(c[1], c[0], 0x0c0c0400), hi = __builtin_amdgcn_perm(c[3], c[2], 0x04000c0c);
+    word[w] = lo | hi;
+  }
+  if (j + kVec<T> <= dim) {
+    __builtin_memcpy(row + j, word, kVec<T>);
+  } else {
+#pragma unroll
+    for (int i = 0; i < kVec<T>; i++)
+      if (j + i < dim) row[j + i] = (int8_t)(word[i / 4] >> (8 * (i % 4)));
+  }
+}
+
+template <class T, int G, int E, int R>
 __global__ __launch_bounds__(256) void quantize_kernel(const T* __restrict__ x, int64_t n, int64_t dim, int64_t stride,
                                                        int8_t* __restrict__ codes, int64_t code_stride,
                                                        float* __restrict__ scales) {
-  const int64_t row = (int64_t)blockIdx.x * 4 + threadIdx.x / kWave;
-  const int lane = lane_id();
-  if (row >= n) return;
-  const T* src = x + row * stride;
-  float top = 0.f;
-  bool odd = false;  // an infinity or a NaN in the row
-  for (int64_t j = lane; j < dim; j += kWave) {
-    const float v = fabsf((float)src[j]);
-    odd |= !(v < __builtin_inff());
-    top = fmaxf(top, v);
+  constexpr int kGroups = 256 / G;
+  const int lane = threadIdx.x % G;
+  const int64_t first = (int64_t)blockIdx.x * kGroups * R + threadIdx.x / G;
+  float v[R][E * kVec<T>];
+#pragma unroll
+  for (int r = 0; r < R; r++) {
+    const int64_t row = min(first + r * kGroups, n - 1);
+#pragma unroll
+    for (int e = 0; e < E; e++) load_floats(x + row * stride, (int64_t)(e * G + lane) * kVec<T>, dim, v[r] + e * kVec<T>);
   }
-  top = wave_max(top);
-  odd = __any(odd);
-  const bool some = !odd && top >= kTiny;
-  const float inv = some ? 127.f / top : 0.f;
-  for (int64_t j = lane; j < dim; j += kWave)
-    codes[row * code_stride + j] = some ? (int8_t)rintf((float)src[j] * inv) : (int8_t)0;
-  if (lane == 0) scales[row] = odd ? __builtin_nanf("") : some ? top / 127.f : 0.f;
+#pragma unroll
+  for (int r = 0; r < R; r++) {
+    const int64_t row = first + r * kGroups;
+    uint32_t top = 0;
+#pragma unroll
+    for (int i = 0; i < E * kVec<T>; i++) top = max(top, __float_as_uint(v[r][i]) & 0x7fffffffu);
+    const RowScale s = scale_of(group_max<G>(top));
+    if (row >= n) continue;
+#pragma unroll
+    for (int e = 0; e < E; e++)
+      store_codes<T>(codes + row * code_stride, (int64_t)(e * G + lane) * kVec<T>, dim, v[r] + e * kVec<T>, s.inv);
+    if (lane == 0) scales[row] = s.scale;
+  }
+}
+
+// Rows longer than a wave holds: one workgroup per row, which is read again (from the
+// caches) for the rounding.
+template <class T>
+__global__ __launch_bounds__(256) void quantize_long_kernel(const T* __restrict__ x, int64_t dim, int64_t stride,
+                                                            int8_t* __restrict__ codes, int64_t code_stride,
+                                                            float* __restrict__ scales) {
+  __shared__ uint32_t tops[4];
+  const int64_t row = blockIdx.x;
+  const T* src = x + row * stride;
+  uint32_t top = 0;
+  for (int64_t j = (int64_t)threadIdx.x * kVec<T>; j < dim; j += 256 * kVec<T>) {
+    float v[kVec<T>];
+    load_floats(src, j, dim, v);
+#pragma unroll
+    for (int i = 0; i < kVec<T>; i++) top = max(top, __float_as_uint(v[i]) & 0x7fffffffu);
+  }
+  top = group_max<64>(top);
+  if (lane_id() == 0) tops[wave_id()] = top;
+  __syncthreads();
+  const RowScale s = scale_of(max(max(tops[0], tops[1]), max(tops[2], tops[3])));
+  for (int64_t j = (int64_t)threadIdx.x * kVec<T>; j < dim; j += 256 * kVec<T>) {
+    float v[kVec<T>];
+    load_floats(src, j, dim, v);
+    store_codes<T>(codes + row * code_stride, j, dim, v, s.inv);
+  }
+  if (threadIdx.x == 0) scales[row] = s.scale;
 }
 
 // ---- product -------------------------------------------------------------------
@@ -655,8 +781,22 @@ __global__ __launch_bounds__(256) void product_small_kernel(Product<O> p, int64_
 template <class T>
 void quantize(const void* x, int64_t n, int64_t dim, int64_t stride, int8_t* codes, int64_t code_stride, float* scales,
               hipStream_t st) {
-  hipLaunchKernelGGL(quantize_kernel<T>, dim3((unsigned)((n + 3) / 4)), dim3(256), 0, st, static_cast<const T*>(x), n,
-                     dim, stride, codes, code_stride, scales);
+  const T* in = static_cast<const T*>(x);
+  auto go = [&](auto* kernel, int64_t rows) {
+    hipLaunchKernelGGL(kernel, dim3((unsigned)((n + rows - 1) / rows)), dim3(256), 0, st, in, n, dim, stride, codes,
+                       code_stride, scales);
+  };
+  const int64_t vectors = (dim + kVec<T> - 1) / kVec<T>;
+  if (vectors <= 8) go(quantize_kernel<T, 8, 1, 4>, 128);
+  else if (vectors <= 16) go(quantize_kernel<T, 16, 1, 4>, 64);
+  else if (vectors <= 32) go(quantize_kernel<T, 32, 1, 4>, 32);
+  else if (vectors <= 64) go(quantize_kernel<T, 64, 1, 4>, 16);
+  else if (vectors <= 128) go(quantize_kernel<T, 64, 2, 2>, 8);
+  else if (vectors <= 256) go(quantize_kernel<T, 64, 4, 1>, 4);
+  else if (vectors <= 512) go(quantize_kernel<T, 64, 8, 1>, 4);
+  else
+    hipLaunchKernelGGL(quantize_long_kernel<T>, dim3((unsigned)n), dim3(256), 0, st, in, dim, stride, codes, code_stride,
+                       scales);
   HIP_OK(hipGetLastError());
 }
 
