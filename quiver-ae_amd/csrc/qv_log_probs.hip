@@ -128,21 +128,48 @@ __device__ __forceinline__ uint64_t merge_desc(uint64_t a, uint64_t b) {
   return key;
 }
 
-// A wave's best keys: entry i of the list in lane i.  Candidates wait in LDS, 64 of
-// them are sorted and merged at once: a tenth of what placing them one by one
-// costs.
+constexpr uint32_t kLowest = 0x00800000u;  // the lowest finite value's rank
+
+// The largest t (of the top 16 bits) that at least k of the lanes' ranks reach.
+__device__ __forceinline__ uint32_t kth_of_lanes(uint32_t rank, int k) {
+  uint32_t t = 0;
+#pragma unroll
+  for (uint32_t bit = 0x80000000u; bit >= 0x10000u; bit >>= 1)
+    if (__popcll(__ballot(rank >= (t | bit))) >= k) t |= bit;
+  return t;
+}
+
+// Descending across the wave; the first `count` lanes hold distinct keys, the others 0.
+// Few are placed by counting the larger ones (4 instructions each, the bitonic sort
+// about 230).
+__device__ __forceinline__ uint64_t sort_desc(uint64_t key, int count) {
+  if (count > 40) return wave_sort_desc(key);
+  const int lane = lane_id();
+  int place = 0;
+  for (int l = 0; l < count; l++) place += read_lane_u64(key, l) > key ? 1 : 0;
+  const int to = (lane < count ? place : lane) << 2;
+  return ((uint64_t)(uint32_t)__builtin_amdgcn_ds_permute(to, (int)(uint32_t)(key >> 32)) << 32) |
+         (uint32_t)__builtin_amdgcn_ds_permute(to, (int)(uint32_t)key);
+}
+
+// A wave's best keys: entry i of the list in lane i.  Candidates wait in LDS until
+// there are 64 of them, or the pass ends.
 constexpr int kPool = 128;
 
 struct Best {
   uint64_t list = 0;
   uint64_t* pool;  // [kPool], this wave's
-  int count = 0;
+  int count = 0;   // in the pool
+  bool some = false;
   int k;
 
   __device__ Best(uint64_t* pool_, int k_) : pool(pool_), k(k_) {}
 
-  __device__ __forceinline__ void merge(uint64_t key) { list = merge_desc(list, wave_sort_desc(key)); }
-
+  __device__ __forceinline__ void merge(uint64_t key, int n) {
+    key = sort_desc(key, n);
+    list = some ? merge_desc(list, key) : key;
+    some = true;
+  }
   __device__ __forceinline__ void offer(bool take, uint64_t key) {
     const uint64_t mask = __ballot(take);
     if (mask == 0) return;
@@ -151,18 +178,27 @@ struct Best {
     if (count >= kWave) {
       __builtin_amdgcn_fence(__ATOMIC_ACQ_REL, "wavefront");
       count -= kWave;
-      merge(pool[count + lane_id()]);
+      merge(pool[count + lane_id()], kWave);
       __builtin_amdgcn_fence(__ATOMIC_ACQ_REL, "wavefront");
     }
   }
   __device__ __forceinline__ void finish() {
     if (count == 0) return;
     __builtin_amdgcn_fence(__ATOMIC_ACQ_REL, "wavefront");
-    merge(lane_id() < count ? pool[lane_id()] : 0);
+    merge(lane_id() < count ? pool[lane_id()] : 0, count);
     count = 0;
   }
-  // The k-th key so far (0 while there are fewer).
-  __device__ __forceinline__ uint64_t last() const { return read_lane_u64(list, k - 1); }
+  // Another wave's list and pool, of which only keys from `least` on can matter.
+  __device__ __forceinline__ void take(uint64_t other_list, const uint64_t* other_pool, int other_count, uint64_t least) {
+    if (__any(other_list != 0)) {
+      list = some ? merge_desc(list, other_list) : other_list;
+      some = true;
+    }
+    if (other_count) {
+      const uint64_t key = lane_id() < other_count ? other_pool[lane_id()] : 0;
+      offer(key && key >= least, key);
+    }
+  }
 };
 
 // ---- sums ----------------------------------------------------------------------
@@ -230,11 +266,16 @@ struct Pass {
 
   __device__ Pass(float c_, uint64_t* pool, int k) : c(c_), best(pool, k) {}
 
-  __device__ __forceinline__ void values(const float (&v)[N], int column, bool first) {
-    float top = v[0];
+  __device__ __forceinline__ void values(const float (&v)[N], int column) {
+    float top;
+    if constexpr (N == 16) {
+      top = max3(max3(v[0], v[1], v[2]), max3(v[3], v[4], v[5]), max3(v[6], v[7], v[8]));
+      top = max3(top, max3(v[9], v[10], v[11]), max3(v[12], v[13], max2(v[14], v[15])));
+    } else {
+      top = max2(v[0], v[1]);
 #pragma unroll
-    for (int i = 1; i + 1 < N; i += 2) top = max3(top, v[i], v[i + 1]);
-    if constexpr (N % 2 == 0) top = max2(top, v[N - 1]);
+      for (int i = 2; i < N; i += 2) top = max3(top, v[i], v[i + 1]);
+    }
     if (__any(top > sum.m)) {
       sum.move(max2(sum.m, top), c);
       mc = scaled(sum.m, c);
@@ -260,36 +301,33 @@ struct Pass {
     sum.s = sum.s + s;
     sum.w = sum.w + w;
     if constexpr (TOP) {
-      if (first) {
-        // the k-th of the lanes' largest: k values are at least that large
-        const uint64_t order = wave_sort_desc(rank_key(top, (uint32_t)lane_id()));
-        least = max2(least, value_of((uint32_t)(read_lane_u64(order, best.k - 1) >> 32)));
-      }
       if (__any(top >= least)) {
+        // k lanes have seen a value that large: about 64 ln(64 / (64 - k)) values pass in all
+        least = max2(least, value_of(max(kLowest, kth_of_lanes(rank_of(sum.m), best.k))));
 #pragma unroll
         for (int i = 0; i < N; i++) {
           const int at = column + (i / kVec<T>)*kWave * kVec<T> + i % kVec<T>;
           best.offer(v[i] >= least, rank_key(v[i], (uint32_t)at));
         }
-        raise(best.last());
       }
     }
   }
-  __device__ __forceinline__ void raise(uint64_t key) {
-    if (key) least = max2(least, value_of((uint32_t)(key >> 32)));
-  }
 
-  // Batches [b, end) in steps; shared: the block's largest k-th value so far (ranks), or null.
+  // Batches b, b + step, ... of columns [from, to), the next one's values on their way; shared: the largest `least` of
+  // the workgroup's waves (as a rank), or null.
   __device__ void run(const T* __restrict__ x, int64_t from, int64_t to, int b, int step, uint32_t* shared) {
     const int lane = lane_id();
-    bool first = true;
-    for (int64_t at = from + (int64_t)b * kBatch; at < to; at += (int64_t)step * kBatch) {
-      float v[N];
-      const int64_t mine = at + lane * kVec<T>;
-      if (at + kBatch <= to) {
-        raw4 r[U];
+    raw4 r[U];
+    int64_t at = from + (int64_t)b * kBatch;
+    auto load = [&](int64_t where) {
 #pragma unroll
-        for (int u = 0; u < U; u++) r[u] = load_raw(x + mine + u * kWave * kVec<T>);
+      for (int u = 0; u < U; u++) r[u] = load_raw(x + where + (u * kWave + lane) * kVec<T>);
+    };
+    if (at + kBatch <= to) load(at);
+    while (at < to) {
+      float v[N];
+      const int64_t mine = at + lane * kVec<T>, next = at + (int64_t)step * kBatch;
+      if (at + kBatch <= to) {
 #pragma unroll
         for (int u = 0; u < U; u++) unpack<T>(r[u], v + u * kVec<T>);
       } else {
@@ -297,12 +335,12 @@ struct Pass {
         for (int u = 0; u < U; u++)
           load_tail(x + mine + u * kWave * kVec<T>, to - mine - u * kWave * kVec<T>, v + u * kVec<T>);
       }
+      if (next + kBatch <= to) load(next);
       if (TOP && shared) least = max2(least, value_of(max(rank_of(least), *(volatile uint32_t*)shared)));
-      values(v, (int)mine, first);
+      values(v, (int)mine);
       if (TOP && shared && lane == 0) atomicMax(shared, rank_of(least));
-      first = false;
+      at = next;
     }
-    if constexpr (TOP) best.finish();
     sum.fold(c);
   }
 };
@@ -355,6 +393,7 @@ __global__ __launch_bounds__(256) void log_probs_wave_kernel(const T* __restrict
   const T* x = logits + row * stride;
   Pass<T, U, TOP> pass(c, TOP ? pool + wave * kPool : pool, o.topk);
   pass.run(x, 0, cols, 0, 1, nullptr);
+  if constexpr (TOP) pass.best.finish();
   finish_row(x, row, cols, pass.sum, pass.best.list, c, inv_t, o);
 }
 
@@ -366,7 +405,9 @@ __global__ __launch_bounds__(256) void log_probs_block_kernel(const T* __restric
                                                               float4* __restrict__ part,
                                                               uint64_t* __restrict__ part_keys) {
   __shared__ uint64_t pool[TOP ? 4 * kPool : 1];
+  __shared__ uint64_t lists[TOP ? 4 : 1][kWave];
   __shared__ float4 sums[4];
+  __shared__ int counts[4];
   __shared__ uint32_t least;
   const int tid = threadIdx.x, wave = wave_id(), lane = lane_id();
   const int64_t row = blockIdx.x / (unsigned)splits;
@@ -379,18 +420,24 @@ __global__ __launch_bounds__(256) void log_probs_block_kernel(const T* __restric
   Pass<T, U, TOP> pass(c, TOP ? pool + wave * kPool : pool, o.topk);
   const int64_t from = (int64_t)split * chunk;
   pass.run(x, from, min((int64_t)cols, from + chunk), wave, 4, &least);
-  if (lane == 0) sums[wave] = pass.sum.packed();
-  if constexpr (TOP) pool[wave * kPool + lane] = pass.best.list;
+  if (lane == 0) {
+    sums[wave] = pass.sum.packed();
+    counts[wave] = pass.best.count;
+  }
+  if constexpr (TOP) lists[wave][lane] = pass.best.list;
   __syncthreads();
   if (wave) return;
   Sums sum = Sums::of(sums[0]);
 #pragma unroll
   for (int q = 1; q < 4; q++) sum.add(Sums::of(sums[q]), c);
-  uint64_t list = pass.best.list;
+  Best& best = pass.best;
   if constexpr (TOP) {
+    const uint64_t from_least = (uint64_t)least << 32;
 #pragma unroll
-    for (int q = 1; q < 4; q++) list = merge_desc(list, pool[q * kPool + lane]);
+    for (int q = 1; q < 4; q++) best.take(lists[q][lane], pool + q * kPool, counts[q], from_least);
+    best.finish();
   }
+  const uint64_t list = best.list;
   if (splits == 1) {
     finish_row(x, row, cols, sum, list, c, inv_t, o);
   } else {
@@ -405,7 +452,9 @@ __global__ __launch_bounds__(256) void join_kernel(const T* __restrict__ logits,
                                                    float inv_t, int splits, Out o, const float4* __restrict__ part,
                                                    const uint64_t* __restrict__ part_keys) {
   __shared__ uint64_t pool[TOP ? 4 * kPool : 1];
+  __shared__ uint64_t lists[TOP ? 4 : 1][kWave], leasts[4];
   __shared__ float4 sums[4];
+  __shared__ int counts[4];
   const int tid = threadIdx.x, wave = wave_id(), lane = lane_id();
   const int64_t row = blockIdx.x;
   Sums sum;
@@ -416,30 +465,33 @@ __global__ __launch_bounds__(256) void join_kernel(const T* __restrict__ logits,
   Best best(TOP ? pool + wave * kPool : pool, o.topk);
   if constexpr (TOP) {
     const uint64_t* keys = part_keys + row * splits * o.topk;
-    // the k-th of 64 chunks' largest keys: k keys are at least that large
+    // k of 64 chunks have a key with a rank that large
     const int head = wave * kWave + lane;
-    const uint64_t order = wave_sort_desc(head < splits ? keys[(int64_t)head * o.topk] : 0);
-    uint64_t least = read_lane_u64(order, o.topk - 1);
+    const uint64_t least = (uint64_t)kth_of_lanes(head < splits ? (uint32_t)(keys[(int64_t)head * o.topk] >> 32) : 0, o.topk) << 32;
     const int total = splits * o.topk;
     for (int i = wave * kWave; i < total; i += 256) {
       const uint64_t key = i + lane < total ? keys[i + lane] : 0;
       best.offer(key && key >= least, key);
-      least = umax64(least, best.last());
     }
-    best.finish();
-    pool[wave * kPool + lane] = best.list;
+    lists[wave][lane] = best.list;
+    if (lane == 0) leasts[wave] = least;
   }
-  if (lane == 0) sums[wave] = sum.packed();
+  if (lane == 0) {
+    sums[wave] = sum.packed();
+    counts[wave] = best.count;
+  }
   __syncthreads();
   if (wave) return;
   sum = Sums::of(sums[0]);
 #pragma unroll
   for (int q = 1; q < 4; q++) sum.add(Sums::of(sums[q]), c);
-  uint64_t list = best.list;
   if constexpr (TOP) {
+    const uint64_t least = umax64(umax64(leasts[0], leasts[1]), umax64(leasts[2], leasts[3]));
 #pragma unroll
-    for (int q = 1; q < 4; q++) list = merge_desc(list, pool[q * kPool + lane]);
+    for (int q = 1; q < 4; q++) best.take(lists[q][lane], pool + q * kPool, counts[q], least);
+    best.finish();
   }
+  const uint64_t list = best.list;
   finish_row(logits + row * stride, row, cols, sum, list, c, inv_t, o);
 }
 
