@@ -153,9 +153,11 @@ __device__ __forceinline__ uint64_t sort_desc(uint64_t key, int count) {
 }
 
 // A wave's best keys: entry i of the list in lane i.  Candidates wait in LDS until
-// there are 64 of them, or the pass ends.
+// there are 64 of them, or the pass ends; VALUES: as a value's bits and its column,
+// which become a key when they are sorted.
 constexpr int kPool = 128;
 
+template <bool VALUES>
 struct Best {
   uint64_t list = 0;
   uint64_t* pool;  // [kPool], this wave's
@@ -165,38 +167,42 @@ struct Best {
 
   __device__ Best(uint64_t* pool_, int k_) : pool(pool_), k(k_) {}
 
+  __device__ __forceinline__ uint64_t waiting(int i, int n) const {
+    const uint64_t c = i < n ? pool[i] : 0;
+    return !VALUES ? c : i < n ? rank_key(__uint_as_float((uint32_t)(c >> 32)), (uint32_t)c) : 0;
+  }
   __device__ __forceinline__ void merge(uint64_t key, int n) {
     key = sort_desc(key, n);
     list = some ? merge_desc(list, key) : key;
     some = true;
   }
-  __device__ __forceinline__ void offer(bool take, uint64_t key) {
+  __device__ __forceinline__ void offer(bool take, uint64_t candidate) {
     const uint64_t mask = __ballot(take);
     if (mask == 0) return;
-    if (take) pool[count + __builtin_amdgcn_mbcnt_hi((uint32_t)(mask >> 32), __builtin_amdgcn_mbcnt_lo((uint32_t)mask, 0))] = key;
+    if (take) pool[count + __builtin_amdgcn_mbcnt_hi((uint32_t)(mask >> 32), __builtin_amdgcn_mbcnt_lo((uint32_t)mask, 0))] = candidate;
     count += __popcll(mask);
     if (count >= kWave) {
       __builtin_amdgcn_fence(__ATOMIC_ACQ_REL, "wavefront");
       count -= kWave;
-      merge(pool[count + lane_id()], kWave);
+      merge(waiting(count + lane_id(), kPool), kWave);
       __builtin_amdgcn_fence(__ATOMIC_ACQ_REL, "wavefront");
     }
   }
   __device__ __forceinline__ void finish() {
     if (count == 0) return;
     __builtin_amdgcn_fence(__ATOMIC_ACQ_REL, "wavefront");
-    merge(lane_id() < count ? pool[lane_id()] : 0, count);
+    merge(waiting(lane_id(), count), count);
     count = 0;
   }
-  // Another wave's list and pool, of which only keys from `least` on can matter.
-  __device__ __forceinline__ void take(uint64_t other_list, const uint64_t* other_pool, int other_count, uint64_t least) {
+  // Another wave's list and pool, of which only ranks from `least` on can matter.
+  __device__ __forceinline__ void take(uint64_t other_list, const Best& other, uint32_t least) {
     if (__any(other_list != 0)) {
       list = some ? merge_desc(list, other_list) : other_list;
       some = true;
     }
-    if (other_count) {
-      const uint64_t key = lane_id() < other_count ? other_pool[lane_id()] : 0;
-      offer(key && key >= least, key);
+    if (other.count) {
+      const uint64_t key = other.waiting(lane_id(), other.count);
+      offer(key && (uint32_t)(key >> 32) >= least, lane_id() < other.count ? other.pool[lane_id()] : 0);
     }
   }
 };
@@ -262,11 +268,12 @@ struct Pass {
   float c, mc = 0.f;
   bool big = false;
   float least = -__FLT_MAX__;  // values below it are not among the k largest
-  Best best;
+  Best<true> best;
 
   __device__ Pass(float c_, uint64_t* pool, int k) : c(c_), best(pool, k) {}
 
-  __device__ __forceinline__ void values(const float (&v)[N], int column) {
+  // `shared`: the four waves' bounds when all of them have batches (ranks), or null.
+  __device__ __forceinline__ void values(const float (&v)[N], int column, bool first, volatile uint32_t* shared) {
     float top;
     if constexpr (N == 16) {
       top = max3(max3(v[0], v[1], v[2]), max3(v[3], v[4], v[5]), max3(v[6], v[7], v[8]));
@@ -301,22 +308,32 @@ struct Pass {
     sum.s = sum.s + s;
     sum.w = sum.w + w;
     if constexpr (TOP) {
-      if (__any(top >= least)) {
-        // k lanes have seen a value that large: about 64 ln(64 / (64 - k)) values pass in all
-        least = max2(least, value_of(max(kLowest, kth_of_lanes(rank_of(sum.m), best.k))));
+      if (first || __any(top >= least)) {
+        // k lanes have seen a value that large (then about 64 ln(64 / (64 - k)) values pass in all), or a quarter of k
+        // in each of the four waves, which is a good third of what passes by their own bounds
+        uint32_t t;
+        if (shared) {
+          t = kth_of_lanes(rank_of(sum.m), (best.k + 3) / 4);
+          if (lane_id() == 0) shared[wave_id()] = t;
+          if (first) __syncthreads();
+          t = min(min(shared[0], shared[1]), min(shared[2], shared[3]));
+        } else {
+          t = kth_of_lanes(rank_of(sum.m), best.k);
+        }
+        least = max2(least, value_of(max(kLowest, t)));
 #pragma unroll
         for (int i = 0; i < N; i++) {
           const int at = column + (i / kVec<T>)*kWave * kVec<T> + i % kVec<T>;
-          best.offer(v[i] >= least, rank_key(v[i], (uint32_t)at));
+          best.offer(v[i] >= least, (uint64_t)__float_as_uint(v[i]) << 32 | (uint32_t)at);
         }
       }
     }
   }
 
-  // Batches b, b + step, ... of columns [from, to), the next one's values on their way; shared: the largest `least` of
-  // the workgroup's waves (as a rank), or null.
-  __device__ void run(const T* __restrict__ x, int64_t from, int64_t to, int b, int step, uint32_t* shared) {
+  // Batches b, b + step, ... of columns [from, to), the next one's values on their way.
+  __device__ void run(const T* __restrict__ x, int64_t from, int64_t to, int b, int step, volatile uint32_t* shared) {
     const int lane = lane_id();
+    bool first = true;
     raw4 r[U];
     int64_t at = from + (int64_t)b * kBatch;
     auto load = [&](int64_t where) {
@@ -336,9 +353,8 @@ struct Pass {
           load_tail(x + mine + u * kWave * kVec<T>, to - mine - u * kWave * kVec<T>, v + u * kVec<T>);
       }
       if (next + kBatch <= to) load(next);
-      if (TOP && shared) least = max2(least, value_of(max(rank_of(least), *(volatile uint32_t*)shared)));
-      values(v, (int)mine);
-      if (TOP && shared && lane == 0) atomicMax(shared, rank_of(least));
+      values(v, (int)mine, first, shared);
+      first = false;
       at = next;
     }
     sum.fold(c);
@@ -408,18 +424,19 @@ __global__ __launch_bounds__(256) void log_probs_block_kernel(const T* __restric
   __shared__ uint64_t lists[TOP ? 4 : 1][kWave];
   __shared__ float4 sums[4];
   __shared__ int counts[4];
-  __shared__ uint32_t least;
+  __shared__ uint32_t bounds[4];
   const int tid = threadIdx.x, wave = wave_id(), lane = lane_id();
   const int64_t row = blockIdx.x / (unsigned)splits;
   const int split = (int)(blockIdx.x - row * splits);
   const T* x = logits + row * stride;
   if constexpr (TOP) {
-    if (tid == 0) least = 0;
+    if (tid < 4) bounds[tid] = 0;
     __syncthreads();
   }
-  Pass<T, U, TOP> pass(c, TOP ? pool + wave * kPool : pool, o.topk);
-  const int64_t from = (int64_t)split * chunk;
-  pass.run(x, from, min((int64_t)cols, from + chunk), wave, 4, &least);
+  using P = Pass<T, U, TOP>;
+  P pass(c, TOP ? pool + wave * kPool : pool, o.topk);
+  const int64_t from = (int64_t)split * chunk, to = min((int64_t)cols, from + chunk);
+  pass.run(x, from, to, wave, 4, to - from > 3 * P::kBatch ? bounds : nullptr);
   if (lane == 0) {
     sums[wave] = pass.sum.packed();
     counts[wave] = pass.best.count;
@@ -430,11 +447,15 @@ __global__ __launch_bounds__(256) void log_probs_block_kernel(const T* __restric
   Sums sum = Sums::of(sums[0]);
 #pragma unroll
   for (int q = 1; q < 4; q++) sum.add(Sums::of(sums[q]), c);
-  Best& best = pass.best;
+  Best<true>& best = pass.best;
   if constexpr (TOP) {
-    const uint64_t from_least = (uint64_t)least << 32;
+    const uint32_t least = min(min(bounds[0], bounds[1]), min(bounds[2], bounds[3]));
 #pragma unroll
-    for (int q = 1; q < 4; q++) best.take(lists[q][lane], pool + q * kPool, counts[q], from_least);
+    for (int q = 1; q < 4; q++) {
+      Best<true> other(pool + q * kPool, o.topk);
+      other.count = counts[q];
+      best.take(lists[q][lane], other, least);
+    }
     best.finish();
   }
   const uint64_t list = best.list;
@@ -452,7 +473,8 @@ __global__ __launch_bounds__(256) void join_kernel(const T* __restrict__ logits,
                                                    float inv_t, int splits, Out o, const float4* __restrict__ part,
                                                    const uint64_t* __restrict__ part_keys) {
   __shared__ uint64_t pool[TOP ? 4 * kPool : 1];
-  __shared__ uint64_t lists[TOP ? 4 : 1][kWave], leasts[4];
+  __shared__ uint64_t lists[TOP ? 4 : 1][kWave];
+  __shared__ uint32_t leasts[4];
   __shared__ float4 sums[4];
   __shared__ int counts[4];
   const int tid = threadIdx.x, wave = wave_id(), lane = lane_id();
@@ -462,16 +484,16 @@ __global__ __launch_bounds__(256) void join_kernel(const T* __restrict__ logits,
     sum.add(Sums::of(part[row * splits + i]), c);
   }
   sum.fold(c);
-  Best best(TOP ? pool + wave * kPool : pool, o.topk);
+  Best<false> best(TOP ? pool + wave * kPool : pool, o.topk);
   if constexpr (TOP) {
     const uint64_t* keys = part_keys + row * splits * o.topk;
     // k of 64 chunks have a key with a rank that large
     const int head = wave * kWave + lane;
-    const uint64_t least = (uint64_t)kth_of_lanes(head < splits ? (uint32_t)(keys[(int64_t)head * o.topk] >> 32) : 0, o.topk) << 32;
+    const uint32_t least = kth_of_lanes(head < splits ? (uint32_t)(keys[(int64_t)head * o.topk] >> 32) : 0, o.topk);
     const int total = splits * o.topk;
     for (int i = wave * kWave; i < total; i += 256) {
       const uint64_t key = i + lane < total ? keys[i + lane] : 0;
-      best.offer(key && key >= least, key);
+      best.offer(key && (uint32_t)(key >> 32) >= least, key);
     }
     lists[wave][lane] = best.list;
     if (lane == 0) leasts[wave] = least;
@@ -486,9 +508,13 @@ __global__ __launch_bounds__(256) void join_kernel(const T* __restrict__ logits,
 #pragma unroll
   for (int q = 1; q < 4; q++) sum.add(Sums::of(sums[q]), c);
   if constexpr (TOP) {
-    const uint64_t least = umax64(umax64(leasts[0], leasts[1]), umax64(leasts[2], leasts[3]));
+    const uint32_t least = max(max(leasts[0], leasts[1]), max(leasts[2], leasts[3]));
 #pragma unroll
-    for (int q = 1; q < 4; q++) best.take(lists[q][lane], pool + q * kPool, counts[q], least);
+    for (int q = 1; q < 4; q++) {
+      Best<false> other(pool + q * kPool, o.topk);
+      other.count = counts[q];
+      best.take(lists[q][lane], other, least);
+    }
     best.finish();
   }
   const uint64_t list = best.list;
@@ -630,7 +656,7 @@ constexpr int64_t kStep = 4096;  // columns: one batch of each of a workgroup's 
 Plan plan_of(int64_t rows, int64_t cols) {
   if (cols <= 1024 || (rows >= 4096 && cols <= 8192)) return {true, 1, cols};
   const int64_t most = (cols + kStep - 1) / kStep;
-  const int64_t want = std::min<int64_t>(std::min<int64_t>(most, 1024), (2048 + rows - 1) / rows);
+  const int64_t want = std::min<int64_t>(most, std::max<int64_t>(1, 1024 / rows));
   const int64_t steps = (most + want - 1) / want;
   return {false, (int)((most + steps - 1) / steps), steps * kStep};
 }

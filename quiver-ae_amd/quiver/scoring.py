@@ -18,48 +18,50 @@ falls back to torch.
 """
 from __future__ import annotations
 
-from dataclasses import dataclass
+from dataclasses import dataclass, replace
 
 import torch
 
 from . import _lib
 
 _TYPES = {torch.float32: _lib.QV_FLOAT, torch.bfloat16: _lib.QV_BFLOAT16, torch.float16: _lib.QV_FLOAT16}
+_CODES = (torch.int8,)
+
+# These calls take a few microseconds on the GPU for a small batch, so the checks
+# below avoid what torch's Python layer is slow at (device objects, stream objects,
+# repeated shapes).
+_raw_stream = torch._C._cuda_getCurrentRawStream
 
 
 def _device(*tensors: torch.Tensor) -> int:
     """The one GPU that every tensor is on."""
-    index = None
+    index = tensors[0].get_device()
     for t in tensors:
-        if not t.is_cuda:
-            raise ValueError("tensors must be on the GPU")
-        if index is None:
-            index = t.get_device()
-        elif t.get_device() != index:
+        if t.get_device() != index:
             raise ValueError("tensors must be on one GPU")
+    if index < 0:
+        raise ValueError("tensors must be on the GPU")
     return index
 
 
-def _stream(device: int) -> int:
-    return torch.cuda.current_stream(device).cuda_stream
-
-
-def _matrix(name: str, t: torch.Tensor, types) -> int:
-    """Checks a row-major matrix; its row stride."""
+def _matrix(name: str, t: torch.Tensor, types) -> tuple[int, int, int]:
+    """Checks a row-major matrix; its rows, columns and row stride."""
     if t.dtype not in types:
         raise ValueError(f"{name} has the type {t.dtype}; " + " or ".join(str(x) for x in types) + " is needed")
-    if t.dim() != 2:
+    shape = t.shape
+    if len(shape) != 2:
         raise ValueError(f"{name} must have two dimensions")
-    rows, cols = t.shape
-    if cols > 1 and t.stride(1) != 1:
+    rows, cols = shape
+    stride, step = t.stride()
+    if step != 1 and cols > 1:
         raise ValueError(f"{name} must be contiguous along its rows")
     # one row, or none, has no stride of its own
-    return t.stride(0) if rows > 1 else max(cols, 1)
+    return rows, cols, stride if rows > 1 else max(cols, 1)
 
 
-def _vector(name: str, t: torch.Tensor, shape, dtype=torch.float32) -> int:
-    if t.dtype != dtype or tuple(t.shape) != tuple(shape) or not t.is_contiguous():
-        raise ValueError(f"{name} must be a contiguous {dtype} tensor of shape {tuple(shape)}")
+def _vector(name: str, t: torch.Tensor, shape: tuple, dtype=torch.float32) -> int:
+    if t.dtype != dtype or t.shape != shape or not t.is_contiguous():
+        raise ValueError(f"{name} must be a contiguous {dtype} tensor of shape {shape}")
     return t.data_ptr()
 
 
@@ -70,19 +72,18 @@ def quantize_rows(x: torch.Tensor, *, out: tuple[torch.Tensor, torch.Tensor] | N
     number, halves to even.  A row of zeros (below 2^-119) has the scale 0, a
     row with an infinity or a NaN the scale NaN and zero codes.
     """
-    stride = _matrix("x", x, _TYPES)
-    n, d = x.shape
+    n, d, stride = _matrix("x", x, _TYPES)
     if out is None:
         out = (torch.empty((n, d), dtype=torch.int8, device=x.device),
                torch.empty(n, dtype=torch.float32, device=x.device))
     codes, scales = out
-    code_stride = _matrix("codes", codes, (torch.int8,))
-    if codes.shape != x.shape:
+    code_rows, code_cols, code_stride = _matrix("codes", codes, _CODES)
+    if code_rows != n or code_cols != d:
         raise ValueError("codes and x differ in shape")
     at = _vector("scales", scales, (n,))
     device = _device(x, codes, scales)
     _lib.check(_lib.load().qv_quantize_rows(x.data_ptr(), _TYPES[x.dtype], n, d, stride, codes.data_ptr(), code_stride,
-                                            at, device, _stream(device)))
+                                            at, device, _raw_stream(device)))
     return out
 
 
@@ -94,30 +95,28 @@ def int8_product(a: torch.Tensor, a_scales: torch.Tensor, b: torch.Tensor, b_sca
     The sums are exact; the rest is fp32, rounded once to ``dtype``.  A bias of
     -inf takes a column out of ``log_probs``.
     """
-    a_stride, b_stride = _matrix("a", a, (torch.int8,)), _matrix("b", b, (torch.int8,))
-    (m, k), n = a.shape, b.shape[0]
-    if b.shape[1] != k:
+    m, k, a_stride = _matrix("a", a, _CODES)
+    n, k_b, b_stride = _matrix("b", b, _CODES)
+    if k_b != k:
         raise ValueError("a and b differ in the length of their rows")
     if out is None:
         if dtype not in _TYPES:
             raise ValueError("dtype must be float32, bfloat16 or float16")
         out = torch.empty((m, n), dtype=dtype, device=a.device)
-    out_stride = _matrix("out", out, _TYPES)
-    if tuple(out.shape) != (m, n):
+    out_rows, out_cols, out_stride = _matrix("out", out, _TYPES)
+    if out_rows != m or out_cols != n:
         raise ValueError(f"out must have the shape {(m, n)}")
     at_a, at_b = _vector("a_scales", a_scales, (m,)), _vector("b_scales", b_scales, (n,))
-    tensors = [a, a_scales, b, b_scales, out]
-    at_bias = None
-    if bias is not None:
-        at_bias = _vector("bias", bias, (n,))
-        tensors.append(bias)
-    device = _device(*tensors)
+    if bias is None:
+        at_bias, device = None, _device(a, a_scales, b, b_scales, out)
+    else:
+        at_bias, device = _vector("bias", bias, (n,)), _device(a, a_scales, b, b_scales, out, bias)
     _lib.check(_lib.load().qv_int8_product(a.data_ptr(), a_stride, at_a, m, b.data_ptr(), b_stride, at_b, at_bias, n, k,
-                                           out.data_ptr(), _TYPES[out.dtype], out_stride, device, _stream(device)))
+                                           out.data_ptr(), _TYPES[out.dtype], out_stride, device, _raw_stream(device)))
     return out
 
 
-@dataclass
+@dataclass(frozen=True, eq=False)
 class LogProbs:
     """What ``log_probs`` gives; ``stats`` is what its gradient needs again."""
 
@@ -129,45 +128,58 @@ class LogProbs:
     stats: torch.Tensor      # [n, 2] largest logit, ln of the sum of exp((x - it) / temperature)
     temperature: float
     _workspace: torch.Tensor
+    _device: int
+    _at: tuple               # the buffers' addresses, in the order above
+
+    @staticmethod
+    def empty(n: int, v: int, t: int, k: int, temperature: float, device: torch.device) -> "LogProbs":
+        """Buffers for ``log_probs`` of n rows of v columns with t targets and k alternatives."""
+        if not 0 <= k <= _lib.QV_LOG_PROBS_MAX_TOPK:
+            raise ValueError(f"top_k must be in [0, {_lib.QV_LOG_PROBS_MAX_TOPK}]")
+        if t > _lib.QV_LOG_PROBS_MAX_TARGETS:
+            raise ValueError(f"at most {_lib.QV_LOG_PROBS_MAX_TARGETS} targets per row")
+        if device.type != "cuda":
+            raise ValueError("tensors must be on the GPU")
+
+        def new(*shape, dtype=torch.float32):
+            return torch.empty(shape, dtype=dtype, device=device)
+
+        return LogProbs.of(new(n, t), new(n), new(n), new(n, k, dtype=torch.int32), new(n, k), new(n, 2), temperature,
+                           new(_lib.load().qv_log_probs_workspace(n, v, k), dtype=torch.uint8))
+
+    @staticmethod
+    def of(target, entropy, logsumexp, top_ids, top, stats, temperature, workspace) -> "LogProbs":
+        parts = (target, entropy, logsumexp, top_ids, top, stats, workspace)
+        return LogProbs(target, entropy, logsumexp, top_ids, top, stats, temperature, workspace, stats.get_device(),
+                        tuple(p.data_ptr() for p in parts))
 
 
 def _given(targets: torch.Tensor | None, rows: int) -> tuple[int | None, int]:
     """(address, columns per row) of int32 targets [n, t] or [n]."""
     if targets is None:
         return None, 0
-    per_row = targets.shape[1] if targets.dim() == 2 else 1
-    shape = (rows, per_row) if targets.dim() == 2 else (rows,)
-    return _vector("targets", targets, shape, torch.int32), per_row
+    shape = targets.shape
+    per_row = shape[1] if len(shape) == 2 else 1
+    return _vector("targets", targets, (rows, per_row) if len(shape) == 2 else (rows,), torch.int32), per_row
 
 
 def _forward(logits, targets, top_k, temperature, out) -> LogProbs:
-    stride = _matrix("logits", logits, _TYPES)
-    n, v = logits.shape
+    n, v, stride = _matrix("logits", logits, _TYPES)
     at_targets, t = _given(targets, n)
     temperature = float(temperature)
-    lib = _lib.load()
     if out is None:
-        if not 0 <= top_k <= _lib.QV_LOG_PROBS_MAX_TOPK:
-            raise ValueError(f"top_k must be in [0, {_lib.QV_LOG_PROBS_MAX_TOPK}]")
-        if t > _lib.QV_LOG_PROBS_MAX_TARGETS:
-            raise ValueError(f"at most {_lib.QV_LOG_PROBS_MAX_TARGETS} targets per row")
-
-        def empty(*shape, dtype=torch.float32):
-            return torch.empty(shape, dtype=dtype, device=logits.device)
-
-        out = LogProbs(empty(n, t), empty(n), empty(n), empty(n, top_k, dtype=torch.int32), empty(n, top_k),
-                       empty(n, 2), temperature,
-                       empty(lib.qv_log_probs_workspace(n, v, top_k), dtype=torch.uint8))
-    out.temperature = temperature
-    at_target, at_top = _vector("out.target", out.target, (n, t)), _vector("out.top", out.top, (n, top_k))
-    at_ids = _vector("out.top_ids", out.top_ids, (n, top_k), torch.int32)
-    at_entropy, at_lse = _vector("out.entropy", out.entropy, (n,)), _vector("out.logsumexp", out.logsumexp, (n,))
-    at_stats = _vector("out.stats", out.stats, (n, 2))
-    device = _device(logits, out.target, out.entropy, out.logsumexp, out.top, out.top_ids, out.stats, out._workspace,
-                     *(() if targets is None else (targets,)))
-    _lib.check(lib.qv_log_probs(logits.data_ptr(), _TYPES[logits.dtype], n, v, stride, temperature, at_targets, t,
-                                top_k, at_target, at_entropy, at_lse, at_stats, at_ids, at_top,
-                                out._workspace.data_ptr(), out._workspace.numel(), device, _stream(device)))
+        out = LogProbs.empty(n, v, t, top_k, temperature, logits.device)
+    elif out.target.shape != (n, t) or out.top.shape != (n, top_k):
+        raise ValueError("out was made for another number of rows, targets or alternatives")
+    elif out.temperature != temperature:
+        out = replace(out, temperature=temperature)
+    device = _device(logits) if targets is None else _device(logits, targets)
+    if device != out._device:
+        raise ValueError("tensors must be on one GPU")
+    at_target, at_entropy, at_lse, at_ids, at_top, at_stats, at_work = out._at
+    _lib.check(_lib.load().qv_log_probs(logits.data_ptr(), _TYPES[logits.dtype], n, v, stride, temperature, at_targets,
+                                        t, top_k, at_target, at_entropy, at_lse, at_stats, at_ids, at_top, at_work,
+                                        out._workspace.shape[0], device, _raw_stream(device)))
     return out
 
 
@@ -188,8 +200,9 @@ class _LogProbsFunction(torch.autograd.Function):
         def plain(g):
             return None if g is None else g.contiguous()
 
-        grad = _gradient(logits, stats, entropy, top_ids, ctx.temperature, targets, plain(g_target),
-                         plain(g_entropy), plain(g_lse), plain(g_top), None)
+        grad = _gradient(logits, stats.data_ptr(), entropy.data_ptr(), top_ids.data_ptr(), top_ids.shape[1],
+                         logits.get_device(), ctx.temperature, targets, plain(g_target), plain(g_entropy), plain(g_lse),
+                         plain(g_top), None)
         return grad, None, None, None
 
 
@@ -210,34 +223,36 @@ def log_probs(logits: torch.Tensor, targets: torch.Tensor | None = None, *, top_
             raise ValueError("out= cannot be given for logits that require a gradient")
         target, entropy, lse, ids, top, stats, workspace = _LogProbsFunction.apply(logits, targets, top_k,
                                                                                   float(temperature))
-        return LogProbs(target, entropy, lse, ids, top, stats, float(temperature), workspace)
+        return LogProbs.of(target, entropy, lse, ids, top, stats, float(temperature), workspace)
     return _forward(logits, targets, top_k, temperature, out)
 
 
-def _gradient(logits, stats, entropy, top_ids, temperature, targets, g_target, g_entropy, g_lse, g_top, out):
-    stride = _matrix("logits", logits, _TYPES)
-    n, v = logits.shape
+def _gradient(logits, at_stats, at_entropy, at_ids, k, device, temperature, targets, g_target, g_entropy, g_lse, g_top,
+              out):
+    n, v, stride = _matrix("logits", logits, _TYPES)
     at_targets, t = _given(targets, n)
-    k = top_ids.shape[1]
     if out is None:
         out = torch.empty((n, v), dtype=logits.dtype, device=logits.device)
-    out_stride = _matrix("out", out, (logits.dtype,))
-    if out.shape != logits.shape:
+    out_rows, out_cols, out_stride = _matrix("out", out, (logits.dtype,))
+    if out_rows != n or out_cols != v:
         raise ValueError("out and logits differ in shape")
-    at_stats, at_entropy = _vector("stats", stats, (n, 2)), _vector("entropy", entropy, (n,))
-    at_ids = _vector("top_ids", top_ids, (n, k), torch.int32)
-    tensors, given = [logits, out, stats, entropy, top_ids], []
+    tensors = [logits, out]
     if targets is not None:
         tensors.append(targets)
-    for name, g, shape in (("grad_target", g_target, (n, t)), ("grad_entropy", g_entropy, (n,)),
-                           ("grad_logsumexp", g_lse, (n,)), ("grad_top", g_top, (n, k))):
-        given.append(None if g is None else _vector(name, g, shape))
-        if g is not None:
-            tensors.append(g)
-    device = _device(*tensors)
+
+    def given(name, g, shape):
+        if g is None:
+            return None
+        tensors.append(g)
+        return _vector(name, g, shape)
+
+    at = (given("grad_target", g_target, (n, t)), given("grad_entropy", g_entropy, (n,)),
+          given("grad_logsumexp", g_lse, (n,)), given("grad_top", g_top, (n, k)))
+    if _device(*tensors) != device:
+        raise ValueError("tensors must be on one GPU")
     _lib.check(_lib.load().qv_log_probs_grad(logits.data_ptr(), _TYPES[logits.dtype], n, v, stride, temperature,
-                                             at_stats, at_entropy, at_targets, t, at_ids, k, *given, out.data_ptr(),
-                                             out_stride, device, _stream(device)))
+                                             at_stats, at_entropy, at_targets, t, at_ids, k, *at, out.data_ptr(),
+                                             out_stride, device, _raw_stream(device)))
     return out
 
 
@@ -250,8 +265,11 @@ def log_probs_grad(logits: torch.Tensor, result: LogProbs, targets: torch.Tensor
     ``result`` and ``targets`` as they were for ``log_probs``; ``out`` may be
     the logits themselves.  What autograd runs, for training loops without it.
     """
-    return _gradient(logits, result.stats, result.entropy, result.top_ids, result.temperature, targets, grad_target,
-                     grad_entropy, grad_logsumexp, grad_top, out)
+    if result.entropy.shape[0] != logits.shape[0]:
+        raise ValueError("result was made for another number of rows")
+    _, at_entropy, _, at_ids, _, at_stats, _ = result._at
+    return _gradient(logits, at_stats, at_entropy, at_ids, result.top.shape[1], result._device, result.temperature,
+                     targets, grad_target, grad_entropy, grad_logsumexp, grad_top, out)
 
 
 class DenseCatalogue:
@@ -299,4 +317,4 @@ class DenseCatalogue:
                                    temperature=temperature))
         joined = [torch.cat([getattr(p, f) for p in parts])
                   for f in ("target", "entropy", "logsumexp", "top_ids", "top", "stats")]
-        return LogProbs(*joined, float(temperature), parts[-1]._workspace)
+        return LogProbs.of(*joined, float(temperature), parts[-1]._workspace)
