@@ -97,6 +97,28 @@ __device__ __forceinline__ float max3(float a, float b, float c) {
   return r;
 }
 
+// A commutative f folded over the wave, the same in every lane: neighbours 1, 2, 4 and 8
+// apart by DPP (within quads, then the mirrored half row and the rotated row, whose lanes
+// agree by then), 16 and 32 by the permlane swaps.
+template <class F>
+__device__ __forceinline__ float wave_fold(float v, F f) {
+  auto dpp = [&](auto control) {
+    constexpr int kControl = decltype(control)::value;
+    v = f(v, __uint_as_float((uint32_t)__builtin_amdgcn_mov_dpp((int)__float_as_uint(v), kControl, 0xF, 0xF, true)));
+  };
+  dpp(std::integral_constant<int, 0xB1>());   // quad_perm [1,0,3,2]
+  dpp(std::integral_constant<int, 0x4E>());   // quad_perm [2,3,0,1]
+  dpp(std::integral_constant<int, 0x141>());  // row_half_mirror
+  dpp(std::integral_constant<int, 0x128>());  // row_ror:8
+  const auto p = __builtin_amdgcn_permlane16_swap(__float_as_uint(v), __float_as_uint(v), false, false);
+  v = f(__uint_as_float(p[0]), __uint_as_float(p[1]));
+  const auto q = __builtin_amdgcn_permlane32_swap(__float_as_uint(v), __float_as_uint(v), false, false);
+  return f(__uint_as_float(q[0]), __uint_as_float(q[1]));
+}
+__device__ __forceinline__ float wave_sum(float v) {
+  return wave_fold(v, [](float a, float b) { return a + b; });
+}
+
 // ---- keys of the alternatives --------------------------------------------------
 
 // Orders as the values do, larger first by larger key, equal values (the two
@@ -146,7 +168,10 @@ __device__ __forceinline__ uint64_t sort_desc(uint64_t key, int count) {
   if (count > 40) return wave_sort_desc(key);
   const int lane = lane_id();
   int place = 0;
-  for (int l = 0; l < count; l++) place += read_lane_u64(key, l) > key ? 1 : 0;
+  for (int l = 0; l < count; l += 4) {  // (what it counts past `count` are zeros)
+#pragma unroll
+    for (int e = 0; e < 4; e++) place += read_lane_u64(key, l + e) > key ? 1 : 0;
+  }
   const int to = (lane < count ? place : lane) << 2;
   return ((uint64_t)(uint32_t)__builtin_amdgcn_ds_permute(to, (int)(uint32_t)(key >> 32)) << 32) |
          (uint32_t)__builtin_amdgcn_ds_permute(to, (int)(uint32_t)key);
@@ -247,15 +272,9 @@ struct Sums {
   }
   // Over the wave, in a fixed order, the same in every lane.
   __device__ __forceinline__ void fold(float c) {
-    float to = m;
-#pragma unroll
-    for (int x = 1; x < kWave; x *= 2) to = max2(to, __shfl_xor(to, x));
-    move(to, c);
-#pragma unroll
-    for (int x = 1; x < kWave; x *= 2) {
-      s = s + __shfl_xor(s, x);
-      w = w + __shfl_xor(w, x);
-    }
+    move(wave_fold(m, [](float a, float b) { return max2(a, b); }), c);
+    s = wave_sum(s);
+    w = wave_sum(w);
   }
 };
 
@@ -273,16 +292,15 @@ struct Pass {
   __device__ Pass(float c_, uint64_t* pool, int k) : c(c_), best(pool, k) {}
 
   // `shared`: the four waves' bounds when all of them have batches (ranks), or null.
-  __device__ __forceinline__ void values(const float (&v)[N], int column, bool first, volatile uint32_t* shared) {
-    float top;
-    if constexpr (N == 16) {
-      top = max3(max3(v[0], v[1], v[2]), max3(v[3], v[4], v[5]), max3(v[6], v[7], v[8]));
-      top = max3(top, max3(v[9], v[10], v[11]), max3(v[12], v[13], max2(v[14], v[15])));
-    } else {
-      top = max2(v[0], v[1]);
+  __device__ __forceinline__ void values(const float (&v)[N], int column, int turn, volatile uint32_t* shared) {
+    constexpr int kGroup = 4;
+    float part[N / kGroup], top;
 #pragma unroll
-      for (int i = 2; i < N; i += 2) top = max3(top, v[i], v[i + 1]);
-    }
+    for (int g = 0; g < N / kGroup; g++)
+      part[g] = max2(max3(v[kGroup * g], v[kGroup * g + 1], v[kGroup * g + 2]), v[kGroup * g + 3]);
+    if constexpr (N == 4) top = part[0];
+    else if constexpr (N == 8) top = max2(part[0], part[1]);
+    else top = max2(max3(part[0], part[1], part[2]), part[3]);
     if (__any(top > sum.m)) {
       sum.move(max2(sum.m, top), c);
       mc = scaled(sum.m, c);
@@ -308,23 +326,30 @@ struct Pass {
     sum.s = sum.s + s;
     sum.w = sum.w + w;
     if constexpr (TOP) {
-      if (first || __any(top >= least)) {
+      if (turn == 0 || __any(top >= least)) {
         // k lanes have seen a value that large (then about 64 ln(64 / (64 - k)) values pass in all), or a quarter of k
-        // in each of the four waves, which is a good third of what passes by their own bounds
-        uint32_t t;
-        if (shared) {
-          t = kth_of_lanes(rank_of(sum.m), (best.k + 3) / 4);
-          if (lane_id() == 0) shared[wave_id()] = t;
-          if (first) __syncthreads();
-          t = min(min(shared[0], shared[1]), min(shared[2], shared[3]));
-        } else {
-          t = kth_of_lanes(rank_of(sum.m), best.k);
+        // in each of the four waves, which is a good third of what passes by their own bounds; renewed in turns 0, 1,
+        // 3, 7, ...
+        if ((turn & (turn + 1)) == 0) {
+          uint32_t t;
+          if (shared) {
+            t = kth_of_lanes(rank_of(sum.m), (best.k + 3) / 4);
+            if (lane_id() == 0) shared[wave_id()] = t;
+            if (turn == 0) __syncthreads();
+            t = min(min(shared[0], shared[1]), min(shared[2], shared[3]));
+          } else {
+            t = kth_of_lanes(rank_of(sum.m), best.k);
+          }
+          least = max2(least, value_of(max(kLowest, t)));
         }
-        least = max2(least, value_of(max(kLowest, t)));
 #pragma unroll
-        for (int i = 0; i < N; i++) {
-          const int at = column + (i / kVec<T>)*kWave * kVec<T> + i % kVec<T>;
-          best.offer(v[i] >= least, (uint64_t)__float_as_uint(v[i]) << 32 | (uint32_t)at);
+        for (int g = 0; g < N / kGroup; g++) {
+          if (!__any(part[g] >= least)) continue;
+#pragma unroll
+          for (int i = kGroup * g; i < kGroup * (g + 1); i++) {
+            const int at = column + (i / kVec<T>)*kWave * kVec<T> + i % kVec<T>;
+            best.offer(v[i] >= least, (uint64_t)__float_as_uint(v[i]) << 32 | (uint32_t)at);
+          }
         }
       }
     }
@@ -333,7 +358,7 @@ struct Pass {
   // Batches b, b + step, ... of columns [from, to), the next one's values on their way.
   __device__ void run(const T* __restrict__ x, int64_t from, int64_t to, int b, int step, volatile uint32_t* shared) {
     const int lane = lane_id();
-    bool first = true;
+    int turn = 0;
     raw4 r[U];
     int64_t at = from + (int64_t)b * kBatch;
     auto load = [&](int64_t where) {
@@ -353,8 +378,7 @@ struct Pass {
           load_tail(x + mine + u * kWave * kVec<T>, to - mine - u * kWave * kVec<T>, v + u * kVec<T>);
       }
       if (next + kBatch <= to) load(next);
-      values(v, (int)mine, first, shared);
-      first = false;
+      values(v, (int)mine, turn++, shared);
       at = next;
     }
     sum.fold(c);
@@ -565,10 +589,7 @@ __global__ __launch_bounds__(256) void log_probs_grad_kernel(const T* logits, in
     weight[h] = t ? g.g_target[at] : g.g_top[at];
     if (id[h] >= 0) total = total + weight[h];
   }
-  if (named) {
-#pragma unroll
-    for (int q = 1; q < kWave; q *= 2) total = total + __shfl_xor(total, q);
-  }
+  if (named) total = wave_sum(total);
   if (g.g_lse) total = total - g.g_lse[row];
   const float ge = g.g_entropy ? g.g_entropy[row] : 0.f, h = g.g_entropy ? g.entropy[row] : 0.f;
   const float nan = __builtin_nanf("");
