@@ -519,16 +519,16 @@ __global__ __launch_bounds__(64 * WM * WN, 1) void product_deep_kernel(Product<O
 // ring of two lines in LDS in which an element's place follows its address: a line is
 // written whole as soon as its last column is there, and only the first and the last
 // one of a walk are written in parts.
-template <int KS, class O>
+template <int KS, bool BIAS, class O>
 __global__ __launch_bounds__(256, KS == 4 ? 3 : 2) void product_panel_kernel(Product<O> p, int64_t panels, int64_t tiles_n,
                                                                int64_t slices) {
   constexpr int PC = 2 * KS, kRow = 32 * KS, L = 64 * PC / 256, kRows = 256 / PC;
   constexpr int S = (int)sizeof(O), E = 128 / S, V = 16 / S;   // elements of a line, of 16 bytes
   constexpr int kRing = 256, Y = E / 32;  // bytes of a row's ring; 32-column results to a line
   __shared__ __align__(16) char lds[2][64 * kRow];
-  __shared__ __align__(16) char rings[4][32 * kRing];
+  __shared__ __align__(256) char rings[4][32 * kRing];
   __shared__ __align__(16) float sa[128];
-  __shared__ float sb[2][2][64];  // a tile's scales and biases
+  __shared__ float sb[2][BIAS ? 2 : 1][64];  // a tile's scales and biases
   const int tid = threadIdx.x, wave = wave_id(), lane = lane_id(), row = lane % 32, half = lane / 32;
   const int64_t t = tile_of_block(blockIdx.x, panels * slices), slice = t / panels, i0 = (t - slice * panels) * 128;
   const int64_t first = tiles_n * slice / slices, end = tiles_n * (slice + 1) / slices;
@@ -536,8 +536,8 @@ __global__ __launch_bounds__(256, KS == 4 ? 3 : 2) void product_panel_kernel(Pro
   auto swap = [](int r) { return KS == 4 ? r / 2 & 7 : r & 15; };  // as in the tiles, for rows of 128 or 256 bytes
   i4 rb[L];
   float rs = 0.f;
-  const bool scales = tid < 128 && (tid < 64 || p.bias);
-  const float* scale_of = tid < 64 ? p.b_scales : p.bias;
+  const bool scales = tid < (BIAS ? 128 : 64);
+  const float* scale_of = !BIAS || tid < 64 ? p.b_scales : p.bias;
   auto load = [&](int64_t tile) {
     const int8_t* b = p.b + tile * 64 * p.b_stride;
     const int last = (int)min(p.n - 1 - tile * 64, (int64_t)63);
@@ -551,7 +551,7 @@ __global__ __launch_bounds__(256, KS == 4 ? 3 : 2) void product_panel_kernel(Pro
       const int r = r0 + q * kRows;
       *reinterpret_cast<i4*>(lds[buffer] + r * kRow + (piece ^ swap(r)) * 16) = rb[q];
     }
-    if (tid < 128) sb[buffer][tid / 64][tid % 64] = scales ? rs : -0.f;  // x + -0 is x
+    if (scales) sb[buffer][tid / 64][tid % 64] = rs;
   };
   load(first);
   const int64_t it = i0 + wave * 32;  // the wave's rows
@@ -571,7 +571,8 @@ __global__ __launch_bounds__(256, KS == 4 ? 3 : 2) void product_panel_kernel(Pro
   char* ring = rings[wave];
   // where the columns of a line go in the ring, register 4 g + e of result y; those of the next line
   // half a ring on
-  int place[Y][16];
+  uint32_t place[Y][16];
+  typedef __attribute__((address_space(3))) O lds_o;
 #pragma unroll
   for (int g = 0; g < 4; g++)
 #pragma unroll
@@ -579,7 +580,7 @@ __global__ __launch_bounds__(256, KS == 4 ? 3 : 2) void product_panel_kernel(Pro
 #pragma unroll
       for (int y = 0; y < Y; y++) {
         const int at = (int)(first & 1) * 64 + 32 * y + row + shift(8 * g + 4 * half + e);
-        place[y][4 * g + e] = 4 * half * kRing + (at * S & (kRing - 1));
+        place[y][4 * g + e] = lds_addr(ring) + 4 * half * kRing + (at * S & (kRing - 1));
       }
   // lines as they leave: 8 lanes a line, 8 rows at once
   constexpr int G = 4;
@@ -654,18 +655,37 @@ __global__ __launch_bounds__(256, KS == 4 ? 3 : 2) void product_panel_kernel(Pro
       for (int y = 0; y < Y; y++) {
         const int j = (l * Y + y) * 32 + row;
         scale[y] = sb[buffer][0][j];
-        add[y] = sb[buffer][1][j];
+        add[y] = BIAS ? sb[buffer][BIAS][j] : 0.f;
       }
 #pragma unroll
       for (int g = 0; g < 4; g++) {
         const f4 s = *reinterpret_cast<const f4*>(sa + wave * 32 + 8 * g + 4 * half);
 #pragma unroll
-        for (int e = 0; e < 4; e++)
+        for (int e = 0; e < 4; e += 2)
 #pragma unroll
           for (int y = 0; y < Y; y++) {
-            const float x = ((float)acc[l * Y + y][4 * g + e] * s[e]) * scale[y] + add[y];
-            *reinterpret_cast<O*>(ring + place[y][4 * g + e] + (8 * g + e) * kRing) = (O)x;
-            place[y][4 * g + e] ^= 128;
+            typedef float f2 __attribute__((ext_vector_type(2)));
+            typedef O o2 __attribute__((ext_vector_type(2)));
+            f2 x;
+#pragma unroll
+            for (int d = 0; d < 2; d++) {
+              x[d] = ((float)acc[l * Y + y][4 * g + e + d] * s[e + d]) * scale[y];
+              if constexpr (BIAS) x[d] = x[d] + add[y];
+            }
+            o2 out;
+            if constexpr (std::is_same<O, bf16>::value) {  // two at once, which the compiler takes apart
+              uint32_t both;
+              asm("v_cvt_pk_bf16_f32 %0, %1, %2" : "=v"(both) : "v"(x[0]), "v"(x[1]));
+              out = __builtin_bit_cast(o2, both);
+            } else {
+              out = __builtin_convertvector(x, o2);
+            }
+#pragma unroll
+            for (int d = 0; d < 2; d++) {
+              uint32_t& at = place[y][4 * g + e + d];
+              ((lds_o*)(uintptr_t)at)[(8 * g + e + d) * kRing / S] = out[d];
+              at ^= 128;
+            }
           }
       }
       __builtin_amdgcn_fence(__ATOMIC_ACQ_REL, "wavefront");
@@ -829,8 +849,8 @@ void launch_panels(const Product<O>& p, hipStream_t st) {
   const int64_t panels = (p.m + 127) / 128, tiles_n = (p.n + 63) / 64;
   // as many workgroups as run at once, each with a like share of b's tiles
   const int64_t slices = std::min(tiles_n, std::max<int64_t>(1, 256 * (KS == 4 ? 3 : 2) / panels));
-  hipLaunchKernelGGL((product_panel_kernel<KS, O>), dim3((unsigned)(panels * slices)), dim3(256), 0, st, p, panels,
-                     tiles_n, slices);
+  auto* kernel = p.bias ? product_panel_kernel<KS, true, O> : product_panel_kernel<KS, false, O>;
+  hipLaunchKernelGGL(kernel, dim3((unsigned)(panels * slices)), dim3(256), 0, st, p, panels, tiles_n, slices);
   HIP_OK(hipGetLastError());
 }
 
