@@ -393,10 +393,24 @@ struct Out {
   float* top;
 };
 
-// A row's results from its sums (in every lane) and its list, by one wave.
+// A lane's given column and its logit, asked for before the row's pass.
+struct Given {
+  int32_t column = -1;
+  float logit = 0.f;
+};
 template <class T>
-__device__ __forceinline__ void finish_row(const T* __restrict__ x, int64_t row, int cols, const Sums& sum,
-                                           uint64_t list, float c, float inv_t, const Out& o) {
+__device__ __forceinline__ Given given_of(const T* __restrict__ x, int64_t row, int cols, const Out& o) {
+  Given g;
+  if (lane_id() < o.per_row) {
+    g.column = o.targets[row * o.per_row + lane_id()];
+    if (g.column >= 0 && g.column < cols) g.logit = (float)x[g.column];
+  }
+  return g;
+}
+
+// A row's results from its sums (in every lane) and its list, by one wave.
+__device__ __forceinline__ void finish_row(const Given& given, int64_t row, int cols, const Sums& sum, uint64_t list,
+                                           float c, float inv_t, const Out& o) {
   const int lane = lane_id();
   const bool odd = sum.s != sum.s, empty = sum.s == 0.f;
   const float nan = __builtin_nanf("");
@@ -412,8 +426,8 @@ __device__ __forceinline__ void finish_row(const T* __restrict__ x, int64_t row,
     o.stats[2 * row + 1] = ln_s;
   }
   if (lane < o.per_row) {
-    const int32_t j = o.targets[row * o.per_row + lane];
-    o.target[row * o.per_row + lane] = j < 0 ? 0.f : j >= cols ? nan : lp((float)x[j]);
+    const int32_t j = given.column;
+    o.target[row * o.per_row + lane] = j < 0 ? 0.f : j >= cols ? nan : lp(given.logit);
   }
   if (lane < o.topk) {
     const bool none = odd || list == 0;
@@ -431,10 +445,11 @@ __global__ __launch_bounds__(256) void log_probs_wave_kernel(const T* __restrict
   const int64_t row = (int64_t)blockIdx.x * 4 + wave;
   if (row >= rows) return;
   const T* x = logits + row * stride;
+  const Given given = given_of(x, row, cols, o);
   Pass<T, U, TOP> pass(c, TOP ? pool + wave * kPool : pool, o.topk);
   pass.run(x, 0, cols, 0, 1, nullptr);
   if constexpr (TOP) pass.best.finish();
-  finish_row(x, row, cols, pass.sum, pass.best.list, c, inv_t, o);
+  finish_row(given, row, cols, pass.sum, pass.best.list, c, inv_t, o);
 }
 
 // One workgroup per chunk of a row.  With one chunk per row its results, else the
@@ -457,6 +472,8 @@ __global__ __launch_bounds__(256) void log_probs_block_kernel(const T* __restric
     if (tid < 4) bounds[tid] = 0;
     __syncthreads();
   }
+  Given given;
+  if (splits == 1 && wave == 0) given = given_of(x, row, cols, o);
   using P = Pass<T, U, TOP>;
   P pass(c, TOP ? pool + wave * kPool : pool, o.topk);
   const int64_t from = (int64_t)split * chunk, to = min((int64_t)cols, from + chunk);
@@ -484,7 +501,7 @@ __global__ __launch_bounds__(256) void log_probs_block_kernel(const T* __restric
   }
   const uint64_t list = best.list;
   if (splits == 1) {
-    finish_row(x, row, cols, sum, list, c, inv_t, o);
+    finish_row(given, row, cols, sum, list, c, inv_t, o);
   } else {
     if (lane == 0) part[blockIdx.x] = sum.packed();
     if (TOP && lane < o.topk) part_keys[(int64_t)blockIdx.x * o.topk + lane] = list;
@@ -503,6 +520,16 @@ __global__ __launch_bounds__(256) void join_kernel(const T* __restrict__ logits,
   __shared__ int counts[4];
   const int tid = threadIdx.x, wave = wave_id(), lane = lane_id();
   const int64_t row = blockIdx.x;
+  Given given;
+  if (wave == 0) given = given_of(logits + row * stride, row, cols, o);
+  // the first keys are asked for before the sums
+  const uint64_t* keys = TOP ? part_keys + row * splits * o.topk : nullptr;
+  const int head = wave * kWave + lane, total = splits * o.topk;
+  uint64_t of_chunk = 0, ahead = 0;
+  if constexpr (TOP) {
+    if (head < splits) of_chunk = keys[(int64_t)head * o.topk];
+    if (head < total) ahead = keys[head];
+  }
   Sums sum;
   for (int i = tid; i < splits; i += 256) {
     sum.add(Sums::of(part[row * splits + i]), c);
@@ -510,13 +537,11 @@ __global__ __launch_bounds__(256) void join_kernel(const T* __restrict__ logits,
   sum.fold(c);
   Best<false> best(TOP ? pool + wave * kPool : pool, o.topk);
   if constexpr (TOP) {
-    const uint64_t* keys = part_keys + row * splits * o.topk;
     // k of 64 chunks have a key with a rank that large
-    const int head = wave * kWave + lane;
-    const uint32_t least = kth_of_lanes(head < splits ? (uint32_t)(keys[(int64_t)head * o.topk] >> 32) : 0, o.topk);
-    const int total = splits * o.topk;
+    const uint32_t least = kth_of_lanes((uint32_t)(of_chunk >> 32), o.topk);
     for (int i = wave * kWave; i < total; i += 256) {
-      const uint64_t key = i + lane < total ? keys[i + lane] : 0;
+      const uint64_t key = ahead;
+      ahead = i + 256 + lane < total ? keys[i + 256 + lane] : 0;
       best.offer(key && (uint32_t)(key >> 32) >= least, key);
     }
     lists[wave][lane] = best.list;
@@ -542,7 +567,7 @@ __global__ __launch_bounds__(256) void join_kernel(const T* __restrict__ logits,
     best.finish();
   }
   const uint64_t list = best.list;
-  finish_row(logits + row * stride, row, cols, sum, list, c, inv_t, o);
+  finish_row(given, row, cols, sum, list, c, inv_t, o);
 }
 
 // ---- gradient ------------------------------------------------------------------
