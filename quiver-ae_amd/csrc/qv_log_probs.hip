@@ -219,18 +219,38 @@ struct Best {
     merge(waiting(lane_id(), count), count);
     count = 0;
   }
-  // Another wave's list and pool, of which only ranks from `least` on can matter.
-  __device__ __forceinline__ void take(uint64_t other_list, const Best& other, uint32_t least) {
-    if (__any(other_list != 0)) {
-      list = some ? merge_desc(list, other_list) : other_list;
-      some = true;
-    }
-    if (other.count) {
-      const uint64_t key = other.waiting(lane_id(), other.count);
-      offer(key && (uint32_t)(key >> 32) >= least, lane_id() < other.count ? other.pool[lane_id()] : 0);
-    }
+  // Puts what is left of the list and the pool, from rank `least` on, behind the other waves' in `all`.
+  __device__ __forceinline__ void hand_over(uint64_t* all, int* total, uint32_t least) const {
+    auto put = [&](uint64_t key) {
+      const bool take = key && (uint32_t)(key >> 32) >= least;
+      const uint64_t mask = __ballot(take);
+      if (mask == 0) return;
+      int at = 0;
+      if (lane_id() == 0) at = atomicAdd(total, __popcll(mask));
+      at = read_lane_i32(at, 0);
+      if (take) all[at + __builtin_amdgcn_mbcnt_hi((uint32_t)(mask >> 32), __builtin_amdgcn_mbcnt_lo((uint32_t)mask, 0))] = key;
+    };
+    if (some) put(list);
+    if (count) put(waiting(lane_id(), count));
   }
 };
+
+// The best of what W waves handed over, by one wave, whatever order it lies in.
+__device__ __forceinline__ uint64_t best_of(const uint64_t* all, int total, uint64_t* pool, int k) {
+  Best<false> best(pool, k);
+  for (int i = 0; i < total; i += kWave) {
+    const uint64_t key = i + lane_id() < total ? all[i + lane_id()] : 0;
+    best.offer(key != 0, key);
+  }
+  best.finish();
+  return best.list;
+}
+
+// The bound that a workgroup's waves give together, from one each that ceil(k / waves) of its values reach.
+__device__ __forceinline__ uint32_t common_bound(const volatile uint32_t* bounds, int waves, int k) {
+  const int share = (k + waves - 1) / waves;
+  return kth_of_lanes(lane_id() < waves ? bounds[lane_id()] : 0, (k + share - 1) / share);
+}
 
 // ---- sums ----------------------------------------------------------------------
 
@@ -291,8 +311,8 @@ struct Pass {
 
   __device__ Pass(float c_, uint64_t* pool, int k) : c(c_), best(pool, k) {}
 
-  // `shared`: the four waves' bounds when all of them have batches (ranks), or null.
-  __device__ __forceinline__ void values(const float (&v)[N], int column, int turn, volatile uint32_t* shared) {
+  // `shared`: the `waves` waves' bounds when all of them have batches (ranks), or null.
+  __device__ __forceinline__ void values(const float (&v)[N], int column, int turn, int waves, volatile uint32_t* shared) {
     constexpr int kGroup = 4;
     float part[N / kGroup], top;
 #pragma unroll
@@ -327,16 +347,16 @@ struct Pass {
     sum.w = sum.w + w;
     if constexpr (TOP) {
       if (turn == 0 || __any(top >= least)) {
-        // k lanes have seen a value that large (then about 64 ln(64 / (64 - k)) values pass in all), or a quarter of k
-        // in each of the four waves, which is a good third of what passes by their own bounds; renewed in turns 0, 1,
-        // 3, 7, ...
+        // k lanes have seen a value that large (then about 64 ln(64 / (64 - k)) values pass in all), or their share of k
+        // in each of the workgroup's waves (with four of them a third of what passes by their own bounds); renewed in
+        // turns 0, 1, 3, 7, ...
         if ((turn & (turn + 1)) == 0) {
           uint32_t t;
           if (shared) {
-            t = kth_of_lanes(rank_of(sum.m), (best.k + 3) / 4);
+            t = kth_of_lanes(rank_of(sum.m), (best.k + waves - 1) / waves);
             if (lane_id() == 0) shared[wave_id()] = t;
             if (turn == 0) __syncthreads();
-            t = min(min(shared[0], shared[1]), min(shared[2], shared[3]));
+            t = common_bound(shared, waves, best.k);
           } else {
             t = kth_of_lanes(rank_of(sum.m), best.k);
           }
@@ -378,7 +398,7 @@ struct Pass {
           load_tail(x + mine + u * kWave * kVec<T>, to - mine - u * kWave * kVec<T>, v + u * kVec<T>);
       }
       if (next + kBatch <= to) load(next);
-      values(v, (int)mine, turn++, shared);
+      values(v, (int)mine, turn++, step, shared);
       at = next;
     }
     sum.fold(c);
@@ -452,24 +472,25 @@ __global__ __launch_bounds__(256) void log_probs_wave_kernel(const T* __restrict
   finish_row(given, row, cols, pass.sum, pass.best.list, c, inv_t, o);
 }
 
-// One workgroup per chunk of a row.  With one chunk per row its results, else the
+// One workgroup of W waves per chunk of a row.  With one chunk per row its results, else the
 // chunk's sums and keys, for join_kernel.
-template <class T, int U, bool TOP>
-__global__ __launch_bounds__(256) void log_probs_block_kernel(const T* __restrict__ logits, int cols, int64_t stride,
+template <class T, int U, bool TOP, int W>
+__global__ __launch_bounds__(64 * W) void log_probs_block_kernel(const T* __restrict__ logits, int cols, int64_t stride,
                                                               float c, float inv_t, int64_t chunk, int splits, Out o,
                                                               float4* __restrict__ part,
                                                               uint64_t* __restrict__ part_keys) {
-  __shared__ uint64_t pool[TOP ? 4 * kPool : 1];
-  __shared__ uint64_t lists[TOP ? 4 : 1][kWave];
-  __shared__ float4 sums[4];
-  __shared__ int counts[4];
-  __shared__ uint32_t bounds[4];
+  __shared__ uint64_t pool[TOP ? W * kPool : 1];
+  __shared__ uint64_t all[TOP ? 2 * W * kWave : 1];
+  __shared__ float4 sums[W];
+  __shared__ uint32_t bounds[W];
+  __shared__ int total;
   const int tid = threadIdx.x, wave = wave_id(), lane = lane_id();
   const int64_t row = blockIdx.x / (unsigned)splits;
   const int split = (int)(blockIdx.x - row * splits);
   const T* x = logits + row * stride;
   if constexpr (TOP) {
-    if (tid < 4) bounds[tid] = 0;
+    if (tid < W) bounds[tid] = 0;
+    if (tid == 0) total = 0;
     __syncthreads();
   }
   Given given;
@@ -477,29 +498,18 @@ __global__ __launch_bounds__(256) void log_probs_block_kernel(const T* __restric
   using P = Pass<T, U, TOP>;
   P pass(c, TOP ? pool + wave * kPool : pool, o.topk);
   const int64_t from = (int64_t)split * chunk, to = min((int64_t)cols, from + chunk);
-  pass.run(x, from, to, wave, 4, to - from > 3 * P::kBatch ? bounds : nullptr);
-  if (lane == 0) {
-    sums[wave] = pass.sum.packed();
-    counts[wave] = pass.best.count;
+  pass.run(x, from, to, wave, W, to - from > (W - 1) * P::kBatch ? bounds : nullptr);
+  if (lane == 0) sums[wave] = pass.sum.packed();
+  if constexpr (TOP) {
+    __syncthreads();
+    pass.best.hand_over(all, &total, common_bound(bounds, W, o.topk));
   }
-  if constexpr (TOP) lists[wave][lane] = pass.best.list;
   __syncthreads();
   if (wave) return;
   Sums sum = Sums::of(sums[0]);
 #pragma unroll
-  for (int q = 1; q < 4; q++) sum.add(Sums::of(sums[q]), c);
-  Best<true>& best = pass.best;
-  if constexpr (TOP) {
-    const uint32_t least = min(min(bounds[0], bounds[1]), min(bounds[2], bounds[3]));
-#pragma unroll
-    for (int q = 1; q < 4; q++) {
-      Best<true> other(pool + q * kPool, o.topk);
-      other.count = counts[q];
-      best.take(lists[q][lane], other, least);
-    }
-    best.finish();
-  }
-  const uint64_t list = best.list;
+  for (int q = 1; q < W; q++) sum.add(Sums::of(sums[q]), c);
+  const uint64_t list = TOP ? best_of(all, total, pool, o.topk) : 0;
   if (splits == 1) {
     finish_row(given, row, cols, sum, list, c, inv_t, o);
   } else {
@@ -514,21 +524,21 @@ __global__ __launch_bounds__(256) void join_kernel(const T* __restrict__ logits,
                                                    float inv_t, int splits, Out o, const float4* __restrict__ part,
                                                    const uint64_t* __restrict__ part_keys) {
   __shared__ uint64_t pool[TOP ? 4 * kPool : 1];
-  __shared__ uint64_t lists[TOP ? 4 : 1][kWave];
+  __shared__ uint64_t all[TOP ? 2 * 4 * kWave : 1];
   __shared__ uint32_t leasts[4];
   __shared__ float4 sums[4];
-  __shared__ int counts[4];
+  __shared__ int total;
   const int tid = threadIdx.x, wave = wave_id(), lane = lane_id();
   const int64_t row = blockIdx.x;
   Given given;
   if (wave == 0) given = given_of(logits + row * stride, row, cols, o);
   // the first keys are asked for before the sums
   const uint64_t* keys = TOP ? part_keys + row * splits * o.topk : nullptr;
-  const int head = wave * kWave + lane, total = splits * o.topk;
+  const int head = wave * kWave + lane, keys_of_row = splits * o.topk;
   uint64_t of_chunk = 0, ahead = 0;
   if constexpr (TOP) {
     if (head < splits) of_chunk = keys[(int64_t)head * o.topk];
-    if (head < total) ahead = keys[head];
+    if (head < keys_of_row) ahead = keys[head];
   }
   Sums sum;
   for (int i = tid; i < splits; i += 256) {
@@ -538,35 +548,25 @@ __global__ __launch_bounds__(256) void join_kernel(const T* __restrict__ logits,
   Best<false> best(TOP ? pool + wave * kPool : pool, o.topk);
   if constexpr (TOP) {
     // k of 64 chunks have a key with a rank that large
-    const uint32_t least = kth_of_lanes((uint32_t)(of_chunk >> 32), o.topk);
-    for (int i = wave * kWave; i < total; i += 256) {
+    const uint32_t mine = kth_of_lanes((uint32_t)(of_chunk >> 32), o.topk);
+    if (lane == 0) leasts[wave] = mine;
+    if (tid == 0) total = 0;
+    __syncthreads();
+    const uint32_t least = max(max(leasts[0], leasts[1]), max(leasts[2], leasts[3]));
+    for (int i = wave * kWave; i < keys_of_row; i += 256) {
       const uint64_t key = ahead;
-      ahead = i + 256 + lane < total ? keys[i + 256 + lane] : 0;
+      ahead = i + 256 + lane < keys_of_row ? keys[i + 256 + lane] : 0;
       best.offer(key && (uint32_t)(key >> 32) >= least, key);
     }
-    lists[wave][lane] = best.list;
-    if (lane == 0) leasts[wave] = least;
+    best.hand_over(all, &total, least);
   }
-  if (lane == 0) {
-    sums[wave] = sum.packed();
-    counts[wave] = best.count;
-  }
+  if (lane == 0) sums[wave] = sum.packed();
   __syncthreads();
   if (wave) return;
   sum = Sums::of(sums[0]);
 #pragma unroll
   for (int q = 1; q < 4; q++) sum.add(Sums::of(sums[q]), c);
-  if constexpr (TOP) {
-    const uint32_t least = max(max(leasts[0], leasts[1]), max(leasts[2], leasts[3]));
-#pragma unroll
-    for (int q = 1; q < 4; q++) {
-      Best<false> other(pool + q * kPool, o.topk);
-      other.count = counts[q];
-      best.take(lists[q][lane], other, least);
-    }
-    best.finish();
-  }
-  const uint64_t list = best.list;
+  const uint64_t list = TOP ? best_of(all, total, pool, o.topk) : 0;
   finish_row(given, row, cols, sum, list, c, inv_t, o);
 }
 
@@ -692,19 +692,24 @@ __global__ __launch_bounds__(256) void log_probs_grad_kernel(const T* logits, in
 
 // How a call's rows are cut.
 struct Plan {
-  bool waves;     // one wave per row
+  int waves;      // per workgroup; 1: one wave per row
   int splits;     // chunks per row (workgroups)
   int64_t chunk;  // columns
 };
 
 constexpr int64_t kStep = 4096;  // columns: one batch of each of a workgroup's four waves
 
+// Short rows, and many of up to 8,192 columns, by waves: XXX
+// Rows that fill the 256 CUs evenly with a workgroup of 16 waves each need no join.  Else fewer than 1,024 rows are
+// cut, so that about four workgroups are there for each CU.
 Plan plan_of(int64_t rows, int64_t cols) {
-  if (cols <= 1024 || (rows >= 4096 && cols <= 8192)) return {true, 1, cols};
+  if (cols <= 1024 || (rows >= 4096 && cols <= 8192)) return {1, 1, cols};
+  const int64_t rounds = (rows + 255) / 256;
+  if (rows < 1024 && rows * 5 >= rounds * 256 * 4 && cols >= 4 * kStep) return {16, 1, cols};
   const int64_t most = (cols + kStep - 1) / kStep;
   const int64_t want = std::min<int64_t>(most, std::max<int64_t>(1, 1024 / rows));
   const int64_t steps = (most + want - 1) / want;
-  return {false, (int)((most + steps - 1) / steps), steps * kStep};
+  return {4, (int)((most + steps - 1) / steps), steps * kStep};
 }
 
 template <class T, bool TOP>
@@ -712,7 +717,7 @@ void log_probs(const T* x, int64_t rows, int64_t cols, int64_t stride, float tem
                hipStream_t st) {
   const float c = (float)(1.44269504088896340736 / (double)temperature), inv_t = (float)(1.0 / (double)temperature);
   const Plan p = plan_of(rows, cols);
-  if (p.waves) {
+  if (p.waves == 1) {
     const dim3 grid((unsigned)((rows + 3) / 4));
     if (cols <= kWave * kVec<T>)
       hipLaunchKernelGGL((log_probs_wave_kernel<T, 1, TOP>), grid, dim3(256), 0, st, x, rows, (int)cols, stride, c,
@@ -725,8 +730,9 @@ void log_probs(const T* x, int64_t rows, int64_t cols, int64_t stride, float tem
   }
   float4* part = static_cast<float4*>(work);
   uint64_t* keys = reinterpret_cast<uint64_t*>(part + rows * p.splits);
-  hipLaunchKernelGGL((log_probs_block_kernel<T, 16 / kVec<T>, TOP>), dim3((unsigned)(rows * p.splits)), dim3(256), 0, st, x,
-                     (int)cols, stride, c, inv_t, p.chunk, p.splits, o, part, keys);
+  auto* kernel = p.waves == 16 ? log_probs_block_kernel<T, 16 / kVec<T>, TOP, 16> : log_probs_block_kernel<T, 16 / kVec<T>, TOP, 4>;
+  hipLaunchKernelGGL(kernel, dim3((unsigned)(rows * p.splits)), dim3(64 * p.waves), 0, st, x, (int)cols, stride, c, inv_t,
+                     p.chunk, p.splits, o, part, keys);
   HIP_OK(hipGetLastError());
   if (p.splits > 1) {
     hipLaunchKernelGGL((join_kernel<T, TOP>), dim3((unsigned)rows), dim3(256), 0, st, x, (int)cols, stride, c, inv_t,

@@ -168,7 +168,8 @@ def _run(scoring, x, targets, k, T, seed=1, grads=True):
     (33, 65, 3, 5, 2.0), (1000, 100, 1, 10, 0.05), (17, 128, 0, 20, 1.0), (40, 255, 1, 0, 1.0), (6, 256, 4, 64, 0.1),
     (12, 257, 1, 33, 1.0), (7, 511, 1, 10, 1.0), (300, 513, 1, 1, 1.0), (20, 1000, 5, 50, 0.3), (4, 1023, 1, 10, 1.0),
     (4, 1025, 64, 64, 1.0), (31, 2048, 1, 10, 1.0), (3, 2049, 1, 64, 1.0), (100, 4096, 1, 10, 0.05), (5, 4099, 2, 7, 1.0),
-    (2, 16385, 1, 64, 1.0), (13, 20001, 1, 10, 1.0), (1, 70003, 3, 50, 0.05), (300, 9001, 1, 20, 1.0)])
+    (2, 16385, 1, 64, 1.0), (13, 20001, 1, 10, 1.0), (1, 70003, 3, 50, 0.05), (300, 9001, 1, 20, 1.0), (210, 17001, 1, 20, 1.0),
+    (250, 16385, 2, 64, 0.2), (256, 16400, 1, 1, 1.0), (4100, 1030, 1, 5, 1.0)])
 def test_rows(scoring, dtype, n, v, t, k, T):
     say("log probs", dtype, n, v, t, k, T)
     x, targets = _inputs(dtype, n, v, t, n + v, T)
@@ -178,10 +179,10 @@ def test_rows(scoring, dtype, n, v, t, k, T):
 
 
 @pytest.mark.parametrize("dtype", TYPES)
-@pytest.mark.parametrize("v", [50, 300, 5000, 40000])
-def test_masks(scoring, dtype, v):
+@pytest.mark.parametrize("v, rows", [(50, 14), (300, 14), (5000, 14), (40000, 14), (16500, 252)])
+def test_masks(scoring, dtype, v, rows):
     """Rows with nothing, one value, all equal, the type's lowest value as a mask, huge and tiny values, signed zeros."""
-    say("log probs, masks", dtype, v)
+    say("log probs, masks", dtype, v, rows)
     low = torch.finfo(dtype).min
     x = torch.randn((14, v), device="cuda").to(dtype)
     x[0] = -INF
@@ -203,6 +204,7 @@ def test_masks(scoring, dtype, v):
     x[13, : v // 2] = -INF
     targets = torch.stack([torch.zeros(14, device="cuda"), torch.full((14,), v - 1, device="cuda"),
                            torch.full((14,), -1, device="cuda")], 1).to(torch.int32)
+    x, targets = x.repeat(rows // 14, 1), targets.repeat(rows // 14, 1)  # (more rows: more waves for each)
     for T in (1.0, 0.125):
         _run(scoring, x, targets, 12, T)
 
