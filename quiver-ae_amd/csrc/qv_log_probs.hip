@@ -699,15 +699,24 @@ struct Plan {
 
 constexpr int64_t kStep = 4096;  // columns: one batch of each of a workgroup's four waves
 
-// Short rows, and many of up to 8,192 columns, by waves: XXX
-// Rows that fill the 256 CUs evenly with a workgroup of 16 waves each need no join.  Else fewer than 1,024 rows are
-// cut, so that about four workgroups are there for each CU.
+// Measured with 10 alternatives of bfloat16 (with none in brackets), us by 1, 4 and 16 waves per row and cut into
+// chunks of 4 waves each:
+//   4,096 x 4,096: 14 (9), 23 (12), 72 (33)     2,000 x 20,000: 28 (17), 29 (17), 60 (29)
+//   500 x 32,000: -, 18 (10), 21 (14), 21 (13)  300 x 128,000: -, 41 (22), 34 (24), 31 (20)
+//   200 x 8,000: -, 9 (11), 11 (12), 13 (13)    200 x 128,000: -, 37 (20), 21 (15), 25 (16)
+//   64 x 32,000: -, 16 (8), 13 (8), 16 (10)     64 x 128,000: -, 35 (20), 21 (14), 17 (10)
+// So one wave per row where rows alone fill the GPU or are too short for more; else a workgroup per row, of 16 waves
+// where there is at most one for each CU; and chunks, whose join costs 5 us, where long rows leave CUs without work.
 Plan plan_of(int64_t rows, int64_t cols) {
-  if (cols <= 1024 || (rows >= 4096 && cols <= 8192)) return {1, 1, cols};
-  const int64_t rounds = (rows + 255) / 256;
-  if (rows < 1024 && rows * 5 >= rounds * 256 * 4 && cols >= 4 * kStep) return {16, 1, cols};
+  if (cols <= 1024 || rows >= 2048) return {1, 1, cols};
+  if (rows > 256) {
+    if (rows >= 400 || cols <= 65536) return {4, 1, cols};
+  } else {
+    if (cols <= 8192) return {4, 1, cols};
+    if (cols <= 32768 || (rows > 96 && cols <= 131072) || rows > 204) return {16, 1, cols};
+  }
   const int64_t most = (cols + kStep - 1) / kStep;
-  const int64_t want = std::min<int64_t>(most, std::max<int64_t>(1, 1024 / rows));
+  const int64_t want = std::min<int64_t>(most, 1024 / rows);
   const int64_t steps = (most + want - 1) / want;
   return {4, (int)((most + steps - 1) / steps), steps * kStep};
 }
