@@ -1,11 +1,12 @@
-// qv_dense.hpp -- what the dense scoring calls share: element types, the caller's
-// device, argument checks.
+// qv_dense.hpp -- what the dense scoring calls share: element types and loads, the
+// caller's device, argument checks.
 #pragma once
 
 #include <hip/hip_runtime.h>
 
 #include <cstdint>
 #include <string>
+#include <type_traits>
 
 #include "qv_common.hpp"
 #include "qv_hip_util.hpp"
@@ -42,6 +43,47 @@ inline int value_size(int32_t type) {
   if (type == QV_FLOAT) return 4;
   if (type == QV_BFLOAT16 || type == QV_FLOAT16) return 2;
   fail(QV_EINVAL, "type must be float, bfloat16 or float16");
+}
+
+// 16 bytes of a row at once, whatever the row's alignment (its elements' own).
+typedef uint32_t raw4 __attribute__((ext_vector_type(4)));
+typedef raw4 raw4_any __attribute__((aligned(2), may_alias));
+
+template <class T>
+constexpr int kVec = 16 / (int)sizeof(T);
+
+template <class T>
+__device__ __forceinline__ raw4 load_raw(const T* p) {
+  return *reinterpret_cast<const raw4_any*>(p);
+}
+
+template <class T>
+__device__ __forceinline__ void unpack(raw4 r, float* v) {
+#pragma unroll
+  for (int i = 0; i < 4; i++) {
+    if constexpr (sizeof(T) == 4) {
+      v[i] = __uint_as_float(r[i]);
+    } else if constexpr (std::is_same<T, bf16>::value) {
+      v[2 * i] = __uint_as_float(r[i] << 16);
+      v[2 * i + 1] = __uint_as_float(r[i] & 0xffff0000u);
+    } else {
+      typedef f16 h2 __attribute__((ext_vector_type(2)));
+      const h2 h = __builtin_bit_cast(h2, (uint32_t)r[i]);
+      v[2 * i] = (float)h[0];
+      v[2 * i + 1] = (float)h[1];
+    }
+  }
+}
+
+// The vector at p of which `valid` elements are in the row, `other` past them.
+template <class T>
+__device__ __forceinline__ void load_tail(const T* p, int64_t valid, float other, float* v) {
+  if (valid >= kVec<T>) {
+    unpack<T>(load_raw(p), v);
+  } else {
+#pragma unroll
+    for (int i = 0; i < kVec<T>; i++) v[i] = i < valid ? (float)p[i] : other;
+  }
 }
 
 // The wave's number in its workgroup, in a scalar register: what is derived from it

@@ -7,6 +7,7 @@ from __future__ import annotations
 
 import ctypes as C
 import os
+import sys
 from pathlib import Path
 
 
@@ -215,6 +216,9 @@ SIGNATURES = {
 }
 
 _lib = None
+# Whether the library was loaded in a process that had not imported torch: it then
+# brought the system's HIP runtime with it, beside which torch's own copy finds no GPU.
+before_torch = False
 
 
 def lib_path() -> Path:
@@ -224,7 +228,7 @@ def lib_path() -> Path:
 
 def load() -> C.CDLL:
     """Load libquiver_hip.so once; raise QuiverError when it is not built."""
-    global _lib
+    global _lib, before_torch
     if _lib is not None:
         return _lib
     path = lib_path()
@@ -238,6 +242,7 @@ def load() -> C.CDLL:
         fn = getattr(lib, name)
         fn.restype = res
         fn.argtypes = args
+    before_torch = "torch" not in sys.modules
     _lib = lib
     return lib
 

@@ -15,14 +15,22 @@ Results can be handed back through ``out=`` to be written again (a loop then
 allocates nothing); a result is ordered with the stream it was made on.  A wrong
 argument raises ``ValueError``, a failing call ``QuiverError``; nothing here
 falls back to torch.
+
+torch brings its own HIP runtime, and a process can hold one: import torch or
+this module before the library is first called (an index opened earlier has
+loaded the system's).
 """
 from __future__ import annotations
 
 from dataclasses import dataclass, replace
 
-import torch
-
 from . import _lib
+
+if _lib.before_torch:
+    raise _lib.QuiverError("libquiver_hip was loaded before torch, so the process would hold two HIP runtimes: "
+                           "import torch (or quiver.scoring) before the first call into the library")
+
+import torch  # noqa: E402
 
 _TYPES = {torch.float32: _lib.QV_FLOAT, torch.bfloat16: _lib.QV_BFLOAT16, torch.float16: _lib.QV_FLOAT16}
 _CODES = (torch.int8,)

@@ -34,7 +34,8 @@ def scoring():
 
     if _lib.device_count() == 0:
         pytest.skip("no GPU")
-    return scoring
+    yield scoring
+    torch.cuda.empty_cache()  # the memory is the other tests' again
 
 
 def say(*a):

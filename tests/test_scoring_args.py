@@ -2,6 +2,9 @@
 from __future__ import annotations
 
 import ctypes as C
+import subprocess
+import sys
+from pathlib import Path
 
 import numpy as np
 import pytest
@@ -157,3 +160,15 @@ def test_python_refusals():
         scoring.log_probs(x, torch.zeros(3, 65, dtype=torch.int32))
     with pytest.raises(ValueError, match="score_bytes"):
         scoring.DenseCatalogue(x, score_bytes=0)
+
+
+@pytest.mark.parametrize("order, says", [("_lib.load(); from quiver import scoring", "loaded before torch"),
+                                         ("from quiver import scoring; _lib.load()", ""),
+                                         ("import torch; _lib.load(); from quiver import scoring", "")])
+def test_one_hip_runtime(order, says):
+    """Loading the library before torch is refused by name, not left to fail as a missing GPU."""
+    package = Path(__file__).resolve().parents[1] / "quiver-ae_amd"
+    run = subprocess.run([sys.executable, "-c", f"import sys; sys.path.insert(0, {str(package)!r}); from quiver import _lib; "
+                          + order], capture_output=True, text=True, timeout=300)
+    assert (run.returncode != 0) == bool(says)
+    assert says in run.stderr
