@@ -1,6 +1,7 @@
 // qv_scores.hip -- rows to 8 bits with a scale each, and the integer product of two
 // such matrices.
 #include <algorithm>
+#include <atomic>
 
 #include "qv_dense.hpp"
 #include "qv_device.hpp"
@@ -208,57 +209,67 @@ __device__ __forceinline__ void put_sums(int32_t* tile, int stride, int j0, cons
   }
 }
 
-// Scales and stores a wave's tile of 32 rows and J columns: 16 bytes of a row per lane.
+// The scales and biases of the 16 bytes of a row, of J columns from j0, that a lane stores.
 template <int J, class O>
-__device__ __forceinline__ void store_tile(const int32_t* tile, int stride, int64_t i0, int64_t j0,
-                                           const Product<O>& p) {
-  constexpr int V = 16 / (int)sizeof(O), L = J / V, R = kWave / L;  // columns per lane, lanes per row, rows at once
-  const int lane = lane_id(), jl = lane % L * V;
-  const int64_t j = j0 + jl;
-  if (j >= p.n) return;
-  const bool whole = j + V <= p.n;
-  float sb[V], add[V];
+struct Columns {
+  static constexpr int V = 16 / (int)sizeof(O), L = J / V, R = kWave / L;  // columns per lane, lanes per row, rows at once
+  float scale[V], add[V];
+  int64_t j;
+  bool whole;
+
+  __device__ __forceinline__ Columns(int64_t j0, const Product<O>& p) : j(j0 + lane_id() % L * V), whole(j + V <= p.n) {
 #pragma unroll
-  for (int v = 0; v < V; v += 4) {
-    if (whole) {
-      const f4 s = *reinterpret_cast<const f4_any*>(p.b_scales + j + v);
-      const f4 t = p.bias ? (f4)*reinterpret_cast<const f4_any*>(p.bias + j + v) : f4{0.f, 0.f, 0.f, 0.f};
+    for (int v = 0; v < V; v += 4) {
+      if (whole) {
+        const f4 s = *reinterpret_cast<const f4_any*>(p.b_scales + j + v);
+        const f4 t = p.bias ? (f4)*reinterpret_cast<const f4_any*>(p.bias + j + v) : f4{0.f, 0.f, 0.f, 0.f};
 #pragma unroll
-      for (int e = 0; e < 4; e++) sb[v + e] = s[e], add[v + e] = t[e];
-    } else {
+        for (int e = 0; e < 4; e++) scale[v + e] = s[e], add[v + e] = t[e];
+      } else {
 #pragma unroll
-      for (int e = 0; e < 4; e++) {
-        const int64_t q = min(j + v + e, p.n - 1);
-        sb[v + e] = p.b_scales[q];
-        add[v + e] = p.bias ? p.bias[q] : 0.f;
+        for (int e = 0; e < 4; e++) {
+          const int64_t q = min(j + v + e, p.n - 1);
+          scale[v + e] = p.b_scales[q];
+          add[v + e] = p.bias ? p.bias[q] : 0.f;
+        }
       }
     }
   }
-#pragma unroll 4
-  for (int r = lane / L; r < 32; r += R) {
+};
+
+// Scales and stores a wave's tile of 32 rows, whose scales `sa` gives, and J columns: 16 bytes of a row per lane.
+template <int J, class O, class F>
+__device__ __forceinline__ void store_tile(const int32_t* tile, int stride, int64_t i0, const Columns<J, O>& c, F sa,
+                                           const Product<O>& p) {
+  using C = Columns<J, O>;
+  if (c.j >= p.n) return;
+  const int lane = lane_id(), jl = lane % C::L * C::V;
+#pragma unroll
+  for (int t = 0; t < 32 / C::R; t++) {
+    const int r = t * C::R + lane / C::L;
     const int64_t i = i0 + r;
     if (i >= p.m) break;
-    const float sa = p.a_scales[i];
+    const float scale = sa(t, r);
     union {
-      O o[V];
+      O o[C::V];
       i4 raw;
     } u;
 #pragma unroll
-    for (int v = 0; v < V; v += 4) {
+    for (int v = 0; v < C::V; v += 4) {
       const i4 sums = *reinterpret_cast<const i4*>(tile + r * stride + jl + v);
 #pragma unroll
       for (int e = 0; e < 4; e++) {
-        const float x = ((float)sums[e] * sa) * sb[v + e];
-        u.o[v + e] = (O)(p.bias ? x + add[v + e] : x);
+        const float x = ((float)sums[e] * scale) * c.scale[v + e];
+        u.o[v + e] = (O)(p.bias ? x + c.add[v + e] : x);
       }
     }
-    O* dst = p.out + i * p.out_stride + j;
-    if (whole) {
+    O* dst = p.out + i * p.out_stride + c.j;
+    if (c.whole) {
       *reinterpret_cast<i4_any*>(dst) = u.raw;
     } else {
 #pragma unroll
-      for (int v = 0; v < V; v++)
-        if (j + v < p.n) dst[v] = u.o[v];
+      for (int v = 0; v < C::V; v++)
+        if (c.j + v < p.n) dst[v] = u.o[v];
     }
   }
 }
@@ -276,7 +287,7 @@ __device__ __forceinline__ int64_t tile_of_block(int64_t block, int64_t tiles) {
 // rows of any alignment and length; 2,048 x 4,096 x 4,096 to bfloat16: 46 us, 1.5 POP/s.
 template <int BM, int BN, int WM, int WN, class O>
 __global__ __launch_bounds__(64 * WM * WN, 1) void product_tile_kernel(Product<O> p, int64_t tiles_m, int64_t tiles_n,
-                                                                       int64_t group) {
+                                                                       int64_t group, int scales_at) {
   constexpr int T = 64 * WM * WN, TM = BM / WM / 32, TN = BN / WN / 32;
   constexpr int LA = BM * 8 / T, LB = BN * 8 / T, kRows = T / 8;
   constexpr int kBuffer = (BM + BN) * kStage;
@@ -333,6 +344,10 @@ __global__ __launch_bounds__(64 * WM * WN, 1) void product_tile_kernel(Product<O
   };
   load(0);
   keep(0);
+  constexpr int J = 32 * TN, kTile = J + 4;
+  const Columns<J, O> columns(j0 + wn * J, p);
+  float* scales = reinterpret_cast<float*>(lds + scales_at);
+  for (int r = tid; r < BM; r += T) scales[r] = p.a_scales[min(i0 + r, p.m - 1)];
   __syncthreads();
   for (int s = 0; s < stages; s++) {
     const bool more = s + 1 < stages;
@@ -351,7 +366,6 @@ __global__ __launch_bounds__(64 * WM * WN, 1) void product_tile_kernel(Product<O
     }
     __syncthreads();
   }
-  constexpr int J = 32 * TN, kTile = J + 4;
   int32_t* tile = reinterpret_cast<int32_t*>(lds) + wave * 32 * kTile;
 #pragma unroll
   for (int x = 0; x < TM; x++) {
@@ -359,7 +373,8 @@ __global__ __launch_bounds__(64 * WM * WN, 1) void product_tile_kernel(Product<O
 #pragma unroll
     for (int y = 0; y < TN; y++) put_sums(tile, kTile, 32 * y, acc[x][y]);
     __builtin_amdgcn_fence(__ATOMIC_ACQ_REL, "wavefront");
-    store_tile<J>(tile, kTile, i0 + (wm * TM + x) * 32, j0 + wn * J, p);
+    const float* sa = scales + (wm * TM + x) * 32;
+    store_tile(tile, kTile, i0 + (wm * TM + x) * 32, columns, [&](int, int r) { return sa[r]; }, p);
   }
 }
 
@@ -393,7 +408,7 @@ constexpr int kWaitFor = (N & 15) | (N >> 4 << 14) | 0x0070;  // s_waitcnt vmcnt
 
 template <int BM, int BN, int WM, int WN, int NB, class O>
 __global__ __launch_bounds__(64 * WM * WN, 1) void product_deep_kernel(Product<O> p, int64_t tiles_m, int64_t tiles_n,
-                                                                       int64_t group) {
+                                                                       int64_t group, int scales_at) {
   constexpr int TM = BM / WM / 32, TN = BN / WN / 32, kRow = 64;
   constexpr int I = (BM + BN) / 16 / (WM * WN);  // loads of 16 rows per wave and stage
   static_assert(I % 2 == 0, "issued in halves");
@@ -449,6 +464,11 @@ __global__ __launch_bounds__(64 * WM * WN, 1) void product_deep_kernel(Product<O
     asm volatile("" ::: "memory");
     __builtin_amdgcn_sched_barrier(0);
   };
+  constexpr int J = 32 * TN, kTile = J + 4;
+  const Columns<J, O> columns(j0 + wn * J, p);
+  float* scales = reinterpret_cast<float*>(lds + scales_at);
+  for (int r = threadIdx.x; r < BM; r += 64 * WM * WN) scales[r] = p.a_scales[min(i0 + r, p.m - 1)];
+  __builtin_amdgcn_s_waitcnt(kWaitFor<0>);  // the waits below count the stages' loads alone
 #pragma unroll
   for (int s = 0; s < NB; s++) {
     issue(s, 0);
@@ -478,7 +498,6 @@ __global__ __launch_bounds__(64 * WM * WN, 1) void product_deep_kernel(Product<O
   }
   __builtin_amdgcn_s_waitcnt(kWaitFor<0>);
   meet();
-  constexpr int J = 32 * TN, kTile = J + 4;
   int32_t* tile = reinterpret_cast<int32_t*>(lds) + wave * 32 * kTile;
 #pragma unroll
   for (int x = 0; x < TM; x++) {
@@ -486,7 +505,8 @@ __global__ __launch_bounds__(64 * WM * WN, 1) void product_deep_kernel(Product<O
 #pragma unroll
     for (int y = 0; y < TN; y++) put_sums(tile, kTile, 32 * y, acc[x][y]);
     __builtin_amdgcn_fence(__ATOMIC_ACQ_REL, "wavefront");
-    store_tile<J>(tile, kTile, i0 + (wm * TM + x) * 32, j0 + wn * J, p);
+    const float* sa = scales + (wm * TM + x) * 32;
+    store_tile(tile, kTile, i0 + (wm * TM + x) * 32, columns, [&](int, int r) { return sa[r]; }, p);
   }
 }
 
@@ -711,6 +731,11 @@ __global__ __launch_bounds__(256) void product_strip_kernel(Product<O> p, int64_
       rb[q] = *reinterpret_cast<const i4_any*>(p.b + r * p.b_stride + from);
     }
   };
+  using C = Columns<32, O>;
+  float sa[32 / C::R];  // of the rows that the lane stores
+#pragma unroll
+  for (int t = 0; t < 32 / C::R; t++) sa[t] = p.a_scales[min((int64_t)(t * C::R + lane / C::L), p.m - 1)];
+  auto scale = [&](int t, int) { return sa[t]; };
   const int s0 = WK == 1 ? 0 : wave;
   int64_t strip = WK == 1 ? (int64_t)blockIdx.x * 4 + wave : blockIdx.x;
   if (WK == 1 && strip >= strips) return;
@@ -746,10 +771,10 @@ __global__ __launch_bounds__(256) void product_strip_kernel(Product<O> p, int64_
         sum[e] = v;
       }
       __syncthreads();
-      if (wave == 0) store_tile<32>(sum, kTile, 0, strip * 32, p);
+      if (wave == 0) store_tile(sum, kTile, 0, C(strip * 32, p), scale, p);
       __syncthreads();
     } else {
-      store_tile<32>(tile, kTile, 0, strip * 32, p);
+      store_tile(tile, kTile, 0, C(strip * 32, p), scale, p);
       __builtin_amdgcn_fence(__ATOMIC_ACQ_REL, "wavefront");
     }
   }
@@ -803,16 +828,30 @@ void quantize(const void* x, int64_t n, int64_t dim, int64_t stride, int8_t* cod
   HIP_OK(hipGetLastError());
 }
 
+// More than 64 KB of LDS is asked for once per kernel and device.
+template <auto* KERNEL>
+void allow_lds(int bytes) {
+  static std::atomic<uint64_t> done{0};
+  if (bytes <= 65536) return;
+  int device = 0;
+  HIP_OK(hipGetDevice(&device));
+  const uint64_t bit = device < 64 ? 1ull << device : 0;
+  if (done.load(std::memory_order_relaxed) & bit) return;
+  HIP_OK(hipFuncSetAttribute(reinterpret_cast<const void*>(KERNEL), hipFuncAttributeMaxDynamicSharedMemorySize, 160 * 1024));
+  done.fetch_or(bit, std::memory_order_relaxed);
+}
+
 template <int BM, int BN, int WM, int WN, class O>
 void launch_tiles(const Product<O>& p, hipStream_t st) {
   const int64_t tm = (p.m + BM - 1) / BM, tn = (p.n + BN - 1) / BN;
   // down a group of tiles' rows first: as many as keep their rows of a within 2 MB of an XCD's L2, eight at least
   const int64_t group = std::min(tm, std::max<int64_t>(8, (2 << 20) / (BM * p.k)));
   const int buffers = p.k > kStage ? 2 : 1;
-  const int lds = std::max(buffers * (BM + BN) * kStage, WM * WN * 32 * (BN / WN + 4) * 4);
-  auto* kernel = product_tile_kernel<BM, BN, WM, WN, O>;
-  if (lds > 65536) HIP_OK(hipFuncSetAttribute(reinterpret_cast<const void*>(kernel), hipFuncAttributeMaxDynamicSharedMemorySize, lds));
-  hipLaunchKernelGGL(kernel, dim3((unsigned)(tm * tn)), dim3(64 * WM * WN), lds, st, p, tm, tn, group);
+  const int scales_at = std::max(buffers * (BM + BN) * kStage, WM * WN * 32 * (BN / WN + 4) * 4);
+  const int lds = scales_at + BM * 4;
+  constexpr auto* kernel = &product_tile_kernel<BM, BN, WM, WN, O>;
+  allow_lds<kernel>(lds);
+  hipLaunchKernelGGL(kernel, dim3((unsigned)(tm * tn)), dim3(64 * WM * WN), lds, st, p, tm, tn, group, scales_at);
   HIP_OK(hipGetLastError());
 }
 
@@ -820,10 +859,11 @@ template <int BM, int BN, int WM, int WN, int NB, class O>
 void launch_deep(const Product<O>& p, hipStream_t st) {
   const int64_t tm = (p.m + BM - 1) / BM, tn = (p.n + BN - 1) / BN;
   const int64_t group = std::min<int64_t>(tm, 8);
-  const int lds = std::max(NB * (BM + BN) * 64, WM * WN * 32 * (BN / WN + 4) * 4);
-  auto* kernel = product_deep_kernel<BM, BN, WM, WN, NB, O>;
-  if (lds > 65536) HIP_OK(hipFuncSetAttribute(reinterpret_cast<const void*>(kernel), hipFuncAttributeMaxDynamicSharedMemorySize, lds));
-  hipLaunchKernelGGL(kernel, dim3((unsigned)(tm * tn)), dim3(64 * WM * WN), lds, st, p, tm, tn, group);
+  const int scales_at = std::max(NB * (BM + BN) * 64, WM * WN * 32 * (BN / WN + 4) * 4);
+  const int lds = scales_at + BM * 4;
+  constexpr auto* kernel = &product_deep_kernel<BM, BN, WM, WN, NB, O>;
+  allow_lds<kernel>(lds);
+  hipLaunchKernelGGL(kernel, dim3((unsigned)(tm * tn)), dim3(64 * WM * WN), lds, st, p, tm, tn, group, scales_at);
   HIP_OK(hipGetLastError());
 }
 
