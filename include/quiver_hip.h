@@ -6,7 +6,8 @@
  * Host buffers are owned by the caller and are never registered with the HIP
  * runtime; device state (graph pages, PQ codes, tables, search scratch) is owned
  * by the library and freed by qv_index_close().  One search may run per index
- * handle at a time; calls are blocking.
+ * handle at a time; calls are blocking (the dense scoring calls are not: they
+ * enqueue on a stream of the caller's).
  *
  * Each entry point names the reference interface it replaces
  * (ruc-system/quiver-ae paths).

@@ -385,7 +385,7 @@ __global__ __launch_bounds__(64 * WM * WN, 1) void product_tile_kernel(Product<O
 // and the next stage's first operands while the second one's do, so the one barrier
 // per stage, between the two, finds the operands of what follows it in registers.
 // Needs 16-byte aligned rows and k a multiple of 64.
-// 4,096^3 to bfloat16: 72 us, 1.9 POP/s (a library's int8 product with a 32-bit result: 69);
+// 4,096^3 to bfloat16: 69 us, 2.0 POP/s (a library's int8 product with a 32-bit result: 69);
 // 8,192^3 of zeros 378 us, 2.9 POP/s, of codes over the whole range 550 us: then power
 // holds the clock at 1.5 GHz (the matrix instruction alone reaches 4.5 and 3.3 POP/s).
 // Loads and LDS reads in runs of their own instead of between the products: 86 us.
@@ -703,8 +703,8 @@ __global__ __launch_bounds__(256, KS == 4 ? 3 : 2) void product_panel_kernel(Pro
 // 1), or a strip's k cut over the WK waves of its workgroup.  A wave's stage of b goes
 // through registers into an LDS area of its own, so no barrier holds it; the next one
 // is in flight meanwhile.  a's operands come from the caches, once for all strips
-// while k is a single stage.  Bound by reading b: 1 x 1M x 128 in 30 us, 4.5 TB/s, 8 x
-// 100,000 x 1,024 in 19 us, 5.3 TB/s.
+// while k is a single stage.  Bound by reading b: 1 x 1M x 128 in 29.5 us, 4.6 TB/s (24.5
+// us over and over, part of b being cached), 8 x 100,000 x 1,024 in 19 us, 5.3 TB/s.
 template <int WK, class O>
 __global__ __launch_bounds__(256) void product_strip_kernel(Product<O> p, int64_t strips, int64_t step) {
   constexpr int kTile = 32 + 4;
