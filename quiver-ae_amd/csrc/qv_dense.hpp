@@ -4,6 +4,7 @@
 
 #include <hip/hip_runtime.h>
 
+#include <algorithm>
 #include <cstdint>
 #include <string>
 #include <type_traits>
@@ -84,6 +85,13 @@ __device__ __forceinline__ void load_tail(const T* p, int64_t valid, float other
 #pragma unroll
     for (int i = 0; i < kVec<T>; i++) v[i] = i < valid ? (float)p[i] : other;
   }
+}
+
+// A launch holds less than 2^32 threads.  f(first, count) launches workgroups first, first + 1, ... of them.
+template <class F>
+void in_launches(int64_t workgroups, int threads, F f) {
+  const int64_t most = (int64_t{1} << 31) / threads;
+  for (int64_t first = 0; first < workgroups; first += most) f(first, (unsigned)std::min(most, workgroups - first));
 }
 
 // The wave's number in its workgroup, in a scalar register: what is derived from it

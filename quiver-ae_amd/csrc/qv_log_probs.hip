@@ -425,10 +425,11 @@ __device__ __forceinline__ void finish_row(const Given& given, int64_t row, int 
 // One wave per row: no barrier, no join.
 template <class T, int U, bool TOP>
 __global__ __launch_bounds__(256) void log_probs_wave_kernel(const T* __restrict__ logits, int64_t rows, int cols,
-                                                             int64_t stride, float c, float inv_t, Out o) {
+                                                             int64_t stride, float c, float inv_t, Out o,
+                                                             int64_t first_block) {
   __shared__ uint64_t pool[TOP ? 4 * kPool : 1];
   const int wave = wave_id();
-  const int64_t row = (int64_t)blockIdx.x * 4 + wave;
+  const int64_t row = (first_block + blockIdx.x) * 4 + wave;
   if (row >= rows) return;
   const T* x = logits + row * stride;
   const Given given = given_of(x, row, cols, o);
@@ -555,9 +556,9 @@ struct Weights {
 template <class T, int U>
 __global__ __launch_bounds__(256) void log_probs_grad_kernel(const T* logits, int64_t units, int cols, int64_t stride,
                                                              float c, float inv_t, int chunk, int splits, Weights g,
-                                                             T* grad, int64_t grad_stride) {
+                                                             T* grad, int64_t grad_stride, int64_t first_block) {
   constexpr int N = U * kVec<T>, kBatch = kWave * N;
-  const int64_t unit = (int64_t)blockIdx.x * 4 + wave_id();
+  const int64_t unit = (first_block + blockIdx.x) * 4 + wave_id();
   if (unit >= units) return;
   const int lane = lane_id();
   const int64_t row = unit / splits;
@@ -693,14 +694,11 @@ void log_probs(const T* x, int64_t rows, int64_t cols, int64_t stride, float tem
   const float c = (float)(1.44269504088896340736 / (double)temperature), inv_t = (float)(1.0 / (double)temperature);
   const Plan p = plan_of(rows, cols);
   if (p.waves == 1) {
-    const dim3 grid((unsigned)((rows + 3) / 4));
-    if (cols <= kWave * kVec<T>)
-      hipLaunchKernelGGL((log_probs_wave_kernel<T, 1, TOP>), grid, dim3(256), 0, st, x, rows, (int)cols, stride, c,
-                         inv_t, o);
-    else
-      hipLaunchKernelGGL((log_probs_wave_kernel<T, 16 / kVec<T>, TOP>), grid, dim3(256), 0, st, x, rows, (int)cols, stride, c,
-                         inv_t, o);
-    HIP_OK(hipGetLastError());
+    auto* kernel = cols <= kWave * kVec<T> ? log_probs_wave_kernel<T, 1, TOP> : log_probs_wave_kernel<T, 16 / kVec<T>, TOP>;
+    in_launches((rows + 3) / 4, 256, [&](int64_t first, unsigned count) {
+      hipLaunchKernelGGL(kernel, dim3(count), dim3(256), 0, st, x, rows, (int)cols, stride, c, inv_t, o, first);
+      HIP_OK(hipGetLastError());
+    });
     return;
   }
   float4* part = static_cast<float4*>(work);
@@ -723,9 +721,11 @@ void log_probs_grad(const T* x, int64_t rows, int64_t cols, int64_t stride, floa
   const float c = (float)(1.44269504088896340736 / (double)temperature), inv_t = (float)(1.0 / (double)temperature);
   const int64_t chunk = 4 * kWave * U * kVec<T>;
   const int64_t splits = (cols + chunk - 1) / chunk, units = rows * splits;
-  hipLaunchKernelGGL((log_probs_grad_kernel<T, U>), dim3((unsigned)((units + 3) / 4)), dim3(256), 0, st, x, units,
-                     (int)cols, stride, c, inv_t, (int)chunk, (int)splits, g, grad, grad_stride);
-  HIP_OK(hipGetLastError());
+  in_launches((units + 3) / 4, 256, [&](int64_t first, unsigned count) {
+    hipLaunchKernelGGL((log_probs_grad_kernel<T, U>), dim3(count), dim3(256), 0, st, x, units, (int)cols, stride, c,
+                       inv_t, (int)chunk, (int)splits, g, grad, grad_stride, first);
+    HIP_OK(hipGetLastError());
+  });
 }
 
 int64_t workspace_of(int64_t rows, int64_t cols, int32_t topk) {

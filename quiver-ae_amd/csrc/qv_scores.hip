@@ -82,10 +82,10 @@ __device__ __forceinline__ void store_codes(int8_t* row, int64_t j, int64_t dim,
 template <class T, int G, int E, int R>
 __global__ __launch_bounds__(256) void quantize_kernel(const T* __restrict__ x, int64_t n, int64_t dim, int64_t stride,
                                                        int8_t* __restrict__ codes, int64_t code_stride,
-                                                       float* __restrict__ scales) {
+                                                       float* __restrict__ scales, int64_t first_block) {
   constexpr int kGroups = 256 / G;
   const int lane = threadIdx.x % G;
-  const int64_t first = (int64_t)blockIdx.x * kGroups * R + threadIdx.x / G;
+  const int64_t first = (first_block + blockIdx.x) * kGroups * R + threadIdx.x / G;
   float v[R][E * kVec<T>];
 #pragma unroll
   for (int r = 0; r < R; r++) {
@@ -116,9 +116,9 @@ __global__ __launch_bounds__(256) void quantize_kernel(const T* __restrict__ x, 
 template <class T>
 __global__ __launch_bounds__(256) void quantize_long_kernel(const T* __restrict__ x, int64_t dim, int64_t stride,
                                                             int8_t* __restrict__ codes, int64_t code_stride,
-                                                            float* __restrict__ scales) {
+                                                            float* __restrict__ scales, int64_t first_block) {
   __shared__ uint32_t tops[4];
-  const int64_t row = blockIdx.x;
+  const int64_t row = first_block + blockIdx.x;
   const T* src = x + row * stride;
   uint32_t top = 0;
   for (int64_t j = (int64_t)threadIdx.x * kVec<T>; j < dim; j += 256 * kVec<T>) {
@@ -784,10 +784,10 @@ __global__ __launch_bounds__(256) void product_strip_kernel(Product<O> p, int64_
 // a 16 x 16 tile of the output per workgroup, one thread per element, both operands'
 // rows staged 64 bytes at a time.
 template <class O>
-__global__ __launch_bounds__(256) void product_small_kernel(Product<O> p, int64_t tiles_n) {
+__global__ __launch_bounds__(256) void product_small_kernel(Product<O> p, int64_t tiles_n, int64_t first_block) {
   __shared__ int8_t sa[16][68], sb[16][68];
   const int tid = threadIdx.x, r = tid / 16, c = tid % 16;
-  const int64_t i0 = (int64_t)blockIdx.x / tiles_n * 16, j0 = (int64_t)blockIdx.x % tiles_n * 16;
+  const int64_t tile = first_block + blockIdx.x, i0 = tile / tiles_n * 16, j0 = tile % tiles_n * 16;
   int32_t acc = 0;
   for (int64_t k0 = 0; k0 < p.k; k0 += 64) {
     for (int u = tid; u < 16 * 64; u += 256) {
@@ -811,8 +811,9 @@ void quantize(const void* x, int64_t n, int64_t dim, int64_t stride, int8_t* cod
               hipStream_t st) {
   const T* in = static_cast<const T*>(x);
   auto go = [&](auto* kernel, int64_t rows) {
-    hipLaunchKernelGGL(kernel, dim3((unsigned)((n + rows - 1) / rows)), dim3(256), 0, st, in, n, dim, stride, codes,
-                       code_stride, scales);
+    in_launches((n + rows - 1) / rows, 256, [&](int64_t first, unsigned count) {
+      hipLaunchKernelGGL(kernel, dim3(count), dim3(256), 0, st, in, n, dim, stride, codes, code_stride, scales, first);
+    });
   };
   const int64_t vectors = (dim + kVec<T> - 1) / kVec<T>;
   if (vectors <= 8) go(quantize_kernel<T, 8, 1, 4>, 128);
@@ -823,8 +824,10 @@ void quantize(const void* x, int64_t n, int64_t dim, int64_t stride, int8_t* cod
   else if (vectors <= 256) go(quantize_kernel<T, 64, 4, 1>, 4);
   else if (vectors <= 512) go(quantize_kernel<T, 64, 8, 1>, 4);
   else
-    hipLaunchKernelGGL(quantize_long_kernel<T>, dim3((unsigned)n), dim3(256), 0, st, in, dim, stride, codes, code_stride,
-                       scales);
+    in_launches(n, 256, [&](int64_t first, unsigned count) {
+      hipLaunchKernelGGL(quantize_long_kernel<T>, dim3(count), dim3(256), 0, st, in, dim, stride, codes, code_stride,
+                         scales, first);
+    });
   HIP_OK(hipGetLastError());
 }
 
@@ -881,8 +884,9 @@ template <class O>
 void product(const Product<O>& p, hipStream_t st) {
   if (p.k < 16 || p.a_stride >= kFar || p.b_stride >= kFar || p.out_stride >= kFarOut) {
     const int64_t tm = (p.m + 15) / 16, tn = (p.n + 15) / 16;
-    if (tm * tn > INT32_MAX) fail(QV_EUNSUPPORTED, "more tiles than one launch has");
-    hipLaunchKernelGGL(product_small_kernel<O>, dim3((unsigned)(tm * tn)), dim3(256), 0, st, p, tn);
+    in_launches(tm * tn, 256, [&](int64_t first, unsigned count) {
+      hipLaunchKernelGGL(product_small_kernel<O>, dim3(count), dim3(256), 0, st, p, tn, first);
+    });
     HIP_OK(hipGetLastError());
   } else if (p.m <= 32) {
     const int64_t strips = (p.n + 31) / 32;
@@ -948,7 +952,7 @@ int qv_int8_product(const int8_t* d_a, int64_t a_stride, const float* d_a_scales
     check_vector("a_scales", d_a_scales, m);
     check_vector("b_scales", d_b_scales, n);
     if (d_bias) check_vector("bias", d_bias, n);
-    if (m > INT32_MAX || n > INT32_MAX || (m + 127) / 128 * ((n + 127) / 128) > INT32_MAX)
+    if (m > INT32_MAX || n > INT32_MAX || (m + 127) / 128 * ((n + 127) / 128) >= 1 << 24)
       qv::fail(QV_EUNSUPPORTED, "more tiles than one launch has");
     const OnDevice on(device);
     const hipStream_t st = static_cast<hipStream_t>(stream);

@@ -371,6 +371,24 @@ def test_long_matrix(scoring):
     assert abs(grad[2, v - 1].item() - (1 - 1 / s)) < 2e-3 and abs(grad[2, 7].item() + math.exp(-1) / s) < 2e-3
 
 
+def test_many_rows(scoring):
+    """More rows than one launch has threads for (2^32, 64 a row)."""
+    n = 2 ** 26 + 77
+    say("log probs and gradient,", n, "rows")
+    place = torch.arange(n, device="cuda") % 11
+    x = torch.stack([torch.zeros(n, device="cuda"), (place - 5).float()], 1)
+    targets = torch.ones(n, dtype=torch.int32, device="cuda")
+    r = scoring.log_probs(x, targets, top_k=1)
+    d = torch.arange(-5, 6, dtype=torch.float64, device="cuda")
+    lp = -torch.log1p(torch.exp(-d))
+    bound = (74 + 82) * U + 4 * U * 7 + U * 6  # |y| <= 5, ln S < 1; lp to a float below
+    assert ((r.target[:, 0] - lp.float()[place]).abs() <= bound).all()
+    assert (r.top_ids[:, 0] == (d > 0)[place]).all()
+    grad = scoring.log_probs_grad(x, r, targets, grad_target=torch.ones((n, 1), device="cuda"), out=x)
+    assert ((grad[:, 1] - (1 - lp.exp()).float()[place]).abs() <= bound + 4 * U).all()
+    assert ((grad[:, 0] + (1 - lp.exp()).float()[place]).abs() <= bound + 4 * U).all()
+
+
 def test_other_stream_reuse_and_repeat(scoring):
     """Results written again through out=, on a stream of their own, in a captured graph; equal calls, equal bits."""
     say("log probs, streams and graphs")

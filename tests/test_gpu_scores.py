@@ -218,6 +218,28 @@ def test_long_catalogue(scoring):
                        torch.bfloat16)
 
 
+def test_many_rows(scoring):
+    """More rows, and more tiles, than one launch is given."""
+    n = 2 ** 30 + 300
+    say("quantize,", n, "rows")
+    x = torch.full((n, 1), 2.0, dtype=torch.bfloat16, device="cuda")
+    x[::3] = -1
+    codes, scales = scoring.quantize_rows(x)
+    negative = x[:, 0] < 0
+    assert (codes[:, 0] == torch.where(negative, -127, 127).to(torch.int8)).all()
+    one = torch.tensor([1 / 127, 2 / 127], device="cuda")
+    assert ((scales - torch.where(negative, one[0], one[1])).abs() <= 2 ** -30).all()  # 2^-24 of 2 / 127
+    del x, codes, scales, negative
+    m, n, k = 46_400, 46_403, 3
+    say("product,", m, n, k)
+    a = torch.randint(-128, 128, (m, k), dtype=torch.int8, device="cuda")
+    b = torch.randint(-128, 128, (n, k), dtype=torch.int8, device="cuda")
+    sa, sb = torch.rand(m, device="cuda"), torch.rand(n, device="cuda")
+    out = scoring.int8_product(a, sa, b, sb, dtype=torch.float16)
+    for lo in (0, m // 2, m - 100):
+        _check_product(out[lo:lo + 100], a[lo:lo + 100], sa[lo:lo + 100], b, sb, None, torch.float16)
+
+
 def test_other_stream_and_order(scoring):
     """Calls follow the current stream's order, and equal calls give equal bits."""
     say("scores on a stream of their own")
