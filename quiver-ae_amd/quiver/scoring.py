@@ -191,6 +191,18 @@ def _forward(logits, targets, top_k, temperature, out) -> LogProbs:
     return out
 
 
+class _Once(torch.autograd.Function):
+    """A gradient made while a graph is recorded: there is no derivative of it, and taking one must not give zeros."""
+
+    @staticmethod
+    def forward(ctx, grad, *inputs):
+        return grad.view_as(grad)
+
+    @staticmethod
+    def backward(ctx, _g):
+        raise _lib.QuiverError("the gradient of log_probs cannot be differentiated again")
+
+
 class _LogProbsFunction(torch.autograd.Function):
     @staticmethod
     def forward(ctx, logits, targets, top_k, temperature):
@@ -211,6 +223,8 @@ class _LogProbsFunction(torch.autograd.Function):
         grad = _gradient(logits, stats.data_ptr(), entropy.data_ptr(), top_ids.data_ptr(), top_ids.shape[1],
                          logits.get_device(), ctx.temperature, targets, plain(g_target), plain(g_entropy), plain(g_lse),
                          plain(g_top), None)
+        if torch.is_grad_enabled():
+            grad = _Once.apply(grad, logits, *(g for g in (g_target, g_entropy, g_lse, g_top) if g is not None))
         return grad, None, None, None
 
 
@@ -224,7 +238,8 @@ def log_probs(logits: torch.Tensor, targets: torch.Tensor | None = None, *, top_
     descending order, the lower column first among equal ones.  -inf takes a
     column out; a row with none left has log probabilities -inf, entropy 0 and
     ids -1, one that holds +inf or NaN has NaN.  With logits that require a
-    gradient the results take part in autograd (``out`` is then refused).
+    gradient the results take part in autograd (``out`` is then refused), once:
+    the gradient has none of its own.
     """
     if torch.is_grad_enabled() and logits.requires_grad:
         if out is not None:

@@ -342,6 +342,19 @@ def test_autograd(scoring):
             scoring.log_probs(leaf, targets, out=plain)
 
 
+def test_no_second_gradient(scoring):
+    """A second derivative is refused, not taken as zero."""
+    from quiver import _lib
+
+    say("log probs, second derivative")
+    leaf = torch.randn((4, 50), device="cuda").requires_grad_()
+    (grad,) = torch.autograd.grad(scoring.log_probs(leaf).entropy.sum(), leaf, create_graph=True)
+    want = scoring.log_probs_grad(leaf.detach(), scoring.log_probs(leaf.detach()), grad_entropy=torch.ones(4, device="cuda"))
+    assert torch.equal(grad, want)
+    with pytest.raises(_lib.QuiverError, match="differentiated again"):
+        (grad.square().sum() + leaf.sum()).backward()
+
+
 def test_empty_sizes(scoring):
     say("log probs, no rows and no columns")
     r = scoring.log_probs(torch.empty((0, 5), device="cuda"), top_k=2)
