@@ -40,6 +40,9 @@ _CODES = (torch.int8,)
 # repeated shapes).
 _raw_stream = torch._C._cuda_getCurrentRawStream
 
+# For tensors given as out=: autograd then refuses a backward pass that needs what they held.
+_written = torch._C._increment_version
+
 
 def _device(*tensors: torch.Tensor) -> int:
     """The one GPU that every tensor is on."""
@@ -81,7 +84,8 @@ def quantize_rows(x: torch.Tensor, *, out: tuple[torch.Tensor, torch.Tensor] | N
     row with an infinity or a NaN the scale NaN and zero codes.
     """
     n, d, stride = _matrix("x", x, _TYPES)
-    if out is None:
+    again = out is not None
+    if not again:
         out = (torch.empty((n, d), dtype=torch.int8, device=x.device),
                torch.empty(n, dtype=torch.float32, device=x.device))
     codes, scales = out
@@ -92,6 +96,8 @@ def quantize_rows(x: torch.Tensor, *, out: tuple[torch.Tensor, torch.Tensor] | N
     device = _device(x, codes, scales)
     _lib.check(_lib.load().qv_quantize_rows(x.data_ptr(), _TYPES[x.dtype], n, d, stride, codes.data_ptr(), code_stride,
                                             at, device, _raw_stream(device)))
+    if again:
+        _written(out)
     return out
 
 
@@ -107,7 +113,8 @@ def int8_product(a: torch.Tensor, a_scales: torch.Tensor, b: torch.Tensor, b_sca
     n, k_b, b_stride = _matrix("b", b, _CODES)
     if k_b != k:
         raise ValueError("a and b differ in the length of their rows")
-    if out is None:
+    again = out is not None
+    if not again:
         if dtype not in _TYPES:
             raise ValueError("dtype must be float32, bfloat16 or float16")
         out = torch.empty((m, n), dtype=dtype, device=a.device)
@@ -121,6 +128,8 @@ def int8_product(a: torch.Tensor, a_scales: torch.Tensor, b: torch.Tensor, b_sca
         at_bias, device = _vector("bias", bias, (n,)), _device(a, a_scales, b, b_scales, out, bias)
     _lib.check(_lib.load().qv_int8_product(a.data_ptr(), a_stride, at_a, m, b.data_ptr(), b_stride, at_b, at_bias, n, k,
                                            out.data_ptr(), _TYPES[out.dtype], out_stride, device, _raw_stream(device)))
+    if again:
+        _written((out,))
     return out
 
 
@@ -137,7 +146,8 @@ class LogProbs:
     temperature: float
     _workspace: torch.Tensor
     _device: int
-    _at: tuple               # the buffers' addresses, in the order above
+    _parts: tuple            # the buffers in the order above, the workspace last
+    _at: tuple               # their addresses
 
     @staticmethod
     def empty(n: int, v: int, t: int, k: int, temperature: float, device: torch.device) -> "LogProbs":
@@ -149,17 +159,21 @@ class LogProbs:
         if device.type != "cuda":
             raise ValueError("tensors must be on the GPU")
 
+        workspace = _lib.load().qv_log_probs_workspace(n, v, k)
+        if workspace < 0:
+            _lib.check(workspace)
+
         def new(*shape, dtype=torch.float32):
             return torch.empty(shape, dtype=dtype, device=device)
 
         return LogProbs.of(new(n, t), new(n), new(n), new(n, k, dtype=torch.int32), new(n, k), new(n, 2), temperature,
-                           new(_lib.load().qv_log_probs_workspace(n, v, k), dtype=torch.uint8))
+                           new(workspace, dtype=torch.uint8))
 
     @staticmethod
     def of(target, entropy, logsumexp, top_ids, top, stats, temperature, workspace) -> "LogProbs":
         parts = (target, entropy, logsumexp, top_ids, top, stats, workspace)
         return LogProbs(target, entropy, logsumexp, top_ids, top, stats, temperature, workspace, stats.get_device(),
-                        tuple(p.data_ptr() for p in parts))
+                        parts, tuple(p.data_ptr() for p in parts))
 
 
 def _given(targets: torch.Tensor | None, rows: int) -> tuple[int | None, int]:
@@ -175,7 +189,8 @@ def _forward(logits, targets, top_k, temperature, out) -> LogProbs:
     n, v, stride = _matrix("logits", logits, _TYPES)
     at_targets, t = _given(targets, n)
     temperature = float(temperature)
-    if out is None:
+    again = out is not None
+    if not again:
         out = LogProbs.empty(n, v, t, top_k, temperature, logits.device)
     elif out.target.shape != (n, t) or out.top.shape != (n, top_k):
         raise ValueError("out was made for another number of rows, targets or alternatives")
@@ -188,6 +203,8 @@ def _forward(logits, targets, top_k, temperature, out) -> LogProbs:
     _lib.check(_lib.load().qv_log_probs(logits.data_ptr(), _TYPES[logits.dtype], n, v, stride, temperature, at_targets,
                                         t, top_k, at_target, at_entropy, at_lse, at_stats, at_ids, at_top, at_work,
                                         out._workspace.shape[0], device, _raw_stream(device)))
+    if again:
+        _written(out._parts)
     return out
 
 
@@ -254,7 +271,8 @@ def _gradient(logits, at_stats, at_entropy, at_ids, k, device, temperature, targ
               out):
     n, v, stride = _matrix("logits", logits, _TYPES)
     at_targets, t = _given(targets, n)
-    if out is None:
+    again = out is not None
+    if not again:
         out = torch.empty((n, v), dtype=logits.dtype, device=logits.device)
     out_rows, out_cols, out_stride = _matrix("out", out, (logits.dtype,))
     if out_rows != n or out_cols != v:
@@ -276,6 +294,8 @@ def _gradient(logits, at_stats, at_entropy, at_ids, k, device, temperature, targ
     _lib.check(_lib.load().qv_log_probs_grad(logits.data_ptr(), _TYPES[logits.dtype], n, v, stride, temperature,
                                              at_stats, at_entropy, at_targets, t, at_ids, k, *at, out.data_ptr(),
                                              out_stride, device, _raw_stream(device)))
+    if again:
+        _written((out,))
     return out
 
 

@@ -355,6 +355,27 @@ def test_no_second_gradient(scoring):
         (grad.square().sum() + leaf.sum()).backward()
 
 
+def test_overwritten(scoring):
+    """A backward pass that needs what out= has overwritten since is refused."""
+    say("results written again before the backward pass")
+    codes, scales = scoring.quantize_rows(torch.randn((40, 64), device="cuda"))
+    logits, weight = scoring.int8_product(codes[:8], scales[:8], codes, scales), torch.ones(8, device="cuda", requires_grad=True)
+    r = scoring.log_probs(logits, top_k=2)
+
+    def writes():
+        yield logits, lambda: scoring.int8_product(codes[:8], scales[:8], codes, scales, out=logits)
+        yield logits, lambda: scoring.log_probs_grad(logits, r, grad_entropy=torch.ones(8, device="cuda"), out=logits)
+        yield r.entropy, lambda: scoring.log_probs(logits, top_k=2, out=r)
+        yield scales, lambda: scoring.quantize_rows(torch.randn((40, 64), device="cuda"), out=(codes, scales))
+
+    for held, write in writes():
+        (held.reshape(-1)[:8] * weight).sum().backward()
+        loss = (held.reshape(-1)[:8] * weight).sum()
+        write()
+        with pytest.raises(RuntimeError, match="modified by an inplace operation"):
+            loss.backward()
+
+
 def test_empty_sizes(scoring):
     say("log probs, no rows and no columns")
     r = scoring.log_probs(torch.empty((0, 5), device="cuda"), top_k=2)

@@ -172,3 +172,11 @@ def test_one_hip_runtime(order, says):
                           + order], capture_output=True, text=True, timeout=300)
     assert (run.returncode != 0) == bool(says)
     assert says in run.stderr
+
+
+def test_buffers_refused(lib):
+    """What the library refuses to size is its error, not an allocation of a negative size."""
+    from quiver import scoring
+
+    with pytest.raises(lib.QuiverError, match="more than 2\\^31 - 1 rows or columns"):
+        scoring.LogProbs.empty(1, 2 ** 31, 0, 4, 1.0, torch.device("cuda"))
