@@ -209,6 +209,79 @@ __device__ __forceinline__ void put_sums(int32_t* tile, int stride, int j0, cons
   }
 }
 
+// Two values in the output's 16 bits, halves to even.
+template <class O>
+__device__ __forceinline__ uint32_t two_of(float x, float y) {
+  if constexpr (std::is_same<O, bf16>::value) {  // at once, which the compiler takes apart
+    uint32_t both;
+    asm("v_cvt_pk_bf16_f32 %0, %1, %2" : "=v"(both) : "v"(x), "v"(y));
+    return both;
+  } else {
+    typedef float f2 __attribute__((ext_vector_type(2)));
+    typedef O o2 __attribute__((ext_vector_type(2)));
+    return __builtin_bit_cast(uint32_t, __builtin_convertvector((f2{x, y}), o2));
+  }
+}
+
+// Scales an instruction's result, 32 columns from j of the rows around the lane's row i, and stores it from the
+// registers: 16 bytes per lane, 32 of each row at once.  Of the four columns that a lane has of every eight, those
+// of 16 bits pass to the other half of the wave and back, eight for a lane.  `sb`, `add`: the columns' scales and
+// biases in LDS.
+template <class O>
+__device__ __forceinline__ void store_sums(const i16v& acc, float sa, const float* sb, const float* add, int64_t i,
+                                           int64_t j, const Product<O>& p) {
+  constexpr int V = 16 / (int)sizeof(O), N = 16 / V;  // columns of a store, stores
+  const int half = lane_id() / 32;
+  float v[16];
+#pragma unroll
+  for (int g = 0; g < 4; g++) {
+    const f4 s = *reinterpret_cast<const f4*>(sb + 8 * g + 4 * half);
+#pragma unroll
+    for (int e = 0; e < 4; e++) v[4 * g + e] = ((float)acc[4 * g + e] * sa) * s[e];
+  }
+  if (p.bias) {
+#pragma unroll
+    for (int g = 0; g < 4; g++) {
+      const f4 t = *reinterpret_cast<const f4*>(add + 8 * g + 4 * half);
+#pragma unroll
+      for (int e = 0; e < 4; e++) v[4 * g + e] = v[4 * g + e] + t[e];
+    }
+  }
+  union {
+    O o[V];
+    uint32_t w[4];
+    i4 raw;
+  } u[N];
+#pragma unroll
+  for (int q = 0; q < N; q++) {
+    if constexpr (sizeof(O) == 4) {
+#pragma unroll
+      for (int e = 0; e < 4; e++) u[q].o[e] = v[4 * q + e];
+    } else {
+#pragma unroll
+      for (int d = 0; d < 2; d++) {
+        const auto both = __builtin_amdgcn_permlane32_swap(two_of<O>(v[8 * q + 2 * d], v[8 * q + 2 * d + 1]),
+                                                           two_of<O>(v[8 * q + 4 + 2 * d], v[8 * q + 5 + 2 * d]), false, false);
+        u[q].w[d] = both[0];
+        u[q].w[2 + d] = both[1];
+      }
+    }
+  }
+  if (i >= p.m) return;
+#pragma unroll
+  for (int q = 0; q < N; q++) {
+    const int64_t at = j + 2 * V * q + V * half;
+    O* dst = p.out + i * p.out_stride + at;
+    if (at + V <= p.n) {
+      *reinterpret_cast<i4_any*>(dst) = u[q].raw;
+    } else {
+#pragma unroll
+      for (int e = 0; e < V; e++)
+        if (at + e < p.n) dst[e] = u[q].o[e];
+    }
+  }
+}
+
 // The scales and biases of the 16 bytes of a row, of J columns from j0, that a lane stores.
 template <int J, class O>
 struct Columns {
@@ -408,7 +481,7 @@ constexpr int kWaitFor = (N & 15) | (N >> 4 << 14) | 0x0070;  // s_waitcnt vmcnt
 
 template <int BM, int BN, int WM, int WN, int NB, class O>
 __global__ __launch_bounds__(64 * WM * WN, 1) void product_deep_kernel(Product<O> p, int64_t tiles_m, int64_t tiles_n,
-                                                                       int64_t group, int scales_at) {
+                                                                       int64_t group) {
   constexpr int TM = BM / WM / 32, TN = BN / WN / 32, kRow = 64;
   constexpr int I = (BM + BN) / 16 / (WM * WN);  // loads of 16 rows per wave and stage
   static_assert(I % 2 == 0, "issued in halves");
@@ -464,10 +537,14 @@ __global__ __launch_bounds__(64 * WM * WN, 1) void product_deep_kernel(Product<O
     asm volatile("" ::: "memory");
     __builtin_amdgcn_sched_barrier(0);
   };
-  constexpr int J = 32 * TN, kTile = J + 4;
-  const Columns<J, O> columns(j0 + wn * J, p);
-  float* scales = reinterpret_cast<float*>(lds + scales_at);
-  for (int r = threadIdx.x; r < BM; r += 64 * WM * WN) scales[r] = p.a_scales[min(i0 + r, p.m - 1)];
+  // scales of the tile's rows and columns, biases
+  float* sa = reinterpret_cast<float*>(lds + NB * kBuffer);
+  float *sb = sa + BM, *add = sb + BN;
+  for (int r = threadIdx.x; r < BM; r += 64 * WM * WN) sa[r] = p.a_scales[min(i0 + r, p.m - 1)];
+  for (int r = threadIdx.x; r < BN; r += 64 * WM * WN) {
+    sb[r] = p.b_scales[min(j0 + r, p.n - 1)];
+    if (p.bias) add[r] = p.bias[min(j0 + r, p.n - 1)];
+  }
   __builtin_amdgcn_s_waitcnt(kWaitFor<0>);  // the waits below count the stages' loads alone
 #pragma unroll
   for (int s = 0; s < NB; s++) {
@@ -496,17 +573,15 @@ __global__ __launch_bounds__(64 * WM * WN, 1) void product_deep_kernel(Product<O
     __builtin_amdgcn_s_waitcnt(kReadsDone);  // long since: said for the compiler, which else waits at the loop's top
     __builtin_amdgcn_sched_barrier(0);
   }
-  __builtin_amdgcn_s_waitcnt(kWaitFor<0>);
-  meet();
-  int32_t* tile = reinterpret_cast<int32_t*>(lds) + wave * 32 * kTile;
+  __builtin_amdgcn_s_waitcnt(kWaitFor<0>);  // no load into LDS outlives the wave
 #pragma unroll
   for (int x = 0; x < TM; x++) {
-    if (x) __builtin_amdgcn_fence(__ATOMIC_ACQ_REL, "wavefront");
+    const int i = (wm * TM + x) * 32 + row;
 #pragma unroll
-    for (int y = 0; y < TN; y++) put_sums(tile, kTile, 32 * y, acc[x][y]);
-    __builtin_amdgcn_fence(__ATOMIC_ACQ_REL, "wavefront");
-    const float* sa = scales + (wm * TM + x) * 32;
-    store_tile(tile, kTile, i0 + (wm * TM + x) * 32, columns, [&](int, int r) { return sa[r]; }, p);
+    for (int y = 0; y < TN; y++) {
+      const int j = (wn * TN + y) * 32;
+      store_sums(acc[x][y], sa[i], sb + j, add + j, i0 + i, j0 + j, p);
+    }
   }
 }
 
@@ -666,22 +741,16 @@ __global__ __launch_bounds__(256, KS == 4 ? 3 : 2) void product_panel_kernel(Pro
         for (int e = 0; e < 4; e += 2)
 #pragma unroll
           for (int y = 0; y < Y; y++) {
-            typedef float f2 __attribute__((ext_vector_type(2)));
             typedef O o2 __attribute__((ext_vector_type(2)));
-            f2 x;
+            float x[2];
 #pragma unroll
             for (int d = 0; d < 2; d++) {
               x[d] = ((float)acc[l * Y + y][4 * g + e + d] * s[e + d]) * scale[y];
               if constexpr (BIAS) x[d] = x[d] + add[y];
             }
             o2 out;
-            if constexpr (std::is_same<O, bf16>::value) {  // two at once, which the compiler takes apart
-              uint32_t both;
-              asm("v_cvt_pk_bf16_f32 %0, %1, %2" : "=v"(both) : "v"(x[0]), "v"(x[1]));
-              out = __builtin_bit_cast(o2, both);
-            } else {
-              out = __builtin_convertvector(x, o2);
-            }
+            if constexpr (sizeof(O) == 2) out = __builtin_bit_cast(o2, two_of<O>(x[0], x[1]));
+            else out = o2{x[0], x[1]};
 #pragma unroll
             for (int d = 0; d < 2; d++) {
               uint32_t& at = place[y][4 * g + e + d];
@@ -862,11 +931,10 @@ template <int BM, int BN, int WM, int WN, int NB, class O>
 void launch_deep(const Product<O>& p, hipStream_t st) {
   const int64_t tm = (p.m + BM - 1) / BM, tn = (p.n + BN - 1) / BN;
   const int64_t group = std::min<int64_t>(tm, 8);
-  const int scales_at = std::max(NB * (BM + BN) * 64, WM * WN * 32 * (BN / WN + 4) * 4);
-  const int lds = scales_at + BM * 4;
+  const int lds = NB * (BM + BN) * 64 + (BM + 2 * BN) * 4;
   constexpr auto* kernel = &product_deep_kernel<BM, BN, WM, WN, NB, O>;
   allow_lds<kernel>(lds);
-  hipLaunchKernelGGL(kernel, dim3((unsigned)(tm * tn)), dim3(64 * WM * WN), lds, st, p, tm, tn, group, scales_at);
+  hipLaunchKernelGGL(kernel, dim3((unsigned)(tm * tn)), dim3(64 * WM * WN), lds, st, p, tm, tn, group);
   HIP_OK(hipGetLastError());
 }
 
