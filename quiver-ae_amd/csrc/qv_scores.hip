@@ -347,6 +347,34 @@ __device__ __forceinline__ void store_tile(const int32_t* tile, int stride, int6
   }
 }
 
+// A tile's scales of BM rows and BN columns, and the columns' biases, in LDS, put there by T threads.
+template <int BM, int BN, int T>
+struct TileScales {
+  static constexpr int kBytes = (BM + 2 * BN) * 4;
+  float* sa;
+
+  template <class O>
+  __device__ __forceinline__ TileScales(char* at, int64_t i0, int64_t j0, const Product<O>& p) : sa(reinterpret_cast<float*>(at)) {
+    for (int r = threadIdx.x; r < BM; r += T) sa[r] = p.a_scales[min(i0 + r, p.m - 1)];
+    for (int r = threadIdx.x; r < BN; r += T) {
+      sa[BM + r] = p.b_scales[min(j0 + r, p.n - 1)];
+      if (p.bias) sa[BM + BN + r] = p.bias[min(j0 + r, p.n - 1)];
+    }
+  }
+  // A wave's results, from row i and column j of the tile at (i0, j0) on.
+  template <int TM, int TN, class O>
+  __device__ __forceinline__ void store(const i16v (&acc)[TM][TN], int i, int j, int64_t i0, int64_t j0, const Product<O>& p) const {
+    const float *sb = sa + BM + j, *add = sb + BN;
+    i += lane_id() % 32;
+#pragma unroll
+    for (int x = 0; x < TM; x++) {
+#pragma unroll
+      for (int y = 0; y < TN; y++)
+        store_sums(acc[x][y], sa[i + 32 * x], sb + 32 * y, add + 32 * y, i0 + i + 32 * x, j0 + j + 32 * y, p);
+    }
+  }
+};
+
 // Workgroups go round the eight XCDs: each XCD gets a run of consecutive tiles.
 __device__ __forceinline__ int64_t tile_of_block(int64_t block, int64_t tiles) {
   const int64_t xcd = block % 8, per = tiles / 8, more = tiles % 8;
@@ -417,10 +445,7 @@ __global__ __launch_bounds__(64 * WM * WN, 1) void product_tile_kernel(Product<O
   };
   load(0);
   keep(0);
-  constexpr int J = 32 * TN, kTile = J + 4;
-  const Columns<J, O> columns(j0 + wn * J, p);
-  float* scales = reinterpret_cast<float*>(lds + scales_at);
-  for (int r = tid; r < BM; r += T) scales[r] = p.a_scales[min(i0 + r, p.m - 1)];
+  const TileScales<BM, BN, T> scales(lds + scales_at, i0, j0, p);
   __syncthreads();
   for (int s = 0; s < stages; s++) {
     const bool more = s + 1 < stages;
@@ -439,16 +464,7 @@ __global__ __launch_bounds__(64 * WM * WN, 1) void product_tile_kernel(Product<O
     }
     __syncthreads();
   }
-  int32_t* tile = reinterpret_cast<int32_t*>(lds) + wave * 32 * kTile;
-#pragma unroll
-  for (int x = 0; x < TM; x++) {
-    if (x) __builtin_amdgcn_fence(__ATOMIC_ACQ_REL, "wavefront");
-#pragma unroll
-    for (int y = 0; y < TN; y++) put_sums(tile, kTile, 32 * y, acc[x][y]);
-    __builtin_amdgcn_fence(__ATOMIC_ACQ_REL, "wavefront");
-    const float* sa = scales + (wm * TM + x) * 32;
-    store_tile(tile, kTile, i0 + (wm * TM + x) * 32, columns, [&](int, int r) { return sa[r]; }, p);
-  }
+  scales.store(acc, wm * TM * 32, wn * TN * 32, i0, j0, p);
 }
 
 // The same tiles where the matrix cores are what bounds the product: stages of 64 bytes
@@ -537,14 +553,7 @@ __global__ __launch_bounds__(64 * WM * WN, 1) void product_deep_kernel(Product<O
     asm volatile("" ::: "memory");
     __builtin_amdgcn_sched_barrier(0);
   };
-  // scales of the tile's rows and columns, biases
-  float* sa = reinterpret_cast<float*>(lds + NB * kBuffer);
-  float *sb = sa + BM, *add = sb + BN;
-  for (int r = threadIdx.x; r < BM; r += 64 * WM * WN) sa[r] = p.a_scales[min(i0 + r, p.m - 1)];
-  for (int r = threadIdx.x; r < BN; r += 64 * WM * WN) {
-    sb[r] = p.b_scales[min(j0 + r, p.n - 1)];
-    if (p.bias) add[r] = p.bias[min(j0 + r, p.n - 1)];
-  }
+  const TileScales<BM, BN, 64 * WM * WN> scales(lds + NB * kBuffer, i0, j0, p);
   __builtin_amdgcn_s_waitcnt(kWaitFor<0>);  // the waits below count the stages' loads alone
 #pragma unroll
   for (int s = 0; s < NB; s++) {
@@ -574,15 +583,7 @@ __global__ __launch_bounds__(64 * WM * WN, 1) void product_deep_kernel(Product<O
     __builtin_amdgcn_sched_barrier(0);
   }
   __builtin_amdgcn_s_waitcnt(kWaitFor<0>);  // no load into LDS outlives the wave
-#pragma unroll
-  for (int x = 0; x < TM; x++) {
-    const int i = (wm * TM + x) * 32 + row;
-#pragma unroll
-    for (int y = 0; y < TN; y++) {
-      const int j = (wn * TN + y) * 32;
-      store_sums(acc[x][y], sa[i], sb + j, add + j, i0 + i, j0 + j, p);
-    }
-  }
+  scales.store(acc, wm * TM * 32, wn * TN * 32, i0, j0, p);
 }
 
 // Short rows, k <= 32 KS, whose product is mostly writing: 32 rows of a stay in a wave's
@@ -919,8 +920,7 @@ void launch_tiles(const Product<O>& p, hipStream_t st) {
   // down a group of tiles' rows first: as many as keep their rows of a within 2 MB of an XCD's L2, eight at least
   const int64_t group = std::min(tm, std::max<int64_t>(8, (2 << 20) / (BM * p.k)));
   const int buffers = p.k > kStage ? 2 : 1;
-  const int scales_at = std::max(buffers * (BM + BN) * kStage, WM * WN * 32 * (BN / WN + 4) * 4);
-  const int lds = scales_at + BM * 4;
+  const int scales_at = buffers * (BM + BN) * kStage, lds = scales_at + TileScales<BM, BN, 64 * WM * WN>::kBytes;
   constexpr auto* kernel = &product_tile_kernel<BM, BN, WM, WN, O>;
   allow_lds<kernel>(lds);
   hipLaunchKernelGGL(kernel, dim3((unsigned)(tm * tn)), dim3(64 * WM * WN), lds, st, p, tm, tn, group, scales_at);
@@ -931,7 +931,7 @@ template <int BM, int BN, int WM, int WN, int NB, class O>
 void launch_deep(const Product<O>& p, hipStream_t st) {
   const int64_t tm = (p.m + BM - 1) / BM, tn = (p.n + BN - 1) / BN;
   const int64_t group = std::min<int64_t>(tm, 8);
-  const int lds = NB * (BM + BN) * 64 + (BM + 2 * BN) * 4;
+  const int lds = NB * (BM + BN) * 64 + TileScales<BM, BN, 64 * WM * WN>::kBytes;
   constexpr auto* kernel = &product_deep_kernel<BM, BN, WM, WN, NB, O>;
   allow_lds<kernel>(lds);
   hipLaunchKernelGGL(kernel, dim3((unsigned)(tm * tn)), dim3(64 * WM * WN), lds, st, p, tm, tn, group);
