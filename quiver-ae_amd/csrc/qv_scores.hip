@@ -226,8 +226,8 @@ __device__ __forceinline__ uint32_t two_of(float x, float y) {
 // Scales an instruction's result, 32 columns from j of the rows around the lane's row i, and stores it from the
 // registers: 16 bytes per lane, 32 of each row at once.  Of the four columns that a lane has of every eight, those
 // of 16 bits pass to the other half of the wave and back, eight for a lane.  `sb`, `add`: the columns' scales and
-// biases in LDS.
-template <class O>
+// biases in LDS.  WHOLE: all of it lies in the output.
+template <bool WHOLE, class O>
 __device__ __forceinline__ void store_sums(const i16v& acc, float sa, const float* sb, const float* add, int64_t i,
                                            int64_t j, const Product<O>& p) {
   constexpr int V = 16 / (int)sizeof(O), N = 16 / V;  // columns of a store, stores
@@ -235,17 +235,9 @@ __device__ __forceinline__ void store_sums(const i16v& acc, float sa, const floa
   float v[16];
 #pragma unroll
   for (int g = 0; g < 4; g++) {
-    const f4 s = *reinterpret_cast<const f4*>(sb + 8 * g + 4 * half);
+    const f4 s = *reinterpret_cast<const f4*>(sb + 8 * g + 4 * half), t = *reinterpret_cast<const f4*>(add + 8 * g + 4 * half);
 #pragma unroll
-    for (int e = 0; e < 4; e++) v[4 * g + e] = ((float)acc[4 * g + e] * sa) * s[e];
-  }
-  if (p.bias) {
-#pragma unroll
-    for (int g = 0; g < 4; g++) {
-      const f4 t = *reinterpret_cast<const f4*>(add + 8 * g + 4 * half);
-#pragma unroll
-      for (int e = 0; e < 4; e++) v[4 * g + e] = v[4 * g + e] + t[e];
-    }
+    for (int e = 0; e < 4; e++) v[4 * g + e] = ((float)acc[4 * g + e] * sa) * s[e] + t[e];
   }
   union {
     O o[V];
@@ -267,12 +259,13 @@ __device__ __forceinline__ void store_sums(const i16v& acc, float sa, const floa
       }
     }
   }
-  if (i >= p.m) return;
+  if (!WHOLE && i >= p.m) return;
+  O* to = p.out + (i * p.out_stride + j + V * half);
 #pragma unroll
   for (int q = 0; q < N; q++) {
     const int64_t at = j + 2 * V * q + V * half;
-    O* dst = p.out + i * p.out_stride + at;
-    if (at + V <= p.n) {
+    O* dst = to + 2 * V * q;
+    if (WHOLE || at + V <= p.n) {
       *reinterpret_cast<i4_any*>(dst) = u[q].raw;
     } else {
 #pragma unroll
@@ -347,31 +340,39 @@ __device__ __forceinline__ void store_tile(const int32_t* tile, int stride, int6
   }
 }
 
-// A tile's scales of BM rows and BN columns, and the columns' biases, in LDS, put there by T threads.
+// A tile's scales of BM rows and BN columns, and the columns' biases (-0, which changes no sum, without), in LDS, put
+// there by T threads.
 template <int BM, int BN, int T>
 struct TileScales {
   static constexpr int kBytes = (BM + 2 * BN) * 4;
   float* sa;
 
+  __device__ __forceinline__ explicit TileScales(char* at) : sa(reinterpret_cast<float*>(at)) {}
   template <class O>
   __device__ __forceinline__ TileScales(char* at, int64_t i0, int64_t j0, const Product<O>& p) : sa(reinterpret_cast<float*>(at)) {
     for (int r = threadIdx.x; r < BM; r += T) sa[r] = p.a_scales[min(i0 + r, p.m - 1)];
     for (int r = threadIdx.x; r < BN; r += T) {
       sa[BM + r] = p.b_scales[min(j0 + r, p.n - 1)];
-      if (p.bias) sa[BM + BN + r] = p.bias[min(j0 + r, p.n - 1)];
+      sa[BM + BN + r] = p.bias ? p.bias[min(j0 + r, p.n - 1)] : -0.f;
     }
   }
   // A wave's results, from row i and column j of the tile at (i0, j0) on.
-  template <int TM, int TN, class O>
-  __device__ __forceinline__ void store(const i16v (&acc)[TM][TN], int i, int j, int64_t i0, int64_t j0, const Product<O>& p) const {
+  template <bool WHOLE, int TM, int TN, class O>
+  __device__ __forceinline__ void store_all(i16v (&acc)[TM][TN], int i, int j, int64_t i0, int64_t j0, const Product<O>& p) const {
     const float *sb = sa + BM + j, *add = sb + BN;
     i += lane_id() % 32;
 #pragma unroll
-    for (int x = 0; x < TM; x++) {
+    for (int x = 0; x < TM; x++)
 #pragma unroll
-      for (int y = 0; y < TN; y++)
-        store_sums(acc[x][y], sa[i + 32 * x], sb + 32 * y, add + 32 * y, i0 + i + 32 * x, j0 + j + 32 * y, p);
-    }
+      for (int y = 0; y < TN; y++) {
+        asm volatile("" : "+a"(acc[x][y]) : : "memory");  // one at a time: none leaves its accumulators before
+        store_sums<WHOLE>(acc[x][y], sa[i + 32 * x], sb + 32 * y, add + 32 * y, i0 + i + 32 * x, j0 + j + 32 * y, p);
+      }
+  }
+  template <int TM, int TN, class O>
+  __device__ __forceinline__ void store(i16v (&acc)[TM][TN], int i, int j, int64_t i0, int64_t j0, const Product<O>& p) const {
+    if (i0 + BM <= p.m && j0 + BN <= p.n) store_all<true>(acc, i, j, i0, j0, p);
+    else store_all<false>(acc, i, j, i0, j0, p);
   }
 };
 
@@ -495,46 +496,62 @@ constexpr int kReadsDone = 0xc07f;  // s_waitcnt lgkmcnt(0)
 template <int N>
 constexpr int kWaitFor = (N & 15) | (N >> 4 << 14) | 0x0070;  // s_waitcnt vmcnt(N) lgkmcnt(0)
 
-template <int BM, int BN, int WM, int WN, int NB, class O>
+template <int BM, int BN, int WM, int WN, int NB, bool MANY, class O>
 __global__ __launch_bounds__(64 * WM * WN, 1) void product_deep_kernel(Product<O> p, int64_t tiles_m, int64_t tiles_n,
                                                                        int64_t group) {
   constexpr int TM = BM / WM / 32, TN = BN / WN / 32, kRow = 64;
+  using Scales = TileScales<BM, BN, 64 * WM * WN>;
   constexpr int I = (BM + BN) / 16 / (WM * WN);  // loads of 16 rows per wave and stage
   static_assert(I % 2 == 0, "issued in halves");
   constexpr int kBuffer = (BM + BN) * kRow;
   extern __shared__ __align__(16) char lds[];
   const int wave = wave_id(), lane = lane_id(), wm = wave / WN, wn = wave % WN;
-  const int64_t t = tile_of_block(blockIdx.x, tiles_m * tiles_n);
-  const int64_t g = t / (group * tiles_n), gm = min(group, tiles_m - g * group), in = t - g * group * tiles_n;
-  const int64_t i0 = (g * group + in % gm) * BM, j0 = in / gm * BN;
-  const int stages = (int)p.k / kRow;
+  const uint32_t stages = (uint32_t)p.k / kRow;  // NB at least
+  const uint32_t tiles = (uint32_t)(tiles_m * tiles_n), tn = (uint32_t)tiles_n, rows = (uint32_t)group;
+  int64_t i0, j0, next_i0, next_j0;
+  auto place_next = [&](uint32_t turn) {
+    const uint32_t t = (uint32_t)tile_of_block(turn, tiles), g = t / (rows * tn), in = t - g * rows * tn;
+    const uint32_t gm = min(rows, (uint32_t)tiles_m - g * rows);
+    next_i0 = (int64_t)(g * rows + in % gm) * BM;
+    next_j0 = (int64_t)(in / gm) * BN;
+  };
 
   // piece q of row r lies at q ^ (r / 4 mod 4): the lanes of a load write 1 KB in a row, so what they load is
   // permuted instead
   const int piece = (lane % 4) ^ (lane / 16);
   const int8_t* src[I];
+  char* scales_at = lds + NB * kBuffer;  // of this tile and the next one
+  // the next tile's rows, and its scales on their way
+  auto turn_to_next = [&](int buffer) {
 #pragma unroll
-  for (int q = 0; q < I; q++) {
-    const int r = (wave * I + q) * 16 + lane / 4;
-    src[q] = (r < BM ? p.a + min(i0 + r, p.m - 1) * p.a_stride : p.b + min(j0 + r - BM, p.n - 1) * p.b_stride) + piece * 16;
-  }
-  // (stages past the last one repeat it: as many loads per turn as the waits count)
-  auto issue = [&](int s, int part) {  // a half of a stage's loads
+    for (int q = 0; q < I; q++) {
+      const int r = (wave * I + q) * 16 + lane / 4;
+      src[q] = (r < BM ? p.a + min(next_i0 + r, p.m - 1) * p.a_stride : p.b + min(next_j0 + r - BM, p.n - 1) * p.b_stride) + piece * 16;
+    }
+    float* to = reinterpret_cast<float*>(scales_at + buffer * Scales::kBytes);
+    for (int r = wave * kWave; r < BM + (p.bias ? 2 : 1) * BN; r += kWave * WM * WN) {
+      const float* from = r < BM        ? p.a_scales + min(next_i0 + r + lane, p.m - 1)
+                          : r < BM + BN ? p.b_scales + min(next_j0 + r - BM + lane, p.n - 1)
+                                        : p.bias + min(next_j0 + r - BM - BN + lane, p.n - 1);
+      __builtin_amdgcn_global_load_lds((const __attribute__((address_space(1))) void*)from,
+                                       (__attribute__((address_space(3))) void*)(to + r), 4, 0, 0);
+    }
+  };
+  // a half of a stage's loads (with one tile, stages past the last one repeat it: as many loads as the waits count)
+  auto issue = [&](uint32_t s, int part) {
     char* to = lds + s % NB * kBuffer + wave * I * 1024;
-    const int from = min(s, stages - 1) * kRow;
+    const uint32_t from = MANY ? 0 : min(s, stages - 1) * kRow;
 #pragma unroll
-    for (int q = part * I / 2; q < (part + 1) * I / 2; q++)
+    for (int q = part * I / 2; q < (part + 1) * I / 2; q++) {
       __builtin_amdgcn_global_load_lds((const __attribute__((address_space(1))) void*)(src[q] + from),
                                        (__attribute__((address_space(3))) void*)(to + q * 1024), 16, 0, 0);
+      if (MANY) src[q] += kRow;
+    }
   };
   i16v acc[TM][TN];
-#pragma unroll
-  for (int x = 0; x < TM; x++)
-#pragma unroll
-    for (int y = 0; y < TN; y++) acc[x][y] = i16v{};
   const int row = lane % 32, half = lane / 32;
   i4 fa[2][TM], fb[2][TN];
-  auto read = [&](int s, int q) {
+  auto read = [&](uint32_t s, int q) {
     const char* from = lds + s % NB * kBuffer + ((2 * q + half) ^ (row / 4 % 4)) * 16 + row * kRow;
 #pragma unroll
     for (int x = 0; x < TM; x++) fa[q][x] = *reinterpret_cast<const i4*>(from + (wm * TM + x) * 32 * kRow);
@@ -553,8 +570,14 @@ __global__ __launch_bounds__(64 * WM * WN, 1) void product_deep_kernel(Product<O
     asm volatile("" ::: "memory");
     __builtin_amdgcn_sched_barrier(0);
   };
-  const TileScales<BM, BN, 64 * WM * WN> scales(lds + NB * kBuffer, i0, j0, p);
-  __builtin_amdgcn_s_waitcnt(kWaitFor<0>);  // the waits below count the stages' loads alone
+  if (!p.bias) {
+    for (int r = threadIdx.x; r < BN; r += 64 * WM * WN)
+#pragma unroll
+      for (int buffer = 0; buffer < 2; buffer++) Scales(scales_at + buffer * Scales::kBytes).sa[BM + BN + r] = -0.f;
+  }
+  uint32_t turn = blockIdx.x;
+  place_next(turn);
+  turn_to_next(0);
 #pragma unroll
   for (int s = 0; s < NB; s++) {
     issue(s, 0);
@@ -564,26 +587,42 @@ __global__ __launch_bounds__(64 * WM * WN, 1) void product_deep_kernel(Product<O
   meet();
   read(0, 0);
   __builtin_amdgcn_s_waitcnt(kReadsDone);
-  for (int s = 0; s < stages; s++) {
-    read(s, 1);
-    issue(s + NB - 1, 1);
-    products(0);
-    between<TM + TN, kDsRead, 1>();
-    between<I / 2, kVmem, 2>();
-    __builtin_amdgcn_sched_barrier(0);
-    // stage s + 1 is there and every wave has read stage s
-    __builtin_amdgcn_s_waitcnt(kWaitFor<(NB - 2) * I>);
-    meet();
-    read(s + 1, 0);
-    issue(s + NB, 0);
-    products(1);
-    between<TM + TN, kDsRead, 1>();
-    between<I / 2, kVmem, 2>();
-    __builtin_amdgcn_s_waitcnt(kReadsDone);  // long since: said for the compiler, which else waits at the loop's top
-    __builtin_amdgcn_sched_barrier(0);
-  }
+  uint32_t s = 0, buffer = 0;
+  do {
+    i0 = next_i0;
+    j0 = next_j0;
+    turn += gridDim.x;
+    if (MANY) place_next(min(turn, tiles - 1));  // (after the last tile some tile's first stages, which nobody reads)
+#pragma unroll
+    for (int x = 0; x < TM; x++)
+#pragma unroll
+      for (int y = 0; y < TN; y++) {
+        acc[x][y] = i16v{};
+        asm volatile("" : "+a"(acc[x][y]));
+      }
+    for (uint32_t left = stages; left > 0; left--, s++) {
+      read(s, 1);
+      issue(s + NB - 1, 1);
+      products(0);
+      between<TM + TN, kDsRead, 1>();
+      between<I / 2, kVmem, 2>();
+      __builtin_amdgcn_sched_barrier(0);
+      // stage s + 1 is there and every wave has read stage s
+      __builtin_amdgcn_s_waitcnt(kWaitFor<(NB - 2) * I>);
+      meet();
+      if (MANY && left == NB) turn_to_next(buffer ^ 1);
+      read(s + 1, 0);
+      issue(s + NB, 0);
+      products(1);
+      between<TM + TN, kDsRead, 1>();
+      between<I / 2, kVmem, 2>();
+      __builtin_amdgcn_s_waitcnt(kReadsDone);  // long since: said for the compiler, which else waits at the loop's top
+      __builtin_amdgcn_sched_barrier(0);
+    }
+    Scales(scales_at + buffer * Scales::kBytes).store(acc, wm * TM * 32, wn * TN * 32, i0, j0, p);
+    buffer ^= 1;
+  } while (MANY && turn < tiles);
   __builtin_amdgcn_s_waitcnt(kWaitFor<0>);  // no load into LDS outlives the wave
-  scales.store(acc, wm * TM * 32, wn * TN * 32, i0, j0, p);
 }
 
 // Short rows, k <= 32 KS, whose product is mostly writing: 32 rows of a stay in a wave's
@@ -927,14 +966,14 @@ void launch_tiles(const Product<O>& p, hipStream_t st) {
   HIP_OK(hipGetLastError());
 }
 
-template <int BM, int BN, int WM, int WN, int NB, class O>
+template <int BM, int BN, int WM, int WN, int NB, bool MANY, class O>
 void launch_deep(const Product<O>& p, hipStream_t st) {
   const int64_t tm = (p.m + BM - 1) / BM, tn = (p.n + BN - 1) / BN;
   const int64_t group = std::min<int64_t>(tm, 8);
-  const int lds = NB * (BM + BN) * 64 + TileScales<BM, BN, 64 * WM * WN>::kBytes;
-  constexpr auto* kernel = &product_deep_kernel<BM, BN, WM, WN, NB, O>;
+  const int lds = NB * (BM + BN) * 64 + 2 * TileScales<BM, BN, 64 * WM * WN>::kBytes;
+  constexpr auto* kernel = &product_deep_kernel<BM, BN, WM, WN, NB, MANY, O>;
   allow_lds<kernel>(lds);
-  hipLaunchKernelGGL(kernel, dim3((unsigned)(tm * tn)), dim3(64 * WM * WN), lds, st, p, tm, tn, group);
+  hipLaunchKernelGGL(kernel, dim3((unsigned)(MANY ? std::min<int64_t>(tm * tn, 256) : tm * tn)), dim3(64 * WM * WN), lds, st, p, tm, tn, group);
   HIP_OK(hipGetLastError());
 }
 
@@ -978,9 +1017,9 @@ void product(const Product<O>& p, hipStream_t st) {
     auto tiles = [&](int64_t size) { return (p.m + size - 1) / size * ((p.n + size - 1) / size); };
     const bool direct = (reinterpret_cast<uintptr_t>(p.a) | reinterpret_cast<uintptr_t>(p.b) | p.a_stride | p.b_stride) % 16 == 0 &&
                         p.k % 64 == 0;
-    if (direct && p.k >= 2048 && tiles(256) >= 200) launch_deep<256, 256, 2, 2, 4>(p, st);
-    else if (direct && tiles(64) <= 512) launch_deep<64, 64, 2, 2, 4>(p, st);
-    else if (direct && tiles(128) <= 256) launch_deep<128, 128, 2, 2, 4>(p, st);
+    if (direct && p.k >= 2048 && tiles(256) >= 200) launch_deep<256, 256, 2, 2, 4, true>(p, st);
+    else if (direct && tiles(64) <= 512) launch_deep<64, 64, 2, 2, 4, false>(p, st);
+    else if (direct && tiles(128) <= 256) launch_deep<128, 128, 2, 2, 4, false>(p, st);
     else if (tiles(64) <= 512) launch_tiles<64, 64, 2, 2>(p, st);
     else launch_tiles<128, 128, 2, 2>(p, st);
   }
