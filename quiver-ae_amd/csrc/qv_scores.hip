@@ -386,7 +386,7 @@ __device__ __forceinline__ int64_t tile_of_block(int64_t block, int64_t tiles) {
 // operands' stages go through registers into LDS, the next one in flight while the
 // matrix cores work on this one; piece q of row r lies at q ^ (r / 2 mod 8), so that the
 // 16 rows that are read at once (64 banks, 256 bytes) lie in 16 different places.  For
-// rows of any alignment and length; 2,048 x 4,096 x 4,096 to bfloat16: 46 us, 1.5 POP/s.
+// rows of any alignment and length; 2,048 x 4,096 x 4,096 to bfloat16: 44 us, 1.6 POP/s.
 template <int BM, int BN, int WM, int WN, class O>
 __global__ __launch_bounds__(64 * WM * WN, 1) void product_tile_kernel(Product<O> p, int64_t tiles_m, int64_t tiles_n,
                                                                        int64_t group, int scales_at) {
@@ -475,10 +475,15 @@ __global__ __launch_bounds__(64 * WM * WN, 1) void product_tile_kernel(Product<O
 // and the next stage's first operands while the second one's do, so the one barrier
 // per stage, between the two, finds the operands of what follows it in registers.
 // Needs 16-byte aligned rows and k a multiple of 64.
-// 4,096^3 to bfloat16: 69 us, 2.0 POP/s (a library's int8 product with a 32-bit result: 69);
-// 8,192^3 of zeros 378 us, 2.9 POP/s, of codes over the whole range 550 us: then power
-// holds the clock at 1.5 GHz (the matrix instruction alone reaches 4.5 and 3.3 POP/s).
-// Loads and LDS reads in runs of their own instead of between the products: 86 us.
+// MANY: one workgroup per CU walks over tiles, and the stages run on from tile to tile:
+// the next tile's first ones are on their way, and its first operands in registers, while
+// the results are stored (10,000 x 50,048 x 512: 457 us, with a workgroup per tile 519).
+// 4,096^3 to bfloat16: 67 us, 2.05 POP/s (a library's int8 product with a 32-bit result:
+// 69), 72 with the results through LDS; 8,192^3 of zeros 349 us, 3.1 POP/s, of codes over
+// the whole range 545 us: then power holds the clock at 1.5 GHz (the matrix instruction
+// alone reaches 4.5 and 3.3 POP/s).  Loads and LDS reads in runs of their own instead of
+// between the products: 86 us.
+//
 // The schedule's next N x (P matrix instructions, one of the given kind): a matrix
 // instruction takes 32 cycles, in which a wave can issue a few others; in a run of
 // their own they would leave the matrix pipe idle.
@@ -1011,13 +1016,15 @@ void product(const Product<O>& p, hipStream_t st) {
     launch_panels<8>(p, st);
   } else {
     // By how many tiles there are for the 256 CUs.  Measured to bfloat16, us, with tiles of 256, 128 and 64 straight
-    // to LDS and of 128 through registers: 4,096^3: 73, 87, 136, 84; 2,048 x 4,096 x 4,096: 56, 48, 73, 46;
-    // 1,024: 53, 26, 42, 31; 512: 51, 22, 20, 29; 64: 45, 20, 13, 27; 4,096 x 4,096 x 1,024: 32, 32, 41, 31;
-    // 1,024 x 20,032 x 512: 42, 28, 32, 27.
+    // to LDS and of 128 through registers: 4,096^3: 71, 108, 156, 96; 2,048 x 4,096 x 4,096: 55, 51, 85, 44;
+    // 1,024: 51, 24, 41, 31; 512: 49, 20, 19, 28; 64: 46, 18, 13, 27; 4,096 x 4,096 x 1,024: 34, 36, 46, 34;
+    // 1,024 x 20,032 x 512: 40, 29, 36, 27; 10,000 x 50,048 x 512: 457, 510, 733, 583.  Tiles of 256 leave CUs without
+    // one in the last turn: 4,096 x 20,032 x 768 (4.9 turns): 97, 119, 171, 106; 512 x 100,032 x 768 (3.05): 74, 77, 103, 63.
     auto tiles = [&](int64_t size) { return (p.m + size - 1) / size * ((p.n + size - 1) / size); };
     const bool direct = (reinterpret_cast<uintptr_t>(p.a) | reinterpret_cast<uintptr_t>(p.b) | p.a_stride | p.b_stride) % 16 == 0 &&
                         p.k % 64 == 0;
-    if (direct && p.k >= 2048 && tiles(256) >= 200) launch_deep<256, 256, 2, 2, 4, true>(p, st);
+    const int64_t turns = (tiles(256) + 255) / 256;
+    if (direct && tiles(256) * 5 >= turns * 256 * 4) launch_deep<256, 256, 2, 2, 4, true>(p, st);
     else if (direct && tiles(64) <= 512) launch_deep<64, 64, 2, 2, 4, false>(p, st);
     else if (direct && tiles(128) <= 256) launch_deep<128, 128, 2, 2, 4, false>(p, st);
     else if (tiles(64) <= 512) launch_tiles<64, 64, 2, 2>(p, st);
