@@ -160,6 +160,17 @@ def test_product(scoring, dtype, m, n, k):
     _check_product(scoring.int8_product(a, sa, b, sb, bias=bias, dtype=dtype), a, sa, b, sb, bias, dtype)
 
 
+# 470 to 770 tiles of 256, which a workgroup takes two or three of; stages of 64 bytes in every remainder of 4
+@pytest.mark.parametrize("dtype", TYPES)
+@pytest.mark.parametrize("m, n, k, bias", [(260, 60001, 320, True), (300, 60160, 384, False), (257, 98000, 448, True),
+                                           (512, 60000, 512, False), (513, 61000, 576, True)])
+def test_product_many_tiles(scoring, dtype, m, n, k, bias):
+    say("product", dtype, m, n, k, bias)
+    a, sa, b, sb, add = _inputs(m, n, k, m + n + k)
+    out = scoring.int8_product(a, sa, b, sb, bias=add if bias else None, dtype=dtype)
+    _check_product(out, a, sa, b, sb, add if bias else None, dtype)
+
+
 @pytest.mark.parametrize("m, n, k", [(1, 40, 131071), (40, 70, 131071), (300, 300, 131071)])
 def test_product_largest_sums(scoring, m, n, k):
     """Every product 127^2, -127 128 or 128^2: sums just inside 32 bits."""
