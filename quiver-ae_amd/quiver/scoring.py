@@ -148,6 +148,7 @@ class LogProbs:
     _device: int
     _parts: tuple            # the buffers in the order above, the workspace last
     _at: tuple               # their addresses
+    _size: tuple             # rows, targets and alternatives per row, bytes of the workspace
 
     @staticmethod
     def empty(n: int, v: int, t: int, k: int, temperature: float, device: torch.device) -> "LogProbs":
@@ -173,7 +174,7 @@ class LogProbs:
     def of(target, entropy, logsumexp, top_ids, top, stats, temperature, workspace) -> "LogProbs":
         parts = (target, entropy, logsumexp, top_ids, top, stats, workspace)
         return LogProbs(target, entropy, logsumexp, top_ids, top, stats, temperature, workspace, stats.get_device(),
-                        parts, tuple(p.data_ptr() for p in parts))
+                        parts, tuple(p.data_ptr() for p in parts), (*target.shape, top.shape[1], workspace.shape[0]))
 
 
 def _given(targets: torch.Tensor | None, rows: int) -> tuple[int | None, int]:
@@ -192,7 +193,7 @@ def _forward(logits, targets, top_k, temperature, out) -> LogProbs:
     again = out is not None
     if not again:
         out = LogProbs.empty(n, v, t, top_k, temperature, logits.device)
-    elif out.target.shape != (n, t) or out.top.shape != (n, top_k):
+    elif out._size[:3] != (n, t, top_k):
         raise ValueError("out was made for another number of rows, targets or alternatives")
     elif out.temperature != temperature:
         out = replace(out, temperature=temperature)
@@ -202,7 +203,7 @@ def _forward(logits, targets, top_k, temperature, out) -> LogProbs:
     at_target, at_entropy, at_lse, at_ids, at_top, at_stats, at_work = out._at
     _lib.check(_lib.load().qv_log_probs(logits.data_ptr(), _TYPES[logits.dtype], n, v, stride, temperature, at_targets,
                                         t, top_k, at_target, at_entropy, at_lse, at_stats, at_ids, at_top, at_work,
-                                        out._workspace.shape[0], device, _raw_stream(device)))
+                                        out._size[3], device, _raw_stream(device)))
     if again:
         _written(out._parts)
     return out
