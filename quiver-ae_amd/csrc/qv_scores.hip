@@ -223,54 +223,86 @@ __device__ __forceinline__ uint32_t two_of(float x, float y) {
   }
 }
 
-// Scales an instruction's result, 32 columns from j of the rows around the lane's row i, and stores it from the
-// registers: 16 bytes per lane, 32 of each row at once.  Of the four columns that a lane has of every eight, those
-// of 16 bits pass to the other half of the wave and back, eight for a lane.  `sb`, `add`: the columns' scales and
-// biases in LDS.  WHOLE: all of it lies in the output.
-template <bool WHOLE, class O>
-__device__ __forceinline__ void store_sums(const i16v& acc, float sa, const float* sb, const float* add, int64_t i,
-                                           int64_t j, const Product<O>& p) {
-  constexpr int V = 16 / (int)sizeof(O), N = 16 / V;  // columns of a store, stores
-  const int half = lane_id() / 32;
-  float v[16];
+// Of P pieces of 16 bytes in each of P lanes, the lane's own one of every lane: the P x P transposed.
+template <int P>
+__device__ __forceinline__ void swap_pieces(i4 (&u)[P]) {
+  auto stage = [&](auto distance, auto control) {
+    constexpr int D = decltype(distance)::value, kControl = decltype(control)::value;
+    const bool up = lane_id() & D;
 #pragma unroll
-  for (int g = 0; g < 4; g++) {
-    const f4 s = *reinterpret_cast<const f4*>(sb + 8 * g + 4 * half), t = *reinterpret_cast<const f4*>(add + 8 * g + 4 * half);
+    for (int q = 0; q < P; q++) {
+      if (q & D) continue;
 #pragma unroll
-    for (int e = 0; e < 4; e++) v[4 * g + e] = ((float)acc[4 * g + e] * sa) * s[e] + t[e];
-  }
-  union {
-    O o[V];
-    uint32_t w[4];
-    i4 raw;
-  } u[N];
+      for (int w = 0; w < 4; w++) {
+        const int lo = u[q][w], hi = u[q | D][w];
+        const int other_lo = __builtin_amdgcn_mov_dpp(lo, kControl, 0xF, 0xF, true);
+        const int other_hi = __builtin_amdgcn_mov_dpp(hi, kControl, 0xF, 0xF, true);
+        u[q][w] = up ? other_hi : lo;
+        u[q | D][w] = up ? hi : other_lo;
+      }
+    }
+  };
+  stage(std::integral_constant<int, 1>(), std::integral_constant<int, 0xB1>());                          // quad_perm [1,0,3,2]
+  if constexpr (P == 4) stage(std::integral_constant<int, 2>(), std::integral_constant<int, 0x4E>());  // quad_perm [2,3,0,1]
+}
+
+// Scales the results of R instructions, 32 R columns from j of the rows around the lane's row i, and stores them from
+// the registers, whole lines of 8 rows at once (half lines of 16 rows with 32 columns of 16 bits).  Of the four columns
+// that a lane has of every eight, those of 16 bits pass to the other half of the wave and back, eight for a lane; then
+// groups of lanes swap rows for pieces of one row.  (Pieces stored as they are, 32 bytes of 32 rows at once, take 5.0
+// for 5.35 TB/s in aligned rows, 2 for 3.8 in others.)  `sb`, `add`: the columns' scales and biases in LDS.  WHOLE:
+// all of it lies in the output.
+template <bool WHOLE, int R, class O>
+__device__ __forceinline__ void store_sums(const i16v* const (&acc)[R], float sa, const float* sb, const float* add,
+                                           int64_t i, int64_t j, const Product<O>& p) {
+  constexpr int V = 16 / (int)sizeof(O), N = 16 / V, P = R * N;  // columns of a piece, pieces of a result, of all
+  const int half = lane_id() / 32, c = lane_id() % P;
+  i4 u[P];
 #pragma unroll
-  for (int q = 0; q < N; q++) {
-    if constexpr (sizeof(O) == 4) {
+  for (int y = 0; y < R; y++) {
+    float v[16];
 #pragma unroll
-      for (int e = 0; e < 4; e++) u[q].o[e] = v[4 * q + e];
-    } else {
+    for (int g = 0; g < 4; g++) {
+      const int at = 32 * y + 8 * g + 4 * half;
+      const f4 s = *reinterpret_cast<const f4*>(sb + at), t = *reinterpret_cast<const f4*>(add + at);
 #pragma unroll
-      for (int d = 0; d < 2; d++) {
-        const auto both = __builtin_amdgcn_permlane32_swap(two_of<O>(v[8 * q + 2 * d], v[8 * q + 2 * d + 1]),
-                                                           two_of<O>(v[8 * q + 4 + 2 * d], v[8 * q + 5 + 2 * d]), false, false);
-        u[q].w[d] = both[0];
-        u[q].w[2 + d] = both[1];
+      for (int e = 0; e < 4; e++) v[4 * g + e] = ((float)(*acc[y])[4 * g + e] * sa) * s[e] + t[e];
+    }
+#pragma unroll
+    for (int q = 0; q < N; q++) {
+      if constexpr (sizeof(O) == 4) {
+#pragma unroll
+        for (int e = 0; e < 4; e++) u[N * y + q][e] = __float_as_int(v[4 * q + e]);
+      } else {
+#pragma unroll
+        for (int d = 0; d < 2; d++) {
+          const auto both = __builtin_amdgcn_permlane32_swap(two_of<O>(v[8 * q + 2 * d], v[8 * q + 2 * d + 1]),
+                                                             two_of<O>(v[8 * q + 4 + 2 * d], v[8 * q + 5 + 2 * d]), false, false);
+          u[N * y + q][d] = (int)both[0];
+          u[N * y + q][2 + d] = (int)both[1];
+        }
       }
     }
   }
-  if (!WHOLE && i >= p.m) return;
-  O* to = p.out + (i * p.out_stride + j + V * half);
+  swap_pieces(u);
+  i -= c;
+  j += 2 * V * c + V * half;
+  O* to = p.out + (i * p.out_stride + j);
+  if (WHOLE || j + V <= p.n) {
 #pragma unroll
-  for (int q = 0; q < N; q++) {
-    const int64_t at = j + 2 * V * q + V * half;
-    O* dst = to + 2 * V * q;
-    if (WHOLE || at + V <= p.n) {
-      *reinterpret_cast<i4_any*>(dst) = u[q].raw;
-    } else {
+    for (int r = 0; r < P; r++)
+      if (WHOLE || i + r < p.m) *reinterpret_cast<i4_any*>(to + r * p.out_stride) = u[r];
+  } else {
+#pragma unroll
+    for (int r = 0; r < P; r++) {
+      union {
+        i4 raw;
+        O o[V];
+      } piece;
+      piece.raw = u[r];
 #pragma unroll
       for (int e = 0; e < V; e++)
-        if (at + e < p.n) dst[e] = u[q].o[e];
+        if (i + r < p.m && j + e < p.n) to[r * p.out_stride + e] = piece.o[e];
     }
   }
 }
@@ -359,14 +391,20 @@ struct TileScales {
   // A wave's results, from row i and column j of the tile at (i0, j0) on.
   template <bool WHOLE, int TM, int TN, class O>
   __device__ __forceinline__ void store_all(i16v (&acc)[TM][TN], int i, int j, int64_t i0, int64_t j0, const Product<O>& p) const {
+    constexpr int R = sizeof(O) == 2 && TN % 2 == 0 ? 2 : 1;
     const float *sb = sa + BM + j, *add = sb + BN;
     i += lane_id() % 32;
 #pragma unroll
     for (int x = 0; x < TM; x++)
 #pragma unroll
-      for (int y = 0; y < TN; y++) {
-        asm volatile("" : "+a"(acc[x][y]) : : "memory");  // one at a time: none leaves its accumulators before
-        store_sums<WHOLE>(acc[x][y], sa[i + 32 * x], sb + 32 * y, add + 32 * y, i0 + i + 32 * x, j0 + j + 32 * y, p);
+      for (int y = 0; y < TN; y += R) {
+        const i16v* from[R];
+#pragma unroll
+        for (int r = 0; r < R; r++) {
+          asm volatile("" : "+a"(acc[x][y + r]) : : "memory");  // in turn: none leaves its accumulators before
+          from[r] = &acc[x][y + r];
+        }
+        store_sums<WHOLE>(from, sa[i + 32 * x], sb + 32 * y, add + 32 * y, i0 + i + 32 * x, j0 + j + 32 * y, p);
       }
   }
   template <int TM, int TN, class O>
@@ -478,11 +516,12 @@ __global__ __launch_bounds__(64 * WM * WN, 1) void product_tile_kernel(Product<O
 // MANY: one workgroup per CU walks over tiles, and the stages run on from tile to tile:
 // the next tile's first ones are on their way, and its first operands in registers, while
 // the results are stored (10,000 x 50,048 x 512: 457 us, with a workgroup per tile 519).
-// 4,096^3 to bfloat16: 67 us, 2.05 POP/s (a library's int8 product with a 32-bit result:
-// 69), 72 with the results through LDS; 8,192^3 of zeros 349 us, 3.1 POP/s, of codes over
-// the whole range 545 us: then power holds the clock at 1.5 GHz (the matrix instruction
-// alone reaches 4.5 and 3.3 POP/s).  Loads and LDS reads in runs of their own instead of
-// between the products: 86 us.
+// 4,096^3 to bfloat16: 67 to 71 us among other work, 2.0 POP/s (a library's int8 product
+// with a 32-bit result: 69), 74 one after the other: then power holds the clock down.
+// 8,192 x 8,192 x 4,096: 263 us (with the results through LDS and a tile per workgroup
+// 273); 8,192^3 of zeros 349 us, 3.1 POP/s, of codes over the whole range 545 us at 1.5
+// GHz (the matrix instruction alone reaches 4.5 and 3.3 POP/s).  Loads and LDS reads in
+// runs of their own instead of between the products: a fifth more.
 //
 // The schedule's next N x (P matrix instructions, one of the given kind): a matrix
 // instruction takes 32 cycles, in which a wave can issue a few others; in a run of
@@ -1019,12 +1058,13 @@ void product(const Product<O>& p, hipStream_t st) {
     // to LDS and of 128 through registers: 4,096^3: 71, 108, 156, 96; 2,048 x 4,096 x 4,096: 55, 51, 85, 44;
     // 1,024: 51, 24, 41, 31; 512: 49, 20, 19, 28; 64: 46, 18, 13, 27; 4,096 x 4,096 x 1,024: 34, 36, 46, 34;
     // 1,024 x 20,032 x 512: 40, 29, 36, 27; 10,000 x 50,048 x 512: 457, 510, 733, 583.  Tiles of 256 leave CUs without
-    // one in the last turn: 4,096 x 20,032 x 768 (4.9 turns): 97, 119, 171, 106; 512 x 100,032 x 768 (3.05): 74, 77, 103, 63.
+    // one in the last turn, or rows of tiles empty: of 256 CUs' tiles, 4,096 x 20,032 x 768 fills 98 % in 5 turns: 97,
+    // 119, 171, 106; 512 x 100,032 x 768 76 % in 4: 74, 77, 103, 63; 300 x 60,001 x 1,024 54 % in 2: 49, -, -, 42.
     auto tiles = [&](int64_t size) { return (p.m + size - 1) / size * ((p.n + size - 1) / size); };
     const bool direct = (reinterpret_cast<uintptr_t>(p.a) | reinterpret_cast<uintptr_t>(p.b) | p.a_stride | p.b_stride) % 16 == 0 &&
                         p.k % 64 == 0;
     const int64_t turns = (tiles(256) + 255) / 256;
-    if (direct && tiles(256) * 5 >= turns * 256 * 4) launch_deep<256, 256, 2, 2, 4, true>(p, st);
+    if (direct && (double)p.m * p.n >= 0.8 * 65536 * 256 * turns) launch_deep<256, 256, 2, 2, 4, true>(p, st);
     else if (direct && tiles(64) <= 512) launch_deep<64, 64, 2, 2, 4, false>(p, st);
     else if (direct && tiles(128) <= 256) launch_deep<128, 128, 2, 2, 4, false>(p, st);
     else if (tiles(64) <= 512) launch_tiles<64, 64, 2, 2>(p, st);
