@@ -341,8 +341,10 @@ struct Pass {
     }
   }
 
-  // Batches b, b + step, ... of columns [from, to), the next one's values on their way.
-  __device__ void run(const T* __restrict__ x, int64_t from, int64_t to, int b, int step, volatile uint32_t* shared) {
+  // Batches b, b + step, ... of columns [from, to), the next one's values on their way.  Always inline: in a function of
+  // its own the uniform bounds count as per-lane ones, with a stack and three times the time.
+  __device__ __forceinline__ void run(const T* __restrict__ x, int64_t from, int64_t to, int b, int step,
+                                      volatile uint32_t* shared) {
     const int lane = lane_id();
     int turn = 0;
     raw4 r[U];
