@@ -209,18 +209,14 @@ __device__ __forceinline__ void put_sums(int32_t* tile, int stride, int j0, cons
   }
 }
 
-// Two values in the output's 16 bits, halves to even.
+// Two values in the output's 16 bits, halves to even.  By instruction: the compiler takes the bfloat16 one apart, and
+// joins float16 to the product before it, whose rounding to fp32 is then left out.
 template <class O>
 __device__ __forceinline__ uint32_t two_of(float x, float y) {
-  if constexpr (std::is_same<O, bf16>::value) {  // at once, which the compiler takes apart
-    uint32_t both;
-    asm("v_cvt_pk_bf16_f32 %0, %1, %2" : "=v"(both) : "v"(x), "v"(y));
-    return both;
-  } else {
-    typedef float f2 __attribute__((ext_vector_type(2)));
-    typedef O o2 __attribute__((ext_vector_type(2)));
-    return __builtin_bit_cast(uint32_t, __builtin_convertvector((f2{x, y}), o2));
-  }
+  uint32_t both;
+  if constexpr (std::is_same<O, bf16>::value) asm("v_cvt_pk_bf16_f32 %0, %1, %2" : "=v"(both) : "v"(x), "v"(y));
+  else asm("v_cvt_pk_f16_f32 %0, %1, %2" : "=v"(both) : "v"(x), "v"(y));
+  return both;
 }
 
 // Of P pieces of 16 bytes in each of P lanes, the lane's own one of every lane: the P x P transposed.

@@ -171,6 +171,21 @@ def test_product_many_tiles(scoring, dtype, m, n, k, bias):
     _check_product(out, a, sa, b, sb, add if bias else None, dtype)
 
 
+# each way that a product takes
+@pytest.mark.parametrize("dtype", TYPES)
+@pytest.mark.parametrize("m, n, k", [(5, 3000, 9), (5, 3000, 100), (20, 700, 2049), (100, 3000, 128), (100, 3001, 200),
+                                     (64, 4096, 1024), (700, 4000, 1024), (512, 60000, 512), (100, 900, 4001),
+                                     (1500, 3300, 1001)])
+def test_product_bits(scoring, dtype, m, n, k):
+    """Exact sums, then fp32 in the written order and one rounding to the type: the same bits from every kernel."""
+    say("product, bits", dtype, m, n, k)
+    a, sa, b, sb, bias = _inputs(m, n, k, m + 3 * n + 5 * k)
+    sa = sa * 0.05
+    want = ((a.double() @ b.double().T.contiguous()).float() * sa[:, None]) * sb[None, :]
+    assert torch.equal(scoring.int8_product(a, sa, b, sb, dtype=dtype), want.to(dtype))
+    assert torch.equal(scoring.int8_product(a, sa, b, sb, bias=bias, dtype=dtype), (want + bias[None, :]).to(dtype))
+
+
 @pytest.mark.parametrize("m, n, k", [(1, 40, 131071), (40, 70, 131071), (300, 300, 131071)])
 def test_product_largest_sums(scoring, m, n, k):
     """Every product 127^2, -127 128 or 128^2: sums just inside 32 bits."""
