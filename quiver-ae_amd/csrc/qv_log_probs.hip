@@ -3,11 +3,17 @@
 //
 // Everything is computed in base 2 relative to a running largest value m: with c =
 // log2(e) / T, s = sum 2^y and w = sum y 2^y over y = x c - m c, a row's ln S is
-// log2(s) ln 2 and its entropy ln 2 (log2(s) - w / s), which no cancellation
-// touches (w <= 0, s >= 1).  One pass over the row: a lane keeps its own m, s and w
-// and moves them to a new m only when a batch of its values holds a larger one.
-// The reference subtracted is fl(m c), not m c, so that y is one fused
-// multiply-add; the difference (fma(-m, c, fl(m c)), exact) enters once at the end.
+// log2(s) ln 2 and its entropy ln 2 (log2(s) - w / s).  One pass over the row: a lane
+// keeps its own m, s and w and moves them to a new m only when a batch of its values
+// holds a larger one.
+// The reference subtracted is fl(m c), not m c, so that y is one fused multiply-add;
+// the difference r = fma(m, c, -fl(m c)), exact, is the y of m itself and enters once at
+// the end.  It is half a unit in the last place of m c at most: 1/32 below |m c| = 2^20,
+// so that s >= 0.97, w <= s / 32, and no cancellation in log2(s) or the entropy passes
+// that.  From 2^20 on (a lane that has seen only masks of some large finite value, or
+// logits and temperatures far from common ones) it would grow past what 2^y can hold:
+// there the reference is m c itself and y = (x - m) c, two instructions.  Sums of lanes on
+// different sides of 2^20 differ by r, which shift_of counts in.
 //
 // What bounds it: reading the logits, beside about 10 vector instructions and one
 // exponential for each.  256 x 200,000 bfloat16 with 20 alternatives: 28 us a pass, 3.7
@@ -27,7 +33,7 @@ namespace {
 
 constexpr float kInf = __builtin_inff();
 constexpr float kLog2e = 1.44269504088896340736f, kLn2 = 0.69314718055994530942f;
-constexpr float kBig = 1e38f;    // |m c| from here on: differences are taken before they are multiplied
+constexpr float kBig = 0x1p20f;  // |m c| from here on: differences are taken before they are multiplied
 constexpr float kNone = -200.f;  // 2^-200 is 0 in fp32: stands for -inf where it would be multiplied by 0
 
 // ---- values ------------------------------------------------------------------
@@ -223,13 +229,18 @@ __device__ __forceinline__ uint32_t common_bound(const volatile uint32_t* bounds
 __device__ __forceinline__ float scaled(float m, float c) { return m == -kInf ? 0.f : m * c; }
 __device__ __forceinline__ bool is_big(float mc) { return !(fabsf(mc) < kBig); }
 
+// What the reference of m lacks of m c; mc: scaled(m, c).
+__device__ __forceinline__ float residue(float m, float mc, float c) { return is_big(mc) ? 0.f : __fmaf_rn(m, c, -mc); }
+
 // log2 of what sums relative to m are multiplied by when the reference becomes
-// to >= m: their two rounded references' difference, or, where those overflow, the
-// difference's product (then 0 or far below every value that counts).
+// to >= m: the two references' difference, of rounded ones as they are, else from the
+// difference of m and to.
 __device__ __forceinline__ float shift_of(float m, float to, float c) {
+  if (m == -kInf) return kNone;
   const float a = scaled(m, c), b = scaled(to, c);
-  const float d = is_big(a) || is_big(b) ? (m == to ? 0.f : (m - to) * c) : a - b;
-  return m == -kInf ? kNone : max2(d, kNone);
+  float d = a - b;
+  if (is_big(a) || is_big(b)) d = m == to ? 0.f : (m - to) * c + (residue(to, b, c) - residue(m, a, c));
+  return max2(d, kNone);
 }
 
 struct Sums {
@@ -403,8 +414,7 @@ __device__ __forceinline__ void finish_row(const Given& given, int64_t row, int 
   const bool odd = sum.s != sum.s, empty = sum.s == 0.f;
   const float nan = __builtin_nanf("");
   const float mc = scaled(sum.m, c);
-  // log2 of the sum relative to m c itself
-  const float log2_s = log2f(sum.s) + (is_big(mc) ? 0.f : __fmaf_rn(-sum.m, c, mc));
+  const float log2_s = log2f(sum.s) - residue(sum.m, mc, c);  // of the sum relative to m c itself
   const float ln_s = odd ? nan : empty ? -kInf : log2_s * kLn2;
   auto lp = [&](float v) { return odd ? nan : v == -kInf ? -kInf : __fmaf_rn(v - sum.m, inv_t, -ln_s); };
   if (lane == 0) {

@@ -481,3 +481,71 @@ def test_catalogue(scoring):
     lp = torch.log_softmax(exact, 1)
     assert (a.target.double() - lp.gather(1, targets.long())).abs().max() < 0.11
     assert ((a.top_ids[:, 0].long() == lp.argmax(1)).double().mean()) > 0.95
+
+
+# one wave per row of one load and of more, 4 and 16 waves, chunks
+RANGE_COLS = [100, 700, 5000, 20000, 40000]
+
+
+@pytest.mark.parametrize("dtype", TYPES)
+@pytest.mark.parametrize("v", RANGE_COLS)
+def test_finite_masks(scoring, dtype, v):
+    """Masks of finite values, in whole lanes, whole rows, the half, the tail, here and there, all but one column."""
+    say("log probs, finite masks", dtype, v)
+    masks = [-1e4, -6e4] if dtype == torch.float16 else [-1e4, -1e9, -1e10, -1e12, -1e20, -1e30, -1e37]
+    g = torch.Generator(device="cuda").manual_seed(v)
+    rows = 6 * len(masks)
+    targets = torch.tensor([0, v // 2, v - 1], dtype=torch.int32, device="cuda").repeat(rows, 1)
+    for T in (0.05, 0.1, 1.0, 2.0):
+        x = torch.randn((rows, v), generator=g, device="cuda") * 3 * T
+        for i, mask in enumerate(masks):
+            at = x[6 * i:6 * i + 6]
+            at[0, :8] = mask
+            at[1] = mask
+            at[2, :v // 2] = mask
+            at[3, v // 3:] = mask
+            at[4, torch.rand(v, generator=g, device="cuda") < 0.9] = mask
+            at[5, :v - 2] = mask
+            at[5, v - 1] = mask
+        _run(scoring, x.to(dtype), targets, 12, T)
+
+
+@pytest.mark.parametrize("dtype", [torch.float32, torch.bfloat16])
+@pytest.mark.parametrize("v", RANGE_COLS)
+def test_large_logits(scoring, dtype, v):
+    """Rows around values up to 1e37, the ones where differences begin to be taken first (2^20 / log2(e) at T = 1) among them."""
+    say("log probs, large logits", dtype, v)
+    g = torch.Generator(device="cuda").manual_seed(v)
+    for T in (0.05, 1.0):
+        limit = 2.0 ** 20 * math.log(2) * T
+        bases = [s * b for b in (1e5, limit, 1e7, 1e9, 3e12, 1e20, 1e30, 1e37) for s in (1, -1)]
+        spread = torch.tensor([max(20 * T, abs(b) * 2.0 ** -21) for b in bases], device="cuda")
+        x = torch.tensor(bases, device="cuda")[:, None] + spread[:, None] * torch.randn((len(bases), v), generator=g, device="cuda")
+        x[2::4, ::5] *= 0.5  # lanes far apart, too
+        targets = torch.tensor([0, v // 2, v - 1], dtype=torch.int32, device="cuda").repeat(len(bases), 1)
+        targets[:, 0] = x.argmax(1)
+        _run(scoring, x.to(dtype), targets, 12, T)
+
+
+@pytest.mark.parametrize("dtype", TYPES)
+@pytest.mark.parametrize("v", RANGE_COLS)
+def test_low_temperatures(scoring, dtype, v):
+    """Nearly greedy temperatures: ties share the probability, the next value has next to none."""
+    say("log probs, low temperatures", dtype, v)
+    g = torch.Generator(device="cuda").manual_seed(v)
+    x = torch.randn((8, v), generator=g, device="cuda") * 3
+    x[1] = 12.7
+    x[2, :] = 12.7
+    x[2, 1::3] = 12.699999
+    x[3, 1:] = 29
+    x[3, 0] = 30
+    x[4] = 0
+    x[5] = -x[1]
+    x[6] = 7.1
+    x[6, v // 2:] = 5
+    x[7] = torch.where(x[7] > 1, 5.3, -1e4)
+    x = x.to(dtype)
+    targets = torch.stack([x.argmax(1), x.argmin(1)], 1).to(torch.int32)
+    for T in (1e-3, 1e-6, 1e-8, 1e-9, 1e-10, 1e-12, 1e-20, 1e-37):
+        # (gradients go with 1 / T: within the type's range only)
+        _run(scoring, x, targets, 12, T, grads=dtype != torch.float16 and T > 1e-30)
