@@ -700,10 +700,14 @@ Plan plan_of(int64_t rows, int64_t cols) {
   return {4, (int)((most + steps - 1) / steps), steps * kStep};
 }
 
+// What the kernels multiply by.
+float log2e_over(float temperature) { return (float)(1.44269504088896340736 / (double)temperature); }
+float one_over(float temperature) { return (float)(1.0 / (double)temperature); }
+
 template <class T, bool TOP>
 void log_probs(const T* x, int64_t rows, int64_t cols, int64_t stride, float temperature, const Out& o, void* work,
                hipStream_t st) {
-  const float c = (float)(1.44269504088896340736 / (double)temperature), inv_t = (float)(1.0 / (double)temperature);
+  const float c = log2e_over(temperature), inv_t = one_over(temperature);
   const Plan p = plan_of(rows, cols);
   if (p.waves == 1) {
     auto* kernel = cols <= kWave * kVec<T> ? log_probs_wave_kernel<T, 1, TOP> : log_probs_wave_kernel<T, 16 / kVec<T>, TOP>;
@@ -730,7 +734,7 @@ template <class T>
 void log_probs_grad(const T* x, int64_t rows, int64_t cols, int64_t stride, float temperature, const Weights& g,
                     T* grad, int64_t grad_stride, hipStream_t st) {
   constexpr int U = 16 / kVec<T>;
-  const float c = (float)(1.44269504088896340736 / (double)temperature), inv_t = (float)(1.0 / (double)temperature);
+  const float c = log2e_over(temperature), inv_t = one_over(temperature);
   const int64_t chunk = 4 * kWave * U * kVec<T>;
   const int64_t splits = (cols + chunk - 1) / chunk, units = rows * splits;
   in_launches((units + 3) / 4, 256, [&](int64_t first, unsigned count) {
@@ -748,8 +752,8 @@ int64_t workspace_of(int64_t rows, int64_t cols, int32_t topk) {
 void check_rows(int32_t type, int64_t rows, int64_t cols, int64_t stride, const void* x, float temperature,
                 const int32_t* targets, int32_t per_row, int32_t topk) {
   check_matrix("logits", x, rows, cols, stride, value_size(type));
-  if (!(temperature > 0.f) || !(1.f / temperature < kInf) || !(1.f / temperature > 0.f))
-    qv::fail(QV_EINVAL, "temperature must be positive, and its reciprocal a finite float");
+  if (!(temperature > 0.f) || !(log2e_over(temperature) < kInf) || !(one_over(temperature) > 0.f))
+    qv::fail(QV_EINVAL, "temperature must be positive and finite, and log2(e) / temperature a finite float");
   if (cols > INT32_MAX || rows > INT32_MAX) qv::fail(QV_EUNSUPPORTED, "more than 2^31 - 1 rows or columns");
   if (per_row < 0) qv::fail(QV_EINVAL, "targets_per_row must not be negative");
   if (per_row > QV_LOG_PROBS_MAX_TARGETS) qv::fail(QV_EUNSUPPORTED, "more than 64 targets per row");

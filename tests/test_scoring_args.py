@@ -180,3 +180,14 @@ def test_buffers_refused(lib):
 
     with pytest.raises(lib.QuiverError, match="more than 2\\^31 - 1 rows or columns"):
         scoring.LogProbs.empty(1, 2 ** 31, 0, 4, 1.0, torch.device("cuda"))
+
+
+@pytest.mark.parametrize("temp, fine", [(1.2e-38, True), (1e-30, True), (1e38, True), (4.2e-39, False), (4e-39, False), (3e-39, False)])
+def test_temperature_range(lib, buf, temp, fine):
+    """A temperature whose reciprocal is finite and log2(e) times it is not would make every row NaN: refused."""
+    L, p = lib.load(), _at(buf)
+    rcs = [L.qv_log_probs(p, lib.QV_FLOAT, 0, 8, 8, temp, None, 0, 0, None, p, p, p, None, None, p, 64, 0, None),
+           L.qv_log_probs_grad(p, lib.QV_FLOAT, 0, 8, 8, temp, p, p, None, 0, None, 0, None, p, None, None, p, 8, 0, None)]
+    assert rcs == [lib.QV_OK if fine else lib.QV_EINVAL] * 2
+    if not fine:
+        assert b"temperature" in L.qv_last_error()
