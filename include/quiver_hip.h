@@ -507,7 +507,7 @@ int qv_int8_product(const int8_t* d_a, int64_t a_stride, const float* d_a_scales
  * A column at -inf has probability 0.  A row with no column above -inf (or with
  * no column): log probabilities and lse -inf, entropy 0.  A row that holds +inf
  * or NaN has no distribution: NaN, ids -1.  temperature: positive and finite,
- * log2(e) / temperature finite too (from 4.3e-39 on).  type as qv_quantize_rows; cols <
+ * 2 log2(e) / temperature finite too (from 8.5e-39 on).  type as qv_quantize_rows; cols <
  * 2^31; targets_per_row in [0, QV_LOG_PROBS_MAX_TARGETS]; topk in [0,
  * QV_LOG_PROBS_MAX_TOPK]; d_targets / d_target may be NULL with targets_per_row
  * 0, d_top_ids / d_top with topk 0; d_entropy and d_lse may be NULL.

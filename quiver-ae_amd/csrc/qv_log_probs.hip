@@ -12,7 +12,8 @@
 // so that s >= 0.97, w <= s / 32, and no cancellation in log2(s) or the entropy passes
 // that.  From 2^20 on (a lane that has seen only masks of some large finite value, or
 // logits and temperatures far from common ones) it would grow past what 2^y can hold:
-// there the reference is m c itself and y = (x - m) c, two instructions.  Sums of lanes on
+// there the reference is m c itself and y = (x - m) c (as half the difference, which no
+// two floats make infinite, and twice c), two instructions.  Sums of lanes on
 // different sides of 2^20 differ by r, which shift_of counts in.
 //
 // What bounds it: reading the logits, beside about 10 vector instructions and one
@@ -229,6 +230,9 @@ __device__ __forceinline__ uint32_t common_bound(const volatile uint32_t* bounds
 __device__ __forceinline__ float scaled(float m, float c) { return m == -kInf ? 0.f : m * c; }
 __device__ __forceinline__ bool is_big(float mc) { return !(fabsf(mc) < kBig); }
 
+// Half of a - b, which is finite where both are (a - b itself passes the largest float at most by a factor of two).
+__device__ __forceinline__ float half_apart(float a, float b) { return __fmaf_rn(a, 0.5f, -0.5f * b); }
+
 // What the reference of m lacks of m c; mc: scaled(m, c).
 __device__ __forceinline__ float residue(float m, float mc, float c) { return is_big(mc) ? 0.f : __fmaf_rn(m, c, -mc); }
 
@@ -239,7 +243,7 @@ __device__ __forceinline__ float shift_of(float m, float to, float c) {
   if (m == -kInf) return kNone;
   const float a = scaled(m, c), b = scaled(to, c);
   float d = a - b;
-  if (is_big(a) || is_big(b)) d = m == to ? 0.f : (m - to) * c + (residue(to, b, c) - residue(m, a, c));
+  if (is_big(a) || is_big(b)) d = m == to ? 0.f : half_apart(m, to) * (2.f * c) + (residue(to, b, c) - residue(m, a, c));
   return max2(d, kNone);
 }
 
@@ -315,7 +319,7 @@ struct Pass {
       const bool far = is_big(mc);
 #pragma unroll
       for (int i = 0; i < N; i++) {
-        const float y = far ? (v[i] - sum.m) * c : __fmaf_rn(v[i], c, -mc), e = __builtin_amdgcn_exp2f(y);
+        const float y = far ? half_apart(v[i], sum.m) * (2.f * c) : __fmaf_rn(v[i], c, -mc), e = __builtin_amdgcn_exp2f(y);
         s = s + e;
         w = __fmaf_rn(e, max2(y, kNone), w);
       }
@@ -416,7 +420,7 @@ __device__ __forceinline__ void finish_row(const Given& given, int64_t row, int 
   const float mc = scaled(sum.m, c);
   const float log2_s = log2f(sum.s) - residue(sum.m, mc, c);  // of the sum relative to m c itself
   const float ln_s = odd ? nan : empty ? -kInf : log2_s * kLn2;
-  auto lp = [&](float v) { return odd ? nan : v == -kInf ? -kInf : __fmaf_rn(v - sum.m, inv_t, -ln_s); };
+  auto lp = [&](float v) { return odd ? nan : v == -kInf ? -kInf : __fmaf_rn(half_apart(v, sum.m), 2.f * inv_t, -ln_s); };
   if (lane == 0) {
     if (o.entropy) o.entropy[row] = odd ? nan : empty ? 0.f : (log2f(sum.s) - sum.w / sum.s) * kLn2;
     if (o.lse) o.lse[row] = odd ? nan : empty ? -kInf : __fmaf_rn(sum.m, inv_t, ln_s);
@@ -600,7 +604,7 @@ __global__ __launch_bounds__(256) void log_probs_grad_kernel(const T* logits, in
   const float a = odd ? nan : empty ? 0.f : -(total + ge * h) * inv_t;
   const float b = empty ? 0.f : -(ge * kLn2) * inv_t;
   auto dense = [&](float v) {
-    const float y = max2(__fmaf_rn(v - m, c, -log2_s), kNone);
+    const float y = max2(__fmaf_rn(half_apart(v, m), 2.f * c, -log2_s), kNone);
     // the instruction gives 0 below 2^-126: probabilities down there are taken 2^64 larger
     const bool low = y < -126.f;
     const float p = __builtin_amdgcn_exp2f(low ? y + 64.f : y);
@@ -752,8 +756,8 @@ int64_t workspace_of(int64_t rows, int64_t cols, int32_t topk) {
 void check_rows(int32_t type, int64_t rows, int64_t cols, int64_t stride, const void* x, float temperature,
                 const int32_t* targets, int32_t per_row, int32_t topk) {
   check_matrix("logits", x, rows, cols, stride, value_size(type));
-  if (!(temperature > 0.f) || !(log2e_over(temperature) < kInf) || !(one_over(temperature) > 0.f))
-    qv::fail(QV_EINVAL, "temperature must be positive and finite, and log2(e) / temperature a finite float");
+  if (!(temperature > 0.f) || !(2.f * log2e_over(temperature) < kInf) || !(one_over(temperature) > 0.f))
+    qv::fail(QV_EINVAL, "temperature must be positive and finite, and 2 log2(e) / temperature a finite float");
   if (cols > INT32_MAX || rows > INT32_MAX) qv::fail(QV_EUNSUPPORTED, "more than 2^31 - 1 rows or columns");
   if (per_row < 0) qv::fail(QV_EINVAL, "targets_per_row must not be negative");
   if (per_row > QV_LOG_PROBS_MAX_TARGETS) qv::fail(QV_EUNSUPPORTED, "more than 64 targets per row");

@@ -549,3 +549,31 @@ def test_low_temperatures(scoring, dtype, v):
     for T in (1e-3, 1e-6, 1e-8, 1e-9, 1e-10, 1e-12, 1e-20, 1e-37):
         # (gradients go with 1 / T: within the type's range only)
         _run(scoring, x, targets, 12, T, grads=dtype != torch.float16 and T > 1e-30)
+
+
+@pytest.mark.parametrize("dtype", [torch.float32, torch.bfloat16])
+@pytest.mark.parametrize("v", RANGE_COLS)
+def test_far_apart(scoring, dtype, v):
+    """Logits that differ by more than the largest float, at temperatures that bring them near to each other again.
+
+    The gradient is that of weights of 1e30, so that it is no subnormal number.
+    """
+    say("log probs, logits far apart", dtype, v)
+    g = torch.Generator(device="cuda").manual_seed(v)
+    x = (torch.rand((6, v), generator=g, device="cuda") * 2 - 1) * 3.38e38
+    x[1] = 3.38e38
+    x[1, v // 2:] = -3.38e38
+    x[2, 1:] = -3.38e38
+    x[2, 0] = 3.38e38
+    x[3] *= 0.01
+    x = x.to(dtype)
+    targets = torch.stack([x.argmax(1), x.argmin(1)], 1).to(torch.int32)
+    for T in (1e36, 1e37, 1e38, 3e38):
+        r, plain = _run(scoring, x, targets, 12, T)
+        rng = np.random.default_rng(v)
+        weights = [(rng.standard_normal(s) * 1e30).astype(np.float32) for s in ((6, 2), 6, 6, (6, 12))]
+        out = scoring.log_probs_grad(x, r, targets, **{
+            "grad_" + name: torch.from_numpy(w).cuda() for name, w in zip(("target", "entropy", "logsumexp", "top"), weights)})
+        want, slack = plain.grad(*[w.astype(np.float64) for w in weights])
+        rel, least = ROUND[dtype]
+        _near(out, want, slack + (np.abs(want) + slack) * rel + least, "gradient of large weights")
