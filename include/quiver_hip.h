@@ -530,7 +530,8 @@ int qv_log_probs(const void* d_logits, int32_t type, int64_t rows, int64_t cols,
  * with absent targets and alternatives (ids < 0) left out, and dx = dz /
  * temperature rounded once to the logits' type.  Any of the four gradients may
  * be NULL (none).  A row with nothing above -inf has the gradient 0, one without
- * a distribution NaN.  d_grad may be the logits themselves. */
+ * a distribution NaN, as one whose target past the row's end (NaN) has a weight
+ * other than 0.  d_grad may be the logits themselves. */
 int qv_log_probs_grad(const void* d_logits, int32_t type, int64_t rows, int64_t cols, int64_t stride,
                       float temperature, const float* d_stats, const float* d_entropy,
                       const int32_t* d_targets, int32_t targets_per_row, const int32_t* d_top_ids,

@@ -595,7 +595,8 @@ __global__ __launch_bounds__(256) void log_probs_grad_kernel(const T* logits, in
     const int64_t at = t ? row * g.per_row + i : row * g.topk + i - g.per_row;
     id[h] = t ? g.targets[at] : g.top_ids[at];
     weight[h] = t ? g.g_target[at] : g.g_top[at];
-    if (id[h] >= 0) total = total + weight[h];
+    // the log probability of a column past the row's end is NaN, and with it the derivative of what weighs it
+    if (id[h] >= 0) total = total + (t && id[h] >= cols && weight[h] != 0.f ? __builtin_nanf("") : weight[h]);
   }
   if (named) total = wave_sum(total);
   if (g.g_lse) total = total - g.g_lse[row];

@@ -252,7 +252,7 @@ def log_probs(logits: torch.Tensor, targets: torch.Tensor | None = None, *, top_
 
     ``targets``: int32 [n, t] or [n], the columns whose log probabilities are
     wanted; a negative one is absent (0, no gradient), one past the row's end
-    gives NaN.  ``top_k`` (up to 64) columns with the largest logits come in
+    gives NaN (and the row a gradient of NaN unless its weight is 0).  ``top_k`` (up to 64) columns with the largest logits come in
     descending order, the lower column first among equal ones.  -inf takes a
     column out; a row with none left has log probabilities -inf, entropy 0 and
     ids -1, one that holds +inf or NaN has NaN.  With logits that require a

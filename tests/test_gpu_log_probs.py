@@ -577,3 +577,20 @@ def test_far_apart(scoring, dtype, v):
         want, slack = plain.grad(*[w.astype(np.float64) for w in weights])
         rel, least = ROUND[dtype]
         _near(out, want, slack + (np.abs(want) + slack) * rel + least, "gradient of large weights")
+
+
+@pytest.mark.parametrize("v", [90, 3000, 50000])
+def test_gradient_past_the_end(scoring, v):
+    """A weighed target past the row's end makes its row's gradient NaN, as the log probability is; with the weight 0 it is absent."""
+    say("log probs, gradient of targets past the end", v)
+    x, targets = _inputs(torch.float32, 4, v, 2, v)
+    absent = targets.clone()
+    targets[1, 1], targets[2, 0], absent[1, 1], absent[2, 0] = v, 2 ** 31 - 1, -1, -1
+    weights = torch.randn((4, 2), device="cuda")
+    weights[2, 0] = 0
+    r = scoring.log_probs(x, targets)
+    grad = scoring.log_probs_grad(x, r, targets, grad_target=weights)
+    assert torch.isnan(r.target[1, 1]) and torch.isnan(grad[1]).all()
+    want = scoring.log_probs_grad(x, r, absent, grad_target=weights)
+    for i in (0, 2, 3):
+        assert torch.equal(grad[i], want[i])
