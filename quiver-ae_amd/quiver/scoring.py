@@ -7,7 +7,8 @@ entropy, the best alternatives (a retriever's hard negatives), the gradient.
 
 ``quantize_rows``, ``int8_product``, ``log_probs`` and ``log_probs_grad`` are
 the C ABI's calls (include/quiver_hip.h) on the current stream of the tensors'
-GPU; none of them waits.  ``log_probs`` takes part in autograd.
+GPU; none of them waits.  ``log_probs`` takes part in autograd (reverse mode);
+where there is no derivative, an argument that asks for one is refused.
 ``DenseCatalogue`` runs them together: a catalogue kept in 8 bits, scored and
 normalised for batches of queries.
 
@@ -31,6 +32,7 @@ if _lib.before_torch:
                            "import torch (or quiver.scoring) before the first call into the library")
 
 import torch  # noqa: E402
+from torch.autograd import forward_ad  # noqa: E402
 
 _TYPES = {torch.float32: _lib.QV_FLOAT, torch.bfloat16: _lib.QV_BFLOAT16, torch.float16: _lib.QV_FLOAT16}
 _CODES = (torch.int8,)
@@ -53,6 +55,26 @@ def _device(*tensors: torch.Tensor) -> int:
     if index < 0:
         raise ValueError("tensors must be on the GPU")
     return index
+
+
+# The two checks below are called only where an argument requires a gradient or a forward-mode level is
+# entered (`forward_ad._current_level >= 0`): reading that is what the other calls pay.
+def _has_tangent(*tensors: torch.Tensor | None) -> bool:
+    """Whether a forward-mode derivative goes with one of them."""
+    if forward_ad._current_level < 0 or not torch._C._is_fwd_grad_enabled():
+        return False
+    return any(t is not None and forward_ad.unpack_dual(t).tangent is not None for t in tensors)
+
+
+def _no_derivative(call: str, *tensors: torch.Tensor | None) -> None:
+    """Results are made outside autograd: a derivative that is asked for is refused, not left out."""
+    if torch.is_grad_enabled():
+        for t in tensors:
+            if t is not None and t.requires_grad:
+                raise ValueError(f"{call} has no derivative, and an argument requires a gradient: detach it, or call "
+                                 "under torch.no_grad()")
+    if _has_tangent(*tensors):
+        raise ValueError(f"{call} has no forward-mode derivative, and an argument has a tangent")
 
 
 def _matrix(name: str, t: torch.Tensor, types) -> tuple[int, int, int]:
@@ -85,6 +107,8 @@ def quantize_rows(x: torch.Tensor, *, out: tuple[torch.Tensor, torch.Tensor] | N
     """
     n, d, stride = _matrix("x", x, _TYPES)
     again = out is not None
+    if x.requires_grad or again and out[1].requires_grad or forward_ad._current_level >= 0:
+        _no_derivative("quantize_rows", x, out[1] if again else None)
     if not again:
         out = (torch.empty((n, d), dtype=torch.int8, device=x.device),
                torch.empty(n, dtype=torch.float32, device=x.device))
@@ -114,6 +138,9 @@ def int8_product(a: torch.Tensor, a_scales: torch.Tensor, b: torch.Tensor, b_sca
     if k_b != k:
         raise ValueError("a and b differ in the length of their rows")
     again = out is not None
+    if (a_scales.requires_grad or b_scales.requires_grad or bias is not None and bias.requires_grad
+            or again and out.requires_grad or forward_ad._current_level >= 0):
+        _no_derivative("int8_product", a_scales, b_scales, bias, out)
     if not again:
         if dtype not in _TYPES:
             raise ValueError("dtype must be float32, bfloat16 or float16")
@@ -235,6 +262,9 @@ class _LogProbsFunction(torch.autograd.Function):
     def backward(ctx, g_target, g_entropy, g_lse, _ids, g_top, _stats, _workspace):
         logits, targets, stats, entropy, top_ids = ctx.saved_tensors
 
+        if _has_tangent(g_target, g_entropy, g_lse, g_top):
+            raise _lib.QuiverError("the gradient of log_probs has no forward-mode derivative")
+
         def plain(g):
             return None if g is None else g.contiguous()
 
@@ -252,19 +282,24 @@ def log_probs(logits: torch.Tensor, targets: torch.Tensor | None = None, *, top_
 
     ``targets``: int32 [n, t] or [n], the columns whose log probabilities are
     wanted; a negative one is absent (0, no gradient), one past the row's end
-    gives NaN (and the row a gradient of NaN unless its weight is 0).  ``top_k`` (up to 64) columns with the largest logits come in
-    descending order, the lower column first among equal ones.  -inf takes a
-    column out; a row with none left has log probabilities -inf, entropy 0 and
-    ids -1, one that holds +inf or NaN has NaN.  With logits that require a
-    gradient the results take part in autograd (``out`` is then refused), once:
-    the gradient has none of its own.
+    gives NaN (and the row a gradient of NaN unless its weight is 0).  ``top_k``
+    (up to 64) columns with the largest logits come in descending order, the
+    lower column first among equal ones.  -inf takes a column out; a row with
+    none left has log probabilities -inf, entropy 0 and ids -1, one that holds
+    +inf or NaN has NaN.  With logits that require a gradient the results take
+    part in autograd (``out`` is then refused), once: the gradient has none of
+    its own, and there is no forward-mode derivative.
     """
-    if torch.is_grad_enabled() and logits.requires_grad:
+    if logits.requires_grad and torch.is_grad_enabled():
         if out is not None:
             raise ValueError("out= cannot be given for logits that require a gradient")
+        if _has_tangent(logits):
+            raise ValueError("log_probs has no forward-mode derivative, and logits has a tangent")
         target, entropy, lse, ids, top, stats, workspace = _LogProbsFunction.apply(logits, targets, top_k,
                                                                                   float(temperature))
         return LogProbs.of(target, entropy, lse, ids, top, stats, float(temperature), workspace)
+    if out is not None and out.entropy.requires_grad or forward_ad._current_level >= 0:
+        _no_derivative("log_probs", logits, None if out is None else out.entropy)
     return _forward(logits, targets, top_k, temperature, out)
 
 
@@ -307,8 +342,16 @@ def log_probs_grad(logits: torch.Tensor, result: LogProbs, targets: torch.Tensor
     """The gradient of a loss with respect to ``logits``, from its gradients with respect to ``result``'s parts.
 
     ``result`` and ``targets`` as they were for ``log_probs``; ``out`` may be
-    the logits themselves.  What autograd runs, for training loops without it.
+    the logits themselves.  What autograd runs, for training loops without it
+    (so logits that require a gradient come detached, or under
+    ``torch.no_grad()``).
     """
+    if (logits.requires_grad or grad_target is not None and grad_target.requires_grad
+            or grad_entropy is not None and grad_entropy.requires_grad
+            or grad_logsumexp is not None and grad_logsumexp.requires_grad
+            or grad_top is not None and grad_top.requires_grad or out is not None and out.requires_grad
+            or forward_ad._current_level >= 0):
+        _no_derivative("log_probs_grad", logits, grad_target, grad_entropy, grad_logsumexp, grad_top, out)
     if result.entropy.shape[0] != logits.shape[0]:
         raise ValueError("result was made for another number of rows")
     _, at_entropy, _, at_ids, _, at_stats, _ = result._at
@@ -322,7 +365,8 @@ class DenseCatalogue:
     ``DenseCatalogue(vectors)`` quantises the rows once.  ``log_probs(queries,
     targets, ...)`` gives each query's distribution over all of them, by inner
     products; the scores exist for one batch of queries at a time, about
-    ``score_bytes`` of them.
+    ``score_bytes`` of them.  Scores have no derivative (vectors, queries or a
+    bias that require a gradient are refused).
     """
 
     def __init__(self, vectors: torch.Tensor, *, bias: torch.Tensor | None = None,

@@ -594,3 +594,22 @@ def test_gradient_past_the_end(scoring, v):
     want = scoring.log_probs_grad(x, r, absent, grad_target=weights)
     for i in (0, 2, 3):
         assert torch.equal(grad[i], want[i])
+
+
+def test_no_tangent_of_the_gradient(scoring):
+    """A backward pass whose incoming gradients have tangents is refused; without them, beside them, it runs."""
+    from torch.autograd import forward_ad
+
+    from quiver import _lib
+
+    say("log probs, forward over reverse")
+    leaf = torch.randn((4, 50), device="cuda").requires_grad_()
+    targets = torch.arange(4, dtype=torch.int32, device="cuda")
+    weights = torch.rand((4, 1), device="cuda")
+    with forward_ad.dual_level():
+        r = scoring.log_probs(leaf, targets)
+        with pytest.raises(_lib.QuiverError, match="forward-mode"):
+            torch.autograd.grad((r.target * forward_ad.make_dual(weights, torch.ones_like(weights))).sum(), leaf)
+        (grad,) = torch.autograd.grad((scoring.log_probs(leaf, targets).target * weights).sum(), leaf)
+    with torch.no_grad():
+        assert torch.equal(grad, scoring.log_probs_grad(leaf, scoring.log_probs(leaf, targets), targets, grad_target=weights))

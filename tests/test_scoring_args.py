@@ -191,3 +191,61 @@ def test_temperature_range(lib, buf, temp, fine):
     assert rcs == [lib.QV_OK if fine else lib.QV_EINVAL] * 2
     if not fine:
         assert b"temperature" in L.qv_last_error()
+
+
+def _calls_without_derivative(wrap):
+    """Every call and argument that a derivative would be lost at; `wrap` makes an argument ask for one."""
+    from quiver import scoring
+
+    x, codes, scales = torch.zeros(3, 8), torch.zeros(3, 8, dtype=torch.int8), torch.zeros(3)
+    empty = torch.zeros(3, 0)
+    r = scoring.LogProbs.of(empty, scales, scales, empty.int(), empty, torch.zeros(3, 2), 1.0, torch.zeros(0))
+    catalogue = scoring.DenseCatalogue.__new__(scoring.DenseCatalogue)
+    catalogue.codes, catalogue.scales, catalogue.bias = codes, scales, None
+    catalogue.score_dtype, catalogue.score_bytes = torch.float32, 1
+    yield lambda: scoring.quantize_rows(wrap(x))
+    yield lambda: scoring.quantize_rows(x, out=(codes, wrap(scales)))
+    yield lambda: scoring.int8_product(codes, wrap(scales), codes, scales)
+    yield lambda: scoring.int8_product(codes, scales, codes, wrap(scales))
+    yield lambda: scoring.int8_product(codes, scales, codes, scales, bias=wrap(scales))
+    yield lambda: scoring.int8_product(codes, scales, codes, scales, out=wrap(torch.zeros(3, 3)))
+    yield lambda: scoring.log_probs(x, out=scoring.LogProbs.of(empty, wrap(scales), scales, empty.int(), empty,
+                                                               torch.zeros(3, 2), 1.0, torch.zeros(0)))
+    yield lambda: scoring.log_probs_grad(wrap(x), r)
+    yield lambda: scoring.log_probs_grad(x, r, grad_target=wrap(empty))
+    yield lambda: scoring.log_probs_grad(x, r, grad_entropy=wrap(scales))
+    yield lambda: scoring.log_probs_grad(x, r, grad_logsumexp=wrap(scales))
+    yield lambda: scoring.log_probs_grad(x, r, grad_top=wrap(empty))
+    yield lambda: scoring.log_probs_grad(x, r, out=wrap(torch.zeros(3, 8)))
+    yield lambda: scoring.DenseCatalogue(wrap(x))
+    yield lambda: catalogue.scores(wrap(x))
+    yield lambda: catalogue.log_probs(wrap(x))
+
+
+def test_gradients_are_not_lost():
+    """A gradient that a call does not have is refused, not left out; under no_grad nobody asks for it."""
+    for call in _calls_without_derivative(lambda t: t.clone().requires_grad_()):
+        with pytest.raises(ValueError, match="requires a gradient"):
+            call()
+        with torch.no_grad(), pytest.raises(ValueError, match="on the GPU"):
+            call()
+
+
+def test_tangents_are_not_lost():
+    """Forward-mode derivatives are refused, those of log_probs among them."""
+    from torch.autograd import forward_ad
+
+    from quiver import scoring
+
+    with forward_ad.dual_level():
+        def dual(t):
+            return forward_ad.make_dual(t.clone(), torch.ones_like(t))
+
+        calls = list(_calls_without_derivative(dual))
+        calls.append(lambda: scoring.log_probs(dual(torch.zeros(3, 8))))
+        calls.append(lambda: scoring.log_probs(dual(torch.zeros(3, 8).requires_grad_())))
+        for call in calls:
+            with pytest.raises(ValueError, match="has a tangent"):
+                call()
+        with pytest.raises(ValueError, match="on the GPU"):
+            scoring.log_probs(torch.zeros(3, 8))
