@@ -126,12 +126,12 @@ def quantize_rows(x: torch.Tensor, *, out: tuple[torch.Tensor, torch.Tensor] | N
 
 
 def int8_product(a: torch.Tensor, a_scales: torch.Tensor, b: torch.Tensor, b_scales: torch.Tensor, *,
-                 bias: torch.Tensor | None = None, dtype: torch.dtype = torch.float32,
+                 bias: torch.Tensor | None = None, dtype: torch.dtype | None = None,
                  out: torch.Tensor | None = None) -> torch.Tensor:
     """``(a . b^T) * a_scales[:, None] * b_scales[None, :] + bias`` of int8 ``a`` [m, k] and ``b`` [n, k].
 
-    The sums are exact; the rest is fp32, rounded once to ``dtype``.  A bias of
-    -inf takes a column out of ``log_probs``.
+    The sums are exact; the rest is fp32, rounded once to ``dtype`` (``out``'s
+    type, or float32).  A bias of -inf takes a column out of ``log_probs``.
     """
     m, k, a_stride = _matrix("a", a, _CODES)
     n, k_b, b_stride = _matrix("b", b, _CODES)
@@ -142,9 +142,13 @@ def int8_product(a: torch.Tensor, a_scales: torch.Tensor, b: torch.Tensor, b_sca
             or again and out.requires_grad or forward_ad._current_level >= 0):
         _no_derivative("int8_product", a_scales, b_scales, bias, out)
     if not again:
-        if dtype not in _TYPES:
+        if dtype is None:
+            dtype = torch.float32
+        elif dtype not in _TYPES:
             raise ValueError("dtype must be float32, bfloat16 or float16")
         out = torch.empty((m, n), dtype=dtype, device=a.device)
+    elif dtype is not None and out.dtype != dtype:
+        raise ValueError(f"out has the type {out.dtype}, and {dtype} is asked for")
     out_rows, out_cols, out_stride = _matrix("out", out, _TYPES)
     if out_rows != m or out_cols != n:
         raise ValueError(f"out must have the shape {(m, n)}")
@@ -384,9 +388,10 @@ class DenseCatalogue:
         return self.codes.shape[0]
 
     def scores(self, queries: torch.Tensor, *, out: torch.Tensor | None = None) -> torch.Tensor:
-        """Inner products of the queries, quantised row by row, with every vector: [n, len(self)]."""
+        """Inner products of the queries, quantised row by row, with every vector: [n, len(self)], of ``out``'s type if given."""
         codes, scales = quantize_rows(queries)
-        return int8_product(codes, scales, self.codes, self.scales, bias=self.bias, dtype=self.score_dtype, out=out)
+        return int8_product(codes, scales, self.codes, self.scales, bias=self.bias,
+                            dtype=self.score_dtype if out is None else None, out=out)
 
     def log_probs(self, queries: torch.Tensor, targets: torch.Tensor | None = None, *, top_k: int = 0,
                   temperature: float = 1.0) -> LogProbs:

@@ -249,3 +249,17 @@ def test_tangents_are_not_lost():
                 call()
         with pytest.raises(ValueError, match="on the GPU"):
             scoring.log_probs(torch.zeros(3, 8))
+
+
+def test_type_of_out():
+    """A type that is asked for beside out= has to be out's; none takes out's."""
+    from quiver import scoring
+
+    codes, scales = torch.zeros(3, 8, dtype=torch.int8), torch.zeros(3)
+    half = torch.zeros(3, 3, dtype=torch.float16)
+    for dtype in (torch.float32, torch.bfloat16, torch.float64):
+        with pytest.raises(ValueError, match="out has the type torch.float16"):
+            scoring.int8_product(codes, scales, codes, scales, dtype=dtype, out=half)
+    for dtype in (None, torch.float16):
+        with pytest.raises(ValueError, match="on the GPU"):
+            scoring.int8_product(codes, scales, codes, scales, dtype=dtype, out=half)
