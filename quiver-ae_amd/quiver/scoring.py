@@ -397,6 +397,7 @@ class DenseCatalogue:
                   temperature: float = 1.0) -> LogProbs:
         """``log_probs`` of the scores, batch by batch of the queries."""
         n = queries.shape[0]
+        _given(targets, n)  # of all batches at once: rows past the queries' would be left out
         row_bytes = max(1, len(self)) * torch.empty((), dtype=self.score_dtype).element_size()
         step = max(1, min(n, self.score_bytes // row_bytes))
         if n <= step:

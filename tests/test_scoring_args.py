@@ -263,3 +263,18 @@ def test_type_of_out():
     for dtype in (None, torch.float16):
         with pytest.raises(ValueError, match="on the GPU"):
             scoring.int8_product(codes, scales, codes, scales, dtype=dtype, out=half)
+
+
+@pytest.mark.parametrize("rows, shape", [(6, (6, 1)), (6, (6,)), (2, (2, 1)), (4, (4, 1, 1))])
+def test_targets_of_a_catalogue(rows, shape):
+    """Targets of another number of rows than the queries are refused, however the queries are cut into batches."""
+    from quiver import scoring
+
+    catalogue = scoring.DenseCatalogue.__new__(scoring.DenseCatalogue)
+    catalogue.codes, catalogue.scales, catalogue.bias = torch.zeros(3, 8, dtype=torch.int8), torch.zeros(3), None
+    catalogue.score_dtype = torch.float32
+    for catalogue.score_bytes in (24, 1 << 30):  # two queries at a time, all at once
+        with pytest.raises(ValueError, match="targets must be"):
+            catalogue.log_probs(torch.zeros(4, 8), torch.zeros(shape, dtype=torch.int32))
+        with pytest.raises(ValueError, match="on the GPU"):
+            catalogue.log_probs(torch.zeros(4, 8), torch.zeros(4, 1, dtype=torch.int32))
