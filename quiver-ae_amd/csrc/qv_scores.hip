@@ -164,8 +164,7 @@ typedef f4 f4_any __attribute__((aligned(4), may_alias));
 
 constexpr int kLoadsDone = 0x0f70;  // s_waitcnt vmcnt(0)
 constexpr int kStage = 128;         // bytes of k per stage
-constexpr int64_t kFar = 1 << 23;     // row strides from here on: 256 rows' offsets pass 31 bits
-constexpr int64_t kFarOut = 1 << 27;  // the same of the output, for 4 rows of floats
+constexpr int64_t kFar = 1 << 23;   // operands' row strides from here on: 256 rows' offsets pass 31 bits
 
 template <class O>
 struct Product {
@@ -929,7 +928,7 @@ __global__ __launch_bounds__(256) void product_strip_kernel(Product<O> p, int64_
   }
 }
 
-// Rows shorter than one piece (16 bytes), or further apart than 32-bit offsets reach:
+// Rows shorter than one piece (16 bytes), or more than 32 rows further apart than 32-bit offsets reach:
 // a 16 x 16 tile of the output per workgroup, one thread per element, both operands'
 // rows staged 64 bytes at a time.
 template <class O>
@@ -1029,7 +1028,8 @@ void launch_panels(const Product<O>& p, hipStream_t st) {
 
 template <class O>
 void product(const Product<O>& p, hipStream_t st) {
-  if (p.k < 16 || p.a_stride >= kFar || p.b_stride >= kFar || p.out_stride >= kFarOut) {
+  // (the strips' offsets, and all of the output's, have 64 bits)
+  if (p.k < 16 || (p.m > 32 && (p.a_stride >= kFar || p.b_stride >= kFar))) {
     const int64_t tm = (p.m + 15) / 16, tn = (p.n + 15) / 16;
     in_launches(tm * tn, 256, [&](int64_t first, unsigned count) {
       hipLaunchKernelGGL(product_small_kernel<O>, dim3(count), dim3(256), 0, st, p, tn, first);

@@ -302,3 +302,61 @@ def test_in_a_graph(scoring):
             graph.replay()
             torch.cuda.synchronize()
             assert torch.equal(out, scoring.int8_product(*scoring.quantize_rows(x.clone()), b, sb, dtype=torch.bfloat16))
+
+
+def test_distant_rows_of_scores(scoring):
+    """Output rows 2^27 elements and more apart, by each way that a product takes; nothing beside the output is written."""
+    rows, stride = 256, 2 ** 27 + 3
+    store = torch.empty(rows * stride, dtype=torch.bfloat16, device="cuda")  # 69 GB
+    for m, n, k in ((1, 300, 96), (3, 3000, 100), (32, 200, 2049), (40, 3000, 100), (100, 1001, 200), (100, 900, 301),
+                    (64, 500, 320), (200, 700, 4096), (256, 56000, 320), (5, 70, 9)):
+        say("product, distant rows of scores", m, n, k)
+        a, sa, b, sb, bias = _inputs(m, n, k, k)
+        wide = store.as_strided((m, n + 16), (stride, 1))
+        wide.fill_(7.0)
+        out = scoring.int8_product(a, sa, b, sb, bias=bias, out=wide[:, 5:5 + n])
+        _check_product(out, a, sa, b, sb, bias, torch.bfloat16)
+        assert (wide[:, :5] == 7).all() and (wide[:, 5 + n:] == 7).all()
+
+
+@pytest.mark.parametrize("m, n, k", [(1, 70, 40), (20, 70, 300), (40, 50, 40), (40, 50, 300)])
+def test_distant_rows_of_codes(scoring, m, n, k):
+    """Operands' rows 2^23 elements and more apart."""
+    say("product, distant rows of codes", m, n, k)
+    a, sa, b, sb, bias = _inputs(m, n, k, k)
+    stride = 2 ** 23 + 5
+    store = torch.empty((m + n) * stride, dtype=torch.int8, device="cuda")
+    far_a, far_b = store.as_strided((m, k), (stride, 1)), store.as_strided((n, k), (stride, 1), m * stride)
+    far_a.copy_(a)
+    far_b.copy_(b)
+    want = scoring.int8_product(a, sa, b, sb, bias=bias)
+    for x, y in ((far_a, b), (a, far_b), (far_a, far_b)):
+        assert torch.equal(scoring.int8_product(x, sa, y, sb, bias=bias), want)
+    _check_product(want, a, sa, b, sb, bias, torch.float32)
+
+
+def test_one_query_of_a_huge_catalogue(scoring):
+    """2^27 rows and more take the time of a few less (three times it at most: it was seven times where they took another way)."""
+    k, most = 16, 2 ** 27 + 77
+    say("product, one query,", most, "rows")
+    b = torch.randint(-128, 128, (most, k), dtype=torch.int8, device="cuda")
+    sb = torch.rand(most, device="cuda")
+    a, sa = b[most - 2:most - 1].clone(), torch.ones(1, device="cuda")
+
+    def timed(n):
+        out = scoring.int8_product(a, sa, b[:n], sb[:n], dtype=torch.bfloat16)
+        for lo in (0, n // 2 - 50, n - 100):
+            _check_product(out[:, lo:lo + 100], a, sa, b[lo:lo + 100], sb[lo:lo + 100], None, torch.bfloat16)
+        times = []
+        for _ in range(5):
+            start, end = torch.cuda.Event(enable_timing=True), torch.cuda.Event(enable_timing=True)
+            start.record()
+            scoring.int8_product(a, sa, b[:n], sb[:n], out=out)
+            end.record()
+            end.synchronize()
+            times.append(start.elapsed_time(end))
+        return min(times)
+
+    under, over = timed(2 ** 27 - 77), timed(most)
+    say(f"{under * 1e3:.0f} us below 2^27 rows, {over * 1e3:.0f} us above")
+    assert over < 3 * under
