@@ -476,7 +476,8 @@ int qv_ground_truth(const void* d_base, int32_t data_type, int64_t n, int32_t di
 
 /* Rows to 8 bits with a scale each: a = max_j |x_ij|, scales[i] = a / 127 and
  * codes[i][j] = x_ij * ((1 / a) * 127) rounded to the nearest whole number (halves
- * to even), each operation in fp32.  A row whose a is below 2^-119 counts as zeros (scale 0);
+ * to even), each operation in fp32 (with a / 2^8 and 127 / 2^8 from a = 2^126 on, where
+ * 1 / a is subnormal).  A row whose a is below 2^-119 counts as zeros (scale 0);
  * one that holds an infinity or a NaN gets the scale NaN and zero codes.  type:
  * QV_FLOAT, QV_BFLOAT16 or QV_FLOAT16. */
 int qv_quantize_rows(const void* d_x, int32_t type, int64_t n, int64_t dim, int64_t x_stride,

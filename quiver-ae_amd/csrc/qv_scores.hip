@@ -22,6 +22,7 @@ namespace {
 // compared as whole numbers, whose order is theirs, with infinities and NaN above all.
 
 constexpr uint32_t kTinyBits = 0x04000000u;  // 2^-119: below it 127 / a comes near the largest float
+constexpr uint32_t kHugeBits = 0x7e800000u;  // 2^126: above it 1 / a is subnormal and keeps fewer bits
 constexpr uint32_t kInfBits = 0x7f800000u;
 
 // Largest value over the group of G lanes (a power of two) that the lane is in.
@@ -49,7 +50,8 @@ __device__ __forceinline__ RowScale scale_of(uint32_t top) {
   const float a = __uint_as_float(top);
   if (top >= kInfBits) return {0.f, __builtin_nanf("")};
   if (top < kTinyBits) return {0.f, 0.f};
-  return {1.f / a * 127.f, a / 127.f};
+  const float h = top >= kHugeBits ? 0x1p-8f : 1.f;  // both products with it are exact
+  return {1.f / (a * h) * (127.f * h), a / 127.f};
 }
 
 // x 127 / a to the nearest whole number, halves to even, in the low byte: adding 1.5 2^23

@@ -360,3 +360,25 @@ def test_one_query_of_a_huge_catalogue(scoring):
     under, over = timed(2 ** 27 - 77), timed(most)
     say(f"{under * 1e3:.0f} us below 2^27 rows, {over * 1e3:.0f} us above")
     assert over < 3 * under
+
+
+@pytest.mark.parametrize("dtype", [torch.float32, torch.bfloat16])
+@pytest.mark.parametrize("n, d", [(3000, 7), (400, 100), (30, 3000)])
+def test_quantize_huge_rows(scoring, dtype, n, d):
+    """Entries all over the type's range: codes as near to x 127 / a as anywhere, though 1 / a is subnormal."""
+    say("quantize huge rows", dtype, n, d)
+    g = torch.Generator(device="cuda").manual_seed(d)
+    big = torch.finfo(dtype).max
+    x = ((torch.rand((n, d), generator=g, device="cuda") * 2 - 1) * big).to(dtype)
+    # near halves, where the reciprocal's last bits decide the code
+    halves = torch.arange(d, device="cuda") % 127 + 0.5
+    a = (torch.rand(n // 2, generator=g, device="cuda") * 0.74 + 0.25) * big
+    x[:n // 2] = (halves * (a[:, None] / 127)).to(dtype)
+    x[:n // 2, 0] = a
+    if dtype == torch.float32:  # the largest errors of a search over rows
+        for i, (top, value) in enumerate((("0x1.fb2cd8p+127", "0x1.f52f4cp+127"), ("0x1.f82df6p+127", "0x1.f631dap+127"),
+                                          ("0x1.f40ffcp+127", "0x1.ee27f2p+127"))):
+            x[i] = 0
+            x[i, 1], x[i, d - 1] = float.fromhex(value), -float.fromhex(top)
+    codes, scales = scoring.quantize_rows(x)
+    _check_rows(x, codes, scales)
