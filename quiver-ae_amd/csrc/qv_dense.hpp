@@ -108,8 +108,9 @@ inline void check_matrix(const char* name, const void* p, int64_t rows, int64_t 
   if (stride > INT64_MAX / 8 / rows) fail(QV_EINVAL, std::string(name) + ": too large");
 }
 
-inline void check_vector(const char* name, const void* p, int64_t count, int size = 4) {
-  if (count > 0) check_matrix(name, p, 1, count, count, size);
+// ... of 4-byte elements.
+inline void check_vector(const char* name, const void* p, int64_t count) {
+  if (count > 0) check_matrix(name, p, 1, count, count, 4);
 }
 
 }  // namespace dense

@@ -197,16 +197,15 @@ __device__ __forceinline__ i16v mfma(i4 x, i4 y, i16v acc) {
   return __builtin_amdgcn_mfma_i32_32x32x32_i8(x, y, acc, 0, 0, 0);
 }
 
-// Puts an instruction's result, 32 columns j from j0 of 32 rows i, into a wave's tile
-// [32][stride] in LDS.
-__device__ __forceinline__ void put_sums(int32_t* tile, int stride, int j0, const i16v& acc) {
+// Puts an instruction's result, 32 columns j of 32 rows i, into a wave's tile [32][stride] in LDS.
+__device__ __forceinline__ void put_sums(int32_t* tile, int stride, const i16v& acc) {
   const int lane = lane_id();
 #pragma unroll
   for (int g = 0; g < 4; g++) {
     i4 v;
 #pragma unroll
     for (int e = 0; e < 4; e++) v[e] = acc[4 * g + e];
-    *reinterpret_cast<i4*>(tile + (lane % 32) * stride + j0 + 8 * g + 4 * (lane / 32)) = v;
+    *reinterpret_cast<i4*>(tile + (lane % 32) * stride + 8 * g + 4 * (lane / 32)) = v;
   }
 }
 
@@ -424,10 +423,10 @@ __device__ __forceinline__ int64_t tile_of_block(int64_t block, int64_t tiles) {
 // rows of any alignment and length; 2,048 x 4,096 x 4,096 to bfloat16: 44 us, 1.6 POP/s.
 template <int BM, int BN, int WM, int WN, class O>
 __global__ __launch_bounds__(64 * WM * WN, 1) void product_tile_kernel(Product<O> p, int64_t tiles_m, int64_t tiles_n,
-                                                                       int64_t group, int scales_at) {
+                                                                       int64_t group) {
   constexpr int T = 64 * WM * WN, TM = BM / WM / 32, TN = BN / WN / 32;
   constexpr int LA = BM * 8 / T, LB = BN * 8 / T, kRows = T / 8;
-  constexpr int kBuffer = (BM + BN) * kStage;
+  constexpr int kBuffer = (BM + BN) * kStage;  // two of them, then the scales
   extern __shared__ __align__(16) char lds[];
   const int tid = threadIdx.x, wave = wave_id(), lane = lane_id();
   const int wm = wave / WN, wn = wave % WN;
@@ -481,7 +480,7 @@ __global__ __launch_bounds__(64 * WM * WN, 1) void product_tile_kernel(Product<O
   };
   load(0);
   keep(0);
-  const TileScales<BM, BN, T> scales(lds + scales_at, i0, j0, p);
+  const TileScales<BM, BN, T> scales(lds + 2 * kBuffer, i0, j0, p);
   __syncthreads();
   for (int s = 0; s < stages; s++) {
     const bool more = s + 1 < stages;
@@ -908,7 +907,7 @@ __global__ __launch_bounds__(256) void product_strip_kernel(Product<O> p, int64_
       __builtin_amdgcn_fence(__ATOMIC_ACQ_REL, "wavefront");
     }
     int32_t* tile = reinterpret_cast<int32_t*>(area);
-    put_sums(tile, kTile, 0, acc);
+    put_sums(tile, kTile, acc);
     __builtin_amdgcn_fence(__ATOMIC_ACQ_REL, "wavefront");
     if constexpr (WK > 1) {
       __syncthreads();
@@ -999,11 +998,10 @@ void launch_tiles(const Product<O>& p, hipStream_t st) {
   const int64_t tm = (p.m + BM - 1) / BM, tn = (p.n + BN - 1) / BN;
   // down a group of tiles' rows first: as many as keep their rows of a within 2 MB of an XCD's L2, eight at least
   const int64_t group = std::min(tm, std::max<int64_t>(8, (2 << 20) / (BM * p.k)));
-  const int buffers = p.k > kStage ? 2 : 1;
-  const int scales_at = buffers * (BM + BN) * kStage, lds = scales_at + TileScales<BM, BN, 64 * WM * WN>::kBytes;
+  constexpr int lds = 2 * (BM + BN) * kStage + TileScales<BM, BN, 64 * WM * WN>::kBytes;
   constexpr auto* kernel = &product_tile_kernel<BM, BN, WM, WN, O>;
   allow_lds<kernel>(lds);
-  hipLaunchKernelGGL(kernel, dim3((unsigned)(tm * tn)), dim3(64 * WM * WN), lds, st, p, tm, tn, group, scales_at);
+  hipLaunchKernelGGL(kernel, dim3((unsigned)(tm * tn)), dim3(64 * WM * WN), lds, st, p, tm, tn, group);
   HIP_OK(hipGetLastError());
 }
 
