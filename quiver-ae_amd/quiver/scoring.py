@@ -46,10 +46,10 @@ _raw_stream = torch._C._cuda_getCurrentRawStream
 _written = torch._C._increment_version
 
 
-def _device(*tensors: torch.Tensor) -> int:
+def _device(first: torch.Tensor, *others: torch.Tensor) -> int:
     """The one GPU that every tensor is on."""
-    index = tensors[0].get_device()
-    for t in tensors:
+    index = first.get_device()
+    for t in others:
         if t.get_device() != index:
             raise ValueError("tensors must be on one GPU")
     if index < 0:
