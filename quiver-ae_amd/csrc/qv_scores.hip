@@ -420,7 +420,8 @@ __device__ __forceinline__ int64_t tile_of_block(int64_t block, int64_t tiles) {
 // operands' stages go through registers into LDS, the next one in flight while the
 // matrix cores work on this one; piece q of row r lies at q ^ (r / 2 mod 8), so that the
 // 16 rows that are read at once (64 banks, 256 bytes) lie in 16 different places.  For
-// rows of any alignment and length; 2,048 x 4,096 x 4,096 to bfloat16: 44 us, 1.6 POP/s.
+// rows of any alignment and length; 2,048 x 4,096 x 4,096 to bfloat16: 44 us, 1.6 POP/s;
+// rows of 4,080: 47 us, of 4,095, which begin at any byte: 63 us.
 template <int BM, int BN, int WM, int WN, class O>
 __global__ __launch_bounds__(64 * WM * WN, 1) void product_tile_kernel(Product<O> p, int64_t tiles_m, int64_t tiles_n,
                                                                        int64_t group) {
@@ -511,10 +512,11 @@ __global__ __launch_bounds__(64 * WM * WN, 1) void product_tile_kernel(Product<O
 // Needs 16-byte aligned rows and k a multiple of 64.
 // MANY: one workgroup per CU walks over tiles, and the stages run on from tile to tile:
 // the next tile's first ones are on their way, and its first operands in registers, while
-// the results are stored (10,000 x 50,048 x 512: 457 us, with a workgroup per tile 519).
+// the results are stored (10,000 x 50,048 x 512: 457 to 490 us, with a workgroup per tile
+// 519 when it took 457).
 // 4,096^3 to bfloat16: 67 to 71 us among other work, 2.0 POP/s (a library's int8 product
 // with a 32-bit result: 69), 74 one after the other: then power holds the clock down.
-// 8,192 x 8,192 x 4,096: 263 us (with the results through LDS and a tile per workgroup
+// 8,192 x 8,192 x 4,096: 252 to 263 us (with the results through LDS and a tile per workgroup
 // 273); 8,192^3 of zeros 349 us, 3.1 POP/s, of codes over the whole range 545 us at 1.5
 // GHz (the matrix instruction alone reaches 4.5 and 3.3 POP/s).  Loads and LDS reads in
 // runs of their own instead of between the products: a fifth more.
@@ -674,8 +676,9 @@ __global__ __launch_bounds__(64 * WM * WN, 1) void product_deep_kernel(Product<O
 // ring of two lines in LDS in which an element's place follows its address: a line is
 // written whole as soon as its last column is there, and only the first and the last
 // one of a walk are written in parts.
-// 10,000 x 50,001 x 128 to bfloat16: 255 us, 3.95 TB/s (tiles with unaligned stores: 503),
-// to float 4.5 TB/s; without its stores the kernel takes 171 us.
+// 10,000 x 50,001 x 128 to bfloat16: 255 us call after call into the same scores, 4.0 TB/s,
+// 264 into others each time (tiles with unaligned stores: 503), to float 4.5 TB/s;
+// without its stores the kernel takes 171 us.
 template <int KS, bool BIAS, class O>
 __global__ __launch_bounds__(256, KS == 4 ? 3 : 2) void product_panel_kernel(Product<O> p, int64_t panels, int64_t tiles_n,
                                                                int64_t slices) {
@@ -852,7 +855,7 @@ __global__ __launch_bounds__(256, KS == 4 ? 3 : 2) void product_panel_kernel(Pro
 // 1), or a strip's k cut over the WK waves of its workgroup.  A wave's stage of b goes
 // through registers into an LDS area of its own, so no barrier holds it; the next one
 // is in flight meanwhile.  a's operands come from the caches, once for all strips
-// while k is a single stage.  Bound by reading b: 1 x 1M x 128 in 29.5 us, 4.6 TB/s (24.5
+// while k is a single stage.  Bound by reading b: 1 x 1M x 128 in 29.5 us, 4.6 TB/s (24
 // us over and over, part of b being cached), 8 x 100,000 x 1,024 in 19 us, 5.3 TB/s.
 template <int WK, class O>
 __global__ __launch_bounds__(256) void product_strip_kernel(Product<O> p, int64_t strips, int64_t step) {
@@ -911,7 +914,7 @@ __global__ __launch_bounds__(256) void product_strip_kernel(Product<O> p, int64_
     __builtin_amdgcn_fence(__ATOMIC_ACQ_REL, "wavefront");
     if constexpr (WK > 1) {
       __syncthreads();
-      // each wave adds up and stores the rows of a quarter of the tile: the sums go to wave 0's tile
+      // every thread adds up its elements of the tiles into wave 0's, and wave 0 stores it
       int32_t* sum = reinterpret_cast<int32_t*>(lds[0]);
       for (int e = threadIdx.x; e < 32 * kTile; e += 256) {
         int32_t v = sum[e];
