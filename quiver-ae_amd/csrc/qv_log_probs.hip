@@ -22,6 +22,7 @@
 // TB/s (73); 10,000 lists of 100 with 10: 9.4 us; one row of 1M: 13 us, of which the two
 // launches are 6.  Gradient: 1,000 x 100,003 floats 139 us, 5.8 TB/s.
 #include <algorithm>
+#include <cmath>
 
 #include "qv_dense.hpp"
 #include "qv_device.hpp"
@@ -36,6 +37,7 @@ constexpr float kInf = __builtin_inff();
 constexpr float kLog2e = 1.44269504088896340736f, kLn2 = 0.69314718055994530942f;
 constexpr float kBig = 0x1p20f;  // |m c| from here on: differences are taken before they are multiplied
 constexpr float kNone = -200.f;  // 2^-200 is 0 in fp32: stands for -inf where it would be multiplied by 0
+constexpr float kHalfNone = -150.f;  // the same where 2^y is squared
 
 // ---- values ------------------------------------------------------------------
 
@@ -565,14 +567,15 @@ struct Weights {
 };
 
 // One wave per chunk of a row: every column by the first two terms, p (a + b log2
-// p), then the columns that targets or alternatives name, whose weights add up in
+// p) / T, then the columns that targets or alternatives name, whose weights add up in
 // their order.  The named columns' logits are read before any column is written
 // (the gradient may take the logits' place); a wave's stores to one address stay
 // in order.
 template <class T, int U>
 __global__ __launch_bounds__(256) void log_probs_grad_kernel(const T* logits, int64_t units, int cols, int64_t stride,
-                                                             float c, float inv_t, int chunk, int splits, Weights g,
-                                                             T* grad, int64_t grad_stride, int64_t first_block) {
+                                                             float c, float inv_t, float root_inv_t, int chunk,
+                                                             int splits, Weights g, T* grad, int64_t grad_stride,
+                                                             int64_t first_block) {
   constexpr int N = U * kVec<T>, kBatch = kWave * N;
   const int64_t unit = (first_block + blockIdx.x) * 4 + wave_id();
   if (unit >= units) return;
@@ -602,14 +605,19 @@ __global__ __launch_bounds__(256) void log_probs_grad_kernel(const T* logits, in
   if (g.g_lse) total = total - g.g_lse[row];
   const float ge = g.g_entropy ? g.g_entropy[row] : 0.f, h = g.g_entropy ? g.entropy[row] : 0.f;
   const float nan = __builtin_nanf("");
-  const float a = odd ? nan : empty ? 0.f : -(total + ge * h) * inv_t;
-  const float b = empty ? 0.f : -(ge * kLn2) * inv_t;
+  const float a = odd ? nan : empty ? 0.f : -(total + ge * h);
+  const float b = empty ? 0.f : -2.f * (ge * kLn2);
+  // Half of log2 p.  The instruction gives 0 below 2^-126, which p passes and its root does not (4,096 x 4,096 bfloat16:
+  // 12.8 us; with such p taken 2^64 larger and back 13.3).
+  auto half_log2 = [&](float v) { return max2(__fmaf_rn(half_apart(v, m), c, -0.5f * log2_s), kHalfNone); };
+  // The root of 1 / T goes with the root of p: 1 / T times a and b may be infinite where p is 0.
   auto dense = [&](float v) {
-    const float y = max2(__fmaf_rn(half_apart(v, m), 2.f * c, -log2_s), kNone);
-    // the instruction gives 0 below 2^-126: probabilities down there are taken 2^64 larger
-    const bool low = y < -126.f;
-    const float p = __builtin_amdgcn_exp2f(low ? y + 64.f : y);
-    return p * (__fmaf_rn(b, y, a) * (low ? 0x1p-64f : 1.f));
+    const float y = half_log2(v), root = __builtin_amdgcn_exp2f(y) * root_inv_t;
+    return __fmaf_rn(b, y, a) * root * root;
+  };
+  auto named_one = [&](float v, float weight) {
+    const float y = half_log2(v), root = __builtin_amdgcn_exp2f(y);
+    return (__fmaf_rn(b, y, a) * root * root + (empty ? 0.f : weight)) * inv_t;
   };
 
   float extra[2] = {0.f, 0.f}, kept[2] = {0.f, 0.f};
@@ -668,7 +676,7 @@ __global__ __launch_bounds__(256) void log_probs_grad_kernel(const T* logits, in
 #pragma unroll
     for (int q = 0; q < 2; q++)
       if (here[q] >> lane & 1)
-        dx[id[q]] = (T)(dense(kept[q]) + (empty ? 0.f : extra[q] * inv_t));
+        dx[id[q]] = (T)named_one(kept[q], extra[q]);
   }
 }
 
@@ -744,7 +752,7 @@ void log_probs_grad(const T* x, int64_t rows, int64_t cols, int64_t stride, floa
   const int64_t splits = (cols + chunk - 1) / chunk, units = rows * splits;
   in_launches((units + 3) / 4, 256, [&](int64_t first, unsigned count) {
     hipLaunchKernelGGL((log_probs_grad_kernel<T, U>), dim3(count), dim3(256), 0, st, x, units, (int)cols, stride, c,
-                       inv_t, (int)chunk, (int)splits, g, grad, grad_stride, first);
+                       inv_t, std::sqrt(inv_t), (int)chunk, (int)splits, g, grad, grad_stride, first);
     HIP_OK(hipGetLastError());
   });
 }

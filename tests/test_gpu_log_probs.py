@@ -14,6 +14,7 @@ and one rounding to the logits' type.
 from __future__ import annotations
 
 import math
+import sys
 
 import numpy as np
 import pytest
@@ -613,3 +614,34 @@ def test_no_tangent_of_the_gradient(scoring):
         (grad,) = torch.autograd.grad((scoring.log_probs(leaf, targets).target * weights).sum(), leaf)
     with torch.no_grad():
         assert torch.equal(grad, scoring.log_probs_grad(leaf, scoring.log_probs(leaf, targets), targets, grad_target=weights))
+
+
+@pytest.mark.parametrize("dtype", [torch.float32, torch.bfloat16])
+@pytest.mark.parametrize("v", [100, 5000, 40000])
+def test_gradient_at_low_temperatures(scoring, dtype, v):
+    """Weights over the temperature pass the largest float times a probability's logarithm: columns without a probability stay 0."""
+    say("log probs, gradient at low temperatures", dtype, v)
+    g = torch.Generator(device="cuda").manual_seed(v)
+    x = torch.randn((5, v), generator=g, device="cuda") * 3
+    x[1] = 12.7
+    x[2, v // 2:] = -1e4
+    x[3, 1:] = 29
+    x[3, 0] = 30
+    x[4, ::2] = -INF
+    x = x.to(dtype)
+    targets = torch.stack([x.argmax(1), x.argmin(1)], 1).to(torch.int32)
+    for T in (1e-30, 1e-35, 1e-36, 1e-37):
+        _run(scoring, x, targets, 12, T)
+
+
+@pytest.fixture(autouse=True)
+def nan_matches_nan_only(monkeypatch):
+    """`_near` asks whether an error is above its bound, which a NaN never is: here, NaN is near to nothing else."""
+    near = _near
+
+    def strict(got, want, slack, what):
+        assert not np.isnan(slack).any(), what
+        np.testing.assert_array_equal(np.isnan(got.double().cpu().numpy()), np.isnan(want), err_msg=what)
+        near(got, want, slack, what)
+
+    monkeypatch.setattr(sys.modules[__name__], "_near", strict)
