@@ -20,7 +20,7 @@
 // exponential for each.  256 x 200,000 bfloat16 with 20 alternatives: 28 us a pass, 3.7
 // TB/s (without alternatives 20.6, 5.0 TB/s); 1,000 x 100,003 floats with 50: 92 us, 4.4
 // TB/s (73); 10,000 lists of 100 with 10: 9.4 us; one row of 1M: 13 us, of which the two
-// launches are 6.  Gradient: 1,000 x 100,003 floats 139 us, 5.8 TB/s.
+// launches are 6.  Gradient: 1,000 x 100,003 floats 137 us, 5.8 TB/s.
 #include <algorithm>
 #include <cmath>
 
