@@ -540,6 +540,56 @@ int qv_log_probs_grad(const void* d_logits, int32_t type, int64_t rows, int64_t 
                       const float* d_g_lse, const float* d_g_top, void* d_grad, int64_t grad_stride,
                       int device, void* stream);
 
+/* Rows in microscaled 4-bit floating point.  A block of 32 values of a row shares
+ * a power of two 2^(s - 127), s one byte (255: the block is NaN); a code is a sign
+ * (bit 3) and one of 0, 1/2, 1, 3/2, 2, 3, 4, 6; two codes to a byte, the first in its
+ * low half.  So a row of dim values is ceil(dim / 2) bytes of codes and ceil(dim / 32)
+ * of scales; the strides are in bytes.
+ *
+ * qv_quantize_rows_mx4: with a the largest magnitude of a block, s is the least for which
+ * a <= 7 2^(s - 127) (0 at least: 2^-127), and a code is x / 2^(s - 127) rounded to the
+ * nearest of those, halves to the even code, magnitudes over 6 to 6: no value is off by
+ * more than half a step.  A block that holds an infinity or a NaN gets the scale 255
+ * and zero codes; a row of odd length ends with a zero code.  type as qv_quantize_rows. */
+int qv_quantize_rows_mx4(const void* d_x, int32_t type, int64_t n, int64_t dim, int64_t x_stride, uint8_t* d_codes,
+                         int64_t code_stride, uint8_t* d_scales, int64_t scale_stride, int device, void* stream);
+
+/* What such rows stand for, rounded to out_type (bfloat16 and float hold it exactly
+ * from 2^-126 on). */
+int qv_mx4_values(const uint8_t* d_codes, int64_t code_stride, const uint8_t* d_scales, int64_t scale_stride, int64_t n,
+                  int64_t dim, void* d_out, int32_t out_type, int64_t out_stride, int device, void* stream);
+
+/* out[i][j] = sum_k a[i][k] b[j][k] + bias[j] of such rows: products exact, their sum and
+ * the bias in fp32, rounded once to out_type.  A row that holds a NaN block gives NaN.
+ * d_bias as qv_int8_product.  k is even (a row of odd length ends with a zero code).
+ * Sums below the smallest normal float may come out as 0. */
+int qv_mx4_product(const uint8_t* d_a, int64_t a_stride, const uint8_t* d_a_scales, int64_t a_scale_stride, int64_t m,
+                   const uint8_t* d_b, int64_t b_stride, const uint8_t* d_b_scales, int64_t b_scale_stride,
+                   const float* d_bias, int64_t n, int64_t k, void* d_out, int32_t out_type, int64_t out_stride, int device,
+                   void* stream);
+
+/* Layer norm of each row: y = (x - mean) / sqrt(var + eps) * weight + bias, mean and
+ * variance (over dim) of the row, in fp32, rounded once to x's type.  Weight and bias
+ * (either may be NULL: 1 and 0) have dim values of param_type.  type and param_type:
+ * QV_FLOAT, QV_BFLOAT16 or QV_FLOAT16.  eps: a positive normal float.  A row that holds
+ * an infinity or a NaN gives NaN.  d_y may be d_x with the same stride. */
+int qv_layer_norm(const void* d_x, int32_t type, int64_t rows, int64_t dim, int64_t x_stride, const void* d_weight,
+                  const void* d_bias, int32_t param_type, float eps, void* d_y, int64_t y_stride, int device, void* stream);
+
+/* The gradient of sum grad y: with x^ = (x - mean) / sqrt(var + eps) and h = grad weight,
+ *   dx = (h - mean(h) - x^ mean(h x^)) / sqrt(var + eps), of x's type (as grad is)
+ *   dweight = sum of grad x^ over the rows, dbias = sum of grad, of param_type
+ * Each of the three may be NULL (not wanted); dweight and dbias of no rows are 0.  The rows'
+ * moments are taken from x again, so nothing is kept from qv_layer_norm.  d_dx may be
+ * d_x or d_grad with the same stride.  d_workspace: qv_layer_norm_grad_workspace bytes (0:
+ * none; negative: a QV_* error), 16-byte aligned, free again once the call's work on
+ * the stream is done. */
+int64_t qv_layer_norm_grad_workspace(int64_t rows, int64_t dim);
+int qv_layer_norm_grad(const void* d_x, int32_t type, int64_t rows, int64_t dim, int64_t x_stride, const void* d_grad,
+                       int64_t grad_stride, const void* d_weight, int32_t param_type, float eps, void* d_dx,
+                       int64_t dx_stride, void* d_dweight, void* d_dbias, void* d_workspace, int64_t workspace_bytes,
+                       int device, void* stream);
+
 /* ---- Synthetic data: the seeded Gaussian mixture of the benchmark configs ----
  * Host generator (CPU) and device generator (HIP) produce identical values for
  * the same arguments.  uint8: centres uniform in [lo, hi], per-dim sigma, rounded

@@ -1,0 +1,629 @@
+// qv_layer_norm.hip -- layer norm over the rows of a matrix, and its gradient with those
+// of the weight and the bias.
+//
+// y = x^ w + b,  x^ = (x - mean) / sqrt(var + eps), mean and var over the row.  With h = g w
+// the gradient is dx = (h - mean(h) - x^ mean(h x^)) / sqrt(var + eps), dw = sum g x^ and
+// db = sum g over the rows.
+//
+// A row is read once and stays in the registers of R threads, E vectors of four values each,
+// between its sums and what is made of them; weights stay there from row to row.  The
+// deviations d = x - mean are summed too: what the mean's rounding left of them comes off
+// again, in d and in var = sum d^2 / n - (sum d / n)^2.  The gradient takes mean(h) and
+// mean(h x^) from the same exchange as var.  A row whose moments are not finite is taken
+// again times 2^-90 (its values may be up to the largest float), so only rows that hold an
+// infinity or a NaN give NaN.  All sums are fp32, in a fixed order.
+#include <algorithm>
+#include <cfloat>
+
+#include "qv_dense.hpp"
+#include "qv_device.hpp"
+
+using namespace qv;
+using namespace qv::dev;
+using namespace qv::dense;
+
+namespace {
+
+typedef float f4 __attribute__((ext_vector_type(4)));
+
+// Four values of a row, whatever the row's alignment.
+template <class T>
+__device__ __forceinline__ f4 load_four(const T* p, int64_t valid) {
+  f4 v = {0.f, 0.f, 0.f, 0.f};
+  if (valid >= 4) {
+    if constexpr (sizeof(T) == 4) {
+      const raw4 r = load_raw(p);
+#pragma unroll
+      for (int i = 0; i < 4; i++) v[i] = __uint_as_float(r[i]);
+    } else {
+      T t[4];
+      __builtin_memcpy(t, p, 8);
+#pragma unroll
+      for (int i = 0; i < 4; i++) v[i] = (float)t[i];
+    }
+  } else {
+#pragma unroll
+    for (int i = 0; i < 3; i++)
+      if (i < valid) v[i] = (float)p[i];
+  }
+  return v;
+}
+
+template <class T>
+__device__ __forceinline__ void store_four(T* p, int64_t valid, f4 v) {
+  T t[4];
+#pragma unroll
+  for (int i = 0; i < 4; i++) t[i] = (T)v[i];
+  if (valid >= 4) {
+    __builtin_memcpy(p, t, 4 * sizeof(T));
+  } else {
+#pragma unroll
+    for (int i = 0; i < 3; i++)
+      if (i < valid) p[i] = t[i];
+  }
+}
+
+// Weights or biases of any of the types; `none` without.
+__device__ __forceinline__ f4 load_params(const void* p, int type, int64_t j, int64_t dim, float none) {
+  if (!p) return f4{none, none, none, none};
+  if (type == QV_FLOAT) return load_four(static_cast<const float*>(p) + j, dim - j);
+  if (type == QV_BFLOAT16) return load_four(static_cast<const bf16*>(p) + j, dim - j);
+  return load_four(static_cast<const f16*>(p) + j, dim - j);
+}
+
+__device__ __forceinline__ void store_param(void* p, int type, int64_t j, float v) {
+  if (type == QV_FLOAT) static_cast<float*>(p)[j] = v;
+  else if (type == QV_BFLOAT16) static_cast<bf16*>(p)[j] = (bf16)v;
+  else static_cast<f16*>(p)[j] = (f16)v;
+}
+
+template <int CONTROL>
+__device__ __forceinline__ float add_dpp(float v) {
+  return v + __uint_as_float((uint32_t)__builtin_amdgcn_mov_dpp((int)__float_as_uint(v), CONTROL, 0xF, 0xF, true));
+}
+
+// The sum over the R lanes (a power of two, up to a wave) that the lane is one of, the same bits in each.
+template <int R>
+__device__ __forceinline__ float lanes_sum(float v) {
+  if constexpr (R >= 2) v = add_dpp<0xB1>(v);
+  if constexpr (R >= 4) v = add_dpp<0x4E>(v);
+  if constexpr (R >= 8) v = add_dpp<0x141>(v);   // row_half_mirror
+  if constexpr (R >= 16) v = add_dpp<0x128>(v);  // row_ror:8
+  if constexpr (R >= 32) {
+    const auto p = __builtin_amdgcn_permlane16_swap(__float_as_uint(v), __float_as_uint(v), false, false);
+    v = __uint_as_float(p[0]) + __uint_as_float(p[1]);
+  }
+  if constexpr (R >= 64) {
+    const auto p = __builtin_amdgcn_permlane32_swap(__float_as_uint(v), __float_as_uint(v), false, false);
+    v = __uint_as_float(p[0]) + __uint_as_float(p[1]);
+  }
+  return v;
+}
+
+// Sums over the R threads of a row: a part of a wave, or whole waves, which exchange theirs through two areas of LDS in
+// turn (so one barrier each: nobody writes an area again before everyone has met at the other one's).
+template <int R, int T>
+struct Row {
+  static constexpr int kWaves = R / kWave;  // of a row, where it has whole ones
+  static constexpr int kFloats = R > kWave ? 2 * 4 * (T / kWave) : 1;
+  float* lds;
+  int turn = 0;
+  bool bad = false, any_bad = false;
+  // CHECK: `bad` is set where a part of the row's v[1] is above `limit` or none at all, `any_bad` where that is so of any row
+  // of the wave, or of the workgroup where rows have more than a wave's threads: all that meet at a barrier agree on it.
+  template <bool CHECK, int N>
+  __device__ __forceinline__ void sum(float (&v)[N], float limit = 0.f) {
+    static_assert(N <= 4, "an area has four sums of each wave");
+#pragma unroll
+    for (int i = 0; i < N; i++) v[i] = lanes_sum<R < kWave ? R : kWave>(v[i]);
+    if constexpr (R > kWave) {
+      float* area = lds + turn * 4 * (T / kWave);
+      turn ^= 1;
+      const int wave = wave_id();
+      if (lane_id() == 0)
+#pragma unroll
+        for (int i = 0; i < N; i++) area[4 * wave + i] = v[i];
+      __syncthreads();
+      const float* from = area + wave / kWaves * kWaves * 4;
+      if constexpr (CHECK) {
+        any_bad = __any(lane_id() < T / kWave && !(area[4 * (lane_id() % (T / kWave)) + 1] <= limit));
+        bad = false;
+#pragma unroll
+        for (int w = 0; w < kWaves; w++) bad |= !(from[4 * w + 1] <= limit);
+      }
+#pragma unroll
+      for (int i = 0; i < N; i++) v[i] = from[i];
+#pragma unroll
+      for (int w = 1; w < kWaves; w++)
+#pragma unroll
+        for (int i = 0; i < N; i++) v[i] += from[4 * w + i];
+    } else if constexpr (CHECK) {
+      bad = !(v[1] <= limit);
+      any_bad = __any(bad);
+    }
+  }
+};
+
+// Rows whose sum of squares passes kLargest, 16 of which add up to a finite sum, are taken times kSmaller: 2^31 squares
+// of the largest float are then below it, and those of rows that passed it far above the smallest float.
+constexpr float kSmaller = 0x1p-90f, kLargest = FLT_MAX / 32.f;
+
+// Turns a thread's part of a row (0 past its end), values(e), into deviations v, of the values times `scale`; returns
+// 1 / sqrt(var + eps) of those.  With GRAD, sums[0] and sums[1] come out as the sums of h = g w and of h d.
+template <bool GRAD, int R, int T, int E, class F>
+__device__ __forceinline__ float centre(F values, f4 (&v)[E], const f4 (&g)[E], const f4 (&w)[E], int lane, int dim,
+                                        float eps, Row<R, T>& row, float& scale, float (&sums)[2]) {
+  const float per = 1.f / (float)dim;
+  scale = 1.f;
+  for (int turn = 0;; turn++) {
+    float s[1] = {0.f};
+#pragma unroll
+    for (int e = 0; e < E; e++) s[0] += (v[e][0] + v[e][1]) + (v[e][2] + v[e][3]);
+    row.template sum<false>(s);
+    const float mean = s[0] * per;
+    float m[GRAD ? 4 : 2] = {};
+#pragma unroll
+    for (int e = 0; e < E; e++) {
+      v[e] = v[e] - mean;
+      if ((e + 1) * R * 4 > dim) {  // not the whole vector of every thread is in the row
+#pragma unroll
+        for (int i = 0; i < 4; i++) v[e][i] = (e * R + lane) * 4 + i < dim ? v[e][i] : 0.f;
+      }
+#pragma unroll
+      for (int i = 0; i < 4; i++) {
+        m[0] += v[e][i];
+        m[1] = __builtin_fmaf(v[e][i], v[e][i], m[1]);
+        if constexpr (GRAD) {
+          const float h = g[e][i] * w[e][i];
+          m[2] += h;
+          m[3] = __builtin_fmaf(h, v[e][i], m[3]);
+        }
+      }
+    }
+    row.template sum<true>(m, kLargest);
+    const float rest = m[0] * per, var = max(m[1] * per - rest * rest, 0.f);
+    const bool bad = row.bad;
+    if (turn == 1 || !row.any_bad) {
+#pragma unroll
+      for (int e = 0; e < E; e++) v[e] = v[e] - rest;
+      if constexpr (GRAD) {
+        sums[0] = m[2];
+        sums[1] = m[3] - rest * m[2];
+      }
+      return 1.f / __builtin_sqrtf(bad ? __builtin_nanf("") : var + eps);
+    }
+    scale = bad ? kSmaller : 1.f;  // (other rows come out as before)
+    if (bad) eps = eps * kSmaller * kSmaller;
+#pragma unroll
+    for (int e = 0; e < E; e++) v[e] = values(e) * scale;
+  }
+}
+
+template <class T, int R, int E, int THREADS>
+__global__ __launch_bounds__(THREADS) void norm_kernel(const T* x, int64_t n, int dim, int64_t stride, const void* weight,
+                                                       const void* bias, int param_type, float eps, T* y, int64_t y_stride) {
+  constexpr int kGroups = THREADS / R;
+  __shared__ float lds[Row<R, THREADS>::kFloats];
+  Row<R, THREADS> across{lds};
+  const int lane = threadIdx.x % R;
+  f4 w[E], b[E];
+#pragma unroll
+  for (int e = 0; e < E; e++) {
+    const int j = (e * R + lane) * 4;
+    w[e] = load_params(weight, param_type, j, dim, 1.f);
+    b[e] = load_params(bias, param_type, j, dim, 0.f);
+  }
+  for (int64_t base = (int64_t)blockIdx.x * kGroups; base < n; base += (int64_t)gridDim.x * kGroups) {
+    const int64_t row = base + threadIdx.x / R;
+    const T* from = x + min(row, n - 1) * stride;
+    auto values = [&](int e) { return load_four(from + (e * R + lane) * 4, dim - (e * R + lane) * 4); };
+    f4 v[E];
+#pragma unroll
+    for (int e = 0; e < E; e++) v[e] = values(e);
+    float scale, none[2];
+    const float rstd = centre<false>(values, v, v, v, lane, dim, eps, across, scale, none);
+    if (row >= n) continue;
+#pragma unroll
+    for (int e = 0; e < E; e++) {
+      const int j = (e * R + lane) * 4;
+      f4 o;
+#pragma unroll
+      for (int i = 0; i < 4; i++) o[i] = __builtin_fmaf(v[e][i] * rstd, w[e][i], b[e][i]);
+      store_four(y + row * y_stride + j, dim - j, o);
+    }
+  }
+}
+
+// Adds up the rows that its groups have seen of a column's sums: `part` of this workgroup, its sums of g x^, then those of g.
+template <class T, int R, int E, int THREADS>
+__global__ __launch_bounds__(THREADS) void norm_grad_kernel(const T* x, int64_t n, int dim, int64_t stride, const T* grad,
+                                                            int64_t grad_stride, const void* weight, int param_type,
+                                                            float eps, T* dx, int64_t dx_stride, float* parts, int pitch) {
+  constexpr int kGroups = THREADS / R;
+  constexpr int kWide = R * E * 4;
+  __shared__ float lds[Row<R, THREADS>::kFloats];
+  __shared__ __align__(16) float columns[kGroups > 1 ? kGroups * kWide : 1];
+  Row<R, THREADS> across{lds};
+  const int lane = threadIdx.x % R, group = threadIdx.x / R;
+  f4 w[E], dw[E], db[E];
+#pragma unroll
+  for (int e = 0; e < E; e++) {
+    w[e] = load_params(weight, param_type, (e * R + lane) * 4, dim, 1.f);
+    dw[e] = db[e] = f4{0.f, 0.f, 0.f, 0.f};
+  }
+  const float per = 1.f / (float)dim;
+  for (int64_t base = (int64_t)blockIdx.x * kGroups; base < n; base += (int64_t)gridDim.x * kGroups) {
+    const int64_t row = base + group, at = min(row, n - 1);
+    const T *from = x + at * stride, *from_g = grad + at * grad_stride;
+    auto values = [&](int e) { return load_four(from + (e * R + lane) * 4, dim - (e * R + lane) * 4); };
+    f4 v[E], g[E];
+#pragma unroll
+    for (int e = 0; e < E; e++) v[e] = values(e);
+#pragma unroll
+    for (int e = 0; e < E; e++) g[e] = load_four(from_g + (e * R + lane) * 4, dim - (e * R + lane) * 4);
+    float scale, sums[2];
+    const float rstd = centre<true>(values, v, g, w, lane, dim, eps, across, scale, sums);
+    if (row >= n) continue;
+    // x^ = d rstd; dx = scale rstd (h - c1 - x^ c2)
+    const float c1 = sums[0] * per, c2 = sums[1] * per * rstd;
+#pragma unroll
+    for (int e = 0; e < E; e++) {
+      const int j = (e * R + lane) * 4;
+      f4 o;
+#pragma unroll
+      for (int i = 0; i < 4; i++) {
+        const float hat = v[e][i] * rstd;
+        o[i] = __builtin_fmaf(-hat, c2, g[e][i] * w[e][i] - c1) * (rstd * scale);
+        dw[e][i] = __builtin_fmaf(g[e][i], hat, dw[e][i]);
+        db[e][i] += g[e][i];
+      }
+      if (dx) store_four(dx + row * dx_stride + j, dim - j, o);
+    }
+  }
+  if (!parts) return;
+  float* part = parts + (int64_t)blockIdx.x * 2 * pitch;
+#pragma unroll
+  for (int of = 0; of < 2; of++) {
+    if constexpr (kGroups == 1) {
+#pragma unroll
+      for (int e = 0; e < E; e++) {
+        const int j = (e * R + lane) * 4;
+        if (j < dim) *reinterpret_cast<f4*>(part + of * pitch + j) = of ? db[e] : dw[e];
+      }
+    } else {
+      if (of) __syncthreads();
+#pragma unroll
+      for (int e = 0; e < E; e++) *reinterpret_cast<f4*>(columns + group * kWide + (e * R + lane) * 4) = of ? db[e] : dw[e];
+      __syncthreads();
+      for (int j = threadIdx.x; j < dim; j += THREADS) {
+        float s = 0.f;
+#pragma unroll
+        for (int q = 0; q < kGroups; q++) s += columns[q * kWide + j];
+        part[of * pitch + j] = s;
+      }
+    }
+  }
+}
+
+// The columns' sums over `count` parts: 32 columns per workgroup, 32 threads each.
+__global__ __launch_bounds__(1024) void join_columns_kernel(const float* parts, int64_t count, int dim, int pitch, void* dweight,
+                                                            void* dbias, int param_type) {
+  __shared__ float sums[32][33];
+  const int column = threadIdx.x % 32, slice = threadIdx.x / 32;
+  const int j = blockIdx.x * 32 + column;
+  void* out = blockIdx.y ? dbias : dweight;
+  if (!out) return;
+  float s = 0.f;
+  if (j < dim)
+    for (int64_t q = slice; q < count; q += 32) s += parts[(q * 2 + blockIdx.y) * pitch + j];
+  sums[slice][column] = s;
+  __syncthreads();
+  if (slice == 0 && j < dim) {
+#pragma unroll
+    for (int q = 1; q < 32; q++) s += sums[q][column];
+    store_param(out, param_type, j, s);
+  }
+}
+
+// ---- rows longer than 16,384 ---------------------------------------------------------
+//
+// A workgroup per row, which is read again for each step (from the caches while it fits).
+// The gradient's columns take what they need of the rows from `Moments`.
+
+struct Moments {
+  float mean, rest, rstd, scale, c1, c2, none[2];
+};
+
+template <bool GRAD, class T>
+__device__ __forceinline__ Moments long_moments(const T* x, const T* g, const void* weight, int param_type, int64_t dim,
+                                                float eps, Row<1024, 1024>& across) {
+  const float per = 1.f / (float)dim;
+  Moments r = {0.f, 0.f, 0.f, 1.f, 0.f, 0.f, {0.f, 0.f}};
+  for (int turn = 0;; turn++) {
+    float s[1] = {0.f};
+    for (int64_t j = threadIdx.x * 4; j < dim; j += 4096) {
+      const f4 v = load_four(x + j, dim - j) * r.scale;
+      s[0] += (v[0] + v[1]) + (v[2] + v[3]);
+    }
+    across.template sum<false>(s);
+    r.mean = s[0] * per;
+    float m[GRAD ? 4 : 2] = {};
+    for (int64_t j = threadIdx.x * 4; j < dim; j += 4096) {
+      const f4 v = load_four(x + j, dim - j);
+      f4 h = {};
+      if constexpr (GRAD) h = load_four(g + j, dim - j) * load_params(weight, param_type, j, dim, 1.f);
+#pragma unroll
+      for (int i = 0; i < 4; i++) {
+        const float d = j + i < dim ? v[i] * r.scale - r.mean : 0.f;
+        m[0] += d;
+        m[1] = __builtin_fmaf(d, d, m[1]);
+        if constexpr (GRAD) {
+          m[2] += h[i];
+          m[3] = __builtin_fmaf(h[i], d, m[3]);
+        }
+      }
+    }
+    across.template sum<true>(m, kLargest);
+    r.rest = m[0] * per;
+    const bool bad = across.bad;
+    if (turn == 1 || !bad) {
+      const float var = max(m[1] * per - r.rest * r.rest, 0.f);
+      r.rstd = 1.f / __builtin_sqrtf(bad ? __builtin_nanf("") : var + eps);
+      if constexpr (GRAD) {
+        r.c1 = m[2] * per;
+        r.c2 = (m[3] - r.rest * m[2]) * per * r.rstd;
+      }
+      return r;
+    }
+    r.scale = kSmaller;
+    eps = eps * kSmaller * kSmaller;
+  }
+}
+
+template <class T>
+__global__ __launch_bounds__(1024) void norm_long_kernel(const T* x, int64_t n, int64_t dim, int64_t stride, const void* weight,
+                                                         const void* bias, int param_type, float eps, T* y, int64_t y_stride) {
+  __shared__ float lds[Row<1024, 1024>::kFloats];
+  Row<1024, 1024> across{lds};
+  for (int64_t row = blockIdx.x; row < n; row += gridDim.x) {
+    const T* from = x + row * stride;
+    const Moments r = long_moments<false, T>(from, nullptr, nullptr, 0, dim, eps, across);
+    for (int64_t j = threadIdx.x * 4; j < dim; j += 4096) {
+      const f4 v = load_four(from + j, dim - j), w = load_params(weight, param_type, j, dim, 1.f),
+               b = load_params(bias, param_type, j, dim, 0.f);
+      f4 o;
+#pragma unroll
+      for (int i = 0; i < 4; i++) o[i] = __builtin_fmaf((v[i] * r.scale - r.mean - r.rest) * r.rstd, w[i], b[i]);
+      store_four(y + row * y_stride + j, dim - j, o);
+    }
+  }
+}
+
+template <class T>
+__global__ __launch_bounds__(1024) void long_moments_kernel(const T* x, int64_t n, int64_t dim, int64_t stride, const T* grad,
+                                                            int64_t grad_stride, const void* weight, int param_type, float eps,
+                                                            Moments* moments) {
+  __shared__ float lds[Row<1024, 1024>::kFloats];
+  Row<1024, 1024> across{lds};
+  for (int64_t row = blockIdx.x; row < n; row += gridDim.x) {
+    const Moments r = long_moments<true, T>(x + row * stride, grad + row * grad_stride, weight, param_type, dim, eps, across);
+    if (threadIdx.x == 0) moments[row] = r;
+  }
+}
+
+// 1,024 columns of every `slices`-th row.
+template <class T>
+__global__ __launch_bounds__(256) void long_columns_kernel(const T* x, int64_t n, int64_t dim, int64_t stride, const T* grad,
+                                                           int64_t grad_stride, const Moments* moments, int slices,
+                                                           float* parts, int pitch) {
+  const int64_t j = ((int64_t)blockIdx.x * 256 + threadIdx.x) * 4;
+  if (j >= dim) return;
+  f4 dw = {0.f, 0.f, 0.f, 0.f}, db = dw;
+  for (int64_t row = blockIdx.y; row < n; row += slices) {
+    const Moments r = moments[row];
+    const f4 v = load_four(x + row * stride + j, dim - j), g = load_four(grad + row * grad_stride + j, dim - j);
+#pragma unroll
+    for (int i = 0; i < 4; i++) {
+      dw[i] = __builtin_fmaf(g[i], (v[i] * r.scale - r.mean - r.rest) * r.rstd, dw[i]);
+      db[i] += g[i];
+    }
+  }
+  float* part = parts + (int64_t)blockIdx.y * 2 * pitch;
+  *reinterpret_cast<f4*>(part + j) = dw;
+  *reinterpret_cast<f4*>(part + pitch + j) = db;
+}
+
+template <class T>
+__global__ __launch_bounds__(256) void long_grad_kernel(const T* x, int64_t n, int64_t dim, int64_t stride, const T* grad,
+                                                        int64_t grad_stride, const void* weight, int param_type,
+                                                        const Moments* moments, T* dx, int64_t dx_stride) {
+  const int64_t j = ((int64_t)blockIdx.x * 256 + threadIdx.x) * 4;
+  if (j >= dim) return;
+  const f4 w = load_params(weight, param_type, j, dim, 1.f);
+  for (int64_t row = blockIdx.y; row < n; row += gridDim.y) {
+    const Moments r = moments[row];
+    const f4 v = load_four(x + row * stride + j, dim - j), h = load_four(grad + row * grad_stride + j, dim - j) * w;
+    f4 o;
+#pragma unroll
+    for (int i = 0; i < 4; i++) {
+      const float hat = (v[i] * r.scale - r.mean - r.rest) * r.rstd;
+      o[i] = __builtin_fmaf(-hat, r.c2, h[i] - r.c1) * (r.rstd * r.scale);
+    }
+    store_four(dx + row * dx_stride + j, dim - j, o);
+  }
+}
+
+// ---- host side -----------------------------------------------------------------------
+
+constexpr int64_t kLong = 16384;    // longer rows do not stay in a workgroup's registers
+constexpr int64_t kGradBlocks = 256;  // workgroups of the gradient, one per CU, and so parts of the columns' sums
+
+// f(threads per row, vectors per thread) for rows of `dim`: the fewest of 3 or 4 vectors each in 4 to 64, 256 or 1,024
+// threads that hold it, so that a third of them at most (a half below 32 values, three quarters past 1,024 and 4,096)
+// stay empty.
+template <class F>
+void by_width(int64_t dim, F f) {
+  auto threads = [&](auto vectors) {
+    using E = decltype(vectors);
+    const int64_t least = (dim + 4 * E::value - 1) / (4 * E::value);
+    if (least <= 4) f(std::integral_constant<int, 4>(), E());
+    else if (least <= 8) f(std::integral_constant<int, 8>(), E());
+    else if (least <= 16) f(std::integral_constant<int, 16>(), E());
+    else if (least <= 32) f(std::integral_constant<int, 32>(), E());
+    else if (least <= 64) f(std::integral_constant<int, 64>(), E());
+    else if (least <= 256) f(std::integral_constant<int, 256>(), E());
+    else f(std::integral_constant<int, 1024>(), E());
+  };
+  int64_t three = 4;
+  while (three * 12 < dim) three *= three < 64 ? 2 : 4;
+  int64_t four = 4;
+  while (four * 16 < dim) four *= four < 64 ? 2 : 4;
+  if (three <= four) threads(std::integral_constant<int, 3>());
+  else threads(std::integral_constant<int, 4>());
+}
+
+int pitch_of(int64_t dim) { return (int)((dim + 3) / 4 * 4); }
+
+int64_t long_slices(int64_t n, int64_t dim) { return std::min<int64_t>(n, std::max<int64_t>(1, 2048 / ((dim + 1023) / 1024))); }
+
+int64_t workspace_bytes(int64_t n, int64_t dim) {
+  if (n == 0 || dim == 0) return 0;
+  if (dim > kLong) return n * (int64_t)sizeof(Moments) + long_slices(n, dim) * 2 * pitch_of(dim) * 4;
+  return std::min(n, kGradBlocks) * 2 * pitch_of(dim) * 4;
+}
+
+template <class T>
+void norm(const void* x, int64_t n, int64_t dim, int64_t stride, const void* weight, const void* bias, int param_type,
+          float eps, void* y, int64_t y_stride, hipStream_t st) {
+  const T* in = static_cast<const T*>(x);
+  T* out = static_cast<T*>(y);
+  if (dim > kLong) {
+    hipLaunchKernelGGL(norm_long_kernel<T>, dim3((unsigned)std::min<int64_t>(n, 1 << 20)), dim3(1024), 0, st, in, n, dim,
+                       stride, weight, bias, param_type, eps, out, y_stride);
+  } else {
+    by_width(dim, [&](auto threads, auto vectors) {
+      constexpr int R = decltype(threads)::value, E = decltype(vectors)::value, T0 = R > 256 ? R : 256;
+      const int64_t blocks = std::min<int64_t>((n + T0 / R - 1) / (T0 / R), 256 * 2048 / T0);
+      hipLaunchKernelGGL((norm_kernel<T, R, E, T0>), dim3((unsigned)blocks), dim3(T0), 0, st, in, n, (int)dim, stride, weight,
+                         bias, param_type, eps, out, y_stride);
+    });
+  }
+  HIP_OK(hipGetLastError());
+}
+
+template <class T>
+void norm_grad(const void* x, int64_t n, int64_t dim, int64_t stride, const void* grad, int64_t grad_stride,
+               const void* weight, int param_type, float eps, void* dx, int64_t dx_stride, void* dweight, void* dbias,
+               void* workspace, hipStream_t st) {
+  const T *in = static_cast<const T*>(x), *g = static_cast<const T*>(grad);
+  T* out = static_cast<T*>(dx);
+  const int pitch = pitch_of(dim);
+  const bool columns = dweight || dbias;
+  float* parts = static_cast<float*>(workspace);
+  int64_t count = 0;
+  if (n > 0 && dim > kLong) {
+    Moments* moments = static_cast<Moments*>(workspace);
+    parts = reinterpret_cast<float*>(moments + n);
+    count = long_slices(n, dim);
+    const unsigned wide = (unsigned)((dim + 1023) / 1024);
+    hipLaunchKernelGGL(long_moments_kernel<T>, dim3((unsigned)std::min<int64_t>(n, 1 << 20)), dim3(1024), 0, st, in, n, dim,
+                       stride, g, grad_stride, weight, param_type, eps, moments);
+    if (columns)
+      hipLaunchKernelGGL(long_columns_kernel<T>, dim3(wide, (unsigned)count), dim3(256), 0, st, in, n, dim, stride, g,
+                         grad_stride, moments, (int)count, parts, pitch);
+    if (dx)
+      hipLaunchKernelGGL(long_grad_kernel<T>, dim3(wide, (unsigned)std::min<int64_t>(n, 1024)), dim3(256), 0, st, in, n, dim,
+                         stride, g, grad_stride, weight, param_type, moments, out, dx_stride);
+  } else if (n > 0) {
+    by_width(dim, [&](auto threads, auto vectors) {
+      constexpr int R = decltype(threads)::value, E = decltype(vectors)::value, T0 = 1024;
+      count = std::min((n + T0 / R - 1) / (T0 / R), kGradBlocks);
+      hipLaunchKernelGGL((norm_grad_kernel<T, R, E, T0>), dim3((unsigned)count), dim3(T0), 0, st, in, n, (int)dim, stride, g,
+                         grad_stride, weight, param_type, eps, out, dx_stride, columns ? parts : nullptr, pitch);
+    });
+  }
+  HIP_OK(hipGetLastError());
+  if (columns) {
+    hipLaunchKernelGGL(join_columns_kernel, dim3((unsigned)((dim + 31) / 32), 2), dim3(1024), 0, st, parts, count, (int)dim,
+                       pitch, dweight, dbias, param_type);
+    HIP_OK(hipGetLastError());
+  }
+}
+
+void check_params(const char* name, const void* p, int64_t dim, int type) {
+  if (p && dim > 0) check_matrix(name, p, 1, dim, dim, value_size(type));
+}
+
+void check_eps(float eps) {
+  if (!(eps >= FLT_MIN && eps <= FLT_MAX)) qv::fail(QV_EINVAL, "eps must be positive, normal and finite");
+}
+
+void check_sizes(int64_t n, int64_t dim) {
+  if (n < 0 || dim < 0) qv::fail(QV_EINVAL, "negative size");
+  if (n > INT32_MAX || dim > INT32_MAX) qv::fail(QV_EUNSUPPORTED, "more than 2^31 - 1 rows or columns");
+}
+
+}  // namespace
+
+extern "C" {
+
+int qv_layer_norm(const void* d_x, int32_t type, int64_t rows, int64_t dim, int64_t x_stride, const void* d_weight,
+                  const void* d_bias, int32_t param_type, float eps, void* d_y, int64_t y_stride, int device, void* stream) {
+  return qv::guard([&] {
+    check_sizes(rows, dim);
+    check_matrix("x", d_x, rows, dim, x_stride, value_size(type));
+    check_matrix("y", d_y, rows, dim, y_stride, value_size(type));
+    value_size(param_type);
+    check_params("weight", d_weight, dim, param_type);
+    check_params("bias", d_bias, dim, param_type);
+    check_eps(eps);
+    if (rows == 0 || dim == 0) return;
+    const OnDevice on(device);
+    const hipStream_t st = static_cast<hipStream_t>(stream);
+    if (type == QV_FLOAT) norm<float>(d_x, rows, dim, x_stride, d_weight, d_bias, param_type, eps, d_y, y_stride, st);
+    else if (type == QV_BFLOAT16) norm<bf16>(d_x, rows, dim, x_stride, d_weight, d_bias, param_type, eps, d_y, y_stride, st);
+    else norm<f16>(d_x, rows, dim, x_stride, d_weight, d_bias, param_type, eps, d_y, y_stride, st);
+  });
+}
+
+int64_t qv_layer_norm_grad_workspace(int64_t rows, int64_t dim) {
+  int64_t bytes = 0;
+  const int rc = qv::guard([&] {
+    check_sizes(rows, dim);
+    bytes = workspace_bytes(rows, dim);
+  });
+  return rc == QV_OK ? bytes : rc;
+}
+
+int qv_layer_norm_grad(const void* d_x, int32_t type, int64_t rows, int64_t dim, int64_t x_stride, const void* d_grad,
+                       int64_t grad_stride, const void* d_weight, int32_t param_type, float eps, void* d_dx,
+                       int64_t dx_stride, void* d_dweight, void* d_dbias, void* d_workspace, int64_t workspace_bytes,
+                       int device, void* stream) {
+  return qv::guard([&] {
+    check_sizes(rows, dim);
+    check_matrix("x", d_x, rows, dim, x_stride, value_size(type));
+    check_matrix("grad", d_grad, rows, dim, grad_stride, value_size(type));
+    if (d_dx) check_matrix("dx", d_dx, rows, dim, dx_stride, value_size(type));
+    value_size(param_type);
+    check_params("weight", d_weight, dim, param_type);
+    check_params("dweight", d_dweight, dim, param_type);
+    check_params("dbias", d_dbias, dim, param_type);
+    check_eps(eps);
+    if (dim == 0 || (!d_dx && !d_dweight && !d_dbias)) return;
+    const int64_t need = ::workspace_bytes(rows, dim);
+    if (need > 0 && (!d_workspace || workspace_bytes < need || reinterpret_cast<uintptr_t>(d_workspace) % 16))
+      qv::fail(QV_EINVAL, "workspace: missing, too small or not 16-byte aligned");
+    const OnDevice on(device);
+    const hipStream_t st = static_cast<hipStream_t>(stream);
+    auto go = [&](auto* t) {
+      using T = std::remove_pointer_t<decltype(t)>;
+      norm_grad<T>(d_x, rows, dim, x_stride, d_grad, grad_stride, d_weight, param_type, eps, d_dx, dx_stride, d_dweight,
+                   d_dbias, d_workspace, st);
+    };
+    if (type == QV_FLOAT) go(static_cast<float*>(nullptr));
+    else if (type == QV_BFLOAT16) go(static_cast<bf16*>(nullptr));
+    else go(static_cast<f16*>(nullptr));
+  });
+}
+
+}  // extern "C"

@@ -1,10 +1,8 @@
 // qv_scores.hip -- rows to 8 bits with a scale each, and the integer product of two
 // such matrices.
 #include <algorithm>
-#include <atomic>
 
-#include "qv_dense.hpp"
-#include "qv_device.hpp"
+#include "qv_product.hpp"
 
 using namespace qv;
 using namespace qv::dev;
@@ -158,15 +156,7 @@ __global__ __launch_bounds__(256) void quantize_long_kernel(const T* __restrict_
 // plain one for rows shorter than a piece.  All sum in int32 and scale in the order of
 // the definition, so they give the same bits.
 
-typedef int32_t i4 __attribute__((ext_vector_type(4)));
-typedef int32_t i16v __attribute__((ext_vector_type(16)));
-typedef float f4 __attribute__((ext_vector_type(4)));
-typedef i4 i4_any __attribute__((aligned(1), may_alias));
-typedef f4 f4_any __attribute__((aligned(4), may_alias));
-
-constexpr int kLoadsDone = 0x0f70;  // s_waitcnt vmcnt(0)
-constexpr int kStage = 128;         // bytes of k per stage
-constexpr int64_t kFar = 1 << 23;   // operands' row strides from here on: 256 rows' offsets pass 31 bits
+constexpr int64_t kFar = 1 << 23;  // operands' row strides from here on: 256 rows' offsets pass 31 bits
 
 template <class O>
 struct Product {
@@ -182,16 +172,6 @@ struct Product {
   O* out;
   int64_t out_stride;
 };
-
-// What a piece starting `over` bytes before its place repeats, zeroed.
-__device__ __forceinline__ i4 without_first(i4 v, int over) {
-#pragma unroll
-  for (int w = 0; w < 4; w++) {
-    const int cut = over - 4 * w;
-    v[w] = cut <= 0 ? v[w] : cut >= 4 ? 0 : (int32_t)((uint32_t)v[w] & (~0u << (8 * cut)));
-  }
-  return v;
-}
 
 __device__ __forceinline__ i16v mfma(i4 x, i4 y, i16v acc) {
   return __builtin_amdgcn_mfma_i32_32x32x32_i8(x, y, acc, 0, 0, 0);
@@ -209,98 +189,22 @@ __device__ __forceinline__ void put_sums(int32_t* tile, int stride, const i16v& 
   }
 }
 
-// Two values in the output's 16 bits, halves to even.  By instruction: the compiler takes the bfloat16 one apart, and
-// joins float16 to the product before it, whose rounding to fp32 is then left out.
-template <class O>
-__device__ __forceinline__ uint32_t two_of(float x, float y) {
-  uint32_t both;
-  if constexpr (std::is_same<O, bf16>::value) asm("v_cvt_pk_bf16_f32 %0, %1, %2" : "=v"(both) : "v"(x), "v"(y));
-  else asm("v_cvt_pk_f16_f32 %0, %1, %2" : "=v"(both) : "v"(x), "v"(y));
-  return both;
-}
-
-// Of P pieces of 16 bytes in each of P lanes, the lane's own one of every lane: the P x P transposed.
-template <int P>
-__device__ __forceinline__ void swap_pieces(i4 (&u)[P]) {
-  auto stage = [&](auto distance, auto control) {
-    constexpr int D = decltype(distance)::value, kControl = decltype(control)::value;
-    const bool up = lane_id() & D;
-#pragma unroll
-    for (int q = 0; q < P; q++) {
-      if (q & D) continue;
-#pragma unroll
-      for (int w = 0; w < 4; w++) {
-        const int lo = u[q][w], hi = u[q | D][w];
-        const int other_lo = __builtin_amdgcn_mov_dpp(lo, kControl, 0xF, 0xF, true);
-        const int other_hi = __builtin_amdgcn_mov_dpp(hi, kControl, 0xF, 0xF, true);
-        u[q][w] = up ? other_hi : lo;
-        u[q | D][w] = up ? hi : other_lo;
-      }
-    }
-  };
-  stage(std::integral_constant<int, 1>(), std::integral_constant<int, 0xB1>());                          // quad_perm [1,0,3,2]
-  if constexpr (P == 4) stage(std::integral_constant<int, 2>(), std::integral_constant<int, 0x4E>());  // quad_perm [2,3,0,1]
-}
-
-// Scales the results of R instructions, 32 R columns from j of the rows around the lane's row i, and stores them from
-// the registers, whole lines of 8 rows at once (half lines of 16 rows with 32 columns of 16 bits).  Of the four columns
-// that a lane has of every eight, those of 16 bits pass to the other half of the wave and back, eight for a lane; then
-// groups of lanes swap rows for pieces of one row.  (Pieces stored as they are, 32 bytes of 32 rows at once, take 5.0
-// for 5.35 TB/s in aligned rows, 2 for 3.8 in others.)  `sb`, `add`: the columns' scales and biases in LDS.  WHOLE:
-// all of it lies in the output.
+// Scales the results of R instructions, 32 R columns from j of the rows around the lane's row i, and stores them.
+// `sb`, `add`: the columns' scales and biases in LDS.
 template <bool WHOLE, int R, class O>
 __device__ __forceinline__ void store_sums(const i16v* const (&acc)[R], float sa, const float* sb, const float* add,
                                            int64_t i, int64_t j, const Product<O>& p) {
-  constexpr int V = 16 / (int)sizeof(O), N = 16 / V, P = R * N;  // columns of a piece, pieces of a result, of all
-  const int half = lane_id() / 32, c = lane_id() % P;
-  i4 u[P];
+  const int half = lane_id() / 32;
+  store_results<WHOLE, R>(
+      [&](int y, int g) {
+        const int at = 32 * y + 8 * g + 4 * half;
+        const f4 s = *reinterpret_cast<const f4*>(sb + at), t = *reinterpret_cast<const f4*>(add + at);
+        f4 v;
 #pragma unroll
-  for (int y = 0; y < R; y++) {
-    float v[16];
-#pragma unroll
-    for (int g = 0; g < 4; g++) {
-      const int at = 32 * y + 8 * g + 4 * half;
-      const f4 s = *reinterpret_cast<const f4*>(sb + at), t = *reinterpret_cast<const f4*>(add + at);
-#pragma unroll
-      for (int e = 0; e < 4; e++) v[4 * g + e] = ((float)(*acc[y])[4 * g + e] * sa) * s[e] + t[e];
-    }
-#pragma unroll
-    for (int q = 0; q < N; q++) {
-      if constexpr (sizeof(O) == 4) {
-#pragma unroll
-        for (int e = 0; e < 4; e++) u[N * y + q][e] = __float_as_int(v[4 * q + e]);
-      } else {
-#pragma unroll
-        for (int d = 0; d < 2; d++) {
-          const auto both = __builtin_amdgcn_permlane32_swap(two_of<O>(v[8 * q + 2 * d], v[8 * q + 2 * d + 1]),
-                                                             two_of<O>(v[8 * q + 4 + 2 * d], v[8 * q + 5 + 2 * d]), false, false);
-          u[N * y + q][d] = (int)both[0];
-          u[N * y + q][2 + d] = (int)both[1];
-        }
-      }
-    }
-  }
-  swap_pieces(u);
-  i -= c;
-  j += 2 * V * c + V * half;
-  O* to = p.out + (i * p.out_stride + j);
-  if (WHOLE || j + V <= p.n) {
-#pragma unroll
-    for (int r = 0; r < P; r++)
-      if (WHOLE || i + r < p.m) *reinterpret_cast<i4_any*>(to + r * p.out_stride) = u[r];
-  } else {
-#pragma unroll
-    for (int r = 0; r < P; r++) {
-      union {
-        i4 raw;
-        O o[V];
-      } piece;
-      piece.raw = u[r];
-#pragma unroll
-      for (int e = 0; e < V; e++)
-        if (i + r < p.m && j + e < p.n) to[r * p.out_stride + e] = piece.o[e];
-    }
-  }
+        for (int e = 0; e < 4; e++) v[e] = ((float)(*acc[y])[4 * g + e] * sa) * s[e] + t[e];
+        return v;
+      },
+      i, j, p.m, p.n, p.out, p.out_stride);
 }
 
 // The scales and biases of the 16 bytes of a row, of J columns from j0, that a lane stores.
@@ -410,12 +314,6 @@ struct TileScales {
   }
 };
 
-// Workgroups go round the eight XCDs: each XCD gets a run of consecutive tiles.
-__device__ __forceinline__ int64_t tile_of_block(int64_t block, int64_t tiles) {
-  const int64_t xcd = block % 8, per = tiles / 8, more = tiles % 8;
-  return xcd * per + min(xcd, more) + block / 8;
-}
-
 // A tile of BM x BN outputs per workgroup, WM x WN waves of 32 TM x 32 TN each.  Both
 // operands' stages go through registers into LDS, the next one in flight while the
 // matrix cores work on this one; piece q of row r lies at q ^ (r / 2 mod 8), so that the
@@ -520,24 +418,6 @@ __global__ __launch_bounds__(64 * WM * WN, 1) void product_tile_kernel(Product<O
 // 273); 8,192^3 of zeros 349 us, 3.1 POP/s, of codes over the whole range 545 us at 1.5
 // GHz (the matrix instruction alone reaches 4.5 and 3.3 POP/s).  Loads and LDS reads in
 // runs of their own instead of between the products: a fifth more.
-//
-// The schedule's next N x (P matrix instructions, one of the given kind): a matrix
-// instruction takes 32 cycles, in which a wave can issue a few others; in a run of
-// their own they would leave the matrix pipe idle.
-constexpr int kMfma = 0x008, kVmem = 0x010, kDsRead = 0x100;
-template <int N, int KIND, int P>
-__device__ __forceinline__ void between() {
-#pragma unroll
-  for (int i = 0; i < N; i++) {
-    __builtin_amdgcn_sched_group_barrier(kMfma, P, 0);
-    __builtin_amdgcn_sched_group_barrier(KIND, 1, 0);
-  }
-}
-
-constexpr int kReadsDone = 0xc07f;  // s_waitcnt lgkmcnt(0)
-template <int N>
-constexpr int kWaitFor = (N & 15) | (N >> 4 << 14) | 0x0070;  // s_waitcnt vmcnt(N) lgkmcnt(0)
-
 template <int BM, int BN, int WM, int WN, int NB, bool MANY, class O>
 __global__ __launch_bounds__(64 * WM * WN, 1) void product_deep_kernel(Product<O> p, int64_t tiles_m, int64_t tiles_n,
                                                                        int64_t group) {
@@ -981,19 +861,6 @@ void quantize(const void* x, int64_t n, int64_t dim, int64_t stride, int8_t* cod
                          scales, first);
     });
   HIP_OK(hipGetLastError());
-}
-
-// More than 64 KB of LDS is asked for once per kernel and device.
-template <auto* KERNEL>
-void allow_lds(int bytes) {
-  static std::atomic<uint64_t> done{0};
-  if (bytes <= 65536) return;
-  int device = 0;
-  HIP_OK(hipGetDevice(&device));
-  const uint64_t bit = device < 64 ? 1ull << device : 0;
-  if (done.load(std::memory_order_relaxed) & bit) return;
-  HIP_OK(hipFuncSetAttribute(reinterpret_cast<const void*>(KERNEL), hipFuncAttributeMaxDynamicSharedMemorySize, 160 * 1024));
-  done.fetch_or(bit, std::memory_order_relaxed);
 }
 
 template <int BM, int BN, int WM, int WN, class O>

@@ -206,6 +206,13 @@ SIGNATURES = {
                             C.c_int, _P]),
     "qv_log_probs_grad": (_I32, [_P, _I32, _I64, _I64, _I64, C.c_float, _P, _P, _P, _I32, _P, _I32, _P, _P, _P, _P,
                                  _P, _I64, C.c_int, _P]),
+    "qv_quantize_rows_mx4": (_I32, [_P, _I32, _I64, _I64, _I64, _P, _I64, _P, _I64, C.c_int, _P]),
+    "qv_mx4_values": (_I32, [_P, _I64, _P, _I64, _I64, _I64, _P, _I32, _I64, C.c_int, _P]),
+    "qv_mx4_product": (_I32, [_P, _I64, _P, _I64, _I64, _P, _I64, _P, _I64, _P, _I64, _I64, _P, _I32, _I64, C.c_int, _P]),
+    "qv_layer_norm": (_I32, [_P, _I32, _I64, _I64, _I64, _P, _P, _I32, C.c_float, _P, _I64, C.c_int, _P]),
+    "qv_layer_norm_grad_workspace": (_I64, [_I64, _I64]),
+    "qv_layer_norm_grad": (_I32, [_P, _I32, _I64, _I64, _I64, _P, _I64, _P, _I32, C.c_float, _P, _I64, _P, _P, _P, _I64,
+                                  C.c_int, _P]),
     "qv_find_index_files": (_I32, [C.c_char_p, C.c_char_p, C.c_char_p, _I32]),
     "qv_read_layout": (_I32, [C.c_char_p, C.c_char_p, C.POINTER(IndexInfo)]),
     "qv_read_index_pages": (_I32, [C.c_char_p, _I64, _P]),

@@ -1,16 +1,19 @@
 """Dense scores and the distribution over them, on torch tensors of one GPU.
 
 What stands next to a graph search: scoring a whole catalogue (or a linear
-layer) by inner products in 8 bits, and what a model's answer or its training
-loss takes from scores -- log probabilities of the relevant columns, the
-entropy, the best alternatives (a retriever's hard negatives), the gradient.
+layer) by inner products in 8 bits or in microscaled 4 bits, what a model's
+answer or its training loss takes from scores -- log probabilities of the
+relevant columns, the entropy, the best alternatives (a retriever's hard
+negatives), the gradient -- and the layer norm that embeddings come from.
 
-``quantize_rows``, ``int8_product``, ``log_probs`` and ``log_probs_grad`` are
-the C ABI's calls (include/quiver_hip.h) on the current stream of the tensors'
-GPU; none of them waits.  ``log_probs`` takes part in autograd (reverse mode);
-where there is no derivative, an argument that asks for one is refused.
-``DenseCatalogue`` runs them together: a catalogue kept in 8 bits, scored and
-normalised for batches of queries.
+``quantize_rows``, ``int8_product``, ``quantize_rows_mx4``, ``mx4_values``,
+``mx4_product``, ``log_probs``, ``log_probs_grad``, ``layer_norm`` and
+``layer_norm_grad`` are the C ABI's calls (include/quiver_hip.h) on the current
+stream of the tensors' GPU; none of them waits.  ``log_probs`` and
+``layer_norm`` take part in autograd (reverse mode); where there is no
+derivative, an argument that asks for one is refused.  ``DenseCatalogue`` runs
+them together: a catalogue kept in 8 or 4 bits, scored and normalised for
+batches of queries.
 
 Results can be handed back through ``out=`` to be written again (a loop then
 allocates nothing); a result is ordered with the stream it was made on.  A wrong
@@ -36,6 +39,7 @@ from torch.autograd import forward_ad  # noqa: E402
 
 _TYPES = {torch.float32: _lib.QV_FLOAT, torch.bfloat16: _lib.QV_BFLOAT16, torch.float16: _lib.QV_FLOAT16}
 _CODES = (torch.int8,)
+_PACKED = (torch.uint8,)
 
 # These calls take a few microseconds on the GPU for a small batch, so the checks
 # below avoid what torch's Python layer is slow at (device objects, stream objects,
@@ -159,6 +163,114 @@ def int8_product(a: torch.Tensor, a_scales: torch.Tensor, b: torch.Tensor, b_sca
         at_bias, device = _vector("bias", bias, (n,)), _device(a, a_scales, b, b_scales, out, bias)
     _lib.check(_lib.load().qv_int8_product(a.data_ptr(), a_stride, at_a, m, b.data_ptr(), b_stride, at_b, at_bias, n, k,
                                            out.data_ptr(), _TYPES[out.dtype], out_stride, device, _raw_stream(device)))
+    if again:
+        _written((out,))
+    return out
+
+
+def _packed(name: str, codes: torch.Tensor, scales: torch.Tensor, scales_name: str = "scales"):
+    """Checks rows of 4-bit codes and their scales: rows, bytes of codes in a row, both row strides."""
+    rows, cols, stride = _matrix(name, codes, _PACKED)
+    scale_rows, blocks, scale_stride = _matrix(scales_name, scales, _PACKED)
+    if scale_rows != rows or blocks != (cols + 15) // 16:
+        raise ValueError(f"{scales_name} must have the shape {(rows, (cols + 15) // 16)}, one for each 16 bytes of {name}")
+    return rows, cols, stride, scale_stride
+
+
+def quantize_rows_mx4(x: torch.Tensor, *, out: tuple[torch.Tensor, torch.Tensor] | None = None):
+    """``(codes uint8 [n, ceil(d / 2)], scales uint8 [n, ceil(d / 32)])``: rows in microscaled 4-bit floating point.
+
+    Each 32 values of a row share a power of two, 2^(scale - 127), the least of
+    which their largest magnitude is 7 times at most; a code is a sign and one of
+    0, 0.5, 1, 1.5, 2, 3, 4, 6, the nearest to the scaled value, halves to the even
+    code.  Two codes to a byte, the first in its low half; a row of odd length
+    ends with a zero code.  Blocks with an infinity or a NaN get the scale 255
+    (NaN) and zero codes.
+    """
+    n, d, stride = _matrix("x", x, _TYPES)
+    if x.requires_grad or forward_ad._current_level >= 0:
+        _no_derivative("quantize_rows_mx4", x)
+    again = out is not None
+    if not again:
+        out = (torch.empty((n, (d + 1) // 2), dtype=torch.uint8, device=x.device),
+               torch.empty((n, (d + 31) // 32), dtype=torch.uint8, device=x.device))
+    codes, scales = out
+    rows, cols, code_stride, scale_stride = _packed("codes", codes, scales)
+    if rows != n or cols != (d + 1) // 2:
+        raise ValueError(f"codes must have the shape {(n, (d + 1) // 2)}")
+    device = _device(x, codes, scales)
+    _lib.check(_lib.load().qv_quantize_rows_mx4(x.data_ptr(), _TYPES[x.dtype], n, d, stride, codes.data_ptr(), code_stride,
+                                                scales.data_ptr(), scale_stride, device, _raw_stream(device)))
+    if again:
+        _written(out)
+    return out
+
+
+def _result(name: str, rows: int, cols: int, dtype: torch.dtype | None, out: torch.Tensor | None, device) -> torch.Tensor:
+    """``out``, which has to be of the type asked for, or a new matrix of it (float32 without)."""
+    if out is None:
+        if dtype is None:
+            dtype = torch.float32
+        elif dtype not in _TYPES:
+            raise ValueError("dtype must be float32, bfloat16 or float16")
+        return torch.empty((rows, cols), dtype=dtype, device=device)
+    if dtype is not None and out.dtype != dtype:
+        raise ValueError(f"{name} has the type {out.dtype}, and {dtype} is asked for")
+    return out
+
+
+def mx4_values(codes: torch.Tensor, scales: torch.Tensor, dim: int | None = None, *, dtype: torch.dtype | None = None,
+               out: torch.Tensor | None = None) -> torch.Tensor:
+    """What ``quantize_rows_mx4``'s rows stand for, [n, dim] of ``dtype`` (``out``'s type, or float32).
+
+    ``dim``: the rows' length, twice the bytes of their codes if it is not given.
+    """
+    n, cols, code_stride, scale_stride = _packed("codes", codes, scales)
+    if dim is None:
+        dim = 2 * cols
+    elif (dim + 1) // 2 != cols:
+        raise ValueError(f"rows of {dim} values have {(dim + 1) // 2} bytes of codes, not {cols}")
+    if out is not None and out.requires_grad or forward_ad._current_level >= 0:
+        _no_derivative("mx4_values", out)
+    again = out is not None
+    out = _result("out", n, dim, dtype, out, codes.device)
+    rows, columns, stride = _matrix("out", out, _TYPES)
+    if rows != n or columns != dim:
+        raise ValueError(f"out must have the shape {(n, dim)}")
+    device = _device(codes, scales, out)
+    _lib.check(_lib.load().qv_mx4_values(codes.data_ptr(), code_stride, scales.data_ptr(), scale_stride, n, dim,
+                                         out.data_ptr(), _TYPES[out.dtype], stride, device, _raw_stream(device)))
+    if again:
+        _written((out,))
+    return out
+
+
+def mx4_product(a: torch.Tensor, a_scales: torch.Tensor, b: torch.Tensor, b_scales: torch.Tensor, *,
+                bias: torch.Tensor | None = None, dtype: torch.dtype | None = None,
+                out: torch.Tensor | None = None) -> torch.Tensor:
+    """``A . B^T + bias`` of the rows that ``a`` and ``b`` stand for (``quantize_rows_mx4``).
+
+    Products are exact, their sums and the bias fp32, rounded once to ``dtype``
+    (``out``'s type, or float32).  A bias of -inf takes a column out of ``log_probs``.
+    """
+    m, cols, a_stride, a_scale_stride = _packed("a", a, a_scales, "a_scales")
+    n, b_cols, b_stride, b_scale_stride = _packed("b", b, b_scales, "b_scales")
+    if b_cols != cols:
+        raise ValueError("a and b differ in the length of their rows")
+    again = out is not None
+    if bias is not None and bias.requires_grad or again and out.requires_grad or forward_ad._current_level >= 0:
+        _no_derivative("mx4_product", bias, out)
+    out = _result("out", m, n, dtype, out, a.device)
+    out_rows, out_cols, out_stride = _matrix("out", out, _TYPES)
+    if out_rows != m or out_cols != n:
+        raise ValueError(f"out must have the shape {(m, n)}")
+    if bias is None:
+        at_bias, device = None, _device(a, a_scales, b, b_scales, out)
+    else:
+        at_bias, device = _vector("bias", bias, (n,)), _device(a, a_scales, b, b_scales, out, bias)
+    _lib.check(_lib.load().qv_mx4_product(a.data_ptr(), a_stride, a_scales.data_ptr(), a_scale_stride, m, b.data_ptr(),
+                                          b_stride, b_scales.data_ptr(), b_scale_stride, at_bias, n, 2 * cols,
+                                          out.data_ptr(), _TYPES[out.dtype], out_stride, device, _raw_stream(device)))
     if again:
         _written((out,))
     return out
@@ -363,23 +475,184 @@ def log_probs_grad(logits: torch.Tensor, result: LogProbs, targets: torch.Tensor
                      targets, grad_target, grad_entropy, grad_logsumexp, grad_top, out)
 
 
-class DenseCatalogue:
-    """Embedding vectors kept in 8 bits and scored exhaustively.
+def _params(dim: int, weight: torch.Tensor | None, bias: torch.Tensor | None):
+    """The type of weight and bias, and their addresses."""
+    dtype = torch.float32
+    for name, p in (("weight", weight), ("bias", bias)):
+        if p is not None:
+            dtype = p.dtype
+            if dtype not in _TYPES:
+                raise ValueError(f"{name} has the type {dtype}; " + " or ".join(str(x) for x in _TYPES) + " is needed")
+    at_weight = None if weight is None else _vector("weight", weight, (dim,), dtype)
+    return dtype, at_weight, None if bias is None else _vector("bias", bias, (dim,), dtype)
 
-    ``DenseCatalogue(vectors)`` quantises the rows once.  ``log_probs(queries,
+
+def _norm(x, weight, bias, eps, out):
+    n, d, stride = _matrix("x", x, _TYPES)
+    dtype, at_weight, at_bias = _params(d, weight, bias)
+    again = out is not None
+    if not again:
+        out = torch.empty((n, d), dtype=x.dtype, device=x.device)
+    rows, cols, out_stride = _matrix("out", out, (x.dtype,))
+    if rows != n or cols != d:
+        raise ValueError("out and x differ in shape")
+    device = _device(*(t for t in (x, out, weight, bias) if t is not None))
+    _lib.check(_lib.load().qv_layer_norm(x.data_ptr(), _TYPES[x.dtype], n, d, stride, at_weight, at_bias, _TYPES[dtype],
+                                         eps, out.data_ptr(), out_stride, device, _raw_stream(device)))
+    if again:
+        _written((out,))
+    return out
+
+
+@dataclass(frozen=True, eq=False)
+class LayerNormGrad:
+    """What ``layer_norm_grad`` gives; None for what was not wanted."""
+
+    x: torch.Tensor | None       # [n, d] of x's type
+    weight: torch.Tensor | None  # [d] of the weight's type
+    bias: torch.Tensor | None    # [d] of the weight's type
+    _workspace: torch.Tensor
+    _size: tuple                 # rows and columns that it was made for
+
+
+def _norm_grad(x, grad, weight, eps, dtype, wanted, out) -> LayerNormGrad:
+    n, d, stride = _matrix("x", x, _TYPES)
+    grad_rows, grad_cols, grad_stride = _matrix("grad", grad, (x.dtype,))
+    if grad_rows != n or grad_cols != d:
+        raise ValueError("grad and x differ in shape")
+    at_weight = _params(d, weight, None)[1]
+    again = out is not None
+    if not again:
+        workspace = _lib.load().qv_layer_norm_grad_workspace(n, d)
+        if workspace < 0:
+            _lib.check(workspace)
+
+        def new(want, shape, type_):
+            return torch.empty(shape, dtype=type_, device=x.device) if want else None
+
+        out = LayerNormGrad(new(wanted[0], (n, d), x.dtype), new(wanted[1], d, dtype), new(wanted[2], d, dtype),
+                            torch.empty(workspace, dtype=torch.uint8, device=x.device), (n, d))
+    elif out._size != (n, d):
+        raise ValueError("out was made for another number of rows or columns")
+    at_x, out_stride = None, d
+    if out.x is not None:
+        out_rows, out_cols, out_stride = _matrix("out.x", out.x, (x.dtype,))
+        if out_rows != n or out_cols != d:
+            raise ValueError("out.x and x differ in shape")
+        at_x = out.x.data_ptr()
+    at = [None if p is None else _vector(name, p, (d,), dtype) for name, p in (("out.weight", out.weight), ("out.bias", out.bias))]
+    device = _device(*(t for t in (x, grad, weight, out.x, out.weight, out.bias, out._workspace) if t is not None))
+    _lib.check(_lib.load().qv_layer_norm_grad(x.data_ptr(), _TYPES[x.dtype], n, d, stride, grad.data_ptr(), grad_stride,
+                                              at_weight, _TYPES[dtype], eps, at_x, out_stride, *at,
+                                              out._workspace.data_ptr(), out._workspace.shape[0], device,
+                                              _raw_stream(device)))
+    if again:
+        _written([t for t in (out.x, out.weight, out.bias) if t is not None])
+    return out
+
+
+class _OnceNorm(torch.autograd.Function):
+    """A gradient made while a graph is recorded: there is no derivative of it, and taking one must not give zeros."""
+
+    @staticmethod
+    def forward(ctx, grad, *inputs):
+        return grad.view_as(grad)
+
+    @staticmethod
+    def backward(ctx, _g):
+        raise _lib.QuiverError("the gradient of layer_norm cannot be differentiated again")
+
+
+class _LayerNormFunction(torch.autograd.Function):
+    @staticmethod
+    def forward(ctx, x, weight, bias, eps):
+        y = _norm(x, weight, bias, eps, None)
+        ctx.eps = eps
+        ctx.dtype = torch.float32 if weight is None and bias is None else (bias if weight is None else weight).dtype
+        ctx.save_for_backward(x, weight)
+        return y
+
+    @staticmethod
+    def backward(ctx, g):
+        x, weight = ctx.saved_tensors
+        if _has_tangent(g):
+            raise _lib.QuiverError("the gradient of layer_norm has no forward-mode derivative")
+        r = _norm_grad(x, g.contiguous(), weight, ctx.eps, ctx.dtype, ctx.needs_input_grad[:3], None)
+        grads = (r.x, r.weight, r.bias)
+        if torch.is_grad_enabled():
+            inputs = [t for t in (g, x, weight) if t is not None]
+            grads = tuple(None if t is None else _OnceNorm.apply(t, *inputs) for t in grads)
+        return (*grads, None)
+
+
+def layer_norm(x: torch.Tensor, weight: torch.Tensor | None = None, bias: torch.Tensor | None = None, *, eps: float = 1e-5,
+               out: torch.Tensor | None = None) -> torch.Tensor:
+    """``(x - mean) / sqrt(var + eps) * weight + bias`` over each row of ``x`` (float32, bfloat16 or float16 [n, d]).
+
+    Mean and variance (over d) in fp32; the result has x's type, rounded once.
+    ``weight`` and ``bias`` [d] are of one type, x's or another of the three.
+    ``eps``: positive (a normal float).  ``out`` may be ``x``.  A row that holds an
+    infinity or a NaN gives NaN.  With arguments that require a gradient the
+    result takes part in autograd (``out`` is then refused), once: the gradient
+    has none of its own, and there is no forward-mode derivative.
+    """
+    if torch.is_grad_enabled() and (x.requires_grad or weight is not None and weight.requires_grad
+                                    or bias is not None and bias.requires_grad):
+        if out is not None:
+            raise ValueError("out= cannot be given for arguments that require a gradient")
+        if _has_tangent(x, weight, bias):
+            raise ValueError("layer_norm has no forward-mode derivative, and an argument has a tangent")
+        return _LayerNormFunction.apply(x, weight, bias, float(eps))
+    if out is not None and out.requires_grad or forward_ad._current_level >= 0:
+        _no_derivative("layer_norm", x, weight, bias, out)
+    return _norm(x, weight, bias, eps, out)
+
+
+def layer_norm_grad(x: torch.Tensor, grad: torch.Tensor, weight: torch.Tensor | None = None, *, eps: float = 1e-5,
+                    wanted: tuple[bool, bool, bool] | None = None, out: LayerNormGrad | None = None) -> LayerNormGrad:
+    """The gradients of x, weight and bias from that of ``layer_norm``'s result.
+
+    ``x``, ``weight`` and ``eps`` as they were for ``layer_norm``, ``grad`` of
+    x's type.  The weight's and bias's come in the weight's type (float32
+    without one).  ``wanted``: which of the three (all of them); ``out``: an
+    earlier result, to be written again.  What autograd runs, for training loops
+    without it (so arguments that require a gradient come detached, or under
+    ``torch.no_grad()``).
+    """
+    outs = () if out is None else (out.x, out.weight, out.bias)
+    if (x.requires_grad or grad.requires_grad or weight is not None and weight.requires_grad
+            or any(t is not None and t.requires_grad for t in outs) or forward_ad._current_level >= 0):
+        _no_derivative("layer_norm_grad", x, grad, weight, *outs)
+    if wanted is None:
+        wanted = (True, True, True)
+    elif out is not None:
+        raise ValueError("wanted cannot be given beside out=, which has what is wanted")
+    return _norm_grad(x, grad, weight, eps, torch.float32 if weight is None else weight.dtype, wanted, out)
+
+
+class DenseCatalogue:
+    """Embedding vectors kept in 8 bits, or in microscaled 4 bits, and scored exhaustively.
+
+    ``DenseCatalogue(vectors)`` quantises the rows once, ``bits=4`` to half the
+    bytes (and about 20 times the error of an inner product), as their queries.  ``log_probs(queries,
     targets, ...)`` gives each query's distribution over all of them, by inner
     products; the scores exist for one batch of queries at a time, about
     ``score_bytes`` of them.  Scores have no derivative (vectors, queries or a
     bias that require a gradient are refused).
     """
 
+    bits = 8
+
     def __init__(self, vectors: torch.Tensor, *, bias: torch.Tensor | None = None,
-                 score_dtype: torch.dtype = torch.float32, score_bytes: int = 1 << 30) -> None:
+                 score_dtype: torch.dtype = torch.float32, score_bytes: int = 1 << 30, bits: int = 8) -> None:
+        if bits not in (8, 4):
+            raise ValueError("bits must be 8 or 4")
         if score_dtype not in _TYPES:
             raise ValueError("score_dtype must be float32, bfloat16 or float16")
         if score_bytes <= 0:
             raise ValueError("score_bytes must be positive")
-        self.codes, self.scales = quantize_rows(vectors)
+        self.bits = bits
+        self.codes, self.scales = self._quantize(vectors)
         if bias is not None:
             _vector("bias", bias, (vectors.shape[0],))
         self.bias, self.score_dtype, self.score_bytes = bias, score_dtype, int(score_bytes)
@@ -387,11 +660,15 @@ class DenseCatalogue:
     def __len__(self) -> int:
         return self.codes.shape[0]
 
+    def _quantize(self, rows: torch.Tensor):
+        return quantize_rows(rows) if self.bits == 8 else quantize_rows_mx4(rows)
+
     def scores(self, queries: torch.Tensor, *, out: torch.Tensor | None = None) -> torch.Tensor:
         """Inner products of the queries, quantised row by row, with every vector: [n, len(self)], of ``out``'s type if given."""
-        codes, scales = quantize_rows(queries)
-        return int8_product(codes, scales, self.codes, self.scales, bias=self.bias,
-                            dtype=self.score_dtype if out is None else None, out=out)
+        codes, scales = self._quantize(queries)
+        product = int8_product if self.bits == 8 else mx4_product
+        return product(codes, scales, self.codes, self.scales, bias=self.bias,
+                       dtype=self.score_dtype if out is None else None, out=out)
 
     def log_probs(self, queries: torch.Tensor, targets: torch.Tensor | None = None, *, top_k: int = 0,
                   temperature: float = 1.0) -> LogProbs:
