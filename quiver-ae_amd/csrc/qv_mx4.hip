@@ -169,6 +169,8 @@ __global__ __launch_bounds__(256) void from_mx4_kernel(const uint8_t* __restrict
 // zeroed in a, so every load is a whole one inside the row and b needs no mask.
 // Rows past the end repeat the last row; what they give is not stored.
 
+constexpr int64_t kFar = 1 << 24;  // row strides from here on: 256 rows' offsets may pass 32 bits
+
 typedef int32_t i8v __attribute__((ext_vector_type(8)));
 typedef float f16v __attribute__((ext_vector_type(16)));
 
@@ -216,6 +218,35 @@ __device__ __forceinline__ i4 short_row(const uint8_t* row, int k) {
   for (int i = 0; i < 15; i++)
     if (i < k) v[i / 4] |= (int)row[i] << (8 * (i % 4));
   return v;
+}
+
+// Stores a wave's results, from row i and column j of the BM x BN tile at (i0, j0) on; `bias`: the tile's columns', in LDS
+// (-0, which changes no sum, without).
+template <int BM, int BN, int TM, int TN, class O>
+__device__ __forceinline__ void store_tile(f16v (&acc)[TM][TN], int i, int j, int64_t i0, int64_t j0, const float* bias,
+                                           const Product<O>& p) {
+  constexpr int R = sizeof(O) == 2 && TN % 2 == 0 ? 2 : 1;
+  const int row = lane_id() % 32, half = lane_id() / 32;
+  auto store = [&](auto whole) {
+#pragma unroll
+    for (int x = 0; x < TM; x++)
+#pragma unroll
+      for (int y = 0; y < TN; y += R) {
+#pragma unroll
+        for (int r = 0; r < R; r++) asm volatile("" : "+a"(acc[x][y + r]) : : "memory");  // in turn: none leaves its accumulators before
+        store_results<decltype(whole)::value, R>(
+            [&](int r, int g) {
+              const f4 t = *reinterpret_cast<const f4*>(bias + j + 32 * (y + r) + 8 * g + 4 * half);
+              f4 v;
+#pragma unroll
+              for (int e = 0; e < 4; e++) v[e] = acc[x][y + r][4 * g + e] + t[e];
+              return v;
+            },
+            i0 + i + 32 * x + row, j0 + j + 32 * y, p.m, p.n, p.out, p.out_stride);
+      }
+  };
+  if (i0 + BM <= p.m && j0 + BN <= p.n) store(std::true_type());
+  else store(std::false_type());
 }
 
 // A tile of BM x BN outputs per workgroup, WM x WN waves of 32 TM x 32 TN each.  Both
@@ -340,25 +371,327 @@ __global__ __launch_bounds__(64 * WM * WN, 1) void product_tile_kernel(Product<O
     products(std::integral_constant<int, 3>());
     __syncthreads();
   }
-  const int64_t i = i0 + wm * TM * 32 + row, j = j0 + wn * TN * 32;
-  constexpr int R = sizeof(O) == 2 && TN % 2 == 0 ? 2 : 1;
-  auto store = [&](auto whole) {
+  store_tile<BM, BN, TM, TN>(acc, wm * TM * 32, wn * TN * 32, i0, j0, add, p);
+}
+
+// The same tiles where the matrix cores are what bounds the product: stages of 64 bytes
+// of k go straight from memory to LDS (no registers, no LDS writes to issue), NB of
+// them at a time, so NB - 1 are on their way while one is used.  A stage is two steps
+// of 32 bytes; the second step's operands are read while the first one's products run,
+// and the next stage's first operands while the second one's do, so the one barrier
+// per stage, between the two, finds the operands of what follows it in registers.
+// Needs 16-byte aligned rows, scales' rows of whole aligned words, k a multiple of 64.
+// MANY: one workgroup per CU walks over tiles, and the stages run on from tile to tile:
+// the next tile's first ones are on their way, and its first operands in registers, while
+// the results are stored.
+template <int BM, int BN, int WM, int WN, int NB, int G, bool MANY, class O>
+__global__ __launch_bounds__(64 * WM * WN, 1) void product_deep_kernel(Product<O> p, int64_t tiles_m, int64_t tiles_n,
+                                                                       int64_t group) {
+  constexpr int TM = BM / WM / 32, TN = BN / WN / 32, kRow = 64, kWaves = WM * WN;
+  constexpr int I = (BM + BN) / 16 / kWaves;                               // loads of 16 rows per wave and stage
+  constexpr int S = (BM + BN + kWave * kWaves - 1) / (kWave * kWaves);     // loads of 64 rows' scales
+  constexpr int SE = G == 1 ? S : 0;  // of which every stage has as many (the waits count these only)
+  static_assert(I % 2 == 0, "issued in halves");
+  constexpr int kBuffer = (BM + BN) * kRow;
+  constexpr int kScales = (BM + BN) * 4 * G, kSlots = G == 1 ? NB : 2;  // scales of G stages
+  extern __shared__ __align__(16) char lds[];
+  const int wave = wave_id(), lane = lane_id(), wm = wave / WN, wn = wave % WN;
+  const uint32_t stages = (uint32_t)p.k / kRow;  // NB at least
+  const uint32_t tiles = (uint32_t)(tiles_m * tiles_n), tn = (uint32_t)tiles_n, rows = (uint32_t)group;
+  int64_t i0, j0, next_i0, next_j0;
+  auto place_next = [&](uint32_t turn) {
+    const uint32_t t = (uint32_t)tile_of_block(turn, tiles), g = t / (rows * tn), in = t - g * rows * tn;
+    const uint32_t gm = min(rows, (uint32_t)tiles_m - g * rows);
+    next_i0 = (int64_t)(g * rows + in % gm) * BM;
+    next_j0 = (int64_t)(in / gm) * BN;
+  };
+
+  // piece q of row r lies at q ^ (r / 4 mod 4): the lanes of a load write 1 KB in a row, so what they load is
+  // permuted instead
+  const int piece = (lane % 4) ^ (lane / 16);
+  // a wave loads rows of one operand only: 16 I of them from `first`, and scales of 64 S from `first_scales`
+  static_assert(BM == BN && kWaves == 4, "two waves for each operand");
+  const int first = wave % 2 * 16 * I, first_scales = wave * S * kWave % BM;
+  const bool of_a = wave < 2, scales_of_a = wave * S * kWave % (BM + BN) < BM;
+  struct Tile {  // where its rows begin, and the lanes' rows from there
+    const uint8_t *rows, *scales;
+    uint32_t row[I], scale[S];
+  } next;
+  const uint8_t *rows_at[2], *scales_at_row;  // of the two halves of a stage's loads
+  uint32_t row_at[I], scale_at[S];
+  char* scales_at = lds + NB * kBuffer;
+  char* bias_at = scales_at + kSlots * kScales;  // of three tiles in turn: other waves may still store the last one
+  // the next tile's rows, and its biases on their way
+  auto find_next = [&](int slot) {
+    const int64_t begin = of_a ? next_i0 : next_j0, scales_begin = scales_of_a ? next_i0 : next_j0;
+    const int64_t stride = of_a ? p.a_stride : p.b_stride, scales_stride = scales_of_a ? p.as_stride : p.bs_stride;
+    const int most = (int)min((of_a ? p.m : p.n) - 1 - begin, (int64_t)BM - 1);
+    const int scales_most = (int)min((scales_of_a ? p.m : p.n) - 1 - scales_begin, (int64_t)BM - 1);
+    next.rows = (of_a ? p.a : p.b) + begin * stride;
+    next.scales = (scales_of_a ? p.a_scales : p.b_scales) + scales_begin * scales_stride;
+#pragma unroll
+    for (int q = 0; q < I; q++) next.row[q] = (uint32_t)min(first + q * 16 + lane / 4, most) * (uint32_t)stride + piece * 16;
+#pragma unroll
+    for (int q = 0; q < S; q++) next.scale[q] = (uint32_t)min(first_scales + q * kWave + lane, scales_most) * (uint32_t)scales_stride;
+    if (p.bias) {
+      float* to = reinterpret_cast<float*>(bias_at) + slot * BN;
+      const int bias_most = (int)min(p.n - 1 - next_j0, (int64_t)BN - 1);
+      for (int r = wave * kWave; r < BN; r += kWave * kWaves)
+        __builtin_amdgcn_global_load_lds((const __attribute__((address_space(1))) void*)(p.bias + next_j0 + min(r + lane, bias_most)),
+                                         (__attribute__((address_space(3))) void*)(to + r), 4, 0, 0);
+    }
+  };
+  auto turn_to_next = [&](bool yes) {
+    rows_at[0] = yes ? next.rows : rows_at[0];
+    rows_at[1] = yes ? next.rows : rows_at[1];
+    scales_at_row = yes ? next.scales : scales_at_row;
+#pragma unroll
+    for (int q = 0; q < I; q++) row_at[q] = yes ? next.row[q] : row_at[q];
+#pragma unroll
+    for (int q = 0; q < S; q++) scale_at[q] = yes ? next.scale[q] : scale_at[q];
+  };
+  // a half of a stage's loads, the scales of it and the next G - 1 with the first one (with one tile, stages past the last
+  // one repeat it: as many loads as the waits count)
+  auto issue = [&](uint32_t s, int part) {
+    if (part == 0 && s % G == 0) {
+      char* to = scales_at + s / G % kSlots * kScales;
+      const uint8_t* from = scales_at_row + (MANY ? 0 : min(s, stages - G) * 4);
+#pragma unroll
+      for (int q = 0; q < S; q++) {
+        const auto there = (__attribute__((address_space(3))) void*)(to + (wave * S + q) * kWave % (BM + BN) * 4 * G);
+        if constexpr (G == 1) __builtin_amdgcn_global_load_lds((const __attribute__((address_space(1))) void*)(from + scale_at[q]), there, 4, 0, 0);
+        else __builtin_amdgcn_global_load_lds((const __attribute__((address_space(1))) void*)(from + scale_at[q]), there, 16, 0, 0);
+      }
+      if (MANY) scales_at_row += 4 * G;
+    }
+    char* to = lds + s % NB * kBuffer + wave * I * 1024;
+    const uint8_t* from = rows_at[part] + (MANY ? 0 : min(s, stages - 1) * kRow);
+#pragma unroll
+    for (int q = part * I / 2; q < (part + 1) * I / 2; q++)
+      __builtin_amdgcn_global_load_lds((const __attribute__((address_space(1))) void*)(from + row_at[q]),
+                                       (__attribute__((address_space(3))) void*)(to + q * 1024), 16, 0, 0);
+    if (MANY) rows_at[part] += kRow;
+  };
+  f16v acc[TM][TN];
+  const int row = lane % 32, half = lane / 32;
+  // step q takes pieces q and 2 + q, so a lane's scales of a stage are two bytes in a row of the four
+  i4 fa[2][TM], fb[2][TN];
+  uint32_t sa[TM], sb[TN], next_sa[TM], next_sb[TN];
+  auto read = [&](uint32_t s, int q) {
+    const char* from = lds + s % NB * kBuffer + ((q + 2 * half) ^ (row / 4 % 4)) * 16 + row * kRow;
+#pragma unroll
+    for (int x = 0; x < TM; x++) fa[q][x] = *reinterpret_cast<const i4*>(from + (wm * TM + x) * 32 * kRow);
+#pragma unroll
+    for (int y = 0; y < TN; y++) fb[q][y] = *reinterpret_cast<const i4*>(from + (BM + (wn * TN + y) * 32) * kRow);
+  };
+  auto read_scales = [&](uint32_t s) {
+    const char* from = scales_at + s / G % kSlots * kScales + row * 4 * G + s % G * 4;
+#pragma unroll
+    for (int x = 0; x < TM; x++) next_sa[x] = *reinterpret_cast<const uint32_t*>(from + (wm * TM + x) * 32 * 4 * G);
+#pragma unroll
+    for (int y = 0; y < TN; y++) next_sb[y] = *reinterpret_cast<const uint32_t*>(from + (BM + (wn * TN + y) * 32) * 4 * G);
+  };
+  auto turn_scales = [&] {
+#pragma unroll
+    for (int x = 0; x < TM; x++) sa[x] = next_sa[x] >> (16 * half);
+#pragma unroll
+    for (int y = 0; y < TN; y++) sb[y] = next_sb[y] >> (16 * half);
+  };
+  auto products = [&](auto step) {
+    constexpr int Q = decltype(step)::value;
 #pragma unroll
     for (int x = 0; x < TM; x++)
 #pragma unroll
-      for (int y = 0; y < TN; y += R)
-        store_results<decltype(whole)::value, R>(
-            [&](int r, int g) {
-              const f4 t = *reinterpret_cast<const f4*>(add + wn * TN * 32 + 32 * (y + r) + 8 * g + 4 * half);
-              f4 v;
-#pragma unroll
-              for (int e = 0; e < 4; e++) v[e] = acc[x][y + r][4 * g + e] + t[e];
-              return v;
-            },
-            i + 32 * x, j + 32 * y, p.m, p.n, p.out, p.out_stride);
+      for (int y = 0; y < TN; y++) acc[x][y] = mfma<Q>(fb[Q][y], sb[y], fa[Q][x], sa[x], acc[x][y]);
   };
-  if (i0 + BM <= p.m && j0 + BN <= p.n) store(std::true_type());
-  else store(std::false_type());
+  auto meet = [] {  // nothing of a stage moves over it
+    asm volatile("" ::: "memory");
+    __builtin_amdgcn_s_barrier();
+    asm volatile("" ::: "memory");
+    __builtin_amdgcn_sched_barrier(0);
+  };
+  if (!p.bias)
+    for (int r = threadIdx.x; r < 3 * BN; r += kWave * kWaves) reinterpret_cast<float*>(bias_at)[r] = -0.f;
+  uint32_t turn = blockIdx.x, slot = 0;
+  place_next(turn);
+  find_next(0);
+  rows_at[0] = rows_at[1] = scales_at_row = nullptr;
+  turn_to_next(true);
+#pragma unroll
+  for (int s = 0; s < NB; s++) {
+    issue(s, 0);
+    if (s + 1 < NB) issue(s, 1);
+  }
+  __builtin_amdgcn_s_waitcnt(kWaitFor<(NB - 2) * (I + SE) + I / 2 + SE>);
+  meet();
+  read(0, 0);
+  read_scales(0);
+  __builtin_amdgcn_s_waitcnt(kReadsDone);
+  // stage s, `last` of its tile of which loads are still to be asked for
+  auto one_stage = [&](uint32_t s, bool last) {
+    turn_scales();
+    read(s, 1);
+    issue(s + NB - 1, 1);
+    products(std::integral_constant<int, 0>());
+    between<TM + TN, kDsRead, 1>();
+    between<I / 2, kVmem, 2>();
+    __builtin_amdgcn_sched_barrier(0);
+    // stage s + 1 is there and every wave has read stage s
+    __builtin_amdgcn_s_waitcnt(kWaitFor<(NB - 2) * (I + SE)>);
+    meet();
+    if (MANY) turn_to_next(last);
+    read(s + 1, 0);
+    read_scales(s + 1);
+    issue(s + NB, 0);
+    products(std::integral_constant<int, 1>());
+    between<TM + TN, kDsRead, 1>();
+    between<I / 2, kVmem, 1>();
+    __builtin_amdgcn_s_waitcnt(kReadsDone);  // long since: said for the compiler, which else waits at the loop's top
+    __builtin_amdgcn_sched_barrier(0);
+  };
+  uint32_t turns = 0;  // groups of G stages so far
+  do {
+    i0 = next_i0;
+    j0 = next_j0;
+    turn += gridDim.x;
+    if (MANY) {  // (after the last tile some tile's first stages, which nobody reads)
+      place_next(min(turn, tiles - 1));
+      find_next(slot == 2 ? 0 : slot + 1);
+    }
+#pragma unroll
+    for (int x = 0; x < TM; x++)
+#pragma unroll
+      for (int y = 0; y < TN; y++) {
+        acc[x][y] = f16v{};
+        asm volatile("" : "+a"(acc[x][y]));
+      }
+    uint32_t left = stages;
+    do {
+      static_assert(G == 1 || G == 4 && NB == 4, "the stages of a group have places of their own");
+#pragma unroll
+      for (int i = 0; i < G; i++) one_stage(turns * G + i, i == 0 && left == NB);
+      turns++;
+      left -= G;
+    } while (left > 0);
+    store_tile<BM, BN, TM, TN>(acc, wm * TM * 32, wn * TN * 32, i0, j0, reinterpret_cast<float*>(bias_at) + slot * BN, p);
+    slot = slot == 2 ? 0 : slot + 1;
+  } while (MANY && turn < tiles);
+  __builtin_amdgcn_s_waitcnt(kWaitFor<0>);  // no load into LDS outlives the wave
+}
+
+// Short rows, k <= 32 KS bytes, whose product is mostly writing: 32 rows of a stay in a wave's
+// registers while its workgroup (128 rows) walks over tiles of 64 rows of b, through
+// LDS with the next two tiles on their way.  Results leave in whole lines (LineRing).
+template <int KS, class O>
+__global__ __launch_bounds__(256, KS == 8 ? 2 : 3) void product_panel_kernel(Product<O> p, int64_t panels, int64_t tiles_n,
+                                                                             int64_t slices) {
+  constexpr int PC = 2 * KS, kRow = 32 * KS, L = 64 * PC / 256, kRows = 256 / PC, Y = LineRing<O>::Y;
+  constexpr int kWords = (KS + 3) / 4;  // of a lane's scales
+  __shared__ __align__(16) char lds[2][64 * kRow];
+  __shared__ __align__(256) char rings[4][LineRing<O>::kBytes];
+  __shared__ __align__(16) uint8_t sc[2][64 * PC];  // a tile's scales
+  __shared__ float sb[2][64];                       // and biases (-0, which changes no sum, without)
+  const int tid = threadIdx.x, wave = wave_id(), lane = lane_id(), row = lane % 32, half = lane / 32;
+  const int64_t t = tile_of_block(blockIdx.x, panels * slices), slice = t / panels, i0 = (t - slice * panels) * 128;
+  const int64_t first = tiles_n * slice / slices, end = tiles_n * (slice + 1) / slices;
+  const int k = (int)p.k, piece = tid % PC, r0 = tid / PC, from = min(piece * 16, k - 16);
+  auto swap = [](int r) { return KS == 2 ? r / 4 & 3 : KS == 4 ? r / 2 & 7 : r & 15; };  // as in the tiles, by the row's bytes
+  i4 rb[L];
+  uint32_t rs = 0;  // KS / 2 bytes of a row's scales
+  float bias = -0.f;
+  auto load = [&](int64_t tile) {
+    const uint8_t* b = p.b + tile * 64 * p.b_stride;
+    const int last = (int)min(p.n - 1 - tile * 64, (int64_t)63);
+#pragma unroll
+    for (int q = 0; q < L; q++) rb[q] = *reinterpret_cast<const i4_any*>(b + ((uint32_t)min(r0 + q * kRows, last) * (uint32_t)p.b_stride + from));
+    const uint8_t* s = p.b_scales + tile * 64 * p.bs_stride + (uint32_t)min(tid / 4, last) * (uint32_t)p.bs_stride;
+    rs = 0;
+#pragma unroll
+    for (int u = 0; u < KS / 2; u++) {
+      const int block = tid % 4 * (KS / 2) + u;
+      if (block < p.blocks) rs |= (uint32_t)s[block] << (8 * u);
+    }
+    if (p.bias && tid < 64) bias = p.bias[tile * 64 + min(tid, last)];
+  };
+  auto keep = [&](int buffer) {
+#pragma unroll
+    for (int q = 0; q < L; q++) {
+      const int r = r0 + q * kRows;
+      *reinterpret_cast<i4*>(lds[buffer] + r * kRow + (piece ^ swap(r)) * 16) = rb[q];
+    }
+    __builtin_memcpy(sc[buffer] + tid * (KS / 2), &rs, KS / 2);
+    if (tid < 64) sb[buffer][tid] = bias;
+  };
+  load(first);
+  const int64_t it = i0 + wave * 32;  // the wave's rows
+  const int rows = (int)min(p.m - it, (int64_t)32);
+  // step q takes pieces q and KS + q, so a lane's scales are KS bytes in a row
+  i4 fa[KS];
+  uint32_t sa[kWords] = {};
+  {
+    const uint8_t* a = p.a + min(it + row, p.m - 1) * p.a_stride;
+    const uint8_t* s = p.a_scales + min(it + row, p.m - 1) * p.as_stride;
+#pragma unroll
+    for (int q = 0; q < KS; q++) {
+      const int block = q + KS * half, at = min(block * 16, k - 16);
+      fa[q] = without_first(*reinterpret_cast<const i4_any*>(a + at), block * 16 - at);
+      if (block < p.blocks) sa[q / 4] |= (uint32_t)s[block] << (8 * (q % 4));
+    }
+  }
+  LineRing<O> ring(rings[wave], p.out, p.out_stride, it, rows, first);
+  keep(0);
+  if (first + 1 < end) load(first + 1);
+  __syncthreads();
+#pragma unroll
+  for (int q = 0; q < KS; q++) asm volatile("" : "+v"(fa[q]));  // these are there: the loop's waits count its own
+#pragma unroll
+  for (int q = 0; q < L; q++) asm volatile("" : "+v"(rb[q]));
+  asm volatile("" : "+v"(rs), "+v"(bias));
+  for (int64_t tile = first; tile < end; tile++) {
+    const int buffer = (int)(tile - first) & 1;
+    const char* b = lds[buffer] + row * kRow;
+    f16v acc[2] = {f16v{}, f16v{}};
+    uint32_t s[2][kWords];
+#pragma unroll
+    for (int y = 0; y < 2; y++) {
+      const uint8_t* at = sc[buffer] + (32 * y + row) * PC + half * KS;
+      if constexpr (KS == 2) s[y][0] = *reinterpret_cast<const uint16_t*>(at);
+      else __builtin_memcpy(s[y], __builtin_assume_aligned(at, KS), KS);
+    }
+    auto step = [&](auto number) {
+      constexpr int Q = decltype(number)::value;
+      if constexpr (Q < KS) {
+#pragma unroll
+        for (int y = 0; y < 2; y++)
+          acc[y] = mfma<Q % 4>(fa[Q], sa[Q / 4], *reinterpret_cast<const i4*>(b + y * 32 * kRow + ((Q + KS * half) ^ swap(row)) * 16),
+                               s[y][Q / 4], acc[y]);
+      }
+    };
+    step(std::integral_constant<int, 0>());
+    step(std::integral_constant<int, 1>());
+    step(std::integral_constant<int, 2>());
+    step(std::integral_constant<int, 3>());
+    step(std::integral_constant<int, 4>());
+    step(std::integral_constant<int, 5>());
+    step(std::integral_constant<int, 6>());
+    step(std::integral_constant<int, 7>());
+    if (tile + 1 < end) keep(buffer ^ 1);
+    if (tile + 2 < end) load(tile + 2);
+#pragma unroll
+    for (int l = 0; l < 2 / Y; l++) {
+#pragma unroll
+      for (int y = 0; y < Y; y++) {
+        const float add = sb[buffer][(l * Y + y) * 32 + row];
+#pragma unroll
+        for (int r = 0; r < 16; r += 2) ring.put(y, r, acc[l * Y + y][r] + add, acc[l * Y + y][r + 1] + add);
+      }
+      __builtin_amdgcn_fence(__ATOMIC_ACQ_REL, "wavefront");
+      ring.leave(tile * (2 / Y) + l, p.n, 128);
+      __builtin_amdgcn_fence(__ATOMIC_ACQ_REL, "wavefront");
+    }
+    __syncthreads();
+  }
+  ring.leave(end * (2 / Y), min(end * 64, p.n), 0);
 }
 
 template <class F>
@@ -402,9 +735,47 @@ void launch_tiles(const Product<O>& p, hipStream_t st) {
   HIP_OK(hipGetLastError());
 }
 
+template <int BM, int BN, int WM, int WN, int NB, int G, bool MANY, class O>
+void launch_deep(const Product<O>& p, hipStream_t st) {
+  const int64_t tm = (p.m + BM - 1) / BM, tn = (p.n + BN - 1) / BN;
+  const int64_t group = std::min<int64_t>(tm, 8);
+  constexpr int lds = NB * (BM + BN) * 64 + (G == 1 ? NB : 2) * (BM + BN) * 4 * G + 3 * BN * 4;
+  constexpr auto* kernel = &product_deep_kernel<BM, BN, WM, WN, NB, G, MANY, O>;
+  allow_lds<kernel>(lds);
+  hipLaunchKernelGGL(kernel, dim3((unsigned)(MANY ? std::min<int64_t>(tm * tn, 256) : tm * tn)), dim3(64 * WM * WN), lds, st, p, tm, tn, group);
+  HIP_OK(hipGetLastError());
+}
+
+template <int KS, class O>
+void launch_panels(const Product<O>& p, hipStream_t st) {
+  const int64_t panels = (p.m + 127) / 128, tiles_n = (p.n + 63) / 64;
+  // as many workgroups as run at once, each with a like share of b's tiles
+  const int64_t slices = std::min(tiles_n, std::max<int64_t>(1, 256 * (KS == 8 ? 2 : 3) / panels));
+  hipLaunchKernelGGL((product_panel_kernel<KS, O>), dim3((unsigned)(panels * slices)), dim3(256), 0, st, p, panels, tiles_n, slices);
+  HIP_OK(hipGetLastError());
+}
+
+int force() { static const int f = getenv("QV_FORCE") ? atoi(getenv("QV_FORCE")) : 0; return f; }
+
 template <class O>
 void product(const Product<O>& p, hipStream_t st) {
+  const bool direct = (reinterpret_cast<uintptr_t>(p.a) | reinterpret_cast<uintptr_t>(p.b) | p.a_stride | p.b_stride | p.k * 0) % 16 == 0 &&
+                      (reinterpret_cast<uintptr_t>(p.a_scales) | reinterpret_cast<uintptr_t>(p.b_scales) | p.as_stride | p.bs_stride) % 4 == 0 &&
+                      p.k % 64 == 0 && p.k >= 256 && p.a_stride < kFar && p.b_stride < kFar && p.as_stride < kFar && p.bs_stride < kFar;
+  const int f = force();
+  const bool four = p.k % 256 == 0 && (reinterpret_cast<uintptr_t>(p.a_scales) | reinterpret_cast<uintptr_t>(p.b_scales) | p.as_stride | p.bs_stride) % 16 == 0;
+  const bool near = p.a_stride < kFar && p.b_stride < kFar && p.as_stride < kFar && p.bs_stride < kFar;
   if (p.k < 16) launch_tiles<64, 64, 2, 2, true>(p, st);
+  else if (near && p.k <= 64 && f == 5) launch_panels<2>(p, st);
+  else if (near && p.k <= 128 && f == 5) launch_panels<4>(p, st);
+  else if (near && p.k <= 256 && f == 5) launch_panels<8>(p, st);
+  else if (direct && four && f == 1) launch_deep<256, 256, 2, 2, 4, 4, true>(p, st);
+  else if (direct && four && f == 2) launch_deep<128, 128, 2, 2, 4, 4, false>(p, st);
+  else if (direct && four && f == 3) launch_deep<64, 64, 2, 2, 4, 4, false>(p, st);
+  else if (direct && f == 1) launch_deep<256, 256, 2, 2, 4, 1, true>(p, st);
+  else if (direct && f == 2) launch_deep<128, 128, 2, 2, 4, 1, false>(p, st);
+  else if (direct && f == 3) launch_deep<64, 64, 2, 2, 4, 1, false>(p, st);
+  else if (f == 4) launch_tiles<128, 128, 2, 2, false>(p, st);
   else launch_tiles<64, 64, 2, 2, false>(p, st);
 }
 

@@ -31,6 +31,7 @@ __device__ __forceinline__ i4 without_first(i4 v, int over) {
 
 // Two values in the output's 16 bits, halves to even.  By instruction: the compiler takes the bfloat16 one apart, and
 // joins float16 to the product before it, whose rounding to fp32 is then left out.
+// (So neither value is a matrix instruction's result itself: the compiler would not wait for it.)
 template <class O>
 __device__ __forceinline__ uint32_t two_of(float x, float y) {
   uint32_t both;
@@ -120,6 +121,100 @@ __device__ __forceinline__ void store_results(F four, int64_t i, int64_t j, int6
     }
   }
 }
+
+// Results of a wave's 32 rows on their way to memory, 64 columns at a time, in whole lines.
+//
+// Memory takes whole aligned lines of 128 bytes at 5.4 TB/s and rows cut elsewhere at
+// 3.3 to 3.8, and rows of an odd length begin anywhere.  So a wave keeps, per row, a
+// ring of two lines in LDS in which an element's place follows its address: a line is
+// written whole as soon as its last column is there, and only the first and the last
+// one of a walk over columns are written in parts.
+template <class O>
+struct LineRing {
+  static constexpr int S = (int)sizeof(O), E = 128 / S, V = 16 / S;  // elements of a line, of 16 bytes
+  static constexpr int kRing = 256, Y = E / 32;                      // bytes of a row's ring; 32-column results to a line
+  static constexpr int kBytes = 32 * kRing;                          // of a wave, aligned to kRing
+  static constexpr int G = 4;                                        // lines leave by 8 lanes each, 8 rows at once
+  char* ring;
+  uint32_t place[Y][16];  // where the lane's columns of a line go in the ring, register 4 g + e of result y; those of the
+                          // next line half a ring on
+  char* line_to[G];
+  int rel[G], rows;
+  int64_t lo;
+
+  // rows [it, it + rows) of `out`, columns from 64 first on
+  __device__ __forceinline__ LineRing(char* ring, O* out, int64_t out_stride, int64_t it, int rows, int64_t first)
+      : ring(ring), rows(rows), lo(first * 64) {
+    const int lane = dev::lane_id(), row = lane % 32, half = lane / 32, c = lane % 8;
+    // elements of its line before a row's first one
+    auto shift = [&](int r) { return (int)(reinterpret_cast<uintptr_t>(out + (it + r) * out_stride) % 128) / S; };
+#pragma unroll
+    for (int g = 0; g < 4; g++)
+#pragma unroll
+      for (int e = 0; e < 4; e++)
+#pragma unroll
+        for (int y = 0; y < Y; y++) {
+          const int at = (int)(first & 1) * 64 + 32 * y + row + shift(8 * g + 4 * half + e);
+          place[y][4 * g + e] = dev::lds_addr(ring) + 4 * half * kRing + (at * S & (kRing - 1));
+        }
+#pragma unroll
+    for (int g = 0; g < G; g++) {
+      const int r = 8 * g + lane / 8, sh = shift(r);
+      rel[g] = c * V - sh;
+      line_to[g] = reinterpret_cast<char*>(out + (it + r) * out_stride + (first * 64 + rel[g]));
+    }
+  }
+  // registers r and r + 1 of the 32 columns' result y of the line to come (two_of's condition holds here too)
+  __device__ __forceinline__ void put(int y, int r, float v0, float v1) {
+    typedef O o2 __attribute__((ext_vector_type(2)));
+    typedef __attribute__((address_space(3))) O lds_o;
+    o2 out;
+    if constexpr (sizeof(O) == 2) out = __builtin_bit_cast(o2, two_of<O>(v0, v1));
+    else out = o2{v0, v1};
+#pragma unroll
+    for (int d = 0; d < 2; d++) {
+      uint32_t& at = place[y][r + d];
+      ((lds_o*)(uintptr_t)at)[(r / 4 * 8 + r % 4 + d) * kRing / S] = out[d];
+      at ^= 128;
+    }
+  }
+  // line number `line` (the E elements from column line E - shift on) of every row, columns [lo, hi) of it
+  __device__ __forceinline__ void leave(int64_t line, int64_t hi, int64_t step) {
+    const int lane = dev::lane_id(), c = lane % 8;
+    const int least = (int)max(lo - line * E, (int64_t)-1024), most = (int)min(hi - line * E, (int64_t)1024);
+    const char* from = ring + (int)(line & 1) * 128 + c * 16;
+    if (rows == 32 && least <= 1 - E && most >= E) {  // whole lines of all rows
+#pragma unroll
+      for (int g = 0; g < G; g++) {
+        *reinterpret_cast<i4*>(line_to[g]) = *reinterpret_cast<const i4*>(from + (8 * g + lane / 8) * kRing);
+        line_to[g] += step;
+      }
+      return;
+    }
+#pragma unroll
+    for (int g = 0; g < G; g++) {
+      const int r = 8 * g + lane / 8;
+      union {
+        i4 raw;
+        O o[V];
+      } u;
+      u.raw = *reinterpret_cast<const i4*>(from + r * kRing);
+      if (r < rows) {
+        if (rel[g] >= least && rel[g] + V <= most) {
+          *reinterpret_cast<i4*>(line_to[g]) = u.raw;
+        } else {
+#pragma unroll
+          for (int v = 0; v < V; v++)
+            if (rel[g] + v >= least && rel[g] + v < most) reinterpret_cast<O*>(line_to[g])[v] = u.o[v];
+        }
+      }
+      line_to[g] += step;
+    }
+    // every store of this way is done: a later wait for loads then need not count them, and on the other way
+    // waits for the loads before its four stores only
+    __builtin_amdgcn_s_waitcnt(kLoadsDone);
+  }
+};
 
 // Workgroups go round the eight XCDs: each XCD gets a run of consecutive tiles.
 __device__ __forceinline__ int64_t tile_of_block(int64_t block, int64_t tiles) {

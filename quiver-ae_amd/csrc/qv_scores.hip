@@ -551,11 +551,7 @@ __global__ __launch_bounds__(64 * WM * WN, 1) void product_deep_kernel(Product<O
 // registers while its workgroup (128 rows) walks over tiles of 64 rows of b, through
 // LDS with the next two tiles on their way.
 //
-// Memory takes whole aligned lines of 128 bytes at 5.4 TB/s and rows cut elsewhere at
-// 3.3 to 3.8, and rows of an odd length begin anywhere.  So a wave keeps, per row, a
-// ring of two lines in LDS in which an element's place follows its address: a line is
-// written whole as soon as its last column is there, and only the first and the last
-// one of a walk are written in parts.
+// Results leave in whole lines (LineRing).
 // 10,000 x 50,001 x 128 to bfloat16: 255 us call after call into the same scores, 4.0 TB/s,
 // 264 into others each time (tiles with unaligned stores: 503), to float 4.5 TB/s;
 // without its stores the kernel takes 171 us.
@@ -563,10 +559,9 @@ template <int KS, bool BIAS, class O>
 __global__ __launch_bounds__(256, KS == 4 ? 3 : 2) void product_panel_kernel(Product<O> p, int64_t panels, int64_t tiles_n,
                                                                int64_t slices) {
   constexpr int PC = 2 * KS, kRow = 32 * KS, L = 64 * PC / 256, kRows = 256 / PC;
-  constexpr int S = (int)sizeof(O), E = 128 / S, V = 16 / S;   // elements of a line, of 16 bytes
-  constexpr int kRing = 256, Y = E / 32;  // bytes of a row's ring; 32-column results to a line
+  constexpr int Y = LineRing<O>::Y;
   __shared__ __align__(16) char lds[2][64 * kRow];
-  __shared__ __align__(256) char rings[4][32 * kRing];
+  __shared__ __align__(256) char rings[4][LineRing<O>::kBytes];
   __shared__ __align__(16) float sa[128];
   __shared__ float sb[2][BIAS ? 2 : 1][64];  // a tile's scales and biases
   const int tid = threadIdx.x, wave = wave_id(), lane = lane_id(), row = lane % 32, half = lane / 32;
@@ -606,69 +601,7 @@ __global__ __launch_bounds__(256, KS == 4 ? 3 : 2) void product_panel_kernel(Pro
     }
   }
   if (tid < 128) sa[tid] = p.a_scales[min(i0 + tid, p.m - 1)];
-  // elements of its line before a row's first one
-  auto shift = [&](int r) { return (int)(reinterpret_cast<uintptr_t>(p.out + (it + r) * p.out_stride) % 128) / S; };
-  char* ring = rings[wave];
-  // where the columns of a line go in the ring, register 4 g + e of result y; those of the next line
-  // half a ring on
-  uint32_t place[Y][16];
-  typedef __attribute__((address_space(3))) O lds_o;
-#pragma unroll
-  for (int g = 0; g < 4; g++)
-#pragma unroll
-    for (int e = 0; e < 4; e++)
-#pragma unroll
-      for (int y = 0; y < Y; y++) {
-        const int at = (int)(first & 1) * 64 + 32 * y + row + shift(8 * g + 4 * half + e);
-        place[y][4 * g + e] = lds_addr(ring) + 4 * half * kRing + (at * S & (kRing - 1));
-      }
-  // lines as they leave: 8 lanes a line, 8 rows at once
-  constexpr int G = 4;
-  const int c = lane % 8;
-  char* line_to[G];
-  int rel[G];
-#pragma unroll
-  for (int g = 0; g < G; g++) {
-    const int r = 8 * g + lane / 8, sh = shift(r);
-    rel[g] = c * V - sh;
-    line_to[g] = reinterpret_cast<char*>(p.out + (it + r) * p.out_stride + (first * 64 + rel[g]));
-  }
-  // line number `line` (the E elements from column line E - shift on) of every row, columns [lo, hi) of it
-  const int64_t lo = first * 64;
-  auto leave = [&](int64_t line, int64_t hi, int64_t step) {
-    const int least = (int)max(lo - line * E, (int64_t)-1024), most = (int)min(hi - line * E, (int64_t)1024);
-    const char* from = ring + (int)(line & 1) * 128 + c * 16;
-    if (rows == 32 && least <= 1 - E && most >= E) {  // whole lines of all rows
-#pragma unroll
-      for (int g = 0; g < G; g++) {
-        *reinterpret_cast<i4*>(line_to[g]) = *reinterpret_cast<const i4*>(from + (8 * g + lane / 8) * kRing);
-        line_to[g] += step;
-      }
-      return;
-    }
-#pragma unroll
-    for (int g = 0; g < G; g++) {
-      const int r = 8 * g + lane / 8;
-      union {
-        i4 raw;
-        O o[V];
-      } u;
-      u.raw = *reinterpret_cast<const i4*>(from + r * kRing);
-      if (r < rows) {
-        if (rel[g] >= least && rel[g] + V <= most) {
-          *reinterpret_cast<i4*>(line_to[g]) = u.raw;
-        } else {
-#pragma unroll
-          for (int v = 0; v < V; v++)
-            if (rel[g] + v >= least && rel[g] + v < most) reinterpret_cast<O*>(line_to[g])[v] = u.o[v];
-        }
-      }
-      line_to[g] += step;
-    }
-    // every store of this way is done: a later wait for loads then need not count them, and on the other way
-    // waits for the loads before its four stores only
-    __builtin_amdgcn_s_waitcnt(kLoadsDone);
-  };
+  LineRing<O> ring(rings[wave], p.out, p.out_stride, it, rows, first);
   keep(0);
   if (first + 1 < end) load(first + 1);
   __syncthreads();
@@ -704,31 +637,22 @@ __global__ __launch_bounds__(256, KS == 4 ? 3 : 2) void product_panel_kernel(Pro
         for (int e = 0; e < 4; e += 2)
 #pragma unroll
           for (int y = 0; y < Y; y++) {
-            typedef O o2 __attribute__((ext_vector_type(2)));
             float x[2];
 #pragma unroll
             for (int d = 0; d < 2; d++) {
               x[d] = ((float)acc[l * Y + y][4 * g + e + d] * s[e + d]) * scale[y];
               if constexpr (BIAS) x[d] = x[d] + add[y];
             }
-            o2 out;
-            if constexpr (sizeof(O) == 2) out = __builtin_bit_cast(o2, two_of<O>(x[0], x[1]));
-            else out = o2{x[0], x[1]};
-#pragma unroll
-            for (int d = 0; d < 2; d++) {
-              uint32_t& at = place[y][4 * g + e + d];
-              ((lds_o*)(uintptr_t)at)[(8 * g + e + d) * kRing / S] = out[d];
-              at ^= 128;
-            }
+            ring.put(y, 4 * g + e, x[0], x[1]);
           }
       }
       __builtin_amdgcn_fence(__ATOMIC_ACQ_REL, "wavefront");
-      leave(tile * (2 / Y) + l, p.n, 128);
+      ring.leave(tile * (2 / Y) + l, p.n, 128);
       __builtin_amdgcn_fence(__ATOMIC_ACQ_REL, "wavefront");
     }
     __syncthreads();
   }
-  leave(end * (2 / Y), min(end * 64, p.n), 0);
+  ring.leave(end * (2 / Y), min(end * 64, p.n), 0);
 }
 
 // Up to 32 rows of a against strips of 32 rows of b, one strip per wave at a time (WK =
