@@ -189,6 +189,7 @@ struct Product {
   int blocks;    // of a row
   O* out;
   int64_t out_stride;
+  bool stream, stream_lines;  // results past the caches: of tiles' pieces, of whole lines
 };
 
 // x: an instruction's rows, y: its columns; the scales are byte S of theirs.
@@ -197,6 +198,13 @@ __device__ __forceinline__ f16v mfma(i4 x, uint32_t scale_x, i4 y, uint32_t scal
   const i8v wx = __builtin_shufflevector(x, x, 0, 1, 2, 3, -1, -1, -1, -1);
   const i8v wy = __builtin_shufflevector(y, y, 0, 1, 2, 3, -1, -1, -1, -1);
   return __builtin_amdgcn_mfma_scale_f32_32x32x64_f8f6f4(wx, wy, acc, 4, 4, S, (int)scale_x, S, (int)scale_y);
+}
+
+// The same of 16 rows, 16 columns and four blocks of each; the scales are their lowest bytes.
+__device__ __forceinline__ f4 mfma16(i4 x, uint32_t scale_x, i4 y, uint32_t scale_y, f4 acc) {
+  const i8v wx = __builtin_shufflevector(x, x, 0, 1, 2, 3, -1, -1, -1, -1);
+  const i8v wy = __builtin_shufflevector(y, y, 0, 1, 2, 3, -1, -1, -1, -1);
+  return __builtin_amdgcn_mfma_scale_f32_16x16x128_f8f6f4(wx, wy, acc, 4, 4, 0, (int)scale_x, 0, (int)scale_y);
 }
 
 // Scales of the eight blocks from `at` on of a row of `blocks`; 0 past its end.
@@ -227,14 +235,14 @@ __device__ __forceinline__ void store_tile(f16v (&acc)[TM][TN], int i, int j, in
                                            const Product<O>& p) {
   constexpr int R = sizeof(O) == 2 && TN % 2 == 0 ? 2 : 1;
   const int row = lane_id() % 32, half = lane_id() / 32;
-  auto store = [&](auto whole) {
+  auto store = [&](auto whole, auto stream) {
 #pragma unroll
     for (int x = 0; x < TM; x++)
 #pragma unroll
       for (int y = 0; y < TN; y += R) {
 #pragma unroll
         for (int r = 0; r < R; r++) asm volatile("" : "+a"(acc[x][y + r]) : : "memory");  // in turn: none leaves its accumulators before
-        store_results<decltype(whole)::value, R>(
+        store_results<decltype(whole)::value, decltype(stream)::value, R>(
             [&](int r, int g) {
               const f4 t = *reinterpret_cast<const f4*>(bias + j + 32 * (y + r) + 8 * g + 4 * half);
               f4 v;
@@ -245,8 +253,9 @@ __device__ __forceinline__ void store_tile(f16v (&acc)[TM][TN], int i, int j, in
             i0 + i + 32 * x + row, j0 + j + 32 * y, p.m, p.n, p.out, p.out_stride);
       }
   };
-  if (i0 + BM <= p.m && j0 + BN <= p.n) store(std::true_type());
-  else store(std::false_type());
+  if (i0 + BM > p.m || j0 + BN > p.n) store(std::false_type(), std::false_type());
+  else if (p.stream) store(std::true_type(), std::true_type());
+  else store(std::true_type(), std::false_type());
 }
 
 // A tile of BM x BN outputs per workgroup, WM x WN waves of 32 TM x 32 TN each.  Both
@@ -381,9 +390,16 @@ __global__ __launch_bounds__(64 * WM * WN, 1) void product_tile_kernel(Product<O
 // and the next stage's first operands while the second one's do, so the one barrier
 // per stage, between the two, finds the operands of what follows it in registers.
 // Needs 16-byte aligned rows, scales' rows of whole aligned words, k a multiple of 64.
+// G: a load brings a row's scales of G stages, 16 bytes for four (k a multiple of 256 and rows
+// of scales 16-byte aligned; then a group's stages are unrolled, with places that are
+// constants), else a word of each, which fetches its line again for the next one where rows
+// are long (4,096^3: 57 us, and 49 before the groups' stages were unrolled).
 // MANY: one workgroup per CU walks over tiles, and the stages run on from tile to tile:
 // the next tile's first ones are on their way, and its first operands in registers, while
 // the results are stored.
+// 4,096^3 to bfloat16: 45 us, 3.1 PFLOP/s, of zeros 37 (a library's 4-bit product with block scales: 70); 8,192^3: 300 us,
+// 3.7 PFLOP/s, of zeros 246 (library: 359).  The matrix instruction alone runs at 6.5 PFLOP/s on varied codes, 8.9 on
+// zeros: LDS (98 KB a stage, 784 of the 1,024 cycles of its products) and power hold it.
 template <int BM, int BN, int WM, int WN, int NB, int G, bool MANY, class O>
 __global__ __launch_bounds__(64 * WM * WN, 1) void product_deep_kernel(Product<O> p, int64_t tiles_m, int64_t tiles_n,
                                                                        int64_t group) {
@@ -579,6 +595,174 @@ __global__ __launch_bounds__(64 * WM * WN, 1) void product_deep_kernel(Product<O
   __builtin_amdgcn_s_waitcnt(kWaitFor<0>);  // no load into LDS outlives the wave
 }
 
+// Stores four columns from j on of row i, with their biases, where they lie in the output.
+template <class O>
+__device__ __forceinline__ void store_four(f4 v, int64_t i, int64_t j, const Product<O>& p) {
+  asm volatile("" : "+v"(v));  // here: a matrix instruction that the compiler moves behind the branch has not all lanes' scales
+  if (i >= p.m) return;
+  O o[4];
+#pragma unroll
+  for (int e = 0; e < 4; e++) o[e] = (O)(p.bias ? v[e] + p.bias[min(j + e, p.n - 1)] : v[e]);
+  O* to = p.out + i * p.out_stride + j;
+  if (j + 4 <= p.n) {
+    __builtin_memcpy(to, o, sizeof(o));
+  } else {
+#pragma unroll
+    for (int e = 0; e < 3; e++)
+      if (j + e < p.n) to[e] = o[e];
+  }
+}
+
+// Up to 16 TM rows of a against strips of 16 rows of b whose blocks one matrix instruction takes, up to 128 values
+// (v_mfma_scale_f32_16x16x128_f8f6f4: what 64 lanes load of 16 such rows is 1 KB in a row).  U strips per wave, straight from
+// memory to the registers.  Bound by reading b: 1 x 1M x 128 to float 13.9 us, 5.2 TB/s.
+template <int U, int TM, class O>
+__global__ __launch_bounds__(256) void product_row_kernel(Product<O> p, int64_t groups, int64_t first_block) {
+  const int lane = lane_id(), row = lane % 16, quarter = lane / 16;
+  const int64_t group = (first_block + blockIdx.x) * 4 + wave_id();
+  if (group >= groups) return;
+  const int k = (int)p.k, place = quarter * 16, at = min(place, k - 16), block = min(quarter, p.blocks - 1);
+  i4 fa[TM], fb[U];
+  uint32_t sa[TM], sb[U];
+#pragma unroll
+  for (int u = 0; u < U; u++) {
+    const int64_t j = min((group * U + u) * 16 + row, p.n - 1);
+    fb[u] = *reinterpret_cast<const i4_any*>(p.b + j * p.b_stride + at);
+    sb[u] = p.b_scales[j * p.bs_stride + block];
+  }
+#pragma unroll
+  for (int x = 0; x < TM; x++) {
+    const int64_t i = min((int64_t)(16 * x + row), p.m - 1);
+    fa[x] = without_first(*reinterpret_cast<const i4_any*>(p.a + i * p.a_stride + at), place - at);
+    sa[x] = p.a_scales[i * p.as_stride + block];
+  }
+#pragma unroll
+  for (int u = 0; u < U; u++)
+#pragma unroll
+    for (int x = 0; x < TM; x++)
+      store_four(mfma16(fb[u], sb[u], fa[x], sa[x], f4{0.f, 0.f, 0.f, 0.f}), 16 * x + row, (group * U + u) * 16 + 4 * quarter, p);
+}
+
+// The same for longer rows: b goes to the registers one turn ahead, U strips of V = 4 / U steps of four blocks.  A lane loads one word of scales, those of
+// one row and step; two exchanges between the quarters of the wave give every lane the word of each.  a and its scales
+// lie in LDS in the order of the lanes.  WK > 1: a strip's blocks are cut over the workgroup's WK waves.
+template <int U, int TM, int WK, class O>
+__global__ __launch_bounds__(WK == 1 ? 256 : 64 * WK) void product_strip_kernel(Product<O> p, int64_t groups) {
+  constexpr int V = 4 / U, kWaves = WK == 1 ? 4 : WK;
+  extern __shared__ __align__(16) char lds[];
+  const int wave = wave_id(), lane = lane_id(), row = lane % 16, quarter = lane / 16;
+  const int k = (int)p.k, blocks = p.blocks, steps = (blocks + 3) / 4, turns = (steps + V - 1) / V;
+  const int64_t step = (int64_t)gridDim.x * (WK == 1 ? 4 : 1);
+  int64_t group = WK == 1 ? (int64_t)blockIdx.x * 4 + wave : blockIdx.x;
+  const int first = WK == 1 ? 0 : wave;
+  const int64_t scales_end = (p.n - 1) * p.bs_stride + blocks;
+
+  i4 next_b[U][V];
+  uint32_t next_scales = 0;
+  auto load = [&](int64_t group, int turn) {
+    const uint8_t* b = p.b + min(group * (16 * U) + row, p.n - 1) * p.b_stride;
+#pragma unroll
+    for (int u = 0; u < U; u++) {
+      const uint8_t* from = u == 0 ? b : p.b + min((group * U + u) * 16 + row, p.n - 1) * p.b_stride;
+#pragma unroll
+      for (int v = 0; v < V; v++)
+        next_b[u][v] = *reinterpret_cast<const i4_any*>(from + min(((turn * V + v) * 4 + quarter) * 16, k - 16));
+    }
+    // the word of this row and step; bytes past the row's end are 0
+    const int block = (turn * V + quarter % V) * 4;
+    const int64_t at = min((group * U + quarter / V) * 16 + row, p.n - 1) * p.bs_stride + min(block, blocks - 1);
+    const int64_t from = min(at, scales_end - 4);
+    uint32_t word;
+    __builtin_memcpy(&word, p.b_scales + from, 4);
+    const int valid = blocks - block;
+    next_scales = valid <= 0 ? 0 : word >> (8 * (int)(at - from)) & (valid >= 4 ? ~0u : (1u << 8 * valid) - 1);
+  };
+  if (group < groups && first < turns) load(group, first);
+
+  // a in LDS: piece q of step s and tile x at ((s TM + x) 64 + 16 q + row) 16, its scale behind them
+  char* sa = lds + steps * TM * 1024;
+  const int pieces = (int)p.m * steps * 4;
+  for (int e = threadIdx.x; e < pieces; e += 4 * 64 * kWaves) {
+    i4 v[4];
+    int at[4];
+    char scale[4];
+#pragma unroll
+    for (int q = 0; q < 4; q++) {
+      const int n = min(e + q * 64 * kWaves, pieces - 1);
+      const int i = n / (steps * 4), block = n - i * (steps * 4), place = block * 16, from = min(place, k - 16);
+      at[q] = (block / 4 * TM + i / 16) * 64 + block % 4 * 16 + i % 16;
+      v[q] = without_first(*reinterpret_cast<const i4_any*>(p.a + i * p.a_stride + from), place - from);
+      scale[q] = block < blocks ? (char)p.a_scales[i * p.as_stride + min(block, blocks - 1)] : 0;
+    }
+#pragma unroll
+    for (int q = 0; q < 4; q++) {
+      *reinterpret_cast<i4*>(lds + at[q] * 16) = v[q];
+      sa[at[q]] = scale[q];
+    }
+  }
+  __syncthreads();
+
+  for (; group < groups; group += step) {
+    f4 acc[TM][U];
+#pragma unroll
+    for (int x = 0; x < TM; x++)
+#pragma unroll
+      for (int u = 0; u < U; u++) acc[x][u] = f4{0.f, 0.f, 0.f, 0.f};
+    for (int turn = first; turn < turns; turn += WK) {
+      i4 b[U][V];
+#pragma unroll
+      for (int u = 0; u < U; u++)
+#pragma unroll
+        for (int v = 0; v < V; v++) b[u][v] = next_b[u][v];
+      const uint32_t word = next_scales;
+      if (turn + WK < turns) load(group, turn + WK);
+      else if (group + step < groups) load(group + step, first);
+      // words[q]: that of quarter q's rows, in every lane
+      uint32_t words[4];
+      {
+        const auto h = __builtin_amdgcn_permlane32_swap(word, word, false, false);
+        const auto lo = __builtin_amdgcn_permlane16_swap(h[0], h[0], false, false);
+        const auto hi = __builtin_amdgcn_permlane16_swap(h[1], h[1], false, false);
+        words[0] = lo[0], words[1] = lo[1], words[2] = hi[0], words[3] = hi[1];
+      }
+#pragma unroll
+      for (int v = 0; v < V; v++) {
+        const int s = turn * V + v;
+        if (V > 1 && s >= steps) break;
+#pragma unroll
+        for (int x = 0; x < TM; x++) {
+          const i4 a = *reinterpret_cast<const i4*>(lds + ((s * TM + x) * 64 + lane) * 16);
+          const uint32_t scale = *reinterpret_cast<const uint8_t*>(sa + (s * TM + x) * 64 + lane);
+#pragma unroll
+          for (int u = 0; u < U; u++) acc[x][u] = mfma16(b[u][v], words[u * V + v] >> (8 * quarter), a, scale, acc[x][u]);
+        }
+      }
+    }
+    if constexpr (WK > 1) {
+      f4* parts = reinterpret_cast<f4*>(lds + steps * TM * 1088);
+#pragma unroll
+      for (int x = 0; x < TM; x++)
+#pragma unroll
+        for (int u = 0; u < U; u++) parts[(wave * TM * U + x * U + u) * 64 + lane] = acc[x][u];
+      __syncthreads();
+      if (wave == 0) {
+#pragma unroll
+        for (int x = 0; x < TM; x++)
+#pragma unroll
+          for (int u = 0; u < U; u++)
+#pragma unroll
+            for (int w = 1; w < WK; w++) acc[x][u] += parts[(w * TM * U + x * U + u) * 64 + lane];
+      }
+      __syncthreads();
+      if (wave) continue;
+    }
+#pragma unroll
+    for (int u = 0; u < U; u++)
+#pragma unroll
+      for (int x = 0; x < TM; x++) store_four(acc[x][u], 16 * x + row, (group * U + u) * 16 + 4 * quarter, p);
+  }
+}
+
 // Short rows, k <= 32 KS bytes, whose product is mostly writing: 32 rows of a stay in a wave's
 // registers while its workgroup (128 rows) walks over tiles of 64 rows of b, through
 // LDS with the next two tiles on their way.  Results leave in whole lines (LineRing).
@@ -638,7 +822,7 @@ __global__ __launch_bounds__(256, KS == 8 ? 2 : 3) void product_panel_kernel(Pro
       if (block < p.blocks) sa[q / 4] |= (uint32_t)s[block] << (8 * (q % 4));
     }
   }
-  LineRing<O> ring(rings[wave], p.out, p.out_stride, it, rows, first);
+  LineRing<O> ring(rings[wave], p.out, p.out_stride, it, rows, first, p.stream_lines);
   keep(0);
   if (first + 1 < end) load(first + 1);
   __syncthreads();
@@ -755,28 +939,83 @@ void launch_panels(const Product<O>& p, hipStream_t st) {
   HIP_OK(hipGetLastError());
 }
 
-int force() { static const int f = getenv("QV_FORCE") ? atoi(getenv("QV_FORCE")) : 0; return f; }
+int strip_lds(int64_t m, int64_t blocks, int u, int wk) {
+  const int tm = m <= 16 ? 1 : 2;
+  return (int)((blocks + 3) / 4) * tm * 1088 + (wk > 1 ? wk * tm * u * 1024 : 0);
+}
+
+template <int U, int WK, class O>
+void launch_strips(const Product<O>& p, hipStream_t st) {
+  const int64_t groups = (p.n + 16 * U - 1) / (16 * U);
+  const int lds = strip_lds(p.m, p.blocks, U, WK);
+  constexpr int kThreads = WK == 1 ? 256 : 64 * WK;
+  // as many workgroups as run at once
+  const int64_t most = 256 * std::min(2048 / kThreads, 160 * 1024 / std::max(lds, 1));
+  const int64_t blocks = std::min(most, WK == 1 ? (groups + 3) / 4 : groups);
+  auto go = [&](auto tiles) {
+    constexpr auto* kernel = &product_strip_kernel<U, decltype(tiles)::value, WK, O>;
+    allow_lds<kernel>(lds);
+    hipLaunchKernelGGL(kernel, dim3((unsigned)blocks), dim3(kThreads), lds, st, p, groups);
+  };
+  if (p.m <= 16) go(std::integral_constant<int, 1>());
+  else go(std::integral_constant<int, 2>());
+  HIP_OK(hipGetLastError());
+}
 
 template <class O>
+void launch_rows(const Product<O>& p, hipStream_t st) {
+  constexpr int U = 2;
+  const int64_t groups = (p.n + 16 * U - 1) / (16 * U);
+  auto* kernel = p.m <= 16 ? product_row_kernel<U, 1, O> : product_row_kernel<U, 2, O>;
+  in_launches((groups + 3) / 4, 256, [&](int64_t first, unsigned count) {
+    hipLaunchKernelGGL(kernel, dim3(count), dim3(256), 0, st, p, groups, first);
+  });
+  HIP_OK(hipGetLastError());
+}
+
+// Which kernel: up to 32 rows read b; rows of up to 256 bytes mostly write the result; longer ones keep the matrix cores busy.
+template <class O>
 void product(const Product<O>& p, hipStream_t st) {
-  const bool direct = (reinterpret_cast<uintptr_t>(p.a) | reinterpret_cast<uintptr_t>(p.b) | p.a_stride | p.b_stride | p.k * 0) % 16 == 0 &&
-                      (reinterpret_cast<uintptr_t>(p.a_scales) | reinterpret_cast<uintptr_t>(p.b_scales) | p.as_stride | p.bs_stride) % 4 == 0 &&
-                      p.k % 64 == 0 && p.k >= 256 && p.a_stride < kFar && p.b_stride < kFar && p.as_stride < kFar && p.bs_stride < kFar;
-  const int f = force();
-  const bool four = p.k % 256 == 0 && (reinterpret_cast<uintptr_t>(p.a_scales) | reinterpret_cast<uintptr_t>(p.b_scales) | p.as_stride | p.bs_stride) % 16 == 0;
-  const bool near = p.a_stride < kFar && p.b_stride < kFar && p.as_stride < kFar && p.bs_stride < kFar;
-  if (p.k < 16) launch_tiles<64, 64, 2, 2, true>(p, st);
-  else if (near && p.k <= 64 && f == 5) launch_panels<2>(p, st);
-  else if (near && p.k <= 128 && f == 5) launch_panels<4>(p, st);
-  else if (near && p.k <= 256 && f == 5) launch_panels<8>(p, st);
-  else if (direct && four && f == 1) launch_deep<256, 256, 2, 2, 4, 4, true>(p, st);
-  else if (direct && four && f == 2) launch_deep<128, 128, 2, 2, 4, 4, false>(p, st);
-  else if (direct && four && f == 3) launch_deep<64, 64, 2, 2, 4, 4, false>(p, st);
-  else if (direct && f == 1) launch_deep<256, 256, 2, 2, 4, 1, true>(p, st);
-  else if (direct && f == 2) launch_deep<128, 128, 2, 2, 4, 1, false>(p, st);
-  else if (direct && f == 3) launch_deep<64, 64, 2, 2, 4, 1, false>(p, st);
-  else if (f == 4) launch_tiles<128, 128, 2, 2, false>(p, st);
-  else launch_tiles<64, 64, 2, 2, false>(p, st);
+  const int64_t scale_bits = reinterpret_cast<uintptr_t>(p.a_scales) | reinterpret_cast<uintptr_t>(p.b_scales) | p.as_stride | p.bs_stride;
+  const int64_t code_bits = reinterpret_cast<uintptr_t>(p.a) | reinterpret_cast<uintptr_t>(p.b) | p.a_stride | p.b_stride;
+  const bool near = std::max({p.a_stride, p.b_stride, p.as_stride, p.bs_stride}) < kFar;
+  const bool direct = near && code_bits % 16 == 0 && scale_bits % 4 == 0 && p.k % 64 == 0;
+  const bool four = direct && scale_bits % 16 == 0 && p.k % 256 == 0;
+  auto tiles = [&](int64_t size) { return (p.m + size - 1) / size * ((p.n + size - 1) / size); };
+  if (p.k < 16) {
+    launch_tiles<64, 64, 2, 2, true>(p, st);
+  } else if (p.m <= 32 && p.blocks <= 4) {
+    launch_rows(p, st);
+  } else if (p.m <= 32 && strip_lds(p.m, p.blocks, 1, 4) <= 150 * 1024) {  // (five blocks: a scales' word lies in any row)
+    // A strip's blocks over four waves where strips alone are too few.  Measured, us, without and with: 1 x 4,096 x 4,096:
+    // 12.8, 7.2; 1 x 20,000 x 4,096: 16.5, 10.8; 1 x 50,000 x 1,024: 8.4, 9.8; 8 x 100,000 x 1,024: 14.5, 16.0.
+    if (p.n >= 32768 || p.blocks <= 16) launch_strips<2, 1>(p, st);
+    else launch_strips<1, 4>(p, st);
+  } else if (near && p.k <= 64) {
+    launch_panels<2>(p, st);
+  } else if (near && p.k <= 128) {
+    launch_panels<4>(p, st);
+  } else if (near && p.k <= 256) {
+    launch_panels<8>(p, st);
+  } else {
+    // By how many tiles there are for the 256 CUs.  Measured to bfloat16, us, with tiles of 256, 128 and 64 straight to LDS
+    // and of 128 and 64 through registers: 4,096^3: 45, 60, 101, 62, 93; 2,048 x 4,096 x 4,096: 35, 30, 45, 30, 42; 1,024:
+    // 31, 16, 24, 25, 23; 512: 28, 13, 12, 21, 14; 64: 28, 11, 7, 19, 12; 10,000 x 50,048 x 1,024: 399, 468, -, 489, -.
+    // Where scales come a word at a time (k no multiple of 512) and rows are long, each word's line is fetched again for
+    // the next: 4,096 x 4,096 x 4,224: 55, 83, 148, 65, -; 2,048: -, 45, 76, 35, 57; 1,024: -, 25, 40, 29, 34; 512: -, 18,
+    // 21, 24, 18; 64: -, 13, 9, 20, 12; 1,024 x 4,096 x 1,152: -, 8.7, 11.2, 10.9, 10.1.
+    // Tiles of 256 where they are filled to 80 % and fill the CUs' turns so (as for 8-bit rows).
+    const int64_t turns = (tiles(256) + 255) / 256;
+    const bool fill = (double)p.m * p.n >= 0.8 * 65536 * 256 * turns && tiles(256) < int64_t{1} << 31;
+    if (four && fill) launch_deep<256, 256, 2, 2, 4, 4, true>(p, st);
+    else if (direct && fill) launch_deep<256, 256, 2, 2, 4, 1, true>(p, st);
+    else if (four && tiles(64) <= 512) launch_deep<64, 64, 2, 2, 4, 4, false>(p, st);
+    else if (four && tiles(128) < 1 << 23) launch_deep<128, 128, 2, 2, 4, 4, false>(p, st);
+    else if (direct && tiles(64) <= 128) launch_deep<64, 64, 2, 2, 4, 1, false>(p, st);
+    else if (direct && tiles(128) <= 256) launch_deep<128, 128, 2, 2, 4, 1, false>(p, st);
+    else if (tiles(64) <= 512) launch_tiles<64, 64, 2, 2, false>(p, st);
+    else launch_tiles<128, 128, 2, 2, false>(p, st);
+  }
 }
 
 // Codes and scales of n rows of dim values.
@@ -838,8 +1077,10 @@ int qv_mx4_product(const uint8_t* d_a, int64_t a_stride, const uint8_t* d_a_scal
     const hipStream_t st = static_cast<hipStream_t>(stream);
     auto go = [&](auto* o) {
       using O = std::remove_pointer_t<decltype(o)>;
+      const bool stream = (double)m * n * size >= kStreamBytes;
+      const bool lines = (reinterpret_cast<uintptr_t>(d_out) | out_stride * size) % 128 == 0;
       product(Product<O>{d_a, a_stride, d_a_scales, a_scale_stride, m, d_b, b_stride, d_b_scales, b_scale_stride, d_bias, n,
-                         k / 2, (int)((k + kBlock - 1) / kBlock), o, out_stride},
+                         k / 2, (int)((k + kBlock - 1) / kBlock), o, out_stride, stream && lines, stream},
               st);
     };
     if (out_type == QV_FLOAT) go(static_cast<float*>(d_out));

@@ -63,13 +63,19 @@ __device__ __forceinline__ void swap_pieces(i4 (&u)[P]) {
   if constexpr (P == 4) stage(std::integral_constant<int, 2>(), std::integral_constant<int, 0x4E>());  // quad_perm [2,3,0,1]
 }
 
+// Results of this size and more do not stay in the 256 MB of the last cache, and whole lines of them written past the
+// caches take less time: 4-bit products of 10,000 x 50,001 x 128 to bfloat16 264 -> 218 us, 10,000 x 50,048 x 1,024 466 ->
+// 399, 2,000 x 50,001 x 100 61 -> 49, but 1,000 x 50,001 x 100, 100 MB, 25.7 -> 27.8.  Lines written in parts take twice
+// the time that way (4,000 x 50,001 x 512: 168 -> 336).
+constexpr int64_t kStreamBytes = 128 << 20;
+
 // Stores the results of R instructions from the registers: 32 R columns from j of the rows around the lane's row i,
 // whole lines of 8 rows at once (half lines of 16 rows with 32 columns of 16 bits).  Of the four columns that a lane
 // has of every eight, those of 16 bits pass to the other half of the wave and back, eight for a lane; then groups of
 // lanes swap rows for pieces of one row.  (Pieces stored as they are, 32 bytes of 32 rows at once, take 5.0 for 5.35
 // TB/s in aligned rows, 2 for 3.8 in others.)  four(y, g): the lane's four results of columns 32 y + 8 g + 4 half on.
-// m, n, out, out_stride: the whole output.  WHOLE: all of it lies in the output.
-template <bool WHOLE, int R, class O, class F>
+// m, n, out, out_stride: the whole output.  WHOLE: all of it lies in the output.  STREAM: past the caches (kStreamBytes).
+template <bool WHOLE, bool STREAM, int R, class O, class F>
 __device__ __forceinline__ void store_results(F four, int64_t i, int64_t j, int64_t m, int64_t n, O* out, int64_t out_stride) {
   constexpr int V = 16 / (int)sizeof(O), N = 16 / V, P = R * N;  // columns of a piece, pieces of a result, of all
   const int half = dev::lane_id() / 32, c = dev::lane_id() % P;
@@ -106,7 +112,10 @@ __device__ __forceinline__ void store_results(F four, int64_t i, int64_t j, int6
   if (WHOLE || j + V <= n) {
 #pragma unroll
     for (int r = 0; r < P; r++)
-      if (WHOLE || i + r < m) *reinterpret_cast<i4_any*>(to + r * out_stride) = u[r];
+      if (WHOLE || i + r < m) {
+        if constexpr (STREAM) __builtin_nontemporal_store(u[r], reinterpret_cast<i4_any*>(to + r * out_stride));
+        else *reinterpret_cast<i4_any*>(to + r * out_stride) = u[r];
+      }
   } else {
 #pragma unroll
     for (int r = 0; r < P; r++) {
@@ -141,10 +150,11 @@ struct LineRing {
   char* line_to[G];
   int rel[G], rows;
   int64_t lo;
+  bool stream;
 
-  // rows [it, it + rows) of `out`, columns from 64 first on
-  __device__ __forceinline__ LineRing(char* ring, O* out, int64_t out_stride, int64_t it, int rows, int64_t first)
-      : ring(ring), rows(rows), lo(first * 64) {
+  // rows [it, it + rows) of `out`, columns from 64 first on; stream: past the caches (kStreamBytes)
+  __device__ __forceinline__ LineRing(char* ring, O* out, int64_t out_stride, int64_t it, int rows, int64_t first, bool stream)
+      : ring(ring), rows(rows), lo(first * 64), stream(stream) {
     const int lane = dev::lane_id(), row = lane % 32, half = lane / 32, c = lane % 8;
     // elements of its line before a row's first one
     auto shift = [&](int r) { return (int)(reinterpret_cast<uintptr_t>(out + (it + r) * out_stride) % 128) / S; };
@@ -184,11 +194,20 @@ struct LineRing {
     const int least = (int)max(lo - line * E, (int64_t)-1024), most = (int)min(hi - line * E, (int64_t)1024);
     const char* from = ring + (int)(line & 1) * 128 + c * 16;
     if (rows == 32 && least <= 1 - E && most >= E) {  // whole lines of all rows
+      i4 u[G];
 #pragma unroll
-      for (int g = 0; g < G; g++) {
-        *reinterpret_cast<i4*>(line_to[g]) = *reinterpret_cast<const i4*>(from + (8 * g + lane / 8) * kRing);
-        line_to[g] += step;
+      for (int g = 0; g < G; g++) u[g] = *reinterpret_cast<const i4*>(from + (8 * g + lane / 8) * kRing);
+      if (stream) {
+        asm volatile("" ::: "memory");  // on both sides: else the two ways become one of ordinary stores
+#pragma unroll
+        for (int g = 0; g < G; g++) __builtin_nontemporal_store(u[g], reinterpret_cast<i4*>(line_to[g]));
+        asm volatile("" ::: "memory");
+      } else {
+#pragma unroll
+        for (int g = 0; g < G; g++) *reinterpret_cast<i4*>(line_to[g]) = u[g];
       }
+#pragma unroll
+      for (int g = 0; g < G; g++) line_to[g] += step;
       return;
     }
 #pragma unroll

@@ -195,7 +195,7 @@ template <bool WHOLE, int R, class O>
 __device__ __forceinline__ void store_sums(const i16v* const (&acc)[R], float sa, const float* sb, const float* add,
                                            int64_t i, int64_t j, const Product<O>& p) {
   const int half = lane_id() / 32;
-  store_results<WHOLE, R>(
+  store_results<WHOLE, false, R>(
       [&](int y, int g) {
         const int at = 32 * y + 8 * g + 4 * half;
         const f4 s = *reinterpret_cast<const f4*>(sb + at), t = *reinterpret_cast<const f4*>(add + at);
@@ -601,7 +601,7 @@ __global__ __launch_bounds__(256, KS == 4 ? 3 : 2) void product_panel_kernel(Pro
     }
   }
   if (tid < 128) sa[tid] = p.a_scales[min(i0 + tid, p.m - 1)];
-  LineRing<O> ring(rings[wave], p.out, p.out_stride, it, rows, first);
+  LineRing<O> ring(rings[wave], p.out, p.out_stride, it, rows, first, false);
   keep(0);
   if (first + 1 < end) load(first + 1);
   __syncthreads();
