@@ -63,11 +63,13 @@ __device__ __forceinline__ void swap_pieces(i4 (&u)[P]) {
   if constexpr (P == 4) stage(std::integral_constant<int, 2>(), std::integral_constant<int, 0x4E>());  // quad_perm [2,3,0,1]
 }
 
-// Results of this size and more do not stay in the 256 MB of the last cache, and whole lines of them written past the
-// caches take less time: 4-bit products of 10,000 x 50,001 x 128 to bfloat16 264 -> 218 us, 10,000 x 50,048 x 1,024 466 ->
-// 399, 2,000 x 50,001 x 100 61 -> 49, but 1,000 x 50,001 x 100, 100 MB, 25.7 -> 27.8.  Lines written in parts take twice
-// the time that way (4,000 x 50,001 x 512: 168 -> 336).
-constexpr int64_t kStreamBytes = 128 << 20;
+// Results of more than the L2s hold together are written past them where they are whole lines.  4-bit products, us,
+// without and with: 10,000 x 50,001 x 128 to bfloat16 264, 218; 10,000 x 50,048 x 1,024 466, 399; 4,096^3 44, 42; 3,000 x
+// 50,001 x 128 78, 69, and 147, 135 with the log probabilities of the result behind it.  Into memory that the last cache
+// (256 MB) does not hold either: 500 x 50,001 x 100 to float16 23.0, 18.1; 1,000 x 50,001 x 100 37.7, 28.1.  Into the same
+// memory again and again: 18.4, 17.9; 25.7, 28.0, and 56, 61 with its log probabilities; worst, 256 x 200,000 x 128 to float:
+// 37, 44 and 76, 93.  Lines in parts take twice the time that way (4,000 x 50,001 x 512 by tiles: 168, 336).
+constexpr int64_t kStreamBytes = 32 << 20;
 
 // Stores the results of R instructions from the registers: 32 R columns from j of the rows around the lane's row i,
 // whole lines of 8 rows at once (half lines of 16 rows with 32 columns of 16 bits).  Of the four columns that a lane
