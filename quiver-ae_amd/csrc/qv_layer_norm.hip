@@ -100,6 +100,45 @@ __device__ __forceinline__ float lanes_sum(float v) {
   return v;
 }
 
+// A thread's part of a row, E vectors of four values, every R-th of the row's: asked for a row ahead, unpacked when they
+// are used.  All loads are whole: the one that the row ends in begins four values before the end, and values() moves
+// what it has down and fills up with zeros.
+template <class T, int R, int E>
+struct Part {
+  uint32_t raw[E][sizeof(T)];
+  __device__ __forceinline__ void load(const T* row, int lane, int dim) {
+#pragma unroll
+    for (int e = 0; e < E; e++) {
+      const int j = (e * R + lane) * 4;
+      if (dim >= 4) {
+        __builtin_memcpy(raw[e], row + min(j, dim - 4), 4 * sizeof(T));
+      } else {
+        T t[4] = {};
+#pragma unroll
+        for (int i = 0; i < 3; i++)
+          if (j + i < dim) t[i] = row[i];
+        __builtin_memcpy(raw[e], t, sizeof(t));
+      }
+    }
+  }
+  __device__ __forceinline__ f4 values(int e, int lane, int dim) const {
+    T t[4];
+    __builtin_memcpy(t, raw[e], sizeof(t));
+    f4 v;
+#pragma unroll
+    for (int i = 0; i < 4; i++) v[i] = (float)t[i];
+    if ((e + 1) * R * 4 > dim) {
+      const int over = dim >= 4 ? (e * R + lane) * 4 - (dim - 4) : (e * R + lane) * 4;
+      if (over > 0) {
+        if (over & 1) v = f4{v[1], v[2], v[3], 0.f};
+        if (over & 2) v = f4{v[2], v[3], 0.f, 0.f};
+        if (over >= 4) v = f4{0.f, 0.f, 0.f, 0.f};
+      }
+    }
+    return v;
+  }
+};
+
 // Sums over the R threads of a row: a part of a wave, or whole waves, which exchange theirs through two areas of LDS in
 // turn (so one barrier each: nobody writes an area again before everyone has met at the other one's).
 template <int R, int T>
@@ -213,15 +252,22 @@ __global__ __launch_bounds__(THREADS) void norm_kernel(const T* x, int64_t n, in
     w[e] = load_params(weight, param_type, j, dim, 1.f);
     b[e] = load_params(bias, param_type, j, dim, 0.f);
   }
-  for (int64_t base = (int64_t)blockIdx.x * kGroups; base < n; base += (int64_t)gridDim.x * kGroups) {
-    const int64_t row = base + threadIdx.x / R;
-    const T* from = x + min(row, n - 1) * stride;
-    auto values = [&](int e) { return load_four(from + (e * R + lane) * 4, dim - (e * R + lane) * 4); };
+  const int64_t step = (int64_t)gridDim.x * kGroups;
+  int64_t row = (int64_t)blockIdx.x * kGroups + threadIdx.x / R;
+  Part<T, R, E> part;
+  part.load(x + min(row, n - 1) * stride, lane, dim);
+  for (int64_t base = (int64_t)blockIdx.x * kGroups; base < n; base += step, row += step) {
     f4 v[E];
 #pragma unroll
-    for (int e = 0; e < E; e++) v[e] = values(e);
+    for (int e = 0; e < E; e++) v[e] = part.values(e, lane, dim);
+    if (base + step < n) part.load(x + min(row + step, n - 1) * stride, lane, dim);
+    auto again = [&](int e) {
+      Part<T, R, E> same;
+      same.load(x + min(row, n - 1) * stride, lane, dim);
+      return same.values(e, lane, dim);
+    };
     float scale, none[2];
-    const float rstd = centre<false>(values, v, v, v, lane, dim, eps, across, scale, none);
+    const float rstd = centre<false>(again, v, v, v, lane, dim, eps, across, scale, none);
     if (row >= n) continue;
 #pragma unroll
     for (int e = 0; e < E; e++) {
@@ -252,17 +298,26 @@ __global__ __launch_bounds__(THREADS) void norm_grad_kernel(const T* x, int64_t 
     dw[e] = db[e] = f4{0.f, 0.f, 0.f, 0.f};
   }
   const float per = 1.f / (float)dim;
-  for (int64_t base = (int64_t)blockIdx.x * kGroups; base < n; base += (int64_t)gridDim.x * kGroups) {
-    const int64_t row = base + group, at = min(row, n - 1);
-    const T *from = x + at * stride, *from_g = grad + at * grad_stride;
-    auto values = [&](int e) { return load_four(from + (e * R + lane) * 4, dim - (e * R + lane) * 4); };
+  const int64_t step = (int64_t)gridDim.x * kGroups;
+  int64_t row = (int64_t)blockIdx.x * kGroups + group;
+  // (a row ahead, as norm_kernel's, takes registers for which fewer waves run: 90 -> 104 us for 65,536 x 1,024 of 16 bits)
+  for (int64_t base = (int64_t)blockIdx.x * kGroups; base < n; base += step, row += step) {
+    Part<T, R, E> part, part_g;
+    part.load(x + min(row, n - 1) * stride, lane, dim);
+    part_g.load(grad + min(row, n - 1) * grad_stride, lane, dim);
     f4 v[E], g[E];
 #pragma unroll
-    for (int e = 0; e < E; e++) v[e] = values(e);
-#pragma unroll
-    for (int e = 0; e < E; e++) g[e] = load_four(from_g + (e * R + lane) * 4, dim - (e * R + lane) * 4);
+    for (int e = 0; e < E; e++) {
+      v[e] = part.values(e, lane, dim);
+      g[e] = part_g.values(e, lane, dim);
+    }
+    auto again = [&](int e) {
+      Part<T, R, E> same;
+      same.load(x + min(row, n - 1) * stride, lane, dim);
+      return same.values(e, lane, dim);
+    };
     float scale, sums[2];
-    const float rstd = centre<true>(values, v, g, w, lane, dim, eps, across, scale, sums);
+    const float rstd = centre<true>(again, v, g, w, lane, dim, eps, across, scale, sums);
     if (row >= n) continue;
     // x^ = d rstd; dx = scale rstd (h - c1 - x^ c2)
     const float c1 = sums[0] * per, c2 = sums[1] * per * rstd;
@@ -281,14 +336,14 @@ __global__ __launch_bounds__(THREADS) void norm_grad_kernel(const T* x, int64_t 
     }
   }
   if (!parts) return;
-  float* part = parts + (int64_t)blockIdx.x * 2 * pitch;
+  float* sums = parts + (int64_t)blockIdx.x * 2 * pitch;
 #pragma unroll
   for (int of = 0; of < 2; of++) {
     if constexpr (kGroups == 1) {
 #pragma unroll
       for (int e = 0; e < E; e++) {
         const int j = (e * R + lane) * 4;
-        if (j < dim) *reinterpret_cast<f4*>(part + of * pitch + j) = of ? db[e] : dw[e];
+        if (j < dim) *reinterpret_cast<f4*>(sums + of * pitch + j) = of ? db[e] : dw[e];
       }
     } else {
       if (of) __syncthreads();
@@ -299,7 +354,7 @@ __global__ __launch_bounds__(THREADS) void norm_grad_kernel(const T* x, int64_t 
         float s = 0.f;
 #pragma unroll
         for (int q = 0; q < kGroups; q++) s += columns[q * kWide + j];
-        part[of * pitch + j] = s;
+        sums[of * pitch + j] = s;
       }
     }
   }
@@ -325,10 +380,10 @@ __global__ __launch_bounds__(1024) void join_columns_kernel(const float* parts, 
   }
 }
 
-// ---- rows longer than 16,384 ---------------------------------------------------------
+// ---- long rows (kLong, kLongGrad) ----------------------------------------------------
 //
-// A workgroup per row, which is read again for each step (from the caches while it fits).
-// The gradient's columns take what they need of the rows from `Moments`.
+// A workgroup per row, which is read again for each step (from the caches while it fits).  The gradient
+// goes column by column then, with what it needs of the rows in `Moments`.
 
 struct Moments {
   float mean, rest, rstd, scale, c1, c2, none[2];
@@ -411,75 +466,90 @@ __global__ __launch_bounds__(1024) void long_moments_kernel(const T* x, int64_t 
   }
 }
 
-// 1,024 columns of every `slices`-th row.
+// 1,024 columns of every gridDim.y-th row: its gradient, and this part of the columns' sums.
 template <class T>
-__global__ __launch_bounds__(256) void long_columns_kernel(const T* x, int64_t n, int64_t dim, int64_t stride, const T* grad,
-                                                           int64_t grad_stride, const Moments* moments, int slices,
-                                                           float* parts, int pitch) {
+__global__ __launch_bounds__(256) void long_grad_kernel(const T* x, int64_t n, int64_t dim, int64_t stride, const T* grad,
+                                                        int64_t grad_stride, const void* weight, int param_type,
+                                                        const Moments* moments, T* dx, int64_t dx_stride, float* parts, int pitch) {
   const int64_t j = ((int64_t)blockIdx.x * 256 + threadIdx.x) * 4;
   if (j >= dim) return;
+  const f4 w = load_params(weight, param_type, j, dim, 1.f);
   f4 dw = {0.f, 0.f, 0.f, 0.f}, db = dw;
-  for (int64_t row = blockIdx.y; row < n; row += slices) {
+  for (int64_t row = blockIdx.y; row < n; row += gridDim.y) {
     const Moments r = moments[row];
     const f4 v = load_four(x + row * stride + j, dim - j), g = load_four(grad + row * grad_stride + j, dim - j);
+    f4 o;
 #pragma unroll
     for (int i = 0; i < 4; i++) {
-      dw[i] = __builtin_fmaf(g[i], (v[i] * r.scale - r.mean - r.rest) * r.rstd, dw[i]);
+      const float hat = (v[i] * r.scale - r.mean - r.rest) * r.rstd;
+      o[i] = __builtin_fmaf(-hat, r.c2, g[i] * w[i] - r.c1) * (r.rstd * r.scale);
+      dw[i] = __builtin_fmaf(g[i], hat, dw[i]);
       db[i] += g[i];
     }
+    if (dx) store_four(dx + row * dx_stride + j, dim - j, o);
   }
+  if (!parts) return;
   float* part = parts + (int64_t)blockIdx.y * 2 * pitch;
   *reinterpret_cast<f4*>(part + j) = dw;
   *reinterpret_cast<f4*>(part + pitch + j) = db;
 }
 
-template <class T>
-__global__ __launch_bounds__(256) void long_grad_kernel(const T* x, int64_t n, int64_t dim, int64_t stride, const T* grad,
-                                                        int64_t grad_stride, const void* weight, int param_type,
-                                                        const Moments* moments, T* dx, int64_t dx_stride) {
-  const int64_t j = ((int64_t)blockIdx.x * 256 + threadIdx.x) * 4;
-  if (j >= dim) return;
-  const f4 w = load_params(weight, param_type, j, dim, 1.f);
-  for (int64_t row = blockIdx.y; row < n; row += gridDim.y) {
-    const Moments r = moments[row];
-    const f4 v = load_four(x + row * stride + j, dim - j), h = load_four(grad + row * grad_stride + j, dim - j) * w;
-    f4 o;
-#pragma unroll
-    for (int i = 0; i < 4; i++) {
-      const float hat = (v[i] * r.scale - r.mean - r.rest) * r.rstd;
-      o[i] = __builtin_fmaf(-hat, r.c2, h[i] - r.c1) * (r.rstd * r.scale);
-    }
-    store_four(dx + row * dx_stride + j, dim - j, o);
-  }
-}
-
 // ---- host side -----------------------------------------------------------------------
 
-constexpr int64_t kLong = 16384;    // longer rows do not stay in a workgroup's registers
-constexpr int64_t kGradBlocks = 256;  // workgroups of the gradient, one per CU, and so parts of the columns' sums
+// Longer rows do not stay in a workgroup's registers; the gradient keeps five values for each of the forward pass's three.
+constexpr int64_t kLong = 16384, kLongGrad = 12288;
 
-// f(threads per row, vectors per thread) for rows of `dim`: the fewest of 3 or 4 vectors each in 4 to 64, 256 or 1,024
-// threads that hold it, so that a third of them at most (a half below 32 values, three quarters past 1,024 and 4,096)
-// stay empty.
-template <class F>
+// The gradient's workgroups for rows of r threads, and so parts of the columns' sums: as many as run at once, or for few
+// rows one per CU, since each part is written and read again.  Measured, us, with 256 of 512 threads and 768 of 256: 4,096 x
+// 768 of 16 bits 12.9, 17.5; 16,384 x 768 24, 27; 65,536 x 768 80, 72; 4,096 x 4,096 39, 39; 60,001 x 1,001 floats 167, 150.
+struct Grid {
+  int threads;
+  int64_t blocks;
+};
+constexpr Grid grad_grid(int64_t n, int r) {
+  const bool few = r <= 256 && n * r <= 64 * 32768;
+  const int threads = few || r > 256 ? 512 : 256;
+  const int64_t groups = threads / r;
+  return {threads, std::min<int64_t>((n + groups - 1) / groups, few ? 256 : r <= 256 ? 768 : 512)};
+}
+
+// f(threads per row, vectors per thread) for rows of `dim`, with one of the given numbers of vectors: the fewest places
+// for them (those past the row stay idle), the number named first if there are several; at most MOST threads.
+// Measured with 1 to 8 vectors: values of 16 bits take 12 to 35 % more with one or two of them, 10 % more with six or eight,
+// floats 10 and 20 % (fewer bytes on their way for each wave, or fewer waves).
+template <int MOST, int FIRST, int... MORE, class F>
 void by_width(int64_t dim, F f) {
-  auto threads = [&](auto vectors) {
-    using E = decltype(vectors);
-    const int64_t least = (dim + 4 * E::value - 1) / (4 * E::value);
-    if (least <= 4) f(std::integral_constant<int, 4>(), E());
-    else if (least <= 8) f(std::integral_constant<int, 8>(), E());
-    else if (least <= 16) f(std::integral_constant<int, 16>(), E());
-    else if (least <= 32) f(std::integral_constant<int, 32>(), E());
-    else if (least <= 64) f(std::integral_constant<int, 64>(), E());
-    else if (least <= 256) f(std::integral_constant<int, 256>(), E());
-    else f(std::integral_constant<int, 1024>(), E());
+  auto threads = [&](int64_t vectors) {
+    int64_t r = 4;
+    while (r * 4 * vectors < dim) r *= 2;
+    return r;
   };
-  int64_t three = 4;
-  while (three * 12 < dim) three *= three < 64 ? 2 : 4;
-  int64_t four = 4;
-  while (four * 16 < dim) four *= four < 64 ? 2 : 4;
-  if (three <= four) threads(std::integral_constant<int, 3>());
-  else threads(std::integral_constant<int, 4>());
+  int best = FIRST;
+  ((best = threads(MORE) <= MOST && (threads(best) > MOST || threads(MORE) * MORE < threads(best) * best) ? MORE : best), ...);
+  const int64_t r = threads(best);
+  auto go = [&](auto vectors) {
+    using E = decltype(vectors);
+    if (E::value != best) return;
+    if (r == 4) f(std::integral_constant<int, 4>(), E());
+    else if (r == 8) f(std::integral_constant<int, 8>(), E());
+    else if (r == 16) f(std::integral_constant<int, 16>(), E());
+    else if (r == 32) f(std::integral_constant<int, 32>(), E());
+    else if (r == 64) f(std::integral_constant<int, 64>(), E());
+    else if (r == 128) f(std::integral_constant<int, 128>(), E());
+    else if (r == 256) f(std::integral_constant<int, 256>(), E());
+    else if (r == 512) f(std::integral_constant<int, 512>(), E());
+    else if constexpr (MOST == 1024) f(std::integral_constant<int, 1024>(), E());
+  };
+  go(std::integral_constant<int, FIRST>());
+  (go(std::integral_constant<int, MORE>()), ...);
+}
+
+// The same for the gradient.  Past 8,192 six vectors: 1,024 threads would not have the registers (5,000 x 12,288 of 16 bits:
+// 126 us, with 1,024 threads 185, as long rows 246).
+template <class F>
+void by_grad_width(int64_t dim, F f) {
+  if (dim > 8192) f(std::integral_constant<int, 512>(), std::integral_constant<int, 6>());
+  else by_width<512, 4, 3>(dim, f);
 }
 
 int pitch_of(int64_t dim) { return (int)((dim + 3) / 4 * 4); }
@@ -488,8 +558,10 @@ int64_t long_slices(int64_t n, int64_t dim) { return std::min<int64_t>(n, std::m
 
 int64_t workspace_bytes(int64_t n, int64_t dim) {
   if (n == 0 || dim == 0) return 0;
-  if (dim > kLong) return n * (int64_t)sizeof(Moments) + long_slices(n, dim) * 2 * pitch_of(dim) * 4;
-  return std::min(n, kGradBlocks) * 2 * pitch_of(dim) * 4;
+  if (dim > kLongGrad) return n * (int64_t)sizeof(Moments) + long_slices(n, dim) * 2 * pitch_of(dim) * 4;
+  int64_t blocks = 0;
+  by_grad_width(dim, [&](auto threads, auto) { blocks = grad_grid(n, decltype(threads)::value).blocks; });
+  return blocks * 2 * pitch_of(dim) * 4;
 }
 
 template <class T>
@@ -501,12 +573,16 @@ void norm(const void* x, int64_t n, int64_t dim, int64_t stride, const void* wei
     hipLaunchKernelGGL(norm_long_kernel<T>, dim3((unsigned)std::min<int64_t>(n, 1 << 20)), dim3(1024), 0, st, in, n, dim,
                        stride, weight, bias, param_type, eps, out, y_stride);
   } else {
-    by_width(dim, [&](auto threads, auto vectors) {
+    auto go = [&](auto threads, auto vectors) {
       constexpr int R = decltype(threads)::value, E = decltype(vectors)::value, T0 = R > 256 ? R : 256;
       const int64_t blocks = std::min<int64_t>((n + T0 / R - 1) / (T0 / R), 256 * 2048 / T0);
       hipLaunchKernelGGL((norm_kernel<T, R, E, T0>), dim3((unsigned)blocks), dim3(T0), 0, st, in, n, (int)dim, stride, weight,
                          bias, param_type, eps, out, y_stride);
-    });
+    };
+    // Short rows of floats that are no whole lines: one vector per thread where that takes no more of them (500,000 x 100:
+    // 90 us, with four vectors 117, 300,000 x 200: 108, 115; whole lines the other way: 500,000 x 128: 106, 99).
+    if (sizeof(T) == 4 && dim <= 256 && dim % 32) by_width<1024, 1, 3, 4>(dim, go);
+    else by_width<1024, 3, 4>(dim, go);
   }
   HIP_OK(hipGetLastError());
 }
@@ -521,26 +597,29 @@ void norm_grad(const void* x, int64_t n, int64_t dim, int64_t stride, const void
   const bool columns = dweight || dbias;
   float* parts = static_cast<float*>(workspace);
   int64_t count = 0;
-  if (n > 0 && dim > kLong) {
+  if (n > 0 && dim > kLongGrad) {
     Moments* moments = static_cast<Moments*>(workspace);
     parts = reinterpret_cast<float*>(moments + n);
     count = long_slices(n, dim);
     const unsigned wide = (unsigned)((dim + 1023) / 1024);
     hipLaunchKernelGGL(long_moments_kernel<T>, dim3((unsigned)std::min<int64_t>(n, 1 << 20)), dim3(1024), 0, st, in, n, dim,
                        stride, g, grad_stride, weight, param_type, eps, moments);
-    if (columns)
-      hipLaunchKernelGGL(long_columns_kernel<T>, dim3(wide, (unsigned)count), dim3(256), 0, st, in, n, dim, stride, g,
-                         grad_stride, moments, (int)count, parts, pitch);
-    if (dx)
-      hipLaunchKernelGGL(long_grad_kernel<T>, dim3(wide, (unsigned)std::min<int64_t>(n, 1024)), dim3(256), 0, st, in, n, dim,
-                         stride, g, grad_stride, weight, param_type, moments, out, dx_stride);
+    hipLaunchKernelGGL(long_grad_kernel<T>, dim3(wide, (unsigned)count), dim3(256), 0, st, in, n, dim, stride, g, grad_stride,
+                       weight, param_type, moments, out, dx_stride, columns ? parts : nullptr, pitch);
   } else if (n > 0) {
-    by_width(dim, [&](auto threads, auto vectors) {
-      constexpr int R = decltype(threads)::value, E = decltype(vectors)::value, T0 = 1024;
-      count = std::min((n + T0 / R - 1) / (T0 / R), kGradBlocks);
-      hipLaunchKernelGGL((norm_grad_kernel<T, R, E, T0>), dim3((unsigned)count), dim3(T0), 0, st, in, n, (int)dim, stride, g,
-                         grad_stride, weight, param_type, eps, out, dx_stride, columns ? parts : nullptr, pitch);
-    });
+    auto go = [&](auto threads, auto vectors) {
+      constexpr int R = decltype(threads)::value, E = decltype(vectors)::value;
+      const Grid grid = grad_grid(n, R);
+      count = grid.blocks;
+      auto launch = [&](auto workgroup) {
+        constexpr int T0 = decltype(workgroup)::value;
+        hipLaunchKernelGGL((norm_grad_kernel<T, R, E, T0>), dim3((unsigned)count), dim3(T0), 0, st, in, n, (int)dim, stride,
+                           g, grad_stride, weight, param_type, eps, out, dx_stride, columns ? parts : nullptr, pitch);
+      };
+      if (R > 256 || grid.threads == 512) launch(std::integral_constant<int, 512>());
+      else if constexpr (R <= 256) launch(std::integral_constant<int, 256>());
+    };
+    by_grad_width(dim, go);
   }
   HIP_OK(hipGetLastError());
   if (columns) {
