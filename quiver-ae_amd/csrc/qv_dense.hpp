@@ -87,6 +87,28 @@ __device__ __forceinline__ void load_tail(const T* p, int64_t valid, float other
   }
 }
 
+// Results of more than the L2s hold together are written past them where they are whole lines.  4-bit products, us,
+// without and with: 10,000 x 50,001 x 128 to bfloat16 264, 218; 10,000 x 50,048 x 1,024 466, 399; 4,096^3 44, 42; 3,000 x
+// 50,001 x 128 78, 69, and 147, 135 with the log probabilities of the result behind it.  Into memory that the last cache
+// (256 MB) does not hold either: 500 x 50,001 x 100 to float16 23.0, 18.1; 1,000 x 50,001 x 100 37.7, 28.1.  Into the same
+// memory again and again: 18.4, 17.9; 25.7, 28.0, and 56, 61 with its log probabilities; worst, 256 x 200,000 x 128 to float:
+// 37, 44 and 76, 93.  Lines in parts take twice the time that way (4,000 x 50,001 x 512 by tiles: 168, 336).  Rows written
+// one after the other: 4-bit values of 1M x 128 to float 105, 81, 1M x 100 115, 71; layer norm of 200,000 x 384 of 16 bits
+// 61, 57, of 60,001 x 1,001 floats 102, 88, and the gradient 150, 144.
+constexpr int64_t kStreamBytes = 32 << 20;
+
+// One store, past the L2 or not.  (The empty assembly keeps the two apart: they would become one ordinary store.)
+template <class V, class P>
+__device__ __forceinline__ void store_past(V v, P* to, bool stream) {
+  if (stream) {
+    asm volatile("" ::: "memory");
+    __builtin_nontemporal_store(v, to);
+    asm volatile("" ::: "memory");
+  } else {
+    *to = v;
+  }
+}
+
 // A launch holds less than 2^32 threads.  f(first, count) launches workgroups first, first + 1, ... of them.
 template <class F>
 void in_launches(int64_t workgroups, int threads, F f) {

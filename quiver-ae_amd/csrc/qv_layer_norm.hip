@@ -49,13 +49,16 @@ __device__ __forceinline__ f4 load_four(const T* p, int64_t valid) {
   return v;
 }
 
+// ... and back, past the L2 if there is more than it holds (kStreamBytes).
 template <class T>
-__device__ __forceinline__ void store_four(T* p, int64_t valid, f4 v) {
+__device__ __forceinline__ void store_four(T* p, int64_t valid, f4 v, bool stream) {
   T t[4];
 #pragma unroll
   for (int i = 0; i < 4; i++) t[i] = (T)v[i];
   if (valid >= 4) {
-    __builtin_memcpy(p, t, 4 * sizeof(T));
+    typedef uint32_t raw __attribute__((ext_vector_type(sizeof(T))));
+    typedef raw raw_any __attribute__((aligned(sizeof(T)), may_alias));
+    store_past(__builtin_bit_cast(raw, t), reinterpret_cast<raw_any*>(p), stream);
   } else {
 #pragma unroll
     for (int i = 0; i < 3; i++)
@@ -240,7 +243,8 @@ __device__ __forceinline__ float centre(F values, f4 (&v)[E], const f4 (&g)[E], 
 
 template <class T, int R, int E, int THREADS>
 __global__ __launch_bounds__(THREADS) void norm_kernel(const T* x, int64_t n, int dim, int64_t stride, const void* weight,
-                                                       const void* bias, int param_type, float eps, T* y, int64_t y_stride) {
+                                                       const void* bias, int param_type, float eps, T* y, int64_t y_stride,
+                                                       bool stream) {
   constexpr int kGroups = THREADS / R;
   __shared__ float lds[Row<R, THREADS>::kFloats];
   Row<R, THREADS> across{lds};
@@ -275,7 +279,7 @@ __global__ __launch_bounds__(THREADS) void norm_kernel(const T* x, int64_t n, in
       f4 o;
 #pragma unroll
       for (int i = 0; i < 4; i++) o[i] = __builtin_fmaf(v[e][i] * rstd, w[e][i], b[e][i]);
-      store_four(y + row * y_stride + j, dim - j, o);
+      store_four(y + row * y_stride + j, dim - j, o, stream);
     }
   }
 }
@@ -284,7 +288,8 @@ __global__ __launch_bounds__(THREADS) void norm_kernel(const T* x, int64_t n, in
 template <class T, int R, int E, int THREADS>
 __global__ __launch_bounds__(THREADS) void norm_grad_kernel(const T* x, int64_t n, int dim, int64_t stride, const T* grad,
                                                             int64_t grad_stride, const void* weight, int param_type,
-                                                            float eps, T* dx, int64_t dx_stride, float* parts, int pitch) {
+                                                            float eps, T* dx, int64_t dx_stride, float* parts, int pitch,
+                                                            bool stream) {
   constexpr int kGroups = THREADS / R;
   constexpr int kWide = R * E * 4;
   __shared__ float lds[Row<R, THREADS>::kFloats];
@@ -332,7 +337,7 @@ __global__ __launch_bounds__(THREADS) void norm_grad_kernel(const T* x, int64_t 
         dw[e][i] = __builtin_fmaf(g[e][i], hat, dw[e][i]);
         db[e][i] += g[e][i];
       }
-      if (dx) store_four(dx + row * dx_stride + j, dim - j, o);
+      if (dx) store_four(dx + row * dx_stride + j, dim - j, o, stream);
     }
   }
   if (!parts) return;
@@ -437,7 +442,8 @@ __device__ __forceinline__ Moments long_moments(const T* x, const T* g, const vo
 
 template <class T>
 __global__ __launch_bounds__(1024) void norm_long_kernel(const T* x, int64_t n, int64_t dim, int64_t stride, const void* weight,
-                                                         const void* bias, int param_type, float eps, T* y, int64_t y_stride) {
+                                                         const void* bias, int param_type, float eps, T* y, int64_t y_stride,
+                                                       bool stream) {
   __shared__ float lds[Row<1024, 1024>::kFloats];
   Row<1024, 1024> across{lds};
   for (int64_t row = blockIdx.x; row < n; row += gridDim.x) {
@@ -449,7 +455,7 @@ __global__ __launch_bounds__(1024) void norm_long_kernel(const T* x, int64_t n, 
       f4 o;
 #pragma unroll
       for (int i = 0; i < 4; i++) o[i] = __builtin_fmaf((v[i] * r.scale - r.mean - r.rest) * r.rstd, w[i], b[i]);
-      store_four(y + row * y_stride + j, dim - j, o);
+      store_four(y + row * y_stride + j, dim - j, o, stream);
     }
   }
 }
@@ -470,7 +476,8 @@ __global__ __launch_bounds__(1024) void long_moments_kernel(const T* x, int64_t 
 template <class T>
 __global__ __launch_bounds__(256) void long_grad_kernel(const T* x, int64_t n, int64_t dim, int64_t stride, const T* grad,
                                                         int64_t grad_stride, const void* weight, int param_type,
-                                                        const Moments* moments, T* dx, int64_t dx_stride, float* parts, int pitch) {
+                                                        const Moments* moments, T* dx, int64_t dx_stride, float* parts, int pitch,
+                                                        bool stream) {
   const int64_t j = ((int64_t)blockIdx.x * 256 + threadIdx.x) * 4;
   if (j >= dim) return;
   const f4 w = load_params(weight, param_type, j, dim, 1.f);
@@ -486,7 +493,7 @@ __global__ __launch_bounds__(256) void long_grad_kernel(const T* x, int64_t n, i
       dw[i] = __builtin_fmaf(g[i], hat, dw[i]);
       db[i] += g[i];
     }
-    if (dx) store_four(dx + row * dx_stride + j, dim - j, o);
+    if (dx) store_four(dx + row * dx_stride + j, dim - j, o, stream);
   }
   if (!parts) return;
   float* part = parts + (int64_t)blockIdx.y * 2 * pitch;
@@ -569,15 +576,16 @@ void norm(const void* x, int64_t n, int64_t dim, int64_t stride, const void* wei
           float eps, void* y, int64_t y_stride, hipStream_t st) {
   const T* in = static_cast<const T*>(x);
   T* out = static_cast<T*>(y);
+  const bool stream = n * dim * (int64_t)sizeof(T) >= kStreamBytes;
   if (dim > kLong) {
     hipLaunchKernelGGL(norm_long_kernel<T>, dim3((unsigned)std::min<int64_t>(n, 1 << 20)), dim3(1024), 0, st, in, n, dim,
-                       stride, weight, bias, param_type, eps, out, y_stride);
+                       stride, weight, bias, param_type, eps, out, y_stride, stream);
   } else {
     auto go = [&](auto threads, auto vectors) {
       constexpr int R = decltype(threads)::value, E = decltype(vectors)::value, T0 = R > 256 ? R : 256;
       const int64_t blocks = std::min<int64_t>((n + T0 / R - 1) / (T0 / R), 256 * 2048 / T0);
       hipLaunchKernelGGL((norm_kernel<T, R, E, T0>), dim3((unsigned)blocks), dim3(T0), 0, st, in, n, (int)dim, stride, weight,
-                         bias, param_type, eps, out, y_stride);
+                         bias, param_type, eps, out, y_stride, stream);
     };
     // Short rows of floats that are no whole lines: one vector per thread where that takes no more of them (500,000 x 100:
     // 90 us, with four vectors 117, 300,000 x 200: 108, 115; whole lines the other way: 500,000 x 128: 106, 99).
@@ -593,6 +601,7 @@ void norm_grad(const void* x, int64_t n, int64_t dim, int64_t stride, const void
                void* workspace, hipStream_t st) {
   const T *in = static_cast<const T*>(x), *g = static_cast<const T*>(grad);
   T* out = static_cast<T*>(dx);
+  const bool stream = n * dim * (int64_t)sizeof(T) >= kStreamBytes;
   const int pitch = pitch_of(dim);
   const bool columns = dweight || dbias;
   float* parts = static_cast<float*>(workspace);
@@ -605,7 +614,7 @@ void norm_grad(const void* x, int64_t n, int64_t dim, int64_t stride, const void
     hipLaunchKernelGGL(long_moments_kernel<T>, dim3((unsigned)std::min<int64_t>(n, 1 << 20)), dim3(1024), 0, st, in, n, dim,
                        stride, g, grad_stride, weight, param_type, eps, moments);
     hipLaunchKernelGGL(long_grad_kernel<T>, dim3(wide, (unsigned)count), dim3(256), 0, st, in, n, dim, stride, g, grad_stride,
-                       weight, param_type, moments, out, dx_stride, columns ? parts : nullptr, pitch);
+                       weight, param_type, moments, out, dx_stride, columns ? parts : nullptr, pitch, stream);
   } else if (n > 0) {
     auto go = [&](auto threads, auto vectors) {
       constexpr int R = decltype(threads)::value, E = decltype(vectors)::value;
@@ -614,7 +623,7 @@ void norm_grad(const void* x, int64_t n, int64_t dim, int64_t stride, const void
       auto launch = [&](auto workgroup) {
         constexpr int T0 = decltype(workgroup)::value;
         hipLaunchKernelGGL((norm_grad_kernel<T, R, E, T0>), dim3((unsigned)count), dim3(T0), 0, st, in, n, (int)dim, stride,
-                           g, grad_stride, weight, param_type, eps, out, dx_stride, columns ? parts : nullptr, pitch);
+                           g, grad_stride, weight, param_type, eps, out, dx_stride, columns ? parts : nullptr, pitch, stream);
       };
       if (R > 256 || grid.threads == 512) launch(std::integral_constant<int, 512>());
       else if constexpr (R <= 256) launch(std::integral_constant<int, 256>());

@@ -105,7 +105,7 @@ template <class T, int R>
 __global__ __launch_bounds__(256) void from_mx4_kernel(const uint8_t* __restrict__ codes, int64_t blocks, int64_t dim,
                                                        int64_t code_stride, const uint8_t* __restrict__ scales,
                                                        int64_t scale_stride, T* __restrict__ out, int64_t stride,
-                                                       uint32_t per_row, uint32_t magic, int64_t first_group) {
+                                                       uint32_t per_row, uint32_t magic, int64_t first_group, bool stream) {
   constexpr int V = kVec<T>, kLanes = kBlock / V, kBlocks = 256 / kLanes;  // values of a lane, lanes of a block
   const int part = threadIdx.x % kLanes, number = threadIdx.x / kLanes;
   const int64_t first = (first_group + blockIdx.x) * (kBlocks * R);
@@ -150,7 +150,7 @@ __global__ __launch_bounds__(256) void from_mx4_kernel(const uint8_t* __restrict
     const int64_t j = (int64_t)block[r] * kBlock + part * V;
     T* to = out + row[r] * stride + j;
     if (j + V <= dim) {
-      *reinterpret_cast<raw4_any*>(to) = u.raw;
+      store_past(u.raw, reinterpret_cast<raw4_any*>(to), stream);
     } else {
 #pragma unroll
       for (int i = 0; i < V; i++)
@@ -906,7 +906,8 @@ void from_mx4(const uint8_t* codes, int64_t n, int64_t dim, int64_t code_stride,
   constexpr int R = 4;
   in_runs(n, dim, 8 * kVec<T> * R, [&](int64_t blocks, uint32_t per_row, uint32_t magic, int64_t first, unsigned count) {
     hipLaunchKernelGGL((from_mx4_kernel<T, R>), dim3(count), dim3(256), 0, st, codes, blocks, dim, code_stride, scales,
-                       scale_stride, static_cast<T*>(out), stride, per_row, magic, first);
+                       scale_stride, static_cast<T*>(out), stride, per_row, magic, first,
+                       n * dim * (int64_t)sizeof(T) >= kStreamBytes);
   });
 }
 

@@ -63,14 +63,6 @@ __device__ __forceinline__ void swap_pieces(i4 (&u)[P]) {
   if constexpr (P == 4) stage(std::integral_constant<int, 2>(), std::integral_constant<int, 0x4E>());  // quad_perm [2,3,0,1]
 }
 
-// Results of more than the L2s hold together are written past them where they are whole lines.  4-bit products, us,
-// without and with: 10,000 x 50,001 x 128 to bfloat16 264, 218; 10,000 x 50,048 x 1,024 466, 399; 4,096^3 44, 42; 3,000 x
-// 50,001 x 128 78, 69, and 147, 135 with the log probabilities of the result behind it.  Into memory that the last cache
-// (256 MB) does not hold either: 500 x 50,001 x 100 to float16 23.0, 18.1; 1,000 x 50,001 x 100 37.7, 28.1.  Into the same
-// memory again and again: 18.4, 17.9; 25.7, 28.0, and 56, 61 with its log probabilities; worst, 256 x 200,000 x 128 to float:
-// 37, 44 and 76, 93.  Lines in parts take twice the time that way (4,000 x 50,001 x 512 by tiles: 168, 336).
-constexpr int64_t kStreamBytes = 32 << 20;
-
 // Stores the results of R instructions from the registers: 32 R columns from j of the rows around the lane's row i,
 // whole lines of 8 rows at once (half lines of 16 rows with 32 columns of 16 bits).  Of the four columns that a lane
 // has of every eight, those of 16 bits pass to the other half of the wave and back, eight for a lane; then groups of
@@ -199,17 +191,11 @@ struct LineRing {
       i4 u[G];
 #pragma unroll
       for (int g = 0; g < G; g++) u[g] = *reinterpret_cast<const i4*>(from + (8 * g + lane / 8) * kRing);
-      if (stream) {
-        asm volatile("" ::: "memory");  // on both sides: else the two ways become one of ordinary stores
 #pragma unroll
-        for (int g = 0; g < G; g++) __builtin_nontemporal_store(u[g], reinterpret_cast<i4*>(line_to[g]));
-        asm volatile("" ::: "memory");
-      } else {
-#pragma unroll
-        for (int g = 0; g < G; g++) *reinterpret_cast<i4*>(line_to[g]) = u[g];
+      for (int g = 0; g < G; g++) {
+        store_past(u[g], reinterpret_cast<i4*>(line_to[g]), stream);
+        line_to[g] += step;
       }
-#pragma unroll
-      for (int g = 0; g < G; g++) line_to[g] += step;
       return;
     }
 #pragma unroll
