@@ -475,30 +475,34 @@ def log_probs_grad(logits: torch.Tensor, result: LogProbs, targets: torch.Tensor
                      targets, grad_target, grad_entropy, grad_logsumexp, grad_top, out)
 
 
-def _params(dim: int, weight: torch.Tensor | None, bias: torch.Tensor | None):
-    """The type of weight and bias, and their addresses."""
-    dtype = torch.float32
-    for name, p in (("weight", weight), ("bias", bias)):
-        if p is not None:
-            dtype = p.dtype
-            if dtype not in _TYPES:
-                raise ValueError(f"{name} has the type {dtype}; " + " or ".join(str(x) for x in _TYPES) + " is needed")
-    at_weight = None if weight is None else _vector("weight", weight, (dim,), dtype)
-    return dtype, at_weight, None if bias is None else _vector("bias", bias, (dim,), dtype)
+def _param(name: str, p: torch.Tensor, dim: int, dtype: torch.dtype | None) -> int:
+    """The address of a weight or bias, of ``dtype`` if that is known already."""
+    if p.dtype not in _TYPES:
+        raise ValueError(f"{name} has the type {p.dtype}; " + " or ".join(str(x) for x in _TYPES) + " is needed")
+    return _vector(name, p, (dim,), p.dtype if dtype is None else dtype)
 
 
 def _norm(x, weight, bias, eps, out):
     n, d, stride = _matrix("x", x, _TYPES)
-    dtype, at_weight, at_bias = _params(d, weight, bias)
+    dtype = at_weight = at_bias = None
+    if bias is not None:
+        dtype, at_bias = bias.dtype, _param("bias", bias, d, None)
+    if weight is not None:
+        dtype, at_weight = weight.dtype if dtype is None else dtype, _param("weight", weight, d, dtype)
     again = out is not None
     if not again:
-        out = torch.empty((n, d), dtype=x.dtype, device=x.device)
-    rows, cols, out_stride = _matrix("out", out, (x.dtype,))
-    if rows != n or cols != d:
-        raise ValueError("out and x differ in shape")
-    device = _device(*(t for t in (x, out, weight, bias) if t is not None))
-    _lib.check(_lib.load().qv_layer_norm(x.data_ptr(), _TYPES[x.dtype], n, d, stride, at_weight, at_bias, _TYPES[dtype],
-                                         eps, out.data_ptr(), out_stride, device, _raw_stream(device)))
+        out, out_stride = torch.empty((n, d), dtype=x.dtype, device=x.device), max(d, 1)
+    else:
+        rows, cols, out_stride = _matrix("out", out, (x.dtype,))
+        if rows != n or cols != d:
+            raise ValueError("out and x differ in shape")
+    if weight is None:
+        device = _device(x, out) if bias is None else _device(x, out, bias)
+    else:
+        device = _device(x, out, weight) if bias is None else _device(x, out, weight, bias)
+    _lib.check(_lib.load().qv_layer_norm(x.data_ptr(), _TYPES[x.dtype], n, d, stride, at_weight, at_bias,
+                                         _lib.QV_FLOAT if dtype is None else _TYPES[dtype], eps, out.data_ptr(), out_stride,
+                                         device, _raw_stream(device)))
     if again:
         _written((out,))
     return out
@@ -512,7 +516,42 @@ class LayerNormGrad:
     weight: torch.Tensor | None  # [d] of the weight's type
     bias: torch.Tensor | None    # [d] of the weight's type
     _workspace: torch.Tensor
-    _size: tuple                 # rows and columns that it was made for
+    _written: tuple              # the first three that are there
+    _made_for: tuple             # rows, columns, types of x and weight
+    _at: tuple                   # addresses of the first three (and x's row stride), the workspace and its bytes
+    _device: int
+
+    @staticmethod
+    def empty(n: int, d: int, dtype: torch.dtype, param_dtype: torch.dtype, wanted: tuple, device) -> "LayerNormGrad":
+        """Buffers for the gradients that are wanted, of n rows of d values."""
+        workspace = _lib.load().qv_layer_norm_grad_workspace(n, d)
+        if workspace < 0:
+            _lib.check(workspace)
+
+        def new(want, shape, type_):
+            return torch.empty(shape, dtype=type_, device=device) if want else None
+
+        return LayerNormGrad.of(new(wanted[0], (n, d), dtype), new(wanted[1], d, param_dtype), new(wanted[2], d, param_dtype),
+                                torch.empty(workspace, dtype=torch.uint8, device=device), (n, d, dtype, param_dtype))
+
+    @staticmethod
+    def of(x, weight, bias, workspace, made_for: tuple) -> "LayerNormGrad":
+        """Given buffers for ``made_for``: rows, columns, types of x and weight."""
+        n, d, dtype, param_dtype = made_for
+        at_x, stride = None, d
+        if x is not None:
+            rows, cols, stride = _matrix("out.x", x, (dtype,))
+            if rows != n or cols != d:
+                raise ValueError("out.x has another number of rows or columns")
+            at_x = x.data_ptr()
+        at_weight, at_bias = (None if p is None else _vector(name, p, (d,), param_dtype)
+                              for name, p in (("out.weight", weight), ("out.bias", bias)))
+        written = tuple(t for t in (x, weight, bias) if t is not None)
+        device = workspace.get_device()
+        if any(t.get_device() != device for t in written):
+            raise ValueError("tensors must be on one GPU")
+        return LayerNormGrad(x, weight, bias, workspace, written, made_for,
+                             (at_x, stride, at_weight, at_bias, workspace.data_ptr(), workspace.shape[0]), device)
 
 
 def _norm_grad(x, grad, weight, eps, dtype, wanted, out) -> LayerNormGrad:
@@ -520,34 +559,19 @@ def _norm_grad(x, grad, weight, eps, dtype, wanted, out) -> LayerNormGrad:
     grad_rows, grad_cols, grad_stride = _matrix("grad", grad, (x.dtype,))
     if grad_rows != n or grad_cols != d:
         raise ValueError("grad and x differ in shape")
-    at_weight = _params(d, weight, None)[1]
+    at_weight = None if weight is None else _param("weight", weight, d, None)
     again = out is not None
+    if again and out._made_for != (n, d, x.dtype, dtype):
+        raise ValueError("out was made for another number of rows or columns, or other types")
+    device = _device(x, grad) if weight is None else _device(x, grad, weight)
     if not again:
-        workspace = _lib.load().qv_layer_norm_grad_workspace(n, d)
-        if workspace < 0:
-            _lib.check(workspace)
-
-        def new(want, shape, type_):
-            return torch.empty(shape, dtype=type_, device=x.device) if want else None
-
-        out = LayerNormGrad(new(wanted[0], (n, d), x.dtype), new(wanted[1], d, dtype), new(wanted[2], d, dtype),
-                            torch.empty(workspace, dtype=torch.uint8, device=x.device), (n, d))
-    elif out._size != (n, d):
-        raise ValueError("out was made for another number of rows or columns")
-    at_x, out_stride = None, d
-    if out.x is not None:
-        out_rows, out_cols, out_stride = _matrix("out.x", out.x, (x.dtype,))
-        if out_rows != n or out_cols != d:
-            raise ValueError("out.x and x differ in shape")
-        at_x = out.x.data_ptr()
-    at = [None if p is None else _vector(name, p, (d,), dtype) for name, p in (("out.weight", out.weight), ("out.bias", out.bias))]
-    device = _device(*(t for t in (x, grad, weight, out.x, out.weight, out.bias, out._workspace) if t is not None))
+        out = LayerNormGrad.empty(n, d, x.dtype, dtype, wanted, x.device)
+    elif out._device != device:
+        raise ValueError("tensors must be on one GPU")
     _lib.check(_lib.load().qv_layer_norm_grad(x.data_ptr(), _TYPES[x.dtype], n, d, stride, grad.data_ptr(), grad_stride,
-                                              at_weight, _TYPES[dtype], eps, at_x, out_stride, *at,
-                                              out._workspace.data_ptr(), out._workspace.shape[0], device,
-                                              _raw_stream(device)))
+                                              at_weight, _TYPES[dtype], eps, *out._at, device, _raw_stream(device)))
     if again:
-        _written([t for t in (out.x, out.weight, out.bias) if t is not None])
+        _written(out._written)
     return out
 
 
@@ -596,8 +620,8 @@ def layer_norm(x: torch.Tensor, weight: torch.Tensor | None = None, bias: torch.
     result takes part in autograd (``out`` is then refused), once: the gradient
     has none of its own, and there is no forward-mode derivative.
     """
-    if torch.is_grad_enabled() and (x.requires_grad or weight is not None and weight.requires_grad
-                                    or bias is not None and bias.requires_grad):
+    if (x.requires_grad or weight is not None and weight.requires_grad
+            or bias is not None and bias.requires_grad) and torch.is_grad_enabled():
         if out is not None:
             raise ValueError("out= cannot be given for arguments that require a gradient")
         if _has_tangent(x, weight, bias):
@@ -619,13 +643,13 @@ def layer_norm_grad(x: torch.Tensor, grad: torch.Tensor, weight: torch.Tensor | 
     without it (so arguments that require a gradient come detached, or under
     ``torch.no_grad()``).
     """
-    outs = () if out is None else (out.x, out.weight, out.bias)
+    again = out is not None
     if (x.requires_grad or grad.requires_grad or weight is not None and weight.requires_grad
-            or any(t is not None and t.requires_grad for t in outs) or forward_ad._current_level >= 0):
-        _no_derivative("layer_norm_grad", x, grad, weight, *outs)
+            or forward_ad._current_level >= 0 or again and any([t.requires_grad for t in out._written])):
+        _no_derivative("layer_norm_grad", x, grad, weight, *(out._written if again else ()))
     if wanted is None:
         wanted = (True, True, True)
-    elif out is not None:
+    elif again:
         raise ValueError("wanted cannot be given beside out=, which has what is wanted")
     return _norm_grad(x, grad, weight, eps, torch.float32 if weight is None else weight.dtype, wanted, out)
 

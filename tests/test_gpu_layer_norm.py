@@ -10,6 +10,8 @@ n / 256 + 400 additions at most (rows of a workgroup, their parts).  Types round
 """
 from __future__ import annotations
 
+from dataclasses import replace
+
 import pytest
 import torch
 
@@ -181,7 +183,7 @@ def test_huge_rows(scoring, dtype, n, d):
     # 1 / s may be subnormal (down to 2^-128): its product rounds to 2^-149
     _within(r.x, dx, (4 * _additions(d) + 40) * U * parts + 2.0 ** -148 * (1 + parts / rstd), "dx")
     assert torch.isfinite(r.weight).all()
-    _check_grad(type(r)(None, r.weight, r.bias, None, None), x, grad, weight, torch.float32)
+    _check_grad(replace(r, x=None), x, grad, weight, torch.float32)
 
 
 @pytest.mark.parametrize("eps", [2.0 ** -126, 1e-12, 1e-3, 10.0, 1e30])
@@ -211,7 +213,7 @@ def test_strides(scoring, dtype, off):
         assert (store[:, :off] == 7).all() and (store[:, off + d:] == 7).all()
         store.fill_(7.0)
         r = scoring.layer_norm_grad(x, grad, weight)
-        again = type(r)(store[:, off:off + d], r.weight, r.bias, r._workspace, r._size)
+        again = type(r).of(store[:, off:off + d], r.weight, r.bias, r._workspace, r._made_for)
         first = r.x.clone(), r.weight.clone(), r.bias.clone()
         scoring.layer_norm_grad(x, grad, weight, out=again)
         _check_grad(again, x, grad, weight, torch.float32)
@@ -228,7 +230,7 @@ def test_in_place(scoring, n, d):
     for place in ("x", "grad"):
         a, b = x.clone(), grad.clone()
         target = a if place == "x" else b
-        out = type(r)(target, torch.empty_like(r.weight), torch.empty_like(r.bias), r._workspace, r._size)
+        out = type(r).of(target, torch.empty_like(r.weight), torch.empty_like(r.bias), r._workspace, r._made_for)
         scoring.layer_norm_grad(a, b, weight, out=out)
         assert torch.equal(target, r.x) and torch.equal(out.weight, r.weight) and torch.equal(out.bias, r.bias)
     assert torch.equal(scoring.layer_norm(x, weight, bias, out=x), y)
@@ -255,7 +257,7 @@ def test_far_rows(scoring):
     y, r = scoring.layer_norm(x, weight, bias), scoring.layer_norm_grad(x, grad, weight)
     for lo in (0, n // 2, n - 100):
         _check_forward(y[lo:lo + 100], x[lo:lo + 100], weight, bias)
-        part = type(r)(r.x[lo:lo + 100], None, None, None, None)
+        part = replace(r, x=r.x[lo:lo + 100], weight=None, bias=None)
         _check_grad(part, x[lo:lo + 100], grad[lo:lo + 100], weight, torch.float32)
     del y
     sums = torch.zeros(d, dtype=torch.float64, device="cuda")

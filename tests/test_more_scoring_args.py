@@ -96,7 +96,9 @@ def test_python_refusals(lib):
     x = torch.zeros(3, 40)
     codes, scales = torch.zeros(3, 20, dtype=torch.uint8), torch.zeros(3, 2, dtype=torch.uint8)
     rows = codes, scales
-    grads = scoring.LayerNormGrad(x, x[0], x[0], torch.zeros(0, dtype=torch.uint8), (3, 40))
+    none = torch.zeros(0, dtype=torch.uint8)
+    made_for = (3, 40, torch.float32, torch.float32)
+    grads = scoring.LayerNormGrad.of(x, x[0], x[0], none, made_for)
     for call, text in [
             (lambda: scoring.quantize_rows_mx4(x), "on the GPU"),
             (lambda: scoring.mx4_values(*rows), "on the GPU"),
@@ -138,7 +140,12 @@ def test_python_refusals(lib):
             (lambda: scoring.layer_norm_grad(x, x[:2]), "grad and x differ"),
             (lambda: scoring.layer_norm_grad(x, x, x[0, :9]), "weight must be"),
             (lambda: scoring.layer_norm_grad(x[:2], x[:2], out=grads), "another number of rows"),
-            (lambda: scoring.layer_norm_grad(x, x, x[0].half(), out=grads), "out.weight must be"),
+            (lambda: scoring.layer_norm_grad(x, x, x[0].half(), out=grads), "or other types"),
+            (lambda: scoring.layer_norm_grad(x.half(), x.half(), out=grads), "or other types"),
+            (lambda: scoring.LayerNormGrad.of(x[:2], None, None, none, made_for), "out.x has another"),
+            (lambda: scoring.LayerNormGrad.of(x.half(), None, None, none, made_for), "out.x has the type"),
+            (lambda: scoring.LayerNormGrad.of(x, x[0, :9], None, none, made_for), "out.weight must be"),
+            (lambda: scoring.LayerNormGrad.of(x, x[0], x[0].half(), none, made_for), "out.bias must be"),
             (lambda: scoring.layer_norm_grad(x, x, wanted=(1, 1, 0), out=grads), "wanted cannot"),
             (lambda: scoring.layer_norm_grad(x, x, out=grads), "on the GPU")]:
         with pytest.raises(ValueError, match=text):
@@ -162,7 +169,8 @@ def _calls_without_derivative(wrap):
     yield lambda: scoring.layer_norm_grad(x, x, wrap(v))
     for at in range(3):
         outs = [wrap(t) if i == at else t for i, t in enumerate((x, v, v))]
-        yield lambda outs=outs: scoring.layer_norm_grad(x, x, out=scoring.LayerNormGrad(*outs, none, (3, 40)))
+        yield lambda outs=outs: scoring.layer_norm_grad(
+            x, x, out=scoring.LayerNormGrad.of(*outs, none, (3, 40, torch.float32, torch.float32)))
     yield lambda: scoring.DenseCatalogue(wrap(x), bits=4)
 
 
