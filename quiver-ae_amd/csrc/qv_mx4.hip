@@ -61,9 +61,12 @@ __global__ __launch_bounds__(256) void to_mx4_kernel(const T* __restrict__ x, in
     const uint32_t u = (uint32_t)min((int64_t)(threadIdx.x / 4 + 64 * r), blocks - 1 - first);
     places.at(u, row[r], block[r]);
     const int64_t j = (int64_t)block[r] * kBlock + quarter * 8;
-    const T* from = x + row[r] * stride + j;
+    const T* from = x + row[r] * stride;
 #pragma unroll
-    for (int e = 0; e < kVecs; e++) load_tail(from + e * kVec<T>, dim - j - e * kVec<T>, 0.f, v[r] + e * kVec<T>);
+    for (int e = 0; e < kVecs; e++) {
+      if (sizeof(T) == 2 && dim >= kVec<T>) load_near_end(from, j + e * kVec<T>, dim, v[r] + e * kVec<T>);
+      else load_tail(from + j + e * kVec<T>, dim - j - e * kVec<T>, 0.f, v[r] + e * kVec<T>);
+    }
   }
 #pragma unroll
   for (int r = 0; r < R; r++) {
