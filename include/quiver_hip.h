@@ -549,13 +549,14 @@ int qv_log_probs_grad(const void* d_logits, int32_t type, int64_t rows, int64_t 
  * qv_quantize_rows_mx4: with a the largest magnitude of a block, s is the least for which
  * a <= 7 2^(s - 127) (0 at least: 2^-127), and a code is x / 2^(s - 127) rounded to the
  * nearest of those, halves to the even code, magnitudes over 6 to 6: no value is off by
- * more than half a step.  A block that holds an infinity or a NaN gets the scale 255
- * and zero codes; a row of odd length ends with a zero code.  type as qv_quantize_rows. */
+ * more than half a step.  (From 3.5 2^126 on that is 4 2^126, an infinity as a float.)  A
+ * block that holds an infinity or a NaN gets the scale 255 and zero codes; a row of odd
+ * length ends with a zero code.  type as qv_quantize_rows; n and dim < 2^31. */
 int qv_quantize_rows_mx4(const void* d_x, int32_t type, int64_t n, int64_t dim, int64_t x_stride, uint8_t* d_codes,
                          int64_t code_stride, uint8_t* d_scales, int64_t scale_stride, int device, void* stream);
 
-/* What such rows stand for, rounded to out_type (bfloat16 and float hold it exactly
- * from 2^-126 on). */
+/* What such rows stand for, rounded to out_type: float holds it exactly below 2^128, bfloat16
+ * from 2^-126 on, float16 within its range. */
 int qv_mx4_values(const uint8_t* d_codes, int64_t code_stride, const uint8_t* d_scales, int64_t scale_stride, int64_t n,
                   int64_t dim, void* d_out, int32_t out_type, int64_t out_stride, int device, void* stream);
 
@@ -572,7 +573,9 @@ int qv_mx4_product(const uint8_t* d_a, int64_t a_stride, const uint8_t* d_a_scal
  * variance (over dim) of the row, in fp32, rounded once to x's type.  Weight and bias
  * (either may be NULL: 1 and 0) have dim values of param_type.  type and param_type:
  * QV_FLOAT, QV_BFLOAT16 or QV_FLOAT16.  eps: a positive normal float.  A row that holds
- * an infinity or a NaN gives NaN.  d_y may be d_x with the same stride. */
+ * an infinity or a NaN gives NaN; values up to the largest float do not.  d_y may be
+ * d_x with the same stride.  rows < 2^31, dim up to QV_LAYER_NORM_MAX_DIM. */
+#define QV_LAYER_NORM_MAX_DIM 16777216
 int qv_layer_norm(const void* d_x, int32_t type, int64_t rows, int64_t dim, int64_t x_stride, const void* d_weight,
                   const void* d_bias, int32_t param_type, float eps, void* d_y, int64_t y_stride, int device, void* stream);
 

@@ -186,7 +186,7 @@ struct Row {
   }
 };
 
-// Rows whose sum of squares passes kLargest, 16 of which add up to a finite sum, are taken times kSmaller: 2^31 squares
+// Rows whose sum of squares passes kLargest, 16 of which add up to a finite sum, are taken times kSmaller: 2^24 squares
 // of the largest float are then below it, and those of rows that passed it far above the smallest float.
 constexpr float kSmaller = 0x1p-90f, kLargest = FLT_MAX / 32.f;
 
@@ -656,7 +656,8 @@ void check_eps(float eps) {
 
 void check_sizes(int64_t n, int64_t dim) {
   if (n < 0 || dim < 0) qv::fail(QV_EINVAL, "negative size");
-  if (n > INT32_MAX || dim > INT32_MAX) qv::fail(QV_EUNSUPPORTED, "more than 2^31 - 1 rows or columns");
+  if (n > INT32_MAX) qv::fail(QV_EUNSUPPORTED, "more than 2^31 - 1 rows");
+  if (dim > QV_LAYER_NORM_MAX_DIM) qv::fail(QV_EUNSUPPORTED, "rows longer than 2^24, the last whole number before a float leaves some out");
 }
 
 }  // namespace

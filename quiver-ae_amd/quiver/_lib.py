@@ -32,6 +32,7 @@ QV_FLOAT16 = 4
 QV_PRODUCT_MAX_K = 131071
 QV_LOG_PROBS_MAX_TOPK = 64
 QV_LOG_PROBS_MAX_TARGETS = 64
+QV_LAYER_NORM_MAX_DIM = 16777216
 QV_EXIT_NONE = 0
 QV_EXIT_GPRUNING = 2
 QV_ADMIT_STREAMING = 0

@@ -658,7 +658,7 @@ class DenseCatalogue:
     """Embedding vectors kept in 8 bits, or in microscaled 4 bits, and scored exhaustively.
 
     ``DenseCatalogue(vectors)`` quantises the rows once, ``bits=4`` to half the
-    bytes (and about 20 times the error of an inner product), as their queries.  ``log_probs(queries,
+    bytes and 15 to 18 times the error of an inner product, as their queries.  ``log_probs(queries,
     targets, ...)`` gives each query's distribution over all of them, by inner
     products; the scores exist for one batch of queries at a time, about
     ``score_bytes`` of them.  Scores have no derivative (vectors, queries or a

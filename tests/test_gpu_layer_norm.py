@@ -268,6 +268,17 @@ def test_far_rows(scoring):
     _within(r.bias, sums, (n / 256 + 400) * U * mass, "columns")
 
 
+def test_longest_rows(scoring):
+    """Rows of the greatest length that is taken."""
+    from quiver import _lib
+
+    d = _lib.QV_LAYER_NORM_MAX_DIM
+    say("layer norm, rows of", d)
+    x, weight, bias, grad = _rows(3, d, torch.bfloat16, 4)
+    _check_forward(scoring.layer_norm(x, weight, bias), x, weight, bias)
+    _check_grad(scoring.layer_norm_grad(x, grad, weight), x, grad, weight, torch.float32)
+
+
 def test_differences(scoring):
     """The gradient against central differences of the definition in 64 bits, along random directions."""
     say("layer norm, gradient against differences")

@@ -376,6 +376,22 @@ def test_many_rows(scoring):
     torch.cuda.empty_cache()
 
 
+def test_many_rows_of_a_product(scoring):
+    """More rows of a than the panels of one launch have."""
+    m, n, k = 2 ** 30 + 129, 2, 32
+    torch.cuda.empty_cache()
+    say("4-bit product,", m, n, k)
+    a = torch.randint(0, 256, (m, k // 2), dtype=torch.uint8, device="cuda")  # 17 GB
+    sa = torch.full((m, 1), 127, dtype=torch.uint8, device="cuda")
+    sa[::7] = 126
+    b, sb = a[5:7].clone(), sa[5:7].clone()
+    out = scoring.mx4_product(a, sa, b, sb, dtype=torch.bfloat16)
+    for lo in (0, m // 2, m - 300):
+        _check_product(out[lo:lo + 300], a[lo:lo + 300], sa[lo:lo + 300], b, sb, None, torch.bfloat16, exact=True)
+    del a, sa, out
+    torch.cuda.empty_cache()
+
+
 def test_distant_rows(scoring):
     """Operands' and output rows 2^25 elements and more apart; nothing beside the output is written."""
     stride = 2 ** 25 + 3

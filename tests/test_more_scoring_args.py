@@ -76,7 +76,9 @@ def test_norm_refusals(lib, buf):
     assert L.qv_layer_norm(*{**ok, "n": 2 ** 31}.values(), 0, None) == lib.QV_EUNSUPPORTED
     need = L.qv_layer_norm_grad_workspace(2, 8)
     assert need > 0 and L.qv_layer_norm_grad_workspace(0, 8) == 0 and L.qv_layer_norm_grad_workspace(-1, 8) == lib.QV_EINVAL
-    assert L.qv_layer_norm_grad_workspace(1, 2 ** 31) == lib.QV_EUNSUPPORTED
+    most = lib.QV_LAYER_NORM_MAX_DIM
+    assert L.qv_layer_norm_grad_workspace(1, most + 1) == lib.QV_EUNSUPPORTED and L.qv_layer_norm_grad_workspace(1, most) > 0
+    assert L.qv_layer_norm(*{**ok, "dim": most + 1, "xs": most + 1, "ys": most + 1}.values(), 0, None) == lib.QV_EUNSUPPORTED
     ok = dict(x=p, type=lib.QV_FLOAT, n=2, dim=8, xs=8, g=p, gs=8, w=p, params=lib.QV_FLOAT, eps=1e-5, dx=p, dxs=8, dw=p,
               db=p, work=p, bytes=need)
     _refused(lib, L.qv_layer_norm_grad, ok, eps + [
