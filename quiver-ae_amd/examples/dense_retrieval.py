@@ -5,9 +5,11 @@
 1. A catalogue of normalised float vectors (the benchmark's mixture) is kept in 8
    bits and scored exhaustively: each query's distribution over all rows, the log
    probability of the row it was made from, how sure it is (entropy), its ten best
-   rows, and how often the exact nearest row is among them.
+   rows, and how often the exact nearest row is among them.  The same in 4 bits.
 2. A linear map of distorted queries is trained with the contrastive loss over a
    batch and the catalogue's hardest rows, by autograd through ``log_probs``.
+3. The same with a tower that ends in a layer norm, whose weight and bias are
+   trained too.
 """
 from __future__ import annotations
 
@@ -57,6 +59,36 @@ def train(catalogue: scoring.DenseCatalogue, vectors: torch.Tensor, queries: tor
     return losses
 
 
+def tower_loss(queries: torch.Tensor, vectors: torch.Tensor, labels: torch.Tensor, weight: torch.Tensor,
+               gain: torch.Tensor, offset: torch.Tensor) -> torch.Tensor:
+    """The contrastive loss of queries through a linear map and a layer norm, every row of the batch against each."""
+    hidden = scoring.layer_norm(queries @ weight, gain, offset)
+    logits = hidden @ vectors.T
+    # a normalised row has the length sqrt(dim): the temperature grows with it
+    return -scoring.log_probs(logits, labels, temperature=TEMPERATURE * queries.shape[1] ** 0.5).target.mean()
+
+
+def train_tower(vectors: torch.Tensor, queries: torch.Tensor, targets: torch.Tensor, steps: int,
+                rate: float = 0.02) -> list[float]:
+    """Contrastive losses of the steps."""
+    n, dim = queries.shape
+    leaves = [torch.eye(dim, device=queries.device), torch.ones(dim, device=queries.device),
+              torch.zeros(dim, device=queries.device)]
+    for leaf in leaves:
+        leaf.requires_grad_()
+    optimizer = torch.optim.Adam(leaves, lr=rate)
+    labels = torch.arange(n, dtype=torch.int32, device=queries.device)
+    answers_of = vectors[targets.long()]
+    losses = []
+    for _ in range(steps):
+        loss = tower_loss(queries, answers_of, labels, *leaves)
+        optimizer.zero_grad()
+        loss.backward()
+        optimizer.step()
+        losses.append(loss.item())
+    return losses
+
+
 def main(rows: int = 100_000, queries: int = 512, steps: int = 30, dim: int = 96) -> dict:
     base = torch.from_numpy(quiver.mixture(rows, dim, data_type="float", num_centers=max(16, rows // 64), sigma=1.0,
                                            seed=5)).cuda()
@@ -68,10 +100,15 @@ def main(rows: int = 100_000, queries: int = 512, steps: int = 30, dim: int = 96
     result = answers(catalogue, base, near, targets)
     print(f"{queries} queries over {rows} rows: log probability of the answer {result['log_prob']:.3f}, "
           f"entropy {result['entropy']:.3f}, nearest row among the ten best {result['recall']:.3f}")
+    short = answers(scoring.DenseCatalogue(base, bits=4), base, near, targets)
+    print(f"in 4 bits: log probability {short['log_prob']:.3f}, entropy {short['entropy']:.3f}, nearest row among the ten "
+          f"best {short['recall']:.3f}")
     distortion = torch.eye(dim, device="cuda") + 1.5 * torch.randn((dim, dim), generator=g, device="cuda") / dim ** 0.5
     losses = train(catalogue, base, near @ distortion, targets, steps)
     print(f"contrastive loss over {steps} steps: {losses[0]:.4f} -> {losses[-1]:.4f}")
-    return {**result, "losses": losses}
+    tower = train_tower(base, near @ distortion, targets, steps)
+    print(f"with a layer norm over {steps} steps: {tower[0]:.4f} -> {tower[-1]:.4f}")
+    return {**result, "losses": losses, "in_4_bits": short, "tower_losses": tower}
 
 
 if __name__ == "__main__":

@@ -416,3 +416,37 @@ def test_embeddings_to_answers(scoring):
     off = 2.0 ** -23 / (64 * 16) * vectors[:64].double().abs()
     for got, want, slack in ((leaf_w.grad, w64.grad, (off * x64.abs()).sum(0)), (leaf_b.grad, b64.grad, off.sum(0))):
         assert ((got.double() - want).abs() <= 2.0 ** -10 * want.abs().max() + slack).all()
+
+
+def test_example(scoring):
+    """The retrieval example runs, and its tower's gradients are those of the loss in 64 bits."""
+    import importlib.util
+    from pathlib import Path
+
+    say("dense retrieval example, in 4 bits and with a layer norm")
+    path = Path(__file__).resolve().parents[1] / "quiver-ae_amd" / "examples" / "dense_retrieval.py"
+    spec = importlib.util.spec_from_file_location("dense_retrieval_tower", path)
+    example = importlib.util.module_from_spec(spec)
+    spec.loader.exec_module(example)
+    r = example.main(rows=4_000, queries=64, steps=2)
+    assert len(r["tower_losses"]) == 2 and all(0 <= x < 100 for x in r["tower_losses"])
+    assert 0 <= r["in_4_bits"]["recall"] <= 1 and r["in_4_bits"]["entropy"] >= 0
+
+    g = torch.Generator(device="cuda").manual_seed(12)
+    queries, vectors = torch.randn((40, 96), generator=g, device="cuda"), torch.randn((40, 96), generator=g, device="cuda")
+    leaves = [torch.randn((96, 96), generator=g, device="cuda") * 0.1, 1 + 0.1 * torch.randn(96, generator=g, device="cuda"),
+              0.1 * torch.randn(96, generator=g, device="cuda")]
+    labels = torch.arange(40, dtype=torch.int32, device="cuda")
+    for leaf in leaves:
+        leaf.requires_grad_()
+    example.tower_loss(queries, vectors, labels, *leaves).backward()
+    exact = [t.detach().double().requires_grad_() for t in leaves]
+    hidden = queries.double() @ exact[0]
+    d = hidden - hidden.mean(1, keepdim=True)
+    hat = d / torch.sqrt((d * d).mean(1, keepdim=True) + EPS)
+    z = (hat * exact[1] + exact[2]) @ vectors.T.double() / (0.05 * 96 ** 0.5)
+    (-torch.log_softmax(z, 1)[torch.arange(40), torch.arange(40)].mean()).backward()
+    # logits over the temperature are at most 500 here, off by 100 roundings of 2^-24 of their 96 terms' magnitudes: 2^-9; each
+    # gradient is a sum of probabilities (as much off, relatively) times values, and the loss's other sums' errors are far less
+    for got, want in zip(leaves, exact):
+        assert ((got.grad.double() - want.grad).abs() <= 2.0 ** -8 * want.grad.abs().max()).all()
