@@ -190,6 +190,13 @@ struct Row {
 // of the largest float are then below it, and those of rows that passed it far above the smallest float.
 constexpr float kSmaller = 0x1p-90f, kLargest = FLT_MAX / 32.f;
 
+// The variance, of the mean square of deviations from what is the mean but for `rest`.  Where all values are equal, only
+// roundings are left of it, and of the deviations less `rest` as many units of 2^-24 of it as sums have additions in a row:
+// no less than 2^-12 of it keeps their quotients small.  One value of up to 2^20 that differs from the others has more.
+__device__ __forceinline__ float variance(float square, float rest) {
+  return max(__builtin_fmaf(-rest, rest, square), rest * rest * 0x1p-24f);
+}
+
 // Turns a thread's part of a row (0 past its end), values(e), into deviations v, of the values times `scale`; returns
 // 1 / sqrt(var + eps) of those.  With GRAD, sums[0] and sums[1] come out as the sums of h = g w and of h d.
 template <bool GRAD, int R, int T, int E, class F>
@@ -223,7 +230,7 @@ __device__ __forceinline__ float centre(F values, f4 (&v)[E], const f4 (&g)[E], 
       }
     }
     row.template sum<true>(m, kLargest);
-    const float rest = m[0] * per, var = max(m[1] * per - rest * rest, 0.f);
+    const float rest = m[0] * per, var = variance(m[1] * per, rest);
     const bool bad = row.bad;
     if (turn == 1 || !row.any_bad) {
 #pragma unroll
@@ -232,10 +239,11 @@ __device__ __forceinline__ float centre(F values, f4 (&v)[E], const f4 (&g)[E], 
         sums[0] = m[2];
         sums[1] = m[3] - rest * m[2];
       }
-      return 1.f / __builtin_sqrtf(bad ? __builtin_nanf("") : var + eps);
+      const float of_eps = eps * scale * scale;
+      if (var == 0.f) scale = 1.f;  // all deviations are 0, times any scale
+      return 1.f / __builtin_sqrtf(bad ? __builtin_nanf("") : var == 0.f ? eps : var + of_eps);
     }
     scale = bad ? kSmaller : 1.f;  // (other rows come out as before)
-    if (bad) eps = eps * kSmaller * kSmaller;
 #pragma unroll
     for (int e = 0; e < E; e++) v[e] = values(e) * scale;
   }
@@ -427,8 +435,12 @@ __device__ __forceinline__ Moments long_moments(const T* x, const T* g, const vo
     r.rest = m[0] * per;
     const bool bad = across.bad;
     if (turn == 1 || !bad) {
-      const float var = max(m[1] * per - r.rest * r.rest, 0.f);
-      r.rstd = 1.f / __builtin_sqrtf(bad ? __builtin_nanf("") : var + eps);
+      const float var = variance(m[1] * per, r.rest), of_eps = eps * r.scale * r.scale;
+      r.rstd = 1.f / __builtin_sqrtf(bad ? __builtin_nanf("") : var == 0.f ? eps : var + of_eps);
+      if (var == 0.f) {  // all deviations are 0, times any scale
+        r.mean *= 1.f / r.scale;
+        r.scale = 1.f;
+      }
       if constexpr (GRAD) {
         r.c1 = m[2] * per;
         r.c2 = (m[3] - r.rest * m[2]) * per * r.rstd;
@@ -436,7 +448,6 @@ __device__ __forceinline__ Moments long_moments(const T* x, const T* g, const vo
       return r;
     }
     r.scale = kSmaller;
-    eps = eps * kSmaller * kSmaller;
   }
 }
 

@@ -186,6 +186,25 @@ def test_huge_rows(scoring, dtype, n, d):
     _check_grad(replace(r, x=None), x, grad, weight, torch.float32)
 
 
+@pytest.mark.parametrize("value", [3e15, -2.0 ** 125, torch.finfo(torch.float32).max])
+@pytest.mark.parametrize("d", [2, 7, 64, 100, 1000, 1024, 4096, 5000, 12288, 16384, 20000, 65536])
+def test_equal_values(scoring, d, value):
+    """Rows of one value, up to the largest: x^ is 0, and 1 / s that of eps alone.  Where d is a power of two the mean is
+    exact.  Else what is left of the deviations is at most A u of that of the mean, and its root is taken of 2^-24 of the
+    square of that at least: x^ is up to (A + 2) 2^-12, and s not eps's."""
+    say("layer norm, equal values", d, value)
+    x, weight, bias, grad = _rows(6, d, torch.float32, d)
+    x[1:4] = value
+    if d & (d - 1) == 0:
+        _check_forward(scoring.layer_norm(x, weight, bias), x, weight, bias)
+        _check_grad(scoring.layer_norm_grad(x, grad, weight), x, grad, weight, torch.float32)
+    else:
+        hat = scoring.layer_norm(x)[1:4]
+        assert (hat.abs() <= (_additions(d) + 2) * 2.0 ** -12).all(), hat.abs().max()
+        r = scoring.layer_norm_grad(x, grad, weight)
+        assert torch.isfinite(r.x).all() and torch.isfinite(r.weight).all()
+
+
 @pytest.mark.parametrize("eps", [2.0 ** -126, 1e-12, 1e-3, 10.0, 1e30])
 def test_eps(scoring, eps):
     say("layer norm, eps", eps)
