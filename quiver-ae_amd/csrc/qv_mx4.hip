@@ -404,8 +404,8 @@ __global__ __launch_bounds__(64 * WM * WN, 1) void product_tile_kernel(Product<O
 // MANY: one workgroup per CU walks over tiles, and the stages run on from tile to tile:
 // the next tile's first ones are on their way, and its first operands in registers, while
 // the results are stored.
-// 4,096^3 to bfloat16: 45 us, 3.1 PFLOP/s, of zeros 37 (a library's 4-bit product with block scales: 70); 8,192^3: 300 us,
-// 3.7 PFLOP/s, of zeros 246 (library: 359).  The matrix instruction alone runs at 6.5 PFLOP/s on varied codes, 8.9 on
+// 4,096^3 to bfloat16: 42 us, 3.3 PFLOP/s, of zeros 36 (a library's 4-bit product with block scales: 70); 8,192^3: 277 us,
+// 4.0 PFLOP/s, of zeros 218 (library: 359).  The matrix instruction alone runs at 6.5 PFLOP/s on varied codes, 8.9 on
 // zeros: LDS (98 KB a stage, 784 of the 1,024 cycles of its products) and power hold it.
 template <int BM, int BN, int WM, int WN, int NB, int G, bool MANY, class O>
 __global__ __launch_bounds__(64 * WM * WN, 1) void product_deep_kernel(Product<O> p, int64_t tiles_m, int64_t tiles_n,
@@ -602,14 +602,29 @@ __global__ __launch_bounds__(64 * WM * WN, 1) void product_deep_kernel(Product<O
   __builtin_amdgcn_s_waitcnt(kWaitFor<0>);  // no load into LDS outlives the wave
 }
 
-// Stores four columns from j on of row i, with their biases, where they lie in the output.
+// The biases of four columns from j on; -0, which changes no sum, without.
 template <class O>
-__device__ __forceinline__ void store_four(f4 v, int64_t i, int64_t j, const Product<O>& p) {
+__device__ __forceinline__ f4 four_biases(int64_t j, const Product<O>& p) {
+  f4 add = {-0.f, -0.f, -0.f, -0.f};
+  if (p.bias) {
+    if (j + 4 <= p.n) {
+      add = *reinterpret_cast<const f4_any*>(p.bias + j);
+    } else {
+#pragma unroll
+      for (int e = 0; e < 4; e++) add[e] = p.bias[min(j + e, p.n - 1)];
+    }
+  }
+  return add;
+}
+
+// Stores four columns from j on of row i, where they lie in the output.
+template <class O>
+__device__ __forceinline__ void store_four(f4 v, f4 add, int64_t i, int64_t j, const Product<O>& p) {
   asm volatile("" : "+v"(v));  // here: a matrix instruction that the compiler moves behind the branch has not all lanes' scales
   if (i >= p.m) return;
   O o[4];
 #pragma unroll
-  for (int e = 0; e < 4; e++) o[e] = (O)(p.bias ? v[e] + p.bias[min(j + e, p.n - 1)] : v[e]);
+  for (int e = 0; e < 4; e++) o[e] = (O)(v[e] + add[e]);
   O* to = p.out + i * p.out_stride + j;
   if (j + 4 <= p.n) {
     __builtin_memcpy(to, o, sizeof(o));
@@ -622,7 +637,8 @@ __device__ __forceinline__ void store_four(f4 v, int64_t i, int64_t j, const Pro
 
 // Up to 16 TM rows of a against strips of 16 rows of b whose blocks one matrix instruction takes, up to 128 values
 // (v_mfma_scale_f32_16x16x128_f8f6f4: what 64 lanes load of 16 such rows is 1 KB in a row).  U strips per wave, straight from
-// memory to the registers.  Bound by reading b: 1 x 1M x 128 to float 13.9 us, 5.2 TB/s.
+// memory to the registers, and the biases with them.  Bound by reading b: 1 x 1M x 128 to float 13 us, 5.5 TB/s (with
+// biases that each are asked for when their result is there: 19).
 template <int U, int TM, class O>
 __global__ __launch_bounds__(256) void product_row_kernel(Product<O> p, int64_t groups, int64_t first_block) {
   const int lane = lane_id(), row = lane % 16, quarter = lane / 16;
@@ -631,8 +647,10 @@ __global__ __launch_bounds__(256) void product_row_kernel(Product<O> p, int64_t 
   const int k = (int)p.k, place = quarter * 16, at = min(place, k - 16), block = min(quarter, p.blocks - 1);
   i4 fa[TM], fb[U];
   uint32_t sa[TM], sb[U];
+  f4 add[U];  // asked for with the rows
 #pragma unroll
   for (int u = 0; u < U; u++) {
+    add[u] = four_biases((group * U + u) * 16 + 4 * quarter, p);
     const int64_t j = min((group * U + u) * 16 + row, p.n - 1);
     fb[u] = *reinterpret_cast<const i4_any*>(p.b + j * p.b_stride + at);
     sb[u] = p.b_scales[j * p.bs_stride + block];
@@ -647,7 +665,7 @@ __global__ __launch_bounds__(256) void product_row_kernel(Product<O> p, int64_t 
   for (int u = 0; u < U; u++)
 #pragma unroll
     for (int x = 0; x < TM; x++)
-      store_four(mfma16(fb[u], sb[u], fa[x], sa[x], f4{0.f, 0.f, 0.f, 0.f}), 16 * x + row, (group * U + u) * 16 + 4 * quarter, p);
+      store_four(mfma16(fb[u], sb[u], fa[x], sa[x], f4{0.f, 0.f, 0.f, 0.f}), add[u], 16 * x + row, (group * U + u) * 16 + 4 * quarter, p);
 }
 
 // The same for longer rows: b goes to the registers one turn ahead, U strips of V = 4 / U steps of four blocks.  A lane loads one word of scales, those of
@@ -710,7 +728,9 @@ __global__ __launch_bounds__(WK == 1 ? 256 : 64 * WK) void product_strip_kernel(
   __syncthreads();
 
   for (; group < groups; group += step) {
-    f4 acc[TM][U];
+    f4 acc[TM][U], add[U];
+#pragma unroll
+    for (int u = 0; u < U; u++) add[u] = four_biases((group * U + u) * 16 + 4 * quarter, p);
 #pragma unroll
     for (int x = 0; x < TM; x++)
 #pragma unroll
@@ -766,7 +786,7 @@ __global__ __launch_bounds__(WK == 1 ? 256 : 64 * WK) void product_strip_kernel(
 #pragma unroll
     for (int u = 0; u < U; u++)
 #pragma unroll
-      for (int x = 0; x < TM; x++) store_four(acc[x][u], 16 * x + row, (group * U + u) * 16 + 4 * quarter, p);
+      for (int x = 0; x < TM; x++) store_four(acc[x][u], add[u], 16 * x + row, (group * U + u) * 16 + 4 * quarter, p);
   }
 }
 
