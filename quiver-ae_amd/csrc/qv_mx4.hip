@@ -196,7 +196,7 @@ struct Product {
   int blocks;    // of a row
   O* out;
   int64_t out_stride;
-  bool stream, stream_lines;  // results past the caches: of tiles' pieces, of whole lines
+  bool stream, stream_lines;  // results past the caches: where rows are whole lines, through lines
 };
 
 // x: an instruction's rows, y: its columns; the scales are byte S of theirs.
@@ -602,73 +602,146 @@ __global__ __launch_bounds__(64 * WM * WN, 1) void product_deep_kernel(Product<O
   __builtin_amdgcn_s_waitcnt(kWaitFor<0>);  // no load into LDS outlives the wave
 }
 
-// The biases of four columns from j on; -0, which changes no sum, without.
-template <class O>
-__device__ __forceinline__ f4 four_biases(int64_t j, const Product<O>& p) {
-  f4 add = {-0.f, -0.f, -0.f, -0.f};
-  if (p.bias) {
-    if (j + 4 <= p.n) {
-      add = *reinterpret_cast<const f4_any*>(p.bias + j);
-    } else {
-#pragma unroll
-      for (int e = 0; e < 4; e++) add[e] = p.bias[min(j + e, p.n - 1)];
-    }
-  }
-  return add;
+// U strips of 16 rows of b: which of its 16 U rows strip u's are, so that a lane's 4 U results are of columns in a row.
+template <int U>
+__device__ __forceinline__ int strip_row(int u, int row) {
+  return row / 4 * (4 * U) + u * 4 + row % 4;
 }
 
-// Stores four columns from j on of row i, where they lie in the output.
-template <class O>
-__device__ __forceinline__ void store_four(f4 v, f4 add, int64_t i, int64_t j, const Product<O>& p) {
-  asm volatile("" : "+v"(v));  // here: a matrix instruction that the compiler moves behind the branch has not all lanes' scales
-  if (i >= p.m) return;
-  O o[4];
+// The biases of a lane's columns, from j on; -0, which changes no sum, without.
+template <int U, class O>
+__device__ __forceinline__ void load_biases(f4 (&add)[U], int64_t j, const Product<O>& p) {
 #pragma unroll
-  for (int e = 0; e < 4; e++) o[e] = (O)(v[e] + add[e]);
-  O* to = p.out + i * p.out_stride + j;
-  if (j + 4 <= p.n) {
-    __builtin_memcpy(to, o, sizeof(o));
-  } else {
+  for (int u = 0; u < U; u++, j += 4) {
+    add[u] = f4{-0.f, -0.f, -0.f, -0.f};
+    if (!p.bias) continue;
+    if (j + 4 <= p.n) {
+      add[u] = *reinterpret_cast<const f4_any*>(p.bias + j);
+    } else {
 #pragma unroll
-    for (int e = 0; e < 3; e++)
+      for (int e = 0; e < 4; e++) add[u][e] = p.bias[min(j + e, p.n - 1)];
+    }
+  }
+}
+
+// Stores a lane's columns, from j on of row i, where they lie in the output.  32 bytes of them: lanes of two rows exchange
+// halves first, and each store writes 128 bytes in a row of eight rows.
+template <int U, class O>
+__device__ __forceinline__ void store_columns(f4 (&v)[U], const f4 (&add)[U], int64_t i, int64_t j, const Product<O>& p) {
+  constexpr int N = 4 * U, V = kVec<O>;
+  constexpr bool kTwo = N == 2 * V;
+#pragma unroll
+  for (int u = 0; u < U; u++) {
+#pragma unroll
+    for (int e = 0; e < 4; e++) v[u][e] += add[u][e];
+    asm volatile("" : "+v"(v[u]));  // here: a matrix instruction that the compiler moves behind the branch has not all lanes' scales
+  }
+  O o[N];
+#pragma unroll
+  for (int e = 0; e < N; e++) o[e] = (O)v[e / 4][e % 4];
+  raw4 own[2] = {}, other[2] = {};
+  if constexpr (kTwo) {
+    __builtin_memcpy(own, o, sizeof(o));
+#pragma unroll
+    for (int u = 0; u < 2; u++)
+#pragma unroll
+      for (int e = 0; e < 4; e++) other[u][e] = (uint32_t)__builtin_amdgcn_mov_dpp((int)own[u][e], 0xB1, 0xF, 0xF, true);
+  }
+  if (j + N <= p.n) {
+    if constexpr (kTwo) {
+      const bool odd = i & 1;
+      O* to = p.out + (i - odd) * p.out_stride + j + (odd ? V : 0);
+      if (i - odd < p.m) store_past(odd ? other[1] : own[0], reinterpret_cast<raw4_any*>(to), p.stream);
+      if (i - odd + 1 < p.m) store_past(odd ? own[1] : other[0], reinterpret_cast<raw4_any*>(to + p.out_stride), p.stream);
+    } else if (i < p.m) {
+      O* to = p.out + i * p.out_stride + j;
+      if constexpr (N == V) store_past(__builtin_bit_cast(raw4, o), reinterpret_cast<raw4_any*>(to), p.stream);
+      else __builtin_memcpy(to, o, sizeof(o));
+    }
+  } else if (i < p.m) {
+    O* to = p.out + i * p.out_stride + j;
+#pragma unroll
+    for (int e = 0; e < N - 1; e++)
       if (j + e < p.n) to[e] = o[e];
   }
 }
 
-// Up to 16 TM rows of a against strips of 16 rows of b whose blocks one matrix instruction takes, up to 128 values
-// (v_mfma_scale_f32_16x16x128_f8f6f4: what 64 lanes load of 16 such rows is 1 KB in a row).  U strips per wave, straight from
-// memory to the registers, and the biases with them.  Bound by reading b: 1 x 1M x 128 to float 13 us, 5.5 TB/s (with
-// biases that each are asked for when their result is there: 19).
-template <int U, int TM, class O>
-__global__ __launch_bounds__(256) void product_row_kernel(Product<O> p, int64_t groups, int64_t first_block) {
+// Short rows of b, of up to four blocks for each of K matrix instructions, stay in a wave's registers: U strips of 16 of them
+// (v_mfma_scale_f32_16x16x128_f8f6f4: what 64 lanes load of 16 rows of 128 values is 1 KB in a row), with their biases, while 16 TM
+// rows of a at a time go by, the next ones on their way.  Bound by reading b and writing: 1 x 1M x 128 to float 12.5 us, 5.8
+// TB/s (with biases that each are asked for when their result is there: 19); 32 x 900,000 x 128 28 us, 6.3 TB/s (with stores of 64
+// bytes in a row through the L2: 62); 64 x 600,000 x 128 to 16 bits 21 us (with 64 bytes in a row: 25).
+template <int U, int TM, int K, class O>
+__global__ __launch_bounds__(256) void product_row_kernel(Product<O> p, int64_t groups, int64_t first_block, int64_t rows) {
   const int lane = lane_id(), row = lane % 16, quarter = lane / 16;
   const int64_t group = (first_block + blockIdx.x) * 4 + wave_id();
   if (group >= groups) return;
-  const int k = (int)p.k, place = quarter * 16, at = min(place, k - 16), block = min(quarter, p.blocks - 1);
-  i4 fa[TM], fb[U];
-  uint32_t sa[TM], sb[U];
+  const int k = (int)p.k;
+  int at[K], over[K], block[K];  // of a lane's piece of each step: where it begins, what is of the one before, its block
+#pragma unroll
+  for (int q = 0; q < K; q++) {
+    const int place = q * 64 + quarter * 16;
+    at[q] = min(place, k - 16);
+    over[q] = place - at[q];
+    block[q] = min(q * 4 + quarter, p.blocks - 1);
+  }
+  i4 fa[TM][K], fb[U][K];
+  uint32_t sa[TM][K], sb[U][K];
+  const int64_t j0 = group * (16 * U);
   f4 add[U];  // asked for with the rows
+  load_biases<U>(add, j0 + quarter * (4 * U), p);
 #pragma unroll
   for (int u = 0; u < U; u++) {
-    add[u] = four_biases((group * U + u) * 16 + 4 * quarter, p);
-    const int64_t j = min((group * U + u) * 16 + row, p.n - 1);
-    fb[u] = *reinterpret_cast<const i4_any*>(p.b + j * p.b_stride + at);
-    sb[u] = p.b_scales[j * p.bs_stride + block];
-  }
+    const int64_t j = min(j0 + strip_row<U>(u, row), p.n - 1);
 #pragma unroll
-  for (int x = 0; x < TM; x++) {
-    const int64_t i = min((int64_t)(16 * x + row), p.m - 1);
-    fa[x] = without_first(*reinterpret_cast<const i4_any*>(p.a + i * p.a_stride + at), place - at);
-    sa[x] = p.a_scales[i * p.as_stride + block];
+    for (int q = 0; q < K; q++) {
+      fb[u][q] = *reinterpret_cast<const i4_any*>(p.b + j * p.b_stride + at[q]);
+      sb[u][q] = p.b_scales[j * p.bs_stride + block[q]];
+    }
   }
+  int64_t i0 = blockIdx.y * rows;
+  const int64_t end = min(p.m, i0 + rows);
+  auto load = [&] {
 #pragma unroll
-  for (int u = 0; u < U; u++)
+    for (int x = 0; x < TM; x++) {
+      const int64_t i = min(i0 + 16 * x + row, p.m - 1);
+#pragma unroll
+      for (int q = 0; q < K; q++) {
+        fa[x][q] = *reinterpret_cast<const i4_any*>(p.a + i * p.a_stride + at[q]);
+        sa[x][q] = p.a_scales[i * p.as_stride + block[q]];
+      }
+    }
+  };
+  load();
+  for (;;) {
+    i4 a[TM][K];
+    uint32_t scale[TM][K];
 #pragma unroll
     for (int x = 0; x < TM; x++)
-      store_four(mfma16(fb[u], sb[u], fa[x], sa[x], f4{0.f, 0.f, 0.f, 0.f}), add[u], 16 * x + row, (group * U + u) * 16 + 4 * quarter, p);
+#pragma unroll
+      for (int q = 0; q < K; q++) {
+        a[x][q] = without_first(fa[x][q], over[q]);
+        scale[x][q] = sa[x][q];
+      }
+    const int64_t here = i0;
+    i0 += 16 * TM;
+    if (i0 < end) load();
+#pragma unroll
+    for (int x = 0; x < TM; x++) {
+      f4 v[U];
+#pragma unroll
+      for (int u = 0; u < U; u++) {
+        v[u] = f4{0.f, 0.f, 0.f, 0.f};
+#pragma unroll
+        for (int q = 0; q < K; q++) v[u] = mfma16(fb[u][q], sb[u][q], a[x][q], scale[x][q], v[u]);
+      }
+      store_columns<U>(v, add, here + 16 * x + row, j0 + quarter * (4 * U), p);
+    }
+    if (i0 >= end) return;
+  }
 }
 
-// The same for longer rows: b goes to the registers one turn ahead, U strips of V = 4 / U steps of four blocks.  A lane loads one word of scales, those of
+// Few longer rows, up to 16 TM: b goes to the registers one turn ahead, U strips of V = 4 / U steps of four blocks.  A lane loads one word of scales, those of
 // one row and step; two exchanges between the quarters of the wave give every lane the word of each.  a and its scales
 // lie in LDS in the order of the lanes.  WK > 1: a strip's blocks are cut over the workgroup's WK waves.
 template <int U, int TM, int WK, class O>
@@ -685,17 +758,16 @@ __global__ __launch_bounds__(WK == 1 ? 256 : 64 * WK) void product_strip_kernel(
   i4 next_b[U][V];
   uint32_t next_scales = 0;
   auto load = [&](int64_t group, int turn) {
-    const uint8_t* b = p.b + min(group * (16 * U) + row, p.n - 1) * p.b_stride;
 #pragma unroll
     for (int u = 0; u < U; u++) {
-      const uint8_t* from = u == 0 ? b : p.b + min((group * U + u) * 16 + row, p.n - 1) * p.b_stride;
+      const uint8_t* from = p.b + min(group * (16 * U) + strip_row<U>(u, row), p.n - 1) * p.b_stride;
 #pragma unroll
       for (int v = 0; v < V; v++)
         next_b[u][v] = *reinterpret_cast<const i4_any*>(from + min(((turn * V + v) * 4 + quarter) * 16, k - 16));
     }
     // the word of this row and step; bytes past the row's end are 0
     const int block = (turn * V + quarter % V) * 4;
-    const int64_t at = min((group * U + quarter / V) * 16 + row, p.n - 1) * p.bs_stride + min(block, blocks - 1);
+    const int64_t at = min(group * (16 * U) + strip_row<U>(quarter / V, row), p.n - 1) * p.bs_stride + min(block, blocks - 1);
     const int64_t from = min(at, scales_end - 4);
     uint32_t word;
     __builtin_memcpy(&word, p.b_scales + from, 4);
@@ -729,8 +801,7 @@ __global__ __launch_bounds__(WK == 1 ? 256 : 64 * WK) void product_strip_kernel(
 
   for (; group < groups; group += step) {
     f4 acc[TM][U], add[U];
-#pragma unroll
-    for (int u = 0; u < U; u++) add[u] = four_biases((group * U + u) * 16 + 4 * quarter, p);
+    load_biases<U>(add, group * (16 * U) + quarter * (4 * U), p);
 #pragma unroll
     for (int x = 0; x < TM; x++)
 #pragma unroll
@@ -784,9 +855,7 @@ __global__ __launch_bounds__(WK == 1 ? 256 : 64 * WK) void product_strip_kernel(
       if (wave) continue;
     }
 #pragma unroll
-    for (int u = 0; u < U; u++)
-#pragma unroll
-      for (int x = 0; x < TM; x++) store_four(acc[x][u], add[u], 16 * x + row, (group * U + u) * 16 + 4 * quarter, p);
+    for (int x = 0; x < TM; x++) store_columns<U>(acc[x], add, 16 * x + row, group * (16 * U) + quarter * (4 * U), p);
   }
 }
 
@@ -967,61 +1036,80 @@ void launch_panels(const Product<O>& p, hipStream_t st) {
   HIP_OK(hipGetLastError());
 }
 
-int strip_lds(int64_t m, int64_t blocks, int u, int wk) {
-  const int tm = m <= 16 ? 1 : 2;
+int strip_lds(int64_t blocks, int u, int tm, int wk) {
   return (int)((blocks + 3) / 4) * tm * 1088 + (wk > 1 ? wk * tm * u * 1024 : 0);
 }
 
-template <int U, int WK, class O>
+template <int U, int TM, int WK, class O>
 void launch_strips(const Product<O>& p, hipStream_t st) {
   const int64_t groups = (p.n + 16 * U - 1) / (16 * U);
-  const int lds = strip_lds(p.m, p.blocks, U, WK);
+  const int lds = strip_lds(p.blocks, U, TM, WK);
   constexpr int kThreads = WK == 1 ? 256 : 64 * WK;
   // as many workgroups as run at once
   const int64_t most = 256 * std::min(2048 / kThreads, 160 * 1024 / std::max(lds, 1));
   const int64_t blocks = std::min(most, WK == 1 ? (groups + 3) / 4 : groups);
-  auto go = [&](auto tiles) {
-    constexpr auto* kernel = &product_strip_kernel<U, decltype(tiles)::value, WK, O>;
-    allow_lds<kernel>(lds);
-    hipLaunchKernelGGL(kernel, dim3((unsigned)blocks), dim3(kThreads), lds, st, p, groups);
-  };
-  if (p.m <= 16) go(std::integral_constant<int, 1>());
-  else go(std::integral_constant<int, 2>());
+  constexpr auto* kernel = &product_strip_kernel<U, TM, WK, O>;
+  allow_lds<kernel>(lds);
+  hipLaunchKernelGGL(kernel, dim3((unsigned)blocks), dim3(kThreads), lds, st, p, groups);
   HIP_OK(hipGetLastError());
 }
 
-template <class O>
+template <int U, int TM, int K, class O>
 void launch_rows(const Product<O>& p, hipStream_t st) {
-  constexpr int U = 2;
-  const int64_t groups = (p.n + 16 * U - 1) / (16 * U);
-  auto* kernel = p.m <= 16 ? product_row_kernel<U, 1, O> : product_row_kernel<U, 2, O>;
-  in_launches((groups + 3) / 4, 256, [&](int64_t first, unsigned count) {
-    hipLaunchKernelGGL(kernel, dim3(count), dim3(256), 0, st, p, groups, first);
+  const int64_t groups = (p.n + 16 * U - 1) / (16 * U), blocks = (groups + 3) / 4;
+  // a's rows cut over workgroups too where b's alone are too few
+  const int64_t chunks = (p.m + 16 * TM - 1) / (16 * TM), slices = std::min(chunks, std::max<int64_t>(1, 1024 / blocks));
+  const int64_t rows = (chunks + slices - 1) / slices * (16 * TM);
+  in_launches(blocks, 256, [&](int64_t first, unsigned count) {
+    hipLaunchKernelGGL((product_row_kernel<U, TM, K, O>), dim3(count, (unsigned)((p.m + rows - 1) / rows)), dim3(256), 0, st, p,
+                       groups, first, rows);
   });
   HIP_OK(hipGetLastError());
 }
 
-// Which kernel: up to 32 rows read b; rows of up to 256 bytes mostly write the result; longer ones keep the matrix cores busy.
+// Which kernel: rows of up to 128 values, and few of up to 256, stay in registers; large results of short rows leave in
+// whole lines; few longer rows read b; others keep the matrix cores busy.
 template <class O>
 void product(const Product<O>& p, hipStream_t st) {
   const int64_t scale_bits = reinterpret_cast<uintptr_t>(p.a_scales) | reinterpret_cast<uintptr_t>(p.b_scales) | p.as_stride | p.bs_stride;
   const int64_t code_bits = reinterpret_cast<uintptr_t>(p.a) | reinterpret_cast<uintptr_t>(p.b) | p.a_stride | p.b_stride;
   const bool near = std::max({p.a_stride, p.b_stride, p.as_stride, p.bs_stride}) < kFar;
-  const bool panels = near && p.m < 1 << 30;  // (a launch has less than 2^32 threads)
   const bool direct = near && code_bits % 16 == 0 && scale_bits % 4 == 0 && p.k % 64 == 0 && p.k > 256;
   const bool four = direct && scale_bits % 16 == 0 && p.k % 256 == 0;
   auto tiles = [&](int64_t size) { return (p.m + size - 1) / size * ((p.n + size - 1) / size); };
+  // Large results of short rows leave through lines.  Measured, us, panels and what else there is.  Rows of b in registers, from 96
+  // MB on: 1,000 x 50,001 x 100 of 16 bits (100 MB) 28, 31; 10,000 x 50,001 x 128 220, 438; 1,000 x 20,001 x 64 floats (80 MB) 20,
+  // 19; 64 x 600,001 x 128 of 16 bits (77 MB) 27, 24; but rows that are whole lines leave the registers so: 10,000 x 50,048 x 128 219, 209.
+  // Tiles, from 72 MB on, past 64 rows: 100 x 368,912 x 200 of 16 bits (74 MB) 25, 34; 200 x 200,000 x 256 (80 MB) 25, 29; 1,000 x 20,001 x 256
+  // floats (80 MB) 23, 19; 128 x 300,000 x 384 of 16 bits (77 MB) 35, 41; 4,000 x 10,001 x 512 floats (160 MB) 40, 58; 128 x 130,000 x 512
+  // (67 MB) 26, 20; 500 x 40,001 x 256 of 16 bits (40 MB) 18, 16; 64 x 600,000 x 384 (77 MB) 58, 46.
+  const double bytes = (double)p.m * p.n * sizeof(O);
+  const bool lines = near && p.m < 1 << 30;  // (a launch has less than 2^32 threads)
+  const bool panels = lines && bytes >= 72e6 && p.m > 64;
+  constexpr int U = sizeof(O) == 2 ? 4 : 2;  // strips of 32 bytes of a result's row
   if (p.k < 16) {
     launch_tiles<64, 64, 2, 2, true>(p, st);
-  } else if (p.m <= 32 && p.blocks <= 4) {
-    launch_rows(p, st);
-  } else if (p.m <= 32 && strip_lds(p.m, p.blocks, 1, 4) <= 150 * 1024) {  // (five blocks: a scales' word lies in any row)
-    // A strip's blocks over four waves where strips alone are too few.  Measured, us, without and with: 1 x 4,096 x 4,096:
-    // 12.8, 7.2; 1 x 20,000 x 4,096: 16.5, 10.8; 1 x 50,000 x 1,024: 8.4, 9.8; 8 x 100,000 x 1,024: 14.5, 16.0.
-    if (p.n >= 32768 || p.blocks <= 16) launch_strips<2, 1>(p, st);
-    else launch_strips<1, 4>(p, st);
-  } else if (panels && p.k <= 64) {
-    launch_panels<2>(p, st);
+  } else if (p.blocks <= 4) {
+    if (p.m <= 16) launch_rows<U, 1, 1>(p, st);
+    else if (lines && bytes >= 96e6 && !p.stream) launch_panels<2>(p, st);
+    else if (p.m <= 32) launch_rows<U, 2, 1>(p, st);
+    else launch_rows<U, 4, 1>(p, st);
+  } else if (p.blocks <= 8 && p.m <= 32) {
+    // (strips: 16 x 300,000 x 200 to 16 bits 13.9 us, here 9.1; tiles: 32 x 300,000 x 200 20, here 11; 64 x 144,162 x 256 11, here 15)
+    if (p.m <= 16) launch_rows<U, 1, 2>(p, st);
+    else launch_rows<U, 2, 2>(p, st);
+  } else if (p.blocks <= 16 && p.m <= 16) {
+    // (tiles: 16 x 500,000 x 384 34 us, here 24; of 32 rows they take 9.7 for 100,000 x 512, strips 12.3)
+    launch_strips<2, 1, 1>(p, st);
+  } else if (p.m <= 32 && direct && tiles(64) < 1 << 23) {
+    // (strips and tiles through registers, us: 1 x 100,000 x 1,024: 14.0, 14.0, here 12.1; 1 x 16,384 x 16,384: 42, 70, here 37)
+    if (four) launch_deep<64, 64, 2, 2, 4, 4, false>(p, st);
+    else launch_deep<64, 64, 2, 2, 4, 1, false>(p, st);
+  } else if (p.m <= 32 && p.n <= 8192 && strip_lds(p.blocks, 1, 2, 4) <= 150 * 1024) {
+    // A strip's blocks over four waves where tiles are too few.  Measured, us, with tiles and so: 32 x 4,000 x 4,001: 16.7, 12.7; 2,001: 9.4,
+    // 8.0; 32 x 20,000 x 1,001: 7.3, 11.9.
+    if (p.m <= 16) launch_strips<1, 1, 4>(p, st);
+    else launch_strips<1, 2, 4>(p, st);
   } else if (panels && p.k <= 128) {
     launch_panels<4>(p, st);
   } else if (panels && p.k <= 256) {
@@ -1033,16 +1121,18 @@ void product(const Product<O>& p, hipStream_t st) {
     // Where scales come a word at a time (k no multiple of 512) and rows are long, each word's line is fetched again for
     // the next: 4,096 x 4,096 x 4,224: 55, 83, 148, 65, -; 2,048: -, 45, 76, 35, 57; 1,024: -, 25, 40, 29, 34; 512: -, 18,
     // 21, 24, 18; 64: -, 13, 9, 20, 12; 1,024 x 4,096 x 1,152: -, 8.7, 11.2, 10.9, 10.1.
+    // Up to 64 rows, tiles of 64 (64 x 50,000 x 768: 8.3, with tiles of 128 10.5; 64 x 300,000 x 1,024: 48, 56).
     // Tiles of 256 where they are filled to 80 % and fill the CUs' turns so (as for 8-bit rows).
+    const bool narrow = std::min(p.m, p.n) <= 64;
     const int64_t turns = (tiles(256) + 255) / 256;
     const bool fill = (double)p.m * p.n >= 0.8 * 65536 * 256 * turns && tiles(256) < int64_t{1} << 31;
     if (four && fill) launch_deep<256, 256, 2, 2, 4, 4, true>(p, st);
     else if (direct && fill) launch_deep<256, 256, 2, 2, 4, 1, true>(p, st);
     else if (four && tiles(64) <= 512) launch_deep<64, 64, 2, 2, 4, 4, false>(p, st);
-    else if (four && tiles(128) < 1 << 23) launch_deep<128, 128, 2, 2, 4, 4, false>(p, st);
+    else if (four && !narrow && tiles(128) < 1 << 23) launch_deep<128, 128, 2, 2, 4, 4, false>(p, st);
     else if (direct && tiles(64) <= 128) launch_deep<64, 64, 2, 2, 4, 1, false>(p, st);
-    else if (direct && tiles(128) <= 256) launch_deep<128, 128, 2, 2, 4, 1, false>(p, st);
-    else if (tiles(64) <= 512) launch_tiles<64, 64, 2, 2, false>(p, st);
+    else if (direct && !narrow && tiles(128) <= 256) launch_deep<128, 128, 2, 2, 4, 1, false>(p, st);
+    else if (narrow || tiles(64) <= 512) launch_tiles<64, 64, 2, 2, false>(p, st);
     else launch_tiles<128, 128, 2, 2, false>(p, st);
   }
 }

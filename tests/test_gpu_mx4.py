@@ -260,6 +260,39 @@ def test_product_exact(scoring, m, n, k):
         assert torch.equal(scoring.mx4_product(a, sa, b, sb, dtype=dtype), want.float().to(dtype))
 
 
+def _check_exact(scoring, m, n, k, dtype, with_bias):
+    """Sums, and a bias in whole units of theirs, that fp32 holds, and fp32 products of the reference too."""
+    a, sa, b, sb, bias = _inputs(m, n, k, m + 3 * n + 5 * k, near=True)
+    assert 6 * 6 * 16 * (k + 1) < 2 ** 24
+    bias = (bias * 16).round() / 16 if with_bias else None
+    out = scoring.mx4_product(a, sa, b, sb, bias=bias, dtype=dtype)
+    want = values_of(a, sa, 2 * a.shape[1]).float() @ values_of(b, sb, 2 * b.shape[1]).float().T.contiguous()
+    assert torch.equal(out, (want if bias is None else want + bias).to(dtype))
+
+
+@pytest.mark.parametrize("dtype", TYPES)
+@pytest.mark.parametrize("m, n, k", [(1000, 300, 100), (5000, 70, 128), (2001, 33, 64), (130, 1, 32), (77, 4097, 40), (31, 63, 200),
+                                     (32, 5000, 256), (3, 20_000, 640), (32, 5000, 1024), (17, 9000, 1152), (16, 4000, 4001),
+                                     (30, 3000, 2001), (24, 9001, 1001), (9, 777, 500), (64, 40_000, 768), (50, 40_001, 1024),
+                                     (40_000, 64, 640), (90_001, 17, 128)])
+def test_product_few_rows_or_columns(scoring, dtype, m, n, k):
+    say("4-bit product", dtype, m, n, k)
+    _check_exact(scoring, m, n, k, dtype, m % 2 == 1)
+
+
+@pytest.mark.parametrize("m, n, k, dtype", [
+    (1000, 50_001, 100, torch.float16), (70, 720_001, 32, torch.bfloat16), (17, 1_500_001, 64, torch.float32),
+    (129, 375_000, 130, torch.bfloat16), (300, 160_000, 256, torch.float16), (130, 150_001, 450, torch.float32),
+    (66, 300_032, 512, torch.float32), (16, 600_032, 96, torch.float32), (50, 400_064, 128, torch.float16),
+    (30, 600_064, 200, torch.bfloat16), (31, 300_001, 250, torch.float32), (10, 900_032, 400, torch.float32),
+    (13, 1_300_001, 300, torch.float16), (101, 100_032, 128, torch.float32), (64, 300_001, 100, torch.float16),
+    (60, 300_000, 384, torch.bfloat16)])
+def test_product_large_results(scoring, m, n, k, dtype):
+    """Results of more than the caches hold, of whole lines and others."""
+    say("4-bit product, large results", m, n, k, dtype)
+    _check_exact(scoring, m, n, k, dtype, n % 2 == 1)
+
+
 @pytest.mark.parametrize("dtype", TYPES)
 @pytest.mark.parametrize("m, n, k, bias", [(260, 60001, 640, True), (300, 60160, 768, False), (257, 98000, 896, True),
                                            (512, 60000, 1024, False), (513, 61000, 1152, True)])
