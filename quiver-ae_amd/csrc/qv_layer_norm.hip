@@ -313,17 +313,24 @@ __global__ __launch_bounds__(THREADS) void norm_grad_kernel(const T* x, int64_t 
   const float per = 1.f / (float)dim;
   const int64_t step = (int64_t)gridDim.x * kGroups;
   int64_t row = (int64_t)blockIdx.x * kGroups + group;
-  // (a row ahead, as norm_kernel's, takes registers for which fewer waves run: 90 -> 104 us for 65,536 x 1,024 of 16 bits)
-  for (int64_t base = (int64_t)blockIdx.x * kGroups; base < n; base += step, row += step) {
-    Part<T, R, E> part, part_g;
+  // A row of 16 bits ahead, as in norm_kernel, where few waves run anyway (5,000 x 12,288: 131 -> 111 us, 16,641 x 768: 27 -> 26);
+  // else it takes registers for which fewer would (65,536 x 1,024 of 16 bits: 90 -> 104, 16,384 x 768 floats: 39 -> 44).
+  constexpr bool kAhead = THREADS == 512 && sizeof(T) == 2;
+  Part<T, R, E> part, part_g;
+  auto load = [&](int64_t row) {
     part.load(x + min(row, n - 1) * stride, lane, dim);
     part_g.load(grad + min(row, n - 1) * grad_stride, lane, dim);
+  };
+  if (kAhead) load(row);
+  for (int64_t base = (int64_t)blockIdx.x * kGroups; base < n; base += step, row += step) {
+    if (!kAhead) load(row);
     f4 v[E], g[E];
 #pragma unroll
     for (int e = 0; e < E; e++) {
       v[e] = part.values(e, lane, dim);
       g[e] = part_g.values(e, lane, dim);
     }
+    if (kAhead && base + step < n) load(row + step);
     auto again = [&](int e) {
       Part<T, R, E> same;
       same.load(x + min(row, n - 1) * stride, lane, dim);
