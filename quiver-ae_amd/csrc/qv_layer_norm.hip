@@ -538,6 +538,13 @@ constexpr Grid grad_grid(int64_t n, int r) {
   return {threads, std::min<int64_t>((n + groups - 1) / groups, few ? 256 : r <= 256 ? 768 : 512)};
 }
 
+// f(r, vectors), r one of R, 2 R, ... MOST.
+template <int R, int MOST, class F, class E>
+void with_threads(int64_t r, F f, E vectors) {
+  if (r == R) f(std::integral_constant<int, R>(), vectors);
+  else if constexpr (R < MOST) with_threads<2 * R, MOST>(r, f, vectors);
+}
+
 // f(threads per row, vectors per thread) for rows of `dim`, with one of the given numbers of vectors: the fewest places
 // for them (those past the row stay idle), the number named first if there are several; at most MOST threads.
 // Measured with 1 to 8 vectors: values of 16 bits take 12 to 35 % more with one or two of them, 10 % more with six or eight,
@@ -555,25 +562,19 @@ void by_width(int64_t dim, F f) {
   auto go = [&](auto vectors) {
     using E = decltype(vectors);
     if (E::value != best) return;
-    if (r == 4) f(std::integral_constant<int, 4>(), E());
-    else if (r == 8) f(std::integral_constant<int, 8>(), E());
-    else if (r == 16) f(std::integral_constant<int, 16>(), E());
-    else if (r == 32) f(std::integral_constant<int, 32>(), E());
-    else if (r == 64) f(std::integral_constant<int, 64>(), E());
-    else if (r == 128) f(std::integral_constant<int, 128>(), E());
-    else if (r == 256) f(std::integral_constant<int, 256>(), E());
-    else if (r == 512) f(std::integral_constant<int, 512>(), E());
-    else if constexpr (MOST == 1024) f(std::integral_constant<int, 1024>(), E());
+    with_threads<4, MOST>(r, f, E());
   };
   go(std::integral_constant<int, FIRST>());
   (go(std::integral_constant<int, MORE>()), ...);
 }
 
 // The same for the gradient.  Past 8,192 six vectors: 1,024 threads would not have the registers (5,000 x 12,288 of 16 bits:
-// 126 us, with 1,024 threads 185, as long rows 246).
+// 126 us, with 1,024 threads 185, as long rows 246).  Rows of up to 64 values one or two vectors, or three
+// (with four: 1M x 64 of 16 bits 148 us, here 90; 1M x 32 65, 52; 2M x 16 114, 69; 500,000 x 64 floats 93, 80).
 template <class F>
 void by_grad_width(int64_t dim, F f) {
   if (dim > 8192) f(std::integral_constant<int, 512>(), std::integral_constant<int, 6>());
+  else if (dim <= 64) by_width<8, 2, 3, 1>(dim, f);
   else by_width<512, 4, 3>(dim, f);
 }
 
@@ -615,7 +616,12 @@ void norm(const void* x, int64_t n, int64_t dim, int64_t stride, const void* wei
     };
     // Short rows of floats that are no whole lines: one vector per thread where that takes no more of them (500,000 x 100:
     // 90 us, with four vectors 117, 300,000 x 200: 108, 115; whole lines the other way: 500,000 x 128: 106, 99).
-    if (sizeof(T) == 4 && dim <= 256 && dim % 32) by_width<1024, 1, 3, 4>(dim, go);
+    // And rows of up to 64 values: floats one vector (1M x 64: 93 us, with four 105; 1M x 48: 76, with three 92; 2M x 32: 92, 126), 16 bits two
+    // of more than 32 values (1M x 64: 61, with four 113) or one (3M x 16: 49, with three 79).
+    if (sizeof(T) == 4 && dim <= 64) by_width<16, 1>(dim, go);
+    else if (dim <= 32) by_width<8, 1>(dim, go);
+    else if (dim <= 64) by_width<8, 2, 3>(dim, go);
+    else if (sizeof(T) == 4 && dim <= 256 && dim % 32) by_width<64, 1, 3, 4>(dim, go);
     else by_width<1024, 3, 4>(dim, go);
   }
   HIP_OK(hipGetLastError());

@@ -186,6 +186,16 @@ def test_huge_rows(scoring, dtype, n, d):
     _check_grad(replace(r, x=None), x, grad, weight, torch.float32)
 
 
+@pytest.mark.parametrize("dtype", TYPES)
+@pytest.mark.parametrize("n", [1, 1000, 70_001])
+@pytest.mark.parametrize("d", [8, 15, 16, 17, 24, 31, 32, 33, 40, 47, 48, 50, 63, 64])
+def test_short_rows(scoring, dtype, n, d):
+    say("layer norm, short rows", dtype, n, d)
+    x, weight, bias, grad = _rows(n, d, dtype, n + d)
+    _check_forward(scoring.layer_norm(x, weight, bias), x, weight, bias)
+    _check_grad(scoring.layer_norm_grad(x, grad, weight), x, grad, weight, torch.float32)
+
+
 @pytest.mark.parametrize("value", [3e15, -2.0 ** 125, torch.finfo(torch.float32).max])
 @pytest.mark.parametrize("d", [2, 7, 64, 100, 1000, 1024, 4096, 5000, 12288, 16384, 20000, 65536])
 def test_equal_values(scoring, d, value):
