@@ -96,6 +96,13 @@ def _matrix(name: str, t: torch.Tensor, types) -> tuple[int, int, int]:
     return rows, cols, stride if rows > 1 else max(cols, 1)
 
 
+def _whole(t: torch.Tensor) -> None:
+    """Refuses a tensor whose memory was cut below its elements (``untyped_storage().resize_``)."""
+    last = t.storage_offset() + sum((size - 1) * step for size, step in zip(t.shape, t.stride()))
+    if t.numel() and (last + 1) * t.element_size() > t.untyped_storage().nbytes():
+        raise ValueError("a result's memory was made smaller than the result")
+
+
 def _vector(name: str, t: torch.Tensor, shape: tuple, dtype=torch.float32) -> int:
     if t.dtype != dtype or t.shape != shape or not t.is_contiguous():
         raise ValueError(f"{name} must be a contiguous {dtype} tensor of shape {shape}")
@@ -516,9 +523,9 @@ class LayerNormGrad:
     weight: torch.Tensor | None  # [d] of the weight's type
     bias: torch.Tensor | None    # [d] of the weight's type
     _workspace: torch.Tensor
-    _written: tuple              # the first three that are there
     _made_for: tuple             # rows, columns, types of x and weight
     _at: tuple                   # addresses of the first three (and x's row stride), the workspace and its bytes
+    _strides: tuple | None       # of x
     _device: int
 
     @staticmethod
@@ -546,12 +553,31 @@ class LayerNormGrad:
             at_x = x.data_ptr()
         at_weight, at_bias = (None if p is None else _vector(name, p, (d,), param_dtype)
                               for name, p in (("out.weight", weight), ("out.bias", bias)))
-        written = tuple(t for t in (x, weight, bias) if t is not None)
         device = workspace.get_device()
-        if any(t.get_device() != device for t in written):
+        if any(t is not None and t.get_device() != device for t in (x, weight, bias)):
             raise ValueError("tensors must be on one GPU")
-        return LayerNormGrad(x, weight, bias, workspace, written, made_for,
-                             (at_x, stride, at_weight, at_bias, workspace.data_ptr(), workspace.shape[0]), device)
+        return LayerNormGrad(x, weight, bias, workspace, made_for,
+                             (at_x, stride, at_weight, at_bias, workspace.data_ptr(), workspace.shape[0]),
+                             None if x is None else x.stride(), device)
+
+    def _now(self) -> tuple:
+        """(addresses, device), taken again where a tensor is no longer what they were taken of: its memory can be
+        another's after ``t.data = ...``, ``set_`` or ``resize_`` (as ``Module.to`` does to a parameter's gradient)."""
+        x, weight, bias, (n, d, dtype, param_dtype) = self.x, self.weight, self.bias, self._made_for
+        at_x, _, at_weight, at_bias, at_work, _ = self._at
+        if ((at_x is None if x is None else x.data_ptr() == at_x and x.shape == (n, d) and x.stride() == self._strides
+             and x.dtype is dtype)
+                and (at_weight is None if weight is None else weight.data_ptr() == at_weight and weight.numel() == d
+                     and weight.is_contiguous() and weight.dtype is param_dtype)
+                and (at_bias is None if bias is None else bias.data_ptr() == at_bias and bias.numel() == d
+                     and bias.is_contiguous() and bias.dtype is param_dtype)
+                and self._workspace.data_ptr() == at_work):
+            return self._at, self._device
+        for t in (x, weight, bias, self._workspace):
+            if t is not None:
+                _whole(t)
+        same = LayerNormGrad.of(x, weight, bias, self._workspace, self._made_for)
+        return same._at, same._device
 
 
 def _norm_grad(x, grad, weight, eps, dtype, wanted, out) -> LayerNormGrad:
@@ -559,19 +585,30 @@ def _norm_grad(x, grad, weight, eps, dtype, wanted, out) -> LayerNormGrad:
     grad_rows, grad_cols, grad_stride = _matrix("grad", grad, (x.dtype,))
     if grad_rows != n or grad_cols != d:
         raise ValueError("grad and x differ in shape")
-    at_weight = None if weight is None else _param("weight", weight, d, None)
+    if weight is None:
+        at_weight = None
+    elif weight.numel() == d and weight.dim() == 1 and weight.is_contiguous() and weight.dtype in _TYPES:
+        at_weight = weight.data_ptr()
+    else:
+        at_weight = _param("weight", weight, d, None)
     again = out is not None
     if again and out._made_for != (n, d, x.dtype, dtype):
         raise ValueError("out was made for another number of rows or columns, or other types")
     device = _device(x, grad) if weight is None else _device(x, grad, weight)
     if not again:
         out = LayerNormGrad.empty(n, d, x.dtype, dtype, wanted, x.device)
-    elif out._device != device:
-        raise ValueError("tensors must be on one GPU")
+        at = out._at
+    else:
+        at, made_on = out._now()
+        if made_on != device:
+            raise ValueError("tensors must be on one GPU")
     _lib.check(_lib.load().qv_layer_norm_grad(x.data_ptr(), _TYPES[x.dtype], n, d, stride, grad.data_ptr(), grad_stride,
-                                              at_weight, _TYPES[dtype], eps, *out._at, device, _raw_stream(device)))
+                                              at_weight, _TYPES[dtype], eps, *at, device, _raw_stream(device)))
     if again:
-        _written(out._written)
+        to = (out.x, out.weight, out.bias)
+        if to[0] is None or to[1] is None or to[2] is None:
+            to = [t for t in to if t is not None]
+        _written(to)
     return out
 
 
@@ -644,9 +681,11 @@ def layer_norm_grad(x: torch.Tensor, grad: torch.Tensor, weight: torch.Tensor | 
     ``torch.no_grad()``).
     """
     again = out is not None
+    to = (out.x, out.weight, out.bias) if again else (None, None, None)
     if (x.requires_grad or grad.requires_grad or weight is not None and weight.requires_grad
-            or forward_ad._current_level >= 0 or again and any([t.requires_grad for t in out._written])):
-        _no_derivative("layer_norm_grad", x, grad, weight, *(out._written if again else ()))
+            or forward_ad._current_level >= 0 or to[0] is not None and to[0].requires_grad
+            or to[1] is not None and to[1].requires_grad or to[2] is not None and to[2].requires_grad):
+        _no_derivative("layer_norm_grad", x, grad, weight, *to)
     if wanted is None:
         wanted = (True, True, True)
     elif again:

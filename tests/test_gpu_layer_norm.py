@@ -479,3 +479,24 @@ def test_example(scoring):
     # gradient is a sum of probabilities (as much off, relatively) times values, and the loss's other sums' errors are far less
     for got, want in zip(leaves, exact):
         assert ((got.grad.double() - want.grad).abs() <= 2.0 ** -8 * want.grad.abs().max()).all()
+
+
+def test_results_follow_their_memory(scoring):
+    """Where a result's tensors were given other memory, a call writes to that and leaves the old alone; or it is refused."""
+    say("layer norm, results in other memory")
+    x, weight, _, grad = _rows(40, 96, torch.float32, 5)
+    want, r = scoring.layer_norm_grad(x, grad, weight), scoring.layer_norm_grad(x, grad, weight)
+    old = [t.detach() for t in (r.x, r.weight, r.bias)]
+    for t in (r.x, r.weight, r.bias):
+        t.data = torch.zeros_like(t)
+    for t in old:
+        t.fill_(7.0)
+    assert scoring.layer_norm_grad(x, grad, weight, out=r) is r
+    assert all((t == 7).all() for t in old)
+    assert torch.equal(r.x, want.x) and torch.equal(r.weight, want.weight) and torch.equal(r.bias, want.bias)
+    r.weight.data = r.weight.data.half()
+    with pytest.raises(ValueError, match="out.weight must be"):
+        scoring.layer_norm_grad(x, grad, weight, out=r)
+    r.weight.data = torch.zeros(96)  # on the CPU
+    with pytest.raises(ValueError, match="on one GPU"):
+        scoring.layer_norm_grad(x, grad, weight, out=r)

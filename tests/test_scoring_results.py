@@ -1,0 +1,114 @@
+"""Results that are written again (out=): where a tensor's memory has changed hands, calls write to what it holds now."""
+from __future__ import annotations
+
+from dataclasses import replace
+
+import pytest
+import torch
+
+
+class Recorder:
+    """In the library's place: takes the addresses that calls pass on."""
+
+    def qv_layer_norm_grad_workspace(self, n, d):
+        return 64
+
+    def qv_layer_norm_grad(self, *a):
+        self.grad = dict(x=a[10], stride=a[11], weight=a[12], bias=a[13], workspace=a[14])
+        return 0
+
+
+@pytest.fixture
+def recorder(monkeypatch):
+    from quiver import scoring
+
+    r = Recorder()
+    monkeypatch.setattr(scoring._lib, "load", lambda: r)
+    monkeypatch.setattr(scoring, "_device", lambda first, *others: first.get_device())
+    monkeypatch.setattr(scoring, "_raw_stream", lambda device: None)
+    return r
+
+
+N, D = 6, 8
+
+
+def _gradients():
+    from quiver import scoring
+
+    x = torch.zeros(N, D)
+    r = scoring.layer_norm_grad(x, x, torch.zeros(D))
+    return lambda out=r: scoring.layer_norm_grad(x, x, torch.zeros(D), out=out), r
+
+
+def _replaced(t, how):
+    """Gives `t` other memory of the same shape, as torch lets a program do."""
+    if how == "data":
+        t.data = torch.ones_like(t)
+    elif how == "set_":
+        t.set_(torch.ones_like(t))
+    elif how == "resize_":
+        shape = t.shape
+        t.resize_(1000)
+        t.resize_(shape)
+    elif how == "storage":
+        size = t.untyped_storage().nbytes()
+        t.untyped_storage().resize_(4 * size)
+    elif how == "module":  # a parameter's gradient, whose module is moved there and back
+        parameter = torch.nn.Parameter(torch.zeros_like(t))
+        parameter.grad = t
+        module = torch.nn.Module()
+        module.p = parameter
+        module.double().float()
+        assert parameter.grad is t
+
+
+@pytest.mark.parametrize("how", ["data", "set_", "resize_", "storage", "module"])
+@pytest.mark.parametrize("part", ["x", "weight", "bias"])
+def test_gradients_follow_their_memory(recorder, part, how):
+    call, r = _gradients()
+    old = getattr(r, part)
+    kept, at = old.detach(), old.data_ptr()  # kept, so that its address is not given out again
+    _replaced(old, how)
+    assert call() is r and kept is not None
+    for p in ("x", "weight", "bias"):
+        assert recorder.grad[p] == getattr(r, p).data_ptr()
+    assert recorder.grad[part] != at
+
+
+def test_gradients_in_wider_rows(recorder):
+    """A result of rows inside a wider matrix is written with its own stride."""
+    call, r = _gradients()
+    r.x.data = torch.zeros(N, 2 * D)[:, 3:3 + D]
+    call()
+    assert recorder.grad["x"] == r.x.data_ptr() and recorder.grad["stride"] == 2 * D
+    r.x.data = torch.zeros(N, D)
+    call()
+    assert recorder.grad["x"] == r.x.data_ptr() and recorder.grad["stride"] == D
+    without = replace(r, x=None)
+    call(without)
+    assert recorder.grad["x"] is None and recorder.grad["bias"] == r.bias.data_ptr()
+
+
+@pytest.mark.parametrize("part, change, text", [
+    ("weight", lambda t: t.data.half(), "out.weight must be"), ("bias", lambda t: t.data.half(), "out.bias must be"),
+    ("x", lambda t: t.data.half(), "out.x has the type"), ("weight", lambda t: t.data[:D - 1], "out.weight must be"),
+    ("bias", lambda t: torch.zeros(2 * D)[::2], "out.bias must be"), ("x", lambda t: t.data[:, :D - 1], "out.x has another"),
+    ("x", lambda t: t.data[:N - 1], "out.x has another"), ("x", lambda t: t.data.reshape(D, N), "out.x has another"),
+    ("x", lambda t: torch.zeros(D, N).T, "out.x must be contiguous"),
+    ("weight", lambda t: t.data.view(torch.int32), "out.weight must be")])
+def test_gradients_of_another_form_are_refused(recorder, part, change, text):
+    call, r = _gradients()
+    call()
+    del recorder.grad
+    t = getattr(r, part)
+    t.data = change(t)
+    with pytest.raises(ValueError, match=text):
+        call()
+    assert not hasattr(recorder, "grad")
+
+
+def test_gradients_of_less_memory_are_refused(recorder):
+    call, r = _gradients()
+    r.weight.untyped_storage().resize_(8)
+    with pytest.raises(ValueError, match="made smaller"):
+        call()
