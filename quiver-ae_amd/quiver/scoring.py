@@ -46,6 +46,9 @@ _PACKED = (torch.uint8,)
 # repeated shapes).
 _raw_stream = torch._C._cuda_getCurrentRawStream
 
+# Of results that are kept with their addresses.
+_address, _count = torch.Tensor.data_ptr, torch.Tensor.numel
+
 # For tensors given as out=: autograd then refuses a backward pass that needs what they held.
 _written = torch._C._increment_version
 
@@ -296,8 +299,8 @@ class LogProbs:
     temperature: float
     _workspace: torch.Tensor
     _device: int
-    _parts: tuple            # the buffers in the order above, the workspace last
-    _at: tuple               # their addresses
+    _at: tuple               # addresses of the buffers in the order above, the workspace last
+    _counts: tuple           # of their elements, but the workspace's
     _size: tuple             # rows, targets and alternatives per row, bytes of the workspace
 
     @staticmethod
@@ -323,8 +326,29 @@ class LogProbs:
     @staticmethod
     def of(target, entropy, logsumexp, top_ids, top, stats, temperature, workspace) -> "LogProbs":
         parts = (target, entropy, logsumexp, top_ids, top, stats, workspace)
-        return LogProbs(target, entropy, logsumexp, top_ids, top, stats, temperature, workspace, stats.get_device(),
-                        parts, tuple(p.data_ptr() for p in parts), (*target.shape, top.shape[1], workspace.shape[0]))
+        return LogProbs(*parts[:-1], temperature, workspace, stats.get_device(), tuple(map(_address, parts)),
+                        tuple(map(_count, parts[:-1])), (*target.shape, top.shape[1], workspace.shape[0]))
+
+    def _parts(self) -> tuple:
+        return self.target, self.entropy, self.logsumexp, self.top_ids, self.top, self.stats, self._workspace
+
+    def _now(self) -> tuple:
+        """(addresses, device), taken again where a tensor is no longer what they were taken of: its memory can be
+        another's after ``t.data = ...``, ``set_`` or ``resize_``."""
+        a, b, c, d, e, f, g = parts = self._parts()
+        if ((a.data_ptr(), b.data_ptr(), c.data_ptr(), d.data_ptr(), e.data_ptr(), f.data_ptr(), g.data_ptr()) == self._at
+                and (a.numel(), b.numel(), c.numel(), d.numel(), e.numel(), f.numel()) == self._counts):
+            return self._at, self._device
+        n, t, k, nbytes = self._size
+        ids, number = torch.int32, torch.float32
+        for name, part, shape, dtype in zip(("target", "entropy", "logsumexp", "top_ids", "top", "stats", "workspace"), parts,
+                                            ((n, t), (n,), (n,), (n, k), (n, k), (n, 2), (nbytes,)),
+                                            (number, number, number, ids, number, number, self._workspace.dtype)):
+            _vector(f"out.{name}", part, shape, dtype)
+            _whole(part)
+            if part.get_device() != parts[0].get_device():
+                raise ValueError("tensors must be on one GPU")
+        return tuple(map(_address, parts)), parts[0].get_device()
 
 
 def _given(targets: torch.Tensor | None, rows: int) -> tuple[int | None, int]:
@@ -348,14 +372,15 @@ def _forward(logits, targets, top_k, temperature, out) -> LogProbs:
     elif out.temperature != temperature:
         out = replace(out, temperature=temperature)
     device = _device(logits) if targets is None else _device(logits, targets)
-    if device != out._device:
+    at, made_on = out._now() if again else (out._at, out._device)
+    if device != made_on:
         raise ValueError("tensors must be on one GPU")
-    at_target, at_entropy, at_lse, at_ids, at_top, at_stats, at_work = out._at
+    at_target, at_entropy, at_lse, at_ids, at_top, at_stats, at_work = at
     _lib.check(_lib.load().qv_log_probs(logits.data_ptr(), _TYPES[logits.dtype], n, v, stride, temperature, at_targets,
                                         t, top_k, at_target, at_entropy, at_lse, at_stats, at_ids, at_top, at_work,
                                         out._size[3], device, _raw_stream(device)))
     if again:
-        _written(out._parts)
+        _written(out._parts())
     return out
 
 
@@ -475,11 +500,11 @@ def log_probs_grad(logits: torch.Tensor, result: LogProbs, targets: torch.Tensor
             or grad_top is not None and grad_top.requires_grad or out is not None and out.requires_grad
             or forward_ad._current_level >= 0):
         _no_derivative("log_probs_grad", logits, grad_target, grad_entropy, grad_logsumexp, grad_top, out)
-    if result.entropy.shape[0] != logits.shape[0]:
+    if result._size[0] != logits.shape[0]:
         raise ValueError("result was made for another number of rows")
-    _, at_entropy, _, at_ids, _, at_stats, _ = result._at
-    return _gradient(logits, at_stats, at_entropy, at_ids, result.top.shape[1], result._device, result.temperature,
-                     targets, grad_target, grad_entropy, grad_logsumexp, grad_top, out)
+    (_, at_entropy, _, at_ids, _, at_stats, _), device = result._now()
+    return _gradient(logits, at_stats, at_entropy, at_ids, result._size[2], device, result.temperature, targets,
+                     grad_target, grad_entropy, grad_logsumexp, grad_top, out)
 
 
 def _param(name: str, p: torch.Tensor, dim: int, dtype: torch.dtype | None) -> int:

@@ -645,3 +645,26 @@ def nan_matches_nan_only(monkeypatch):
         near(got, want, slack, what)
 
     monkeypatch.setattr(sys.modules[__name__], "_near", strict)
+
+
+def test_results_follow_their_memory(scoring):
+    """Where a result's tensors were given other memory, a call writes to that and leaves the old alone; or it is refused."""
+    say("log probs, results in other memory")
+    x, targets = _inputs(torch.float32, 50, 300, 1, 2)
+    parts = ("target", "entropy", "logsumexp", "top_ids", "top", "stats")
+    want, r = scoring.log_probs(x, targets, top_k=5), scoring.log_probs(x, targets, top_k=5)
+    old = [getattr(r, p).detach() for p in parts]
+    for p in parts:
+        getattr(r, p).data = torch.zeros_like(getattr(r, p))
+    for t in old:
+        t.fill_(7)
+    assert scoring.log_probs(x, targets, top_k=5, out=r) is r
+    assert all((t == 7).all() for t in old)
+    assert all(torch.equal(getattr(r, p), getattr(want, p)) for p in parts)
+    g = torch.ones((50, 1), device="cuda")
+    assert torch.equal(scoring.log_probs_grad(x, r, targets, grad_target=g), scoring.log_probs_grad(x, want, targets, grad_target=g))
+    r.entropy.data = torch.zeros(50)  # on the CPU
+    for call in (lambda: scoring.log_probs(x, targets, top_k=5, out=r),
+                 lambda: scoring.log_probs_grad(x, r, targets, grad_target=g)):
+        with pytest.raises(ValueError, match="on one GPU"):
+            call()

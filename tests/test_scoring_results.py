@@ -17,6 +17,17 @@ class Recorder:
         self.grad = dict(x=a[10], stride=a[11], weight=a[12], bias=a[13], workspace=a[14])
         return 0
 
+    def qv_log_probs_workspace(self, n, v, k):
+        return 64
+
+    def qv_log_probs(self, *a):
+        self.log_probs = dict(target=a[9], entropy=a[10], logsumexp=a[11], stats=a[12], top_ids=a[13], top=a[14])
+        return 0
+
+    def qv_log_probs_grad(self, *a):
+        self.log_probs_grad = dict(stats=a[6], entropy=a[7], top_ids=a[10])
+        return 0
+
 
 @pytest.fixture
 def recorder(monkeypatch):
@@ -112,3 +123,59 @@ def test_gradients_of_less_memory_are_refused(recorder):
     r.weight.untyped_storage().resize_(8)
     with pytest.raises(ValueError, match="made smaller"):
         call()
+
+
+PARTS = ("target", "entropy", "logsumexp", "top_ids", "top", "stats")
+
+
+def _log_probs():
+    from quiver import scoring
+
+    new = [torch.zeros(shape, dtype=dtype) for shape, dtype in (
+        ((N, 1), torch.float32), ((N,), torch.float32), ((N,), torch.float32), ((N, 2), torch.int32), ((N, 2), torch.float32),
+        ((N, 2), torch.float32))]
+    r = scoring.LogProbs.of(*new, 1.0, torch.zeros(64, dtype=torch.uint8))
+    x, targets = torch.zeros(N, D), torch.zeros(N, 1, dtype=torch.int32)
+    return (lambda: scoring.log_probs(x, targets, top_k=2, out=r),
+            lambda: scoring.log_probs_grad(x, r, targets, grad_target=torch.ones(N, 1)), r)
+
+
+@pytest.mark.parametrize("how", ["data", "set_", "resize_", "storage"])
+@pytest.mark.parametrize("part", PARTS)
+def test_log_probs_follow_their_memory(recorder, part, how):
+    """... and their gradient reads what the result holds now."""
+    call, gradient, r = _log_probs()
+    old = getattr(r, part)
+    kept, at = old.detach(), old.data_ptr()
+    _replaced(old, how)
+    assert call() is r and kept is not None
+    for p in PARTS:
+        assert recorder.log_probs[p] == getattr(r, p).data_ptr()
+    assert recorder.log_probs[part] != at
+    gradient()
+    for p in ("stats", "entropy", "top_ids"):
+        assert recorder.log_probs_grad[p] == getattr(r, p).data_ptr()
+
+
+@pytest.mark.parametrize("part, change", [
+    ("target", lambda t: t.data.half()), ("entropy", lambda t: t.data[:N - 1]), ("logsumexp", lambda t: torch.zeros(2 * N)[::2]),
+    ("top_ids", lambda t: t.data.long()), ("top", lambda t: t.data[:, :1]), ("stats", lambda t: torch.zeros(2, N).T),
+    ("entropy", lambda t: t.data.view(torch.float16))])
+def test_log_probs_of_another_form_are_refused(recorder, part, change):
+    call, gradient, r = _log_probs()
+    call()
+    gradient()
+    del recorder.log_probs, recorder.log_probs_grad
+    getattr(r, part).data = change(getattr(r, part))
+    for f in (call, gradient):
+        with pytest.raises(ValueError, match=f"out.{part} must be"):
+            f()
+    assert not hasattr(recorder, "log_probs") and not hasattr(recorder, "log_probs_grad")
+
+
+def test_log_probs_of_less_memory_are_refused(recorder):
+    call, gradient, r = _log_probs()
+    r.stats.untyped_storage().resize_(8)
+    for f in (call, gradient):
+        with pytest.raises(ValueError, match="made smaller"):
+            f()
