@@ -1036,14 +1036,17 @@ void launch_panels(const Product<O>& p, hipStream_t st) {
   HIP_OK(hipGetLastError());
 }
 
-int strip_lds(int64_t blocks, int u, int tm, int wk) {
-  return (int)((blocks + 3) / 4) * tm * 1088 + (wk > 1 ? wk * tm * u * 1024 : 0);
+// In 64 bits: rows may have 2^26 blocks.
+int64_t strip_lds(int64_t blocks, int u, int tm, int wk) {
+  return (blocks + 3) / 4 * tm * 1088 + (wk > 1 ? wk * tm * u * 1024 : 0);
 }
 
 template <int U, int TM, int WK, class O>
 void launch_strips(const Product<O>& p, hipStream_t st) {
   const int64_t groups = (p.n + 16 * U - 1) / (16 * U);
-  const int lds = strip_lds(p.blocks, U, TM, WK);
+  const int64_t need = strip_lds(p.blocks, U, TM, WK);
+  if (need > 160 * 1024) qv::fail(QV_EUNSUPPORTED, "rows too long for strips");
+  const int lds = (int)need;
   constexpr int kThreads = WK == 1 ? 256 : 64 * WK;
   // as many workgroups as run at once
   const int64_t most = 256 * std::min(2048 / kThreads, 160 * 1024 / std::max(lds, 1));

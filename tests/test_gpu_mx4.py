@@ -510,3 +510,25 @@ def test_catalogue(scoring):
         queries, targets, top_k=10, temperature=0.05)
     assert torch.equal(whole.top_ids, parts.top_ids) and torch.equal(whole.target, parts.target)
     assert not (whole.top_ids == 17).any()
+
+
+@pytest.mark.parametrize("m, n, k", [(1, 3, 130_000_000), (20, 3, 130_000_000), (17, 2, 126_400_000), (1, 2, 260_000_000)])
+def test_longest_rows_of_a_product(scoring, m, n, k):
+    """Rows whose codes and scales no workgroup could keep in LDS, by factors that pass 31 bits; codes are 0 but for some."""
+    say("4-bit product, rows of", k)
+    g = torch.Generator(device="cuda").manual_seed(k)
+    at = torch.randint(0, k // 2, (3000,), generator=g, device="cuda").unique()
+    at = torch.cat([at, torch.tensor([0, 15, 16, k // 2 - 1], device="cuda")]).unique()
+    rows = []
+    for count in (m, n):
+        codes = torch.zeros((count, k // 2), dtype=torch.uint8, device="cuda")
+        scales = torch.full((count, -(-k // 32)), 127, dtype=torch.uint8, device="cuda")
+        scales[:, ::5] = 126
+        codes[:, at] = torch.randint(0, 256, (count, at.numel()), generator=g, device="cuda", dtype=torch.uint8)
+        grid = torch.tensor(np.concatenate([GRID, -GRID]), device="cuda")
+        there, s = codes[:, at].long(), torch.exp2(scales[:, at // 16].double() - 127)
+        rows.append((codes, scales, torch.cat([grid[there & 15] * s, grid[there >> 4] * s], 1)))
+    (a, sa, va), (b, sb, vb) = rows
+    out = scoring.mx4_product(a, sa, b, sb)
+    # sums of up to 6,008 products, each a whole number of 2^-4 and at most 36: below 2^18, so exact
+    assert torch.equal(out, (va @ vb.T.contiguous()).float())
