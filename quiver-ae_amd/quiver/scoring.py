@@ -106,6 +106,12 @@ def _whole(t: torch.Tensor) -> None:
         raise ValueError("a result's memory was made smaller than the result")
 
 
+def _bytes(workspace: torch.Tensor) -> None:
+    """A workspace's elements are counted as its bytes: they have to be there, one behind the other."""
+    if workspace.dim() != 1 or not workspace.is_contiguous():
+        raise ValueError("a workspace must be a contiguous vector")
+
+
 def _vector(name: str, t: torch.Tensor, shape: tuple, dtype=torch.float32) -> int:
     if t.dtype != dtype or t.shape != shape or not t.is_contiguous():
         raise ValueError(f"{name} must be a contiguous {dtype} tensor of shape {shape}")
@@ -326,6 +332,7 @@ class LogProbs:
     @staticmethod
     def of(target, entropy, logsumexp, top_ids, top, stats, temperature, workspace) -> "LogProbs":
         parts = (target, entropy, logsumexp, top_ids, top, stats, workspace)
+        _bytes(workspace)
         return LogProbs(*parts[:-1], temperature, workspace, stats.get_device(), tuple(map(_address, parts)),
                         tuple(map(_count, parts[:-1])), (*target.shape, top.shape[1], workspace.shape[0]))
 
@@ -578,6 +585,7 @@ class LayerNormGrad:
             at_x = x.data_ptr()
         at_weight, at_bias = (None if p is None else _vector(name, p, (d,), param_dtype)
                               for name, p in (("out.weight", weight), ("out.bias", bias)))
+        _bytes(workspace)
         device = workspace.get_device()
         if any(t is not None and t.get_device() != device for t in (x, weight, bias)):
             raise ValueError("tensors must be on one GPU")

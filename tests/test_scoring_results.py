@@ -179,3 +179,17 @@ def test_log_probs_of_less_memory_are_refused(recorder):
     for f in (call, gradient):
         with pytest.raises(ValueError, match="made smaller"):
             f()
+
+
+@pytest.mark.parametrize("workspace", [torch.zeros(1, dtype=torch.uint8).expand(1 << 20), torch.zeros(2, 64, dtype=torch.uint8),
+                                       torch.zeros(64, dtype=torch.uint8)[::2]])
+def test_workspaces_are_whole(workspace):
+    """A workspace is as many bytes as it has elements: none that repeats or skips them."""
+    from quiver import scoring
+
+    x = torch.zeros(N, D)
+    with pytest.raises(ValueError, match="workspace must be"):
+        scoring.LayerNormGrad.of(x, x[0], x[0], workspace, (N, D, torch.float32, torch.float32))
+    with pytest.raises(ValueError, match="workspace must be"):
+        scoring.LogProbs.of(x[:, :0], x[:, 0].contiguous(), x[:, 0].contiguous(), x[:, :0].int(), x[:, :0],
+                            x[:, :2].contiguous(), 1.0, workspace)
