@@ -563,20 +563,30 @@ class LayerNormGrad:
     @staticmethod
     def empty(n: int, d: int, dtype: torch.dtype, param_dtype: torch.dtype, wanted: tuple, device) -> "LayerNormGrad":
         """Buffers for the gradients that are wanted, of n rows of d values."""
-        workspace = _lib.load().qv_layer_norm_grad_workspace(n, d)
-        if workspace < 0:
-            _lib.check(workspace)
-
         def new(want, shape, type_):
             return torch.empty(shape, dtype=type_, device=device) if want else None
 
         return LayerNormGrad.of(new(wanted[0], (n, d), dtype), new(wanted[1], d, param_dtype), new(wanted[2], d, param_dtype),
-                                torch.empty(workspace, dtype=torch.uint8, device=device), (n, d, dtype, param_dtype))
+                                LayerNormGrad.workspace(n, d, device), (n, d, dtype, param_dtype))
+
+    @staticmethod
+    def workspace(n: int, d: int, device) -> torch.Tensor:
+        """What the gradients of n rows of d values need beside their buffers; several results may share one on a stream."""
+        size = _lib.load().qv_layer_norm_grad_workspace(n, d)
+        if size < 0:
+            _lib.check(size)
+        return torch.empty(size, dtype=torch.uint8, device=device)
 
     @staticmethod
     def of(x, weight, bias, workspace, made_for: tuple) -> "LayerNormGrad":
-        """Given buffers for ``made_for``: rows, columns, types of x and weight."""
+        """Given buffers (None: not wanted; a gradient's own or x's memory may be its ``x``), a workspace (None: a new one),
+        and what they are ``made_for``: rows, columns, types of x and of the weight."""
         n, d, dtype, param_dtype = made_for
+        if workspace is None:
+            there = [t for t in (x, weight, bias) if t is not None]
+            if not there:
+                raise ValueError("buffers for none of the gradients are given")
+            workspace = LayerNormGrad.workspace(n, d, there[0].device)
         at_x, stride = None, d
         if x is not None:
             rows, cols, stride = _matrix("out.x", x, (dtype,))

@@ -500,3 +500,19 @@ def test_results_follow_their_memory(scoring):
     r.weight.data = torch.zeros(96)  # on the CPU
     with pytest.raises(ValueError, match="on one GPU"):
         scoring.layer_norm_grad(x, grad, weight, out=r)
+
+
+def test_lent_buffers(scoring):
+    """The gradient in x's place and in its own, with buffers of the caller's and one workspace for several results."""
+    say("layer norm, lent buffers")
+    for n, d in ((50, 40), (9, 20000)):
+        x, weight, _, grad = _rows(n, d, torch.bfloat16, d)
+        want = scoring.layer_norm_grad(x, grad, weight)
+        made_for = (n, d, x.dtype, weight.dtype)
+        shared = scoring.LayerNormGrad.workspace(n, d, x.device)
+        for place in (0, 1):
+            for workspace in (None, shared):
+                a, b, dw, db = x.clone(), grad.clone(), torch.empty_like(weight), torch.empty_like(weight)
+                r = scoring.LayerNormGrad.of((a, b)[place], dw, db, workspace, made_for)
+                assert scoring.layer_norm_grad(a, b, weight, out=r) is r
+                assert torch.equal((a, b)[place], want.x) and torch.equal(dw, want.weight) and torch.equal(db, want.bias)

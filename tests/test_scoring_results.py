@@ -193,3 +193,20 @@ def test_workspaces_are_whole(workspace):
     with pytest.raises(ValueError, match="workspace must be"):
         scoring.LogProbs.of(x[:, :0], x[:, 0].contiguous(), x[:, 0].contiguous(), x[:, :0].int(), x[:, :0],
                             x[:, :2].contiguous(), 1.0, workspace)
+
+
+def test_lent_buffers(recorder):
+    """Buffers of a program's own, without a word of what a workspace is: None takes a new one."""
+    from quiver import scoring
+
+    x, weight, bias = torch.zeros(N, D), torch.zeros(D), torch.zeros(D)
+    made_for = (N, D, torch.float32, torch.float32)
+    for buffers in ((x, weight, bias), (x, None, None), (None, None, bias)):
+        r = scoring.LayerNormGrad.of(*buffers, None, made_for)
+        assert r._workspace.shape == (64,) and r._workspace.dtype == torch.uint8
+        scoring.layer_norm_grad(x, torch.ones_like(x), weight, out=r)
+        assert [recorder.grad[p] for p in ("x", "weight", "bias")] == [None if b is None else b.data_ptr() for b in buffers]
+        assert recorder.grad["workspace"] == r._workspace.data_ptr()
+    assert scoring.LayerNormGrad.workspace(N, D, "cpu").shape == (64,)
+    with pytest.raises(ValueError, match="none of the gradients"):
+        scoring.LayerNormGrad.of(None, None, None, None, made_for)
