@@ -583,7 +583,8 @@ int qv_layer_norm(const void* d_x, int32_t type, int64_t rows, int64_t dim, int6
  *   dx = (h - mean(h) - x^ mean(h x^)) / sqrt(var + eps), of x's type (as grad is)
  *   dweight = sum of grad x^ over the rows, dbias = sum of grad, of param_type
  * Each of the three may be NULL (not wanted); dweight and dbias of no rows are 0.  The rows'
- * moments are taken from x again, so nothing is kept from qv_layer_norm.  d_dx may be
+ * moments are taken from x again, so nothing is kept from qv_layer_norm.  x as there; dx is
+ * finite where it is a float and the row's sums of |h| and |h x^| are, whatever h (x - mean) is.  d_dx may be
  * d_x or d_grad with the same stride.  d_workspace: qv_layer_norm_grad_workspace bytes (0:
  * none; negative: a QV_* error), 16-byte aligned, free again once the call's work on
  * the stream is done. */

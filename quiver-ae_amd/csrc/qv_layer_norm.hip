@@ -11,7 +11,8 @@
 // again, in d and in var = sum d^2 / n - (sum d / n)^2.  The gradient takes mean(h) and
 // mean(h x^) from the same exchange as var.  A row whose moments are not finite is taken
 // again times 2^-90 (its values may be up to the largest float), so only rows that hold an
-// infinity or a NaN give NaN.  All sums are fp32, in a fixed order.
+// infinity or a NaN give NaN; one whose sum of h d is none, times about 1 / s.  All sums
+// are fp32, in a fixed order.
 #include <algorithm>
 #include <cfloat>
 
@@ -109,19 +110,29 @@ __device__ __forceinline__ float lanes_sum(float v) {
 template <class T, int R, int E>
 struct Part {
   uint32_t raw[E][sizeof(T)];
+  __device__ __forceinline__ void load_one(int e, const T* row, int lane, int dim, bool four) {
+    const int j = (e * R + lane) * 4;
+    if (four) {
+      __builtin_memcpy(raw[e], row + min(j, dim - 4), 4 * sizeof(T));
+    } else {
+      T t[4] = {};
+#pragma unroll
+      for (int i = 0; i < 3; i++)
+        if (j + i < dim) t[i] = row[i];
+      __builtin_memcpy(raw[e], t, sizeof(t));
+    }
+  }
+  // TOGETHER: all behind one branch; with one for each, some wait for those before.  That is better only in the forward pass of
+  // floats within a wave (us: 60,001 x 1,001 88, together 94, 1M x 128 172, 180; but 5,000 x 16,384 118, each 130, and the
+  // gradient of 16,384 x 768 35, each 41, 200,000 x 128 62, 75, 5,000 x 6,000 90, 107, 500,000 x 64 76, 88).
+  template <bool TOGETHER>
   __device__ __forceinline__ void load(const T* row, int lane, int dim) {
+    if (TOGETHER && dim >= 4) {
 #pragma unroll
-    for (int e = 0; e < E; e++) {
-      const int j = (e * R + lane) * 4;
-      if (dim >= 4) {
-        __builtin_memcpy(raw[e], row + min(j, dim - 4), 4 * sizeof(T));
-      } else {
-        T t[4] = {};
+      for (int e = 0; e < E; e++) load_one(e, row, lane, dim, true);
+    } else {
 #pragma unroll
-        for (int i = 0; i < 3; i++)
-          if (j + i < dim) t[i] = row[i];
-        __builtin_memcpy(raw[e], t, sizeof(t));
-      }
+      for (int e = 0; e < E; e++) load_one(e, row, lane, dim, !TOGETHER && dim >= 4);
     }
   }
   __device__ __forceinline__ f4 values(int e, int lane, int dim) const {
@@ -142,19 +153,32 @@ struct Part {
   }
 };
 
+// Rows whose sum of squares passes kLargest are taken times kSmaller: 2^24 squares of the largest float are then below it, and
+// those of rows that passed it far above the smallest float.
+constexpr float kSmaller = 0x1p-90f, kLargest = FLT_MAX / 2.f;
+
+// Of the sums of d, d^2 and, of four, h and h d: whether what is made of them stays finite.  What the mean's rounding left is
+// at most the root of kLargest, so 2^57 for the sum of h keeps their product finite too.
+template <int N>
+__device__ __forceinline__ bool within(const float (&v)[N], float most) {
+  if constexpr (N == 4) return __builtin_fmaf(__builtin_fabsf(v[2]), 0x1p70f, v[1] + __builtin_fabsf(v[3])) <= most;
+  else return v[1] <= most;
+}
+
 // Sums over the R threads of a row: a part of a wave, or whole waves, which exchange theirs through two areas of LDS in
 // turn (so one barrier each: nobody writes an area again before everyone has met at the other one's).
 template <int R, int T>
 struct Row {
   static constexpr int kWaves = R / kWave;  // of a row, where it has whole ones
   static constexpr int kFloats = R > kWave ? 2 * 4 * (T / kWave) : 1;
-  float* lds;
+  float* lds;  // 16-byte aligned
   int turn = 0;
-  bool bad = false, any_bad = false;
-  // CHECK: `bad` is set where a part of the row's v[1] is above `limit` or none at all, `any_bad` where that is so of any row
-  // of the wave, or of the workgroup where rows have more than a wave's threads: all that meet at a barrier agree on it.
+  bool any_wide = false;
+  // CHECK: `any_wide` is set where a row of the wave is not within() kLargest; or, where rows have more than a wave's threads,
+  // a wave's part of any row of the workgroup not within a 16th of it: all that meet at a barrier agree on it, and no row whose
+  // sums (of 16 parts at most) are not within kLargest is left out.
   template <bool CHECK, int N>
-  __device__ __forceinline__ void sum(float (&v)[N], float limit = 0.f) {
+  __device__ __forceinline__ void sum(float (&v)[N]) {
     static_assert(N <= 4, "an area has four sums of each wave");
 #pragma unroll
     for (int i = 0; i < N; i++) v[i] = lanes_sum<R < kWave ? R : kWave>(v[i]);
@@ -168,10 +192,9 @@ struct Row {
       __syncthreads();
       const float* from = area + wave / kWaves * kWaves * 4;
       if constexpr (CHECK) {
-        any_bad = __any(lane_id() < T / kWave && !(area[4 * (lane_id() % (T / kWave)) + 1] <= limit));
-        bad = false;
-#pragma unroll
-        for (int w = 0; w < kWaves; w++) bad |= !(from[4 * w + 1] <= limit);
+        float part[N];
+        __builtin_memcpy(part, __builtin_assume_aligned(area + 4 * (lane_id() % (T / kWave)), 16), sizeof(part));
+        any_wide = __any(lane_id() < T / kWave && !within(part, kLargest / 16.f));
       }
 #pragma unroll
       for (int i = 0; i < N; i++) v[i] = from[i];
@@ -180,15 +203,10 @@ struct Row {
 #pragma unroll
         for (int i = 0; i < N; i++) v[i] += from[4 * w + i];
     } else if constexpr (CHECK) {
-      bad = !(v[1] <= limit);
-      any_bad = __any(bad);
+      any_wide = __any(!within(v, kLargest));
     }
   }
 };
-
-// Rows whose sum of squares passes kLargest, 16 of which add up to a finite sum, are taken times kSmaller: 2^24 squares
-// of the largest float are then below it, and those of rows that passed it far above the smallest float.
-constexpr float kSmaller = 0x1p-90f, kLargest = FLT_MAX / 32.f;
 
 // The variance, of the mean square of deviations from what is the mean but for `rest`.  Where all values are equal, only
 // roundings are left of it, and of the deviations less `rest` as many units of 2^-24 of it as sums have additions in a row:
@@ -197,11 +215,29 @@ __device__ __forceinline__ float variance(float square, float rest) {
   return max(__builtin_fmaf(-rest, rest, square), rest * rest * 0x1p-24f);
 }
 
+// The mean of h x^ is that of h d times 1 / s.  Where sums of h d are not finite, and with an eps for which products of h with
+// a small d may be lost (they are below 2^-126 for an h of 2^-106 and a d of the root of kSmallEps), values are taken times the
+// power of two below 1 / s, d is then about x^.  (Of values that are not all equal none is more than 2^40 s.)
+constexpr float kSmallEps = 0x1p-40f;
+__device__ __forceinline__ float power_below(float v) { return __uint_as_float(__float_as_uint(v) & 0x7f800000u); }
+
+// What a row's values are to be taken times in the gradient's next turn, after turns 0 and 1.
+__device__ __forceinline__ float next_scale(int turn, float scale, bool bad, bool wide, float var, float rstd, float eps) {
+  if (turn == 0 && bad) return kSmaller;
+  if (var == 0.f) return scale;
+  if (turn == 0 && (wide || eps < kSmallEps)) return power_below(rstd);
+  if (turn == 1 && scale == kSmaller) return kSmaller * power_below(rstd);
+  return scale;
+}
+
 // Turns a thread's part of a row (0 past its end), values(e), into deviations v, of the values times `scale`; returns
-// 1 / sqrt(var + eps) of those.  With GRAD, sums[0] and sums[1] come out as the sums of h = g w and of h d.
+// 1 / sqrt(var + eps) of those.  With GRAD, means[0] and means[1] come out as the means of h = g w and of h x^.
+//
+// Rows out of the ordinary take further turns, from their values on (next_scale).  All that meet take them, and the other rows'
+// results come out as before.
 template <bool GRAD, int R, int T, int E, class F>
 __device__ __forceinline__ float centre(F values, f4 (&v)[E], const f4 (&g)[E], const f4 (&w)[E], int lane, int dim,
-                                        float eps, Row<R, T>& row, float& scale, float (&sums)[2]) {
+                                        float eps, Row<R, T>& row, float& scale, float (&means)[2]) {
   const float per = 1.f / (float)dim;
   scale = 1.f;
   for (int turn = 0;; turn++) {
@@ -229,21 +265,26 @@ __device__ __forceinline__ float centre(F values, f4 (&v)[E], const f4 (&g)[E], 
         }
       }
     }
-    row.template sum<true>(m, kLargest);
+    row.template sum<true>(m);
     const float rest = m[0] * per, var = variance(m[1] * per, rest);
-    const bool bad = row.bad;
-    if (turn == 1 || !row.any_bad) {
+    const bool bad = !(m[1] <= kLargest);
+    const float of_eps = eps * scale * scale;
+    auto root = [&] { return 1.f / __builtin_sqrtf(bad ? __builtin_nanf("") : var == 0.f ? eps : var + of_eps); };
+    float rstd;
+    if constexpr (GRAD) rstd = root();
+    if (GRAD ? turn == 2 || turn == 0 && !row.any_wide && !(eps < kSmallEps) : turn == 1 || !row.any_wide) {
 #pragma unroll
       for (int e = 0; e < E; e++) v[e] = v[e] - rest;
+      if constexpr (!GRAD) rstd = root();
       if constexpr (GRAD) {
-        sums[0] = m[2];
-        sums[1] = m[3] - rest * m[2];
+        means[0] = m[2] * per;
+        means[1] = (m[3] - rest * m[2]) * per * rstd;
       }
-      const float of_eps = eps * scale * scale;
       if (var == 0.f) scale = 1.f;  // all deviations are 0, times any scale
-      return 1.f / __builtin_sqrtf(bad ? __builtin_nanf("") : var == 0.f ? eps : var + of_eps);
+      return rstd;
     }
-    scale = bad ? kSmaller : 1.f;  // (other rows come out as before)
+    if constexpr (GRAD) scale = next_scale(turn, scale, bad, !within(m, kLargest), var, rstd, eps);
+    else scale = bad ? kSmaller : 1.f;
 #pragma unroll
     for (int e = 0; e < E; e++) v[e] = values(e) * scale;
   }
@@ -254,7 +295,7 @@ __global__ __launch_bounds__(THREADS) void norm_kernel(const T* x, int64_t n, in
                                                        const void* bias, int param_type, float eps, T* y, int64_t y_stride,
                                                        bool stream) {
   constexpr int kGroups = THREADS / R;
-  __shared__ float lds[Row<R, THREADS>::kFloats];
+  __shared__ __align__(16) float lds[Row<R, THREADS>::kFloats];
   Row<R, THREADS> across{lds};
   const int lane = threadIdx.x % R;
   f4 w[E], b[E];
@@ -266,16 +307,17 @@ __global__ __launch_bounds__(THREADS) void norm_kernel(const T* x, int64_t n, in
   }
   const int64_t step = (int64_t)gridDim.x * kGroups;
   int64_t row = (int64_t)blockIdx.x * kGroups + threadIdx.x / R;
+  constexpr bool kTogether = R > kWave;
   Part<T, R, E> part;
-  part.load(x + min(row, n - 1) * stride, lane, dim);
+  part.template load<kTogether>(x + min(row, n - 1) * stride, lane, dim);
   for (int64_t base = (int64_t)blockIdx.x * kGroups; base < n; base += step, row += step) {
     f4 v[E];
 #pragma unroll
     for (int e = 0; e < E; e++) v[e] = part.values(e, lane, dim);
-    if (base + step < n) part.load(x + min(row + step, n - 1) * stride, lane, dim);
+    if (base + step < n) part.template load<kTogether>(x + min(row + step, n - 1) * stride, lane, dim);
     auto again = [&](int e) {
       Part<T, R, E> same;
-      same.load(x + min(row, n - 1) * stride, lane, dim);
+      same.template load<kTogether>(x + min(row, n - 1) * stride, lane, dim);
       return same.values(e, lane, dim);
     };
     float scale, none[2];
@@ -300,7 +342,7 @@ __global__ __launch_bounds__(THREADS) void norm_grad_kernel(const T* x, int64_t 
                                                             bool stream) {
   constexpr int kGroups = THREADS / R;
   constexpr int kWide = R * E * 4;
-  __shared__ float lds[Row<R, THREADS>::kFloats];
+  __shared__ __align__(16) float lds[Row<R, THREADS>::kFloats];
   __shared__ __align__(16) float columns[kGroups > 1 ? kGroups * kWide : 1];
   Row<R, THREADS> across{lds};
   const int lane = threadIdx.x % R, group = threadIdx.x / R;
@@ -310,7 +352,6 @@ __global__ __launch_bounds__(THREADS) void norm_grad_kernel(const T* x, int64_t 
     w[e] = load_params(weight, param_type, (e * R + lane) * 4, dim, 1.f);
     dw[e] = db[e] = f4{0.f, 0.f, 0.f, 0.f};
   }
-  const float per = 1.f / (float)dim;
   const int64_t step = (int64_t)gridDim.x * kGroups;
   int64_t row = (int64_t)blockIdx.x * kGroups + group;
   // A row of 16 bits ahead, as in norm_kernel, where few waves run anyway (5,000 x 12,288: 131 -> 111 us, 16,641 x 768: 27 -> 26);
@@ -318,8 +359,8 @@ __global__ __launch_bounds__(THREADS) void norm_grad_kernel(const T* x, int64_t 
   constexpr bool kAhead = THREADS == 512 && sizeof(T) == 2;
   Part<T, R, E> part, part_g;
   auto load = [&](int64_t row) {
-    part.load(x + min(row, n - 1) * stride, lane, dim);
-    part_g.load(grad + min(row, n - 1) * grad_stride, lane, dim);
+    part.template load<true>(x + min(row, n - 1) * stride, lane, dim);
+    part_g.template load<true>(grad + min(row, n - 1) * grad_stride, lane, dim);
   };
   if (kAhead) load(row);
   for (int64_t base = (int64_t)blockIdx.x * kGroups; base < n; base += step, row += step) {
@@ -333,14 +374,14 @@ __global__ __launch_bounds__(THREADS) void norm_grad_kernel(const T* x, int64_t 
     if (kAhead && base + step < n) load(row + step);
     auto again = [&](int e) {
       Part<T, R, E> same;
-      same.load(x + min(row, n - 1) * stride, lane, dim);
+      same.template load<true>(x + min(row, n - 1) * stride, lane, dim);
       return same.values(e, lane, dim);
     };
-    float scale, sums[2];
-    const float rstd = centre<true>(again, v, g, w, lane, dim, eps, across, scale, sums);
+    float scale, means[2];
+    const float rstd = centre<true>(again, v, g, w, lane, dim, eps, across, scale, means);
     if (row >= n) continue;
     // x^ = d rstd; dx = scale rstd (h - c1 - x^ c2)
-    const float c1 = sums[0] * per, c2 = sums[1] * per * rstd;
+    const float c1 = means[0], c2 = means[1];
 #pragma unroll
     for (int e = 0; e < E; e++) {
       const int j = (e * R + lane) * 4;
@@ -438,23 +479,24 @@ __device__ __forceinline__ Moments long_moments(const T* x, const T* g, const vo
         }
       }
     }
-    across.template sum<true>(m, kLargest);
+    across.template sum<true>(m);
     r.rest = m[0] * per;
-    const bool bad = across.bad;
-    if (turn == 1 || !bad) {
-      const float var = variance(m[1] * per, r.rest), of_eps = eps * r.scale * r.scale;
-      r.rstd = 1.f / __builtin_sqrtf(bad ? __builtin_nanf("") : var == 0.f ? eps : var + of_eps);
-      if (var == 0.f) {  // all deviations are 0, times any scale
-        r.mean *= 1.f / r.scale;
-        r.scale = 1.f;
-      }
+    const bool bad = !(m[1] <= kLargest);
+    const float var = variance(m[1] * per, r.rest);
+    r.rstd = 1.f / __builtin_sqrtf(bad ? __builtin_nanf("") : var == 0.f ? eps : var + eps * r.scale * r.scale);
+    if (turn == (GRAD ? 2 : 1) || turn == 0 && !across.any_wide && !(GRAD && eps < kSmallEps)) {
       if constexpr (GRAD) {
         r.c1 = m[2] * per;
         r.c2 = (m[3] - r.rest * m[2]) * per * r.rstd;
       }
+      if (var == 0.f) {  // all deviations are 0, times any scale
+        r.mean *= 1.f / r.scale;
+        r.scale = 1.f;
+      }
       return r;
     }
-    r.scale = kSmaller;
+    if constexpr (GRAD) r.scale = next_scale(turn, r.scale, bad, !within(m, kLargest), var, r.rstd, eps);
+    else if (turn == 0) r.scale = bad ? kSmaller : 1.f;
   }
 }
 
@@ -462,7 +504,7 @@ template <class T>
 __global__ __launch_bounds__(1024) void norm_long_kernel(const T* x, int64_t n, int64_t dim, int64_t stride, const void* weight,
                                                          const void* bias, int param_type, float eps, T* y, int64_t y_stride,
                                                        bool stream) {
-  __shared__ float lds[Row<1024, 1024>::kFloats];
+  __shared__ __align__(16) float lds[Row<1024, 1024>::kFloats];
   Row<1024, 1024> across{lds};
   for (int64_t row = blockIdx.x; row < n; row += gridDim.x) {
     const T* from = x + row * stride;
@@ -482,7 +524,7 @@ template <class T>
 __global__ __launch_bounds__(1024) void long_moments_kernel(const T* x, int64_t n, int64_t dim, int64_t stride, const T* grad,
                                                             int64_t grad_stride, const void* weight, int param_type, float eps,
                                                             Moments* moments) {
-  __shared__ float lds[Row<1024, 1024>::kFloats];
+  __shared__ __align__(16) float lds[Row<1024, 1024>::kFloats];
   Row<1024, 1024> across{lds};
   for (int64_t row = blockIdx.x; row < n; row += gridDim.x) {
     const Moments r = long_moments<true, T>(x + row * stride, grad + row * grad_stride, weight, param_type, dim, eps, across);

@@ -516,3 +516,36 @@ def test_lent_buffers(scoring):
                 r = scoring.LayerNormGrad.of((a, b)[place], dw, db, workspace, made_for)
                 assert scoring.layer_norm_grad(a, b, weight, out=r) is r
                 assert torch.equal((a, b)[place], want.x) and torch.equal(dw, want.weight) and torch.equal(db, want.bias)
+
+
+@pytest.mark.parametrize("dtype", [torch.float32, torch.bfloat16])
+@pytest.mark.parametrize("n, d", [(70, 7), (70, 40), (70, 100), (20, 1000), (20, 2048), (12, 4096), (12, 12000), (10, 20000)])
+def test_wide_gradients(scoring, dtype, n, d):
+    """Gradients and deviations whose products no float holds, or loses, while their quotients are ordinary; other rows' bits stay."""
+    say("layer norm, wide gradients", dtype, n, d)
+    x, weight, _, grad = _rows(n, d, torch.float32, d + 1)
+    plain = scoring.layer_norm_grad(x.to(dtype), grad.to(dtype), weight)
+    for row, of_x, of_grad in ((0, 1e16, 1e22), (1, 1e18, 1e30), (2, 1.0, 1e33), (4, 1e-15, 1e-30), (6, 1e30, 1e-5), (7, 1e25, 1e27)):
+        x[row] *= of_x
+        grad[row] *= of_grad
+    x[3] = x[3].clamp(-1, 1) * 3e38
+    grad[3] *= 1e25
+    x, grad = x.to(dtype), grad.to(dtype)
+    r = scoring.layer_norm_grad(x, grad, weight)
+    assert torch.isfinite(r.x).all() and torch.isfinite(r.weight).all()
+    _check_grad(r, x, grad, weight, torch.float32)
+    assert torch.equal(r.x[[5, 8, 9]], plain.x[[5, 8, 9]])
+    # by themselves too: sums over rows of one size
+    for row in (4, 6):
+        _check_grad(scoring.layer_norm_grad(x[row:row + 1], grad[row:row + 1], weight), x[row:row + 1], grad[row:row + 1], weight,
+                    torch.float32)
+
+
+@pytest.mark.parametrize("d", [7, 100, 1000, 4096, 20000])
+def test_small_gradients(scoring, d):
+    """With an eps near the smallest float, gradients and deviations whose products are lost, while their quotients are not."""
+    say("layer norm, small gradients", d)
+    x, weight, _, grad = _rows(20, d, torch.float32, d + 2, offset=0.0)
+    for eps, of_x, of_grad in ((2.0 ** -126, 1e-18, 1e-25), (2.0 ** -100, 1e-15, 1e-28), (2.0 ** -41, 1e-6, 1e-30)):
+        _check_grad(scoring.layer_norm_grad(x * of_x, grad * of_grad, weight, eps=eps), x * of_x, grad * of_grad, weight,
+                    torch.float32, eps)
