@@ -748,6 +748,7 @@ class DenseCatalogue:
     """
 
     bits = 8
+    dim = None  # of the vectors: in 4 bits an odd one has as many bytes as the next
 
     def __init__(self, vectors: torch.Tensor, *, bias: torch.Tensor | None = None,
                  score_dtype: torch.dtype = torch.float32, score_bytes: int = 1 << 30, bits: int = 8) -> None:
@@ -759,6 +760,7 @@ class DenseCatalogue:
             raise ValueError("score_bytes must be positive")
         self.bits = bits
         self.codes, self.scales = self._quantize(vectors)
+        self.dim = vectors.shape[1]
         if bias is not None:
             _vector("bias", bias, (vectors.shape[0],))
         self.bias, self.score_dtype, self.score_bytes = bias, score_dtype, int(score_bytes)
@@ -772,6 +774,8 @@ class DenseCatalogue:
     def scores(self, queries: torch.Tensor, *, out: torch.Tensor | None = None) -> torch.Tensor:
         """Inner products of the queries, quantised row by row, with every vector: [n, len(self)], of ``out``'s type if given."""
         codes, scales = self._quantize(queries)
+        if self.dim is not None and queries.shape[1] != self.dim:
+            raise ValueError(f"queries have {queries.shape[1]} dimensions, the catalogue's vectors {self.dim}")
         product = int8_product if self.bits == 8 else mx4_product
         return product(codes, scales, self.codes, self.scales, bias=self.bias,
                        dtype=self.score_dtype if out is None else None, out=out)

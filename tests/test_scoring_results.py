@@ -210,3 +210,24 @@ def test_lent_buffers(recorder):
     assert scoring.LayerNormGrad.workspace(N, D, "cpu").shape == (64,)
     with pytest.raises(ValueError, match="none of the gradients"):
         scoring.LayerNormGrad.of(None, None, None, None, made_for)
+
+
+@pytest.mark.parametrize("bits", [8, 4])
+@pytest.mark.parametrize("dim, other", [(7, 8), (8, 7), (33, 34), (8, 6)])
+def test_queries_of_another_length(monkeypatch, bits, dim, other):
+    """Rows of 7 values in 4 bits have as many bytes as rows of 8; queries of another length than the vectors' are refused."""
+    from quiver import scoring
+
+    def quantized(rows):
+        n, d = rows.shape
+        if bits == 8:
+            return torch.zeros((n, d), dtype=torch.int8), torch.zeros(n)
+        return torch.zeros((n, (d + 1) // 2), dtype=torch.uint8), torch.zeros((n, (d + 31) // 32), dtype=torch.uint8)
+
+    monkeypatch.setattr(scoring, "quantize_rows" if bits == 8 else "quantize_rows_mx4", quantized)
+    catalogue = scoring.DenseCatalogue(torch.zeros(5, dim), bits=bits)
+    for call in (catalogue.scores, catalogue.log_probs):
+        with pytest.raises(ValueError, match="dimensions"):
+            call(torch.zeros(3, other))
+        with pytest.raises(ValueError, match="on the GPU"):
+            call(torch.zeros(3, dim))
