@@ -993,14 +993,34 @@ void to_mx4(const void* x, int64_t n, int64_t dim, int64_t stride, uint8_t* code
   });
 }
 
+// Whether values go past the L2 (kStreamBytes), us, past it and through it; into three results in turn.  Rows of whole lines or
+// halves of them: 1M x 128 floats 81, 106; 500,000 x 128 of 16 bits every 160 26, 38.  Rows one behind the other, whose ends'
+// lines meet: of whole 16 bytes, up to 256 of them, 1M x 104 of 16 bits 41, 47, 1M x 52 floats 35, 37 (but 300,000 x 264 of 16 bits
+// 36, 32); results that the last cache does not keep beside the codes, 1.2M x 100 of 16 bits (240 MB) 57, 111, 1M x 99 floats
+// 97, 130, 1M x 100 of 16 bits (200 MB) 48, 54 (with 120 MB 31, 32; longer rows 250,000 x 1,001 of 16 bits 154, 134, 50,000 x
+// 1,004 floats 53, 44; floats that leave only part of a lane's four out of a block 3M x 31 207, 144, 1.5M x 63 150, 124).  Rows
+// apart: 1M x 100 floats every 132 144, 173; but at odd places 300,000 x 96 of 16 bits every 128 35, 15, 1M x 33 of 16 bits
+// every 40 53, 24, 200,000 x 255 of 16 bits every 300 42, 39; 1M x 100 floats every 131 168, 192.
+template <class T>
+bool values_past_the_l2(const T* out, int64_t n, int64_t dim, int64_t stride) {
+  const int64_t row = dim * (int64_t)sizeof(T), bytes = n * row;
+  const int64_t bits = reinterpret_cast<uintptr_t>(out) | stride * (int64_t)sizeof(T) | row;
+  if (bytes < kStreamBytes) return false;
+  if (bits % 64 == 0) return true;
+  if (row > 1040) return false;
+  if (stride > dim) return bits % 16 == 0 && bytes >= int64_t{256} << 20;
+  if (bytes < int64_t{180} << 20) return bits % 16 == 0 && row <= 256;
+  return sizeof(T) == 2 || dim % kBlock <= kBlock - 4;
+}
+
 template <class T>
 void from_mx4(const uint8_t* codes, int64_t n, int64_t dim, int64_t code_stride, const uint8_t* scales, int64_t scale_stride,
               void* out, int64_t stride, hipStream_t st) {
   constexpr int R = 4;
+  const bool past = values_past_the_l2(static_cast<const T*>(out), n, dim, stride);
   in_runs(n, dim, 8 * kVec<T> * R, [&](int64_t blocks, uint32_t per_row, uint32_t magic, int64_t first, unsigned count) {
     hipLaunchKernelGGL((from_mx4_kernel<T, R>), dim3(count), dim3(256), 0, st, codes, blocks, dim, code_stride, scales,
-                       scale_stride, static_cast<T*>(out), stride, per_row, magic, first,
-                       n * dim * (int64_t)sizeof(T) >= kStreamBytes);
+                       scale_stride, static_cast<T*>(out), stride, per_row, magic, first, past);
   });
 }
 

@@ -532,3 +532,21 @@ def test_longest_rows_of_a_product(scoring, m, n, k):
     out = scoring.mx4_product(a, sa, b, sb)
     # sums of up to 6,008 products, each a whole number of 2^-4 and at most 36: below 2^18, so exact
     assert torch.equal(out, (va @ vb.T.contiguous()).float())
+
+
+@pytest.mark.parametrize("n, d, wide, off, dtype", [
+    (500_001, 128, 128, 0, torch.float32), (300_000, 96, 128, 16, torch.bfloat16), (1_200_001, 100, 100, 0, torch.float16),
+    (800_000, 52, 52, 0, torch.float32), (700_000, 100, 132, 0, torch.float32), (500_000, 31, 31, 0, torch.float32),
+    (1_000_003, 33, 40, 1, torch.bfloat16), (60_001, 1001, 1001, 0, torch.float32)])
+def test_values_large_results(scoring, n, d, wide, off, dtype):
+    """Values of more than the L2s hold, past them and through them; nothing beside the rows is written."""
+    say("4-bit values, large results", n, d, wide, off, dtype)
+    g = torch.Generator(device="cuda").manual_seed(d)
+    codes = torch.randint(0, 256, (n, (d + 1) // 2), generator=g, device="cuda", dtype=torch.uint8)
+    scales = torch.randint(120, 130, (n, -(-d // 32)), generator=g, device="cuda", dtype=torch.uint8)
+    store = torch.full((n, wide), 99.0, dtype=dtype, device="cuda")
+    scoring.mx4_values(codes, scales, d, out=store[:, off:off + d])
+    assert (store[:, :off] == 99).all() and (store[:, off + d:] == 99).all()
+    for lo in range(0, n, 100_000):
+        want = values_of(codes[lo:lo + 100_000], scales[lo:lo + 100_000], d).to(dtype)
+        assert torch.equal(store[lo:lo + 100_000, off:off + d], want)
