@@ -549,3 +549,51 @@ def test_small_gradients(scoring, d):
     for eps, of_x, of_grad in ((2.0 ** -126, 1e-18, 1e-25), (2.0 ** -100, 1e-15, 1e-28), (2.0 ** -41, 1e-6, 1e-30)):
         _check_grad(scoring.layer_norm_grad(x * of_x, grad * of_grad, weight, eps=eps), x * of_x, grad * of_grad, weight,
                     torch.float32, eps)
+
+
+@pytest.mark.parametrize("dtype", TYPES)
+@pytest.mark.parametrize("n, d", [(600_001, 16), (300_001, 64), (300_001, 33), (270_001, 100), (140_001, 250), (70_001, 384),
+                                  (40_001, 768), (20_001, 1_500), (20_001, 2_000), (9_001, 2_999), (9_001, 4_000)])
+def test_gradients_of_many_rows(scoring, dtype, n, d):
+    """Workgroups of 256 threads, more rows than run at once: the bias's sums of whole numbers are exact, the weight's have terms
+    of one sign in some columns, so that rows left out show."""
+    say("layer norm, gradients of many rows", dtype, n, d)
+    x, weight, _, grad = _rows(n, d, dtype, n + d)
+    r = scoring.layer_norm_grad(x, grad, weight)
+    _check_grad(r, x, grad, weight, torch.float32)
+    g = torch.Generator(device="cuda").manual_seed(d)
+    whole = torch.randint(-2, 6, (n, d), generator=g, device="cuda").to(dtype)  # sums of up to 3.6M: every partial one is exact
+    signs = torch.sign(x.float() - x.float().mean(1, keepdim=True))
+    r = scoring.layer_norm_grad(x, whole, weight)
+    assert torch.equal(r.bias, whole.double().sum(0).float())
+    _check_grad(replace(r, x=None, bias=None), x, whole, weight, torch.float32)
+    # g of x^'s own sign: every term of the weight's gradient is positive, and their sum far from 0
+    r = scoring.layer_norm_grad(x, signs.to(dtype), weight, wanted=(False, True, False))
+    _check_grad(r, x, signs.to(dtype), weight, torch.float32)
+    assert (r.weight > 0.3 * n).all()
+
+
+def test_far_columns(scoring):
+    """The columns' sums of rows past 2^31 elements from the first: whole numbers, and terms of one sign."""
+    n, d = 2_200_000, 1025
+    say("layer norm, columns of rows past 31 bits")
+    x = torch.empty((n, d), dtype=torch.bfloat16, device="cuda").normal_()
+    grad = torch.ones_like(x)
+    r = scoring.layer_norm_grad(x, grad, wanted=(False, False, True))
+    assert (r.bias == n).all()
+    grad.copy_(torch.sign(x))
+    r = scoring.layer_norm_grad(x, grad, wanted=(False, True, True))
+    want = torch.zeros(2, d, dtype=torch.float64, device="cuda")
+    mass = torch.zeros_like(want)
+    for lo in range(0, n, 100_000):
+        hat = _moments(x[lo:lo + 100_000], EPS)[0]
+        g = grad[lo:lo + 100_000].double()
+        want[0] += (g * hat).sum(0)
+        mass[0] += (g * hat).abs().sum(0)
+        want[1] += g.sum(0)
+        mass[1] += g.abs().sum(0)
+    assert (r.weight > 0.5 * n).all()
+    a = _additions(d)
+    # x^ is off by (a + 8) u |x^| + (a + 4) u, the sum by n / 256 + 400 additions
+    _within(r.weight, want[0], ((n / 256 + 400) + a + 8) * U * mass[0] + (a + 4) * U * n, "weight")
+    assert torch.equal(r.bias, want[1].float())
