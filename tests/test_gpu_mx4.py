@@ -550,3 +550,48 @@ def test_values_large_results(scoring, n, d, wide, off, dtype):
     for lo in range(0, n, 100_000):
         want = values_of(codes[lo:lo + 100_000], scales[lo:lo + 100_000], d).to(dtype)
         assert torch.equal(store[lo:lo + 100_000, off:off + d], want)
+
+
+# rows in the registers (one and two instructions), strips (of a wave, over four waves; every number of blocks in the last step),
+# panels of two, four and eight steps, tiles through registers, and straight to LDS (few, many, walking; words and groups of scales)
+@pytest.mark.parametrize("m, n, k", [
+    (10, 700, 90), (40, 700, 130), (20, 700, 200), (16, 700, 230), (10, 700, 400), (16, 700, 262), (9, 700, 512), (16, 700, 4001),
+    (30, 700, 2001), (5, 8000, 1000), (32, 300, 2080), (129, 150_000, 120), (129, 200_001, 120), (129, 150_001, 250),
+    (130, 140_003, 500), (300, 700, 1001), (20, 900, 1152), (20, 900, 2048), (70, 700, 1152), (600, 700, 1152), (600, 900, 2048),
+    (1024, 1500, 1152), (2000, 2500, 1024), (2000, 2100, 1001), (512, 61_000, 640), (512, 61_000, 1024), (512, 61_001, 1152)])
+def test_product_nan_blocks_of_every_kernel(scoring, m, n, k):
+    """NaN scales in the first, the last and the one before it, at tiles' borders on both sides: their rows are NaN, no other is."""
+    say("4-bit product, NaN blocks", m, n, k)
+    a, sa, b, sb, _ = _inputs(m, n, k, k, near=True)
+    blocks = sa.shape[1]
+    rows_a = sorted({0, m // 2, m - 1} | {r for r in (15, 16, 31, 32, 63, 64, 127, 128, 255, 256) if r < m and r % 3})
+    rows_b = sorted({0, 5, n // 2, n - 1} | {r for r in (15, 16, 31, 32, 63, 64, 127, 128, 255, 256, 511, 512) if r < n and r % 3})
+    at = [0, blocks - 1, max(0, blocks - 2), blocks // 2]
+    want = scoring.mx4_product(a, sa, b, sb)
+    _check_product(want, a, sa, b, sb, None, torch.float32, exact=True)
+    for rows, codes, scales, axis in ((rows_a, a, sa, 0), (rows_b, b, sb, 1)):
+        bad = scales.clone()
+        for i, r in enumerate(rows):
+            bad[r, at[i % 4]] = 255
+        codes = codes.clone()
+        codes[rows[-1]] = 0  # zero codes under a NaN scale too
+        out = scoring.mx4_product(codes, bad, b, sb) if axis == 0 else scoring.mx4_product(a, sa, codes, bad)
+        there = torch.zeros(m if axis == 0 else n, dtype=torch.bool, device="cuda")
+        there[rows] = True
+        if axis == 0:
+            assert torch.isnan(out[there]).all() and torch.equal(out[~there], want[~there])
+        else:
+            assert torch.isnan(out[:, there]).all() and torch.equal(out[:, ~there], want[:, ~there])
+
+
+@pytest.mark.parametrize("m, n, k", [(1, 40, 128), (20, 40, 128), (10, 700, 400), (16, 700, 4001), (30, 700, 2001), (20, 700, 200),
+                                     (300, 300, 1024), (70, 70, 1000)])
+def test_product_large_scales_of_zeros(scoring, m, n, k):
+    """Values near the largest float against zeros: their blocks' scales multiply past it, the products are 0."""
+    say("4-bit product, large scales", m, n, k)
+    x, y = torch.zeros((m, k), device="cuda"), torch.zeros((n, k), device="cuda")
+    x[:, 0::2] = 3e38
+    y[:, 1::2] = -2e38
+    for dtype in TYPES:
+        out = scoring.mx4_product(*scoring.quantize_rows_mx4(x), *scoring.quantize_rows_mx4(y), dtype=dtype)
+        assert (out == 0).all()
