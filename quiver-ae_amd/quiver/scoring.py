@@ -395,12 +395,13 @@ class _Once(torch.autograd.Function):
     """A gradient made while a graph is recorded: there is no derivative of it, and taking one must not give zeros."""
 
     @staticmethod
-    def forward(ctx, grad, *inputs):
+    def forward(ctx, call, grad, *inputs):
+        ctx.call = call
         return grad.view_as(grad)
 
     @staticmethod
     def backward(ctx, _g):
-        raise _lib.QuiverError("the gradient of log_probs cannot be differentiated again")
+        raise _lib.QuiverError(f"the gradient of {ctx.call} cannot be differentiated again")
 
 
 class _LogProbsFunction(torch.autograd.Function):
@@ -427,7 +428,7 @@ class _LogProbsFunction(torch.autograd.Function):
                          logits.get_device(), ctx.temperature, targets, plain(g_target), plain(g_entropy), plain(g_lse),
                          plain(g_top), None)
         if torch.is_grad_enabled():
-            grad = _Once.apply(grad, logits, *(g for g in (g_target, g_entropy, g_lse, g_top) if g is not None))
+            grad = _Once.apply("log_probs", grad, logits, *(g for g in (g_target, g_entropy, g_lse, g_top) if g is not None))
         return grad, None, None, None
 
 
@@ -655,18 +656,6 @@ def _norm_grad(x, grad, weight, eps, dtype, wanted, out) -> LayerNormGrad:
     return out
 
 
-class _OnceNorm(torch.autograd.Function):
-    """A gradient made while a graph is recorded: there is no derivative of it, and taking one must not give zeros."""
-
-    @staticmethod
-    def forward(ctx, grad, *inputs):
-        return grad.view_as(grad)
-
-    @staticmethod
-    def backward(ctx, _g):
-        raise _lib.QuiverError("the gradient of layer_norm cannot be differentiated again")
-
-
 class _LayerNormFunction(torch.autograd.Function):
     @staticmethod
     def forward(ctx, x, weight, bias, eps):
@@ -685,7 +674,7 @@ class _LayerNormFunction(torch.autograd.Function):
         grads = (r.x, r.weight, r.bias)
         if torch.is_grad_enabled():
             inputs = [t for t in (g, x, weight) if t is not None]
-            grads = tuple(None if t is None else _OnceNorm.apply(t, *inputs) for t in grads)
+            grads = tuple(None if t is None else _Once.apply("layer_norm", t, *inputs) for t in grads)
         return (*grads, None)
 
 
