@@ -275,12 +275,12 @@ __device__ __forceinline__ float centre(F values, f4 (&v)[E], const f4 (&g)[E], 
     if (GRAD ? turn == 2 || turn == 0 && !row.any_wide && !(eps < kSmallEps) : turn == 1 || !row.any_wide) {
 #pragma unroll
       for (int e = 0; e < E; e++) v[e] = v[e] - rest;
+      scale = var == 0.f ? 1.f : scale;  // all deviations are 0, times any scale
       if constexpr (!GRAD) rstd = root();
       if constexpr (GRAD) {
         means[0] = m[2] * per;
         means[1] = (m[3] - rest * m[2]) * per * rstd;
       }
-      if (var == 0.f) scale = 1.f;  // all deviations are 0, times any scale
       return rstd;
     }
     if constexpr (GRAD) scale = next_scale(turn, scale, bad, !within(m, kLargest), var, rstd, eps);
