@@ -355,7 +355,8 @@ __global__ __launch_bounds__(THREADS) void norm_grad_kernel(const T* x, int64_t 
   const int64_t step = (int64_t)gridDim.x * kGroups;
   int64_t row = (int64_t)blockIdx.x * kGroups + group;
   // A row of 16 bits ahead, as in norm_kernel, where few waves run anyway (5,000 x 12,288: 131 -> 111 us, 16,641 x 768: 27 -> 26);
-  // else it takes registers for which fewer would (65,536 x 1,024 of 16 bits: 90 -> 104, 16,384 x 768 floats: 39 -> 44).
+  // else it takes registers for which fewer would (65,536 x 1,024 of 16 bits: 91 -> 108).  (Floats where few run would gain too
+  // since their loads are together: 16,384 x 768 35 -> 33, 4,096 x 4,096 53 -> 48; not done.)
   constexpr bool kAhead = THREADS == 512 && sizeof(T) == 2;
   Part<T, R, E> part, part_g;
   auto load = [&](int64_t row) {
@@ -444,7 +445,9 @@ __global__ __launch_bounds__(1024) void join_columns_kernel(const float* parts, 
 // ---- long rows (kLong, kLongGrad) ----------------------------------------------------
 //
 // A workgroup per row, which is read again for each step (from the caches while it fits).  The gradient
-// goes column by column then, with what it needs of the rows in `Moments`.
+// goes column by column then, with what it needs of the rows in `Moments`.  2,000 x 20,000, us (at 4.9 TB/s, each matrix once):
+// floats 90 (66), gradient 173 (98); 16 bits 53 (33), gradient 145 (49); 5,000 x 16,384 of 16 bits, gradient 291 (101); 8 x 1M
+// floats, eight workgroups in all, 325 (13).
 
 struct Moments {
   float mean, rest, rstd, scale, c1, c2, none[2];
@@ -568,7 +571,8 @@ constexpr int64_t kLong = 16384, kLongGrad = 12288;
 
 // The gradient's workgroups for rows of r threads, and so parts of the columns' sums: as many as run at once, or for few
 // rows one per CU, since each part is written and read again.  Measured, us, with 256 of 512 threads and 768 of 256: 4,096 x
-// 768 of 16 bits 12.9, 17.5; 16,384 x 768 24, 27; 65,536 x 768 80, 72; 4,096 x 4,096 39, 39; 60,001 x 1,001 floats 167, 150.
+// 768 of 16 bits 12.9, 17.5; 16,384 x 768 24, 28; 65,536 x 768 77, 72; 4,096 x 4,096 31, 36; 44,479 x 96 14, 18; 60,001 x 1,001
+// floats 147, 147; 500,000 x 64 83, 75.
 struct Grid {
   int threads;
   int64_t blocks;
@@ -611,8 +615,9 @@ void by_width(int64_t dim, F f) {
 }
 
 // The same for the gradient.  Past 8,192 six vectors: 1,024 threads would not have the registers (5,000 x 12,288 of 16 bits:
-// 126 us, with 1,024 threads 185, as long rows 246).  Rows of up to 64 values one or two vectors, or three
-// (with four: 1M x 64 of 16 bits 148 us, here 90; 1M x 32 65, 52; 2M x 16 114, 69; 500,000 x 64 floats 93, 80).
+// 110 us; before a row was asked for ahead 126, then with 1,024 threads 185, as long rows 246).  Rows of up to 64 values one or
+// two vectors, or three (with four: 1M x 64 of 16 bits 143 us, here 90; 1M x 32 65, 51; 2M x 16 114, 67; 500,000 x 64 floats
+// 81, 75).
 template <class F>
 void by_grad_width(int64_t dim, F f) {
   if (dim > 8192) f(std::integral_constant<int, 512>(), std::integral_constant<int, 6>());

@@ -23,7 +23,7 @@ constexpr int kBlock = 32;  // values that share a scale
 // number, gives the scale, the least power of two of which a is 7 times at most (then no
 // value is further than half a step of the codes from its own).  The scaled values are
 // exact, and one instruction rounds two of them, halves to even, magnitudes over 6 to 6.
-// Bound by memory: 1M x 128 floats 109 us, 5.3 TB/s; 1M x 128 of 16 bits 61, 100,000 x 769 43.
+// Bound by memory: 1M x 128 floats 104 to 109 us, 5.3 TB/s; 1M x 128 of 16 bits 63, 100,000 x 769 43.
 
 constexpr uint32_t kInfBits = 0x7f800000u;
 
@@ -103,8 +103,8 @@ __device__ __forceinline__ float scale_of(uint32_t s) {
   return s == 255 ? __builtin_nanf("") : __uint_as_float(s ? s << 23 : 1u << 22);
 }
 
-// Back again, a lane writes 16 bytes of a row: 1M x 128 to float 81 us (lanes of 32 bytes, in two stores, and through the
-// L2: 149).
+// Back again, a lane writes 16 bytes of a row: 1M x 128 to float 81 us call after call, 7.2 TB/s, into one result
+// or three in turn; behind the calls that make the codes 93 (lanes of 32 bytes, in two stores, and through the L2: 149).
 template <class T, int R>
 __global__ __launch_bounds__(256) void from_mx4_kernel(const uint8_t* __restrict__ codes, int64_t blocks, int64_t dim,
                                                        int64_t code_stride, const uint8_t* __restrict__ scales,
@@ -861,7 +861,8 @@ __global__ __launch_bounds__(WK == 1 ? 256 : 64 * WK) void product_strip_kernel(
 
 // Short rows, k <= 32 KS bytes, whose product is mostly writing: 32 rows of a stay in a wave's
 // registers while its workgroup (128 rows) walks over tiles of 64 rows of b, through
-// LDS with the next two tiles on their way.  Results leave in whole lines (LineRing).
+// LDS with the next two tiles on their way.  Results leave in whole lines (LineRing).  (KS = 4 to floats spills two of its 168
+// registers, 12 bytes of a lane.)
 template <int KS, class O>
 __global__ __launch_bounds__(256, KS == 8 ? 2 : 3) void product_panel_kernel(Product<O> p, int64_t panels, int64_t tiles_n,
                                                                              int64_t slices) {
